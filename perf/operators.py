@@ -181,11 +181,11 @@ def _own(s):
     mc = __graft_entry__.load_package()
     c, x = s["case"], s["logits"]
     if c["kind"] == "logprobs":
-        logps, lse = mc.token_logprobs_forward(x, s["targets"], ignore_index=IGNORE, temperature=c["temperature"],
-                                               save_lse=c["train"])
+        logps, stats = mc.token_logprobs_forward(x, s["targets"], ignore_index=IGNORE, temperature=c["temperature"],
+                                                 save_stats=c["train"])
         if not c["train"]:
             return logps
-        return logps, mc.token_logprobs_backward(x, s["targets"], lse, s["dlogps"], ignore_index=IGNORE,
+        return logps, mc.token_logprobs_backward(x, s["targets"], stats, s["dlogps"], ignore_index=IGNORE,
                                                  temperature=c["temperature"])
     if c["kind"] == "preference":
         loss, rewards, stats = mc.preference_loss_forward(

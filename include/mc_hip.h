@@ -32,6 +32,9 @@
  *                    bias of MetalLayerNorm (src/embeddings/metal_bert.rs).
  *   mc_log_softmax_*, mc_cross_entropy_*  cross_entropy_loss and its label
  *                    smoothing (src/training/loss.rs:58-245).
+ *   mc_token_logprobs_*, mc_preference_loss_*, mc_policy_loss_*,
+ *   mc_distill_loss_*  no counterpart in the reference: losses over the same
+ *                    logits for preferences, rewards and teachers.
  *
  * Conventions (all entry points):
  *  - Device buffers are caller-owned, row-major and contiguous; inputs are
@@ -357,6 +360,160 @@ mc_status mc_cross_entropy_fwd(const mc_xent_desc* d, const void* logits, const 
 mc_status mc_cross_entropy_bwd(const mc_xent_desc* d, const void* logits, const uint32_t* targets,
                                const float* stats, const float* dloss, void* dlogits, hipStream_t stream);
 
+/* Losses over the logits [rows, vocab] for what comes after supervised
+ * fine-tuning. No counterpart in the reference, whose only loss is the cross
+ * entropy; targets and ignore_index are as there, T is a temperature in
+ * [1e-6, 1e6], vocab < 2^31 and rows <= 16777215. logits may start at any element.
+ * A row whose target is ignore_index (distillation: whose mask is 0) is not
+ * counted: it is not read, whatever it holds, and its gradient is zero, as is
+ * that of a row whose loss has no gradient. A counted id past the vocabulary
+ * makes the loss NaN and the gradients that depend on it. Sums run in a fixed
+ * order: results are bitwise reproducible. dloss: fp32 [1] on the device, the
+ * gradient of the loss, or NULL for 1. stats of a forward, which its backward
+ * needs, start with each row's maximum and sum of exponentials [rows, 2].
+ *
+ * Log-probabilities of given tokens, l = x[t] / T - log sum exp(x / T), fp32
+ * [rows]; 0 where the row is not counted. stats fp32 [rows, 2] may be NULL. */
+typedef struct mc_logprob_desc {
+    int64_t rows;          /* 1 .. 16777215 */
+    int64_t vocab;         /* 1 .. 2^31 - 1 */
+    int64_t ignore_index;  /* < 0: none */
+    float temperature;
+    int32_t dtype;         /* mc_dtype of logits and dlogits */
+} mc_logprob_desc;
+
+mc_status mc_token_logprobs_fwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets, float* logps,
+                                float* stats, hipStream_t stream);
+
+/* dlogits = dlogps ([j = target] - softmax(x / T)) / T; dlogps fp32 [rows]. */
+mc_status mc_token_logprobs_bwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets,
+                                const float* stats, const float* dlogps, void* dlogits, hipStream_t stream);
+
+/* Preference loss over pairs of sequences: logits [2 pairs, seq, vocab], the
+ * preferred answers first, then the others in the same order; targets
+ * [2 pairs, seq]; ref_logps fp32 [2 pairs, seq], the reference policy's
+ * log-probabilities (mc_token_logprobs_fwd), or NULL for none. With T = 1 and
+ *   s = sum over a sequence's counted tokens of (l - ref) (average: the mean; 0 if there are none)
+ *   d = s_preferred - s_other,  z = beta d - margin
+ * a pair's loss is
+ *   MC_PREF_SIGMOID  -(1 - e) log sigma(z) - e log sigma(-z), e = label_smoothing
+ *   MC_PREF_HINGE    max(0, 1 - z)
+ *   MC_PREF_SQUARED  (d - 1 / (2 beta))^2
+ * and loss (fp32 [1]) their mean over the pairs. rewards fp32 [2 pairs] (may be
+ * NULL) receives beta s, stats fp32 [rows * 2 + 2 pairs] (may be NULL) what the
+ * backward needs, rows = 2 pairs seq. The scores are summed in 64 bits. */
+typedef enum mc_pref_kind {
+    MC_PREF_SIGMOID = 0,
+    MC_PREF_HINGE = 1,
+    MC_PREF_SQUARED = 2,
+} mc_pref_kind;
+
+typedef struct mc_preference_desc {
+    int64_t pairs;          /* >= 1; 2 pairs seq <= 16777215 */
+    int64_t seq;            /* >= 1 */
+    int64_t vocab;          /* 1 .. 2^31 - 1 */
+    int64_t ignore_index;   /* < 0: none */
+    int32_t kind;           /* mc_pref_kind */
+    int32_t average;        /* 0 or 1 */
+    float beta;             /* > 0 */
+    float label_smoothing;  /* [0, 1); 0 unless MC_PREF_SIGMOID */
+    float margin;           /* finite; 0 for MC_PREF_SQUARED */
+    int32_t dtype;
+} mc_preference_desc;
+
+size_t mc_preference_loss_workspace_size(const mc_preference_desc* d);
+
+mc_status mc_preference_loss_fwd(const mc_preference_desc* d, const void* logits, const uint32_t* targets,
+                                 const float* ref_logps, float* loss, float* rewards, float* stats, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream);
+mc_status mc_preference_loss_bwd(const mc_preference_desc* d, const void* logits, const uint32_t* targets,
+                                 const float* stats, const float* dloss, void* dlogits, hipStream_t stream);
+
+/* Clipped policy loss: logits [batch, seq, vocab], targets [batch, seq] (the
+ * sampled tokens), advantages fp32 [batch] or [batch, seq]; old_logps and
+ * ref_logps fp32 [batch, seq], the sampling and the reference policy's
+ * log-probabilities at the same T. Per counted token, r = exp(l - old) (1 when
+ * old_logps is NULL, the gradient then that of l A),
+ *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef kl
+ *   kl = exp(ref - l) - (ref - l) - 1   (0 when ref_logps is NULL)
+ * Where the clipped side is the smaller one the surrogate has no gradient. The
+ * loss (fp32 [1]) is the mean over the counted tokens, or with
+ * MC_MEAN_SEQUENCES the mean over the batch of each sequence's mean, 0 for a
+ * sequence without counted tokens. MC_MEAN_TOKENS without a counted token gives
+ * NaN, as the cross entropy. logps fp32 [batch, seq] receives l; metrics fp32
+ * [2] (may be NULL) kl and the clipped share, averaged as the loss is; stats
+ * fp32 [rows * 3 + 1] (may be NULL) what the backward needs. */
+typedef enum mc_mean {
+    MC_MEAN_TOKENS = 0,
+    MC_MEAN_SEQUENCES = 1,
+} mc_mean;
+
+typedef struct mc_policy_desc {
+    int64_t batch;                 /* >= 1; batch * seq <= 16777215 */
+    int64_t seq;                   /* >= 1 */
+    int64_t vocab;                 /* 1 .. 2^31 - 1 */
+    int64_t ignore_index;          /* < 0: none */
+    int32_t per_token_advantages;  /* 0: [batch], 1: [batch, seq] */
+    int32_t reduction;             /* mc_mean */
+    float clip_low;                /* [0, 1] */
+    float clip_high;               /* >= 0, finite */
+    float kl_coef;                 /* >= 0, finite; > 0 needs ref_logps */
+    float temperature;
+    int32_t dtype;
+} mc_policy_desc;
+
+size_t mc_policy_loss_workspace_size(const mc_policy_desc* d);
+
+mc_status mc_policy_loss_fwd(const mc_policy_desc* d, const void* logits, const uint32_t* targets,
+                             const float* advantages, const float* old_logps, const float* ref_logps, float* loss,
+                             float* logps, float* metrics, float* stats, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream);
+mc_status mc_policy_loss_bwd(const mc_policy_desc* d, const void* logits, const uint32_t* targets, const float* stats,
+                             const float* dloss, void* dlogits, hipStream_t stream);
+
+/* Both in one call, for a training step: the weight of each token is known
+ * from the targets, so loss and gradient need not read the logits twice. */
+size_t mc_policy_loss_fwd_bwd_workspace_size(const mc_policy_desc* d);
+mc_status mc_policy_loss_fwd_bwd(const mc_policy_desc* d, const void* logits, const uint32_t* targets,
+                                 const float* advantages, const float* old_logps, const float* ref_logps,
+                                 const float* dloss, float* loss, float* logps, float* metrics, void* dlogits,
+                                 void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Distillation from a teacher's top logits: teacher_ids int32 and
+ * teacher_logits fp32 [rows, top], in any order; an entry of -inf is left out,
+ * whatever its id (rows of fewer entries), and an id that comes twice counts
+ * twice. p = softmax over the row's entries of teacher_logits / T, or with
+ * teacher_lse fp32 [rows] (the log-sum-exp of all the teacher's logits / T)
+ * p = exp(teacher_logits / T - teacher_lse). With q = softmax(logits / T)
+ *   loss = T^2 mean over the counted rows of sum_k p_k (log p_k - log q_{id k})
+ *   dlogits = dloss (T / counted rows) (q_j sum_k p_k - sum_{k: id k = j} p_k)
+ * mask uint8 [rows] (NULL: every row is counted); no row counted: NaN. A row
+ * whose entries are all left out counts and adds 0. stats fp32 [rows * 2 + 1]. */
+#define MC_DISTILL_MAX_TOP 256
+typedef struct mc_distill_desc {
+    int64_t rows;       /* 1 .. 16777215 */
+    int64_t vocab;      /* 1 .. 2^31 - 1 */
+    int32_t top;        /* 1 .. MC_DISTILL_MAX_TOP */
+    float temperature;
+    int32_t dtype;
+} mc_distill_desc;
+
+size_t mc_distill_loss_workspace_size(const mc_distill_desc* d);
+
+mc_status mc_distill_loss_fwd(const mc_distill_desc* d, const void* logits, const int32_t* teacher_ids,
+                              const float* teacher_logits, const float* teacher_lse, const uint8_t* mask, float* loss,
+                              float* stats, void* workspace, size_t workspace_bytes, hipStream_t stream);
+mc_status mc_distill_loss_bwd(const mc_distill_desc* d, const void* logits, const int32_t* teacher_ids,
+                              const float* teacher_logits, const float* teacher_lse, const uint8_t* mask,
+                              const float* stats, const float* dloss, void* dlogits, hipStream_t stream);
+
+/* Both in one call, as mc_policy_loss_fwd_bwd. */
+size_t mc_distill_loss_fwd_bwd_workspace_size(const mc_distill_desc* d);
+mc_status mc_distill_loss_fwd_bwd(const mc_distill_desc* d, const void* logits, const int32_t* teacher_ids,
+                                  const float* teacher_logits, const float* teacher_lse, const uint8_t* mask,
+                                  const float* dloss, float* loss, void* dlogits, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream);
+
 /* Host-side dropout keep-mask [rows, rank] from a seed (Philox4x32-10; element
  * i = t*rank + j uses counter block i/4, word i%4, key = seed; keep iff
  * (word >> 8) * 2^-24 >= p). Both the GPU path and the CPU reference are fed
@@ -374,7 +531,7 @@ mc_status mc_dropout_mask(uint64_t seed, float p, int64_t rows, int32_t rank, ui
  * base x.W^T / dY.W product only), 1 = rank-r kernels, 2 = RMSNorm,
  * 3 = softmax, 4 = attention (FLOPs of the unmasked score and P.V products),
  * 5 = AdamW (bytes: 28 per element), 6 = LayerNorm / log-softmax /
- * cross-entropy.
+ * cross-entropy and the other losses.
  * Enabling allocates hipEvents (not for allocation-free use). */
 mc_status mc_profile_enable(int32_t on);
 mc_status mc_profile_collect(void);

@@ -14,6 +14,9 @@ from .ops import (  # noqa: F401
     attention_forward,
     cross_entropy_backward,
     cross_entropy_forward,
+    distillation_loss_backward,
+    distillation_loss_forward,
+    distillation_loss_forward_backward,
     dropout_mask,
     layer_norm_backward,
     layer_norm_forward,
@@ -23,9 +26,16 @@ from .ops import (  # noqa: F401
     lora_forward,
     lora_group_backward,
     lora_group_forward,
+    policy_loss_backward,
+    policy_loss_forward,
+    policy_loss_forward_backward,
+    preference_loss_backward,
+    preference_loss_forward,
     rms_norm_backward,
     rms_norm_forward,
     softmax_backward,
     softmax_forward,
+    token_logprobs_backward,
+    token_logprobs_forward,
     transpose_weight,
 )

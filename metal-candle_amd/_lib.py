@@ -88,6 +88,69 @@ class XentDesc(ctypes.Structure):
     ]
 
 
+class LogprobDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("temperature", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+MC_PREF_SIGMOID = 0
+MC_PREF_HINGE = 1
+MC_PREF_SQUARED = 2
+
+
+class PreferenceDesc(ctypes.Structure):
+    _fields_ = [
+        ("pairs", ctypes.c_int64),
+        ("seq", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("kind", ctypes.c_int32),
+        ("average", ctypes.c_int32),
+        ("beta", ctypes.c_float),
+        ("label_smoothing", ctypes.c_float),
+        ("margin", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+MC_MEAN_TOKENS = 0
+MC_MEAN_SEQUENCES = 1
+
+
+class PolicyDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("seq", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("per_token_advantages", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("clip_low", ctypes.c_float),
+        ("clip_high", ctypes.c_float),
+        ("kl_coef", ctypes.c_float),
+        ("temperature", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+MC_DISTILL_MAX_TOP = 256
+
+
+class DistillDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("top", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 class AdamWConfig(ctypes.Structure):
     _fields_ = [
         ("learning_rate", ctypes.c_float),
@@ -117,6 +180,10 @@ _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
 _dp = ctypes.POINTER(LoraDesc)
 _ap = ctypes.POINTER(AttnDesc)
+_lp = ctypes.POINTER(LogprobDesc)
+_rp = ctypes.POINTER(PreferenceDesc)
+_pp = ctypes.POINTER(PolicyDesc)
+_tp = ctypes.POINTER(DistillDesc)
 
 _SIGNATURES = {
     "mc_version": (ctypes.c_char_p, []),
@@ -152,6 +219,21 @@ _SIGNATURES = {
     "mc_cross_entropy_workspace_size": (_sz, [ctypes.POINTER(XentDesc)]),
     "mc_cross_entropy_fwd": (ctypes.c_int, [ctypes.POINTER(XentDesc), _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mc_cross_entropy_bwd": (ctypes.c_int, [ctypes.POINTER(XentDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_token_logprobs_fwd": (ctypes.c_int, [_lp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_token_logprobs_bwd": (ctypes.c_int, [_lp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_preference_loss_workspace_size": (_sz, [_rp]),
+    "mc_preference_loss_fwd": (ctypes.c_int, [_rp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_preference_loss_bwd": (ctypes.c_int, [_rp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_policy_loss_workspace_size": (_sz, [_pp]),
+    "mc_policy_loss_fwd": (ctypes.c_int, [_pp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_policy_loss_bwd": (ctypes.c_int, [_pp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_policy_loss_fwd_bwd_workspace_size": (_sz, [_pp]),
+    "mc_policy_loss_fwd_bwd": (ctypes.c_int, [_pp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_distill_loss_workspace_size": (_sz, [_tp]),
+    "mc_distill_loss_fwd": (ctypes.c_int, [_tp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_distill_loss_bwd": (ctypes.c_int, [_tp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_distill_loss_fwd_bwd_workspace_size": (_sz, [_tp]),
+    "mc_distill_loss_fwd_bwd": (ctypes.c_int, [_tp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mc_adamw_step": (ctypes.c_int, [ctypes.POINTER(AdamWConfig), ctypes.POINTER(AdamWTensor), _i32, _vp]),
     "mc_dropout_mask": (ctypes.c_int, [ctypes.c_uint64, _f32, _i64, _i32, _vp]),
     "mc_profile_enable": (ctypes.c_int, [_i32]),

@@ -723,6 +723,271 @@ mc_status mc_cross_entropy_bwd(const mc_xent_desc* d, const void* logits, const 
                       "cross_entropy backward");
 }
 
+// ------------------------------------------------ losses over log-probabilities
+static mc_status check_vocab(const char* op, int64_t rows, int64_t vocab, int32_t dtype) {
+    mc_status s = check_dtype(dtype, op);
+    if (s != MC_OK) return s;
+    MC_CHECK(rows >= 1 && rows <= kMaxBlockRows && vocab >= 1 && vocab < ((int64_t)1 << 31), MC_ERR_SHAPE,
+             "%s: rows (%lld) must be in [1, %lld] and vocab (%lld) in [1, 2^31 - 1]", op, (long long)rows,
+             (long long)kMaxBlockRows, (long long)vocab);
+    return MC_OK;
+}
+
+static mc_status check_temperature(const char* op, float t) {
+    MC_CHECK(t >= 1e-6f && t <= 1e6f, MC_ERR_VALUE, "%s: temperature must be in [1e-6, 1e6], got %g", op, (double)t);
+    return MC_OK;
+}
+
+static mc_status check_logits(const char* op, int32_t dtype, const void* logits, const void* dlogits) {
+    const uintptr_t es = dtype == MC_F32 ? 4 : 2;
+    MC_CHECK(reinterpret_cast<uintptr_t>(logits) % es == 0 && reinterpret_cast<uintptr_t>(dlogits) % es == 0,
+             MC_ERR_LAYOUT, "%s: logits and dlogits must be aligned to their elements", op);
+    return MC_OK;
+}
+
+static mc_status check_workspace(const char* op, const void* workspace, size_t bytes, size_t need) {
+    MC_CHECK(workspace && bytes >= need, MC_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", op, need,
+             bytes);
+    MC_CHECK(aligned16(workspace), MC_ERR_LAYOUT, "%s: workspace must be 16-byte aligned", op);
+    return MC_OK;
+}
+
+// n sequences of seq rows as rows, 0 if there are too many
+static int64_t seq_rows(int64_t n, int64_t seq) {
+    return n >= 1 && seq >= 1 && n <= kMaxBlockRows && seq <= kMaxBlockRows ? n * seq : 0;
+}
+
+static double logit_bytes(int64_t rows, int64_t vocab, int32_t dtype, double passes) {
+    return (dtype == MC_F32 ? 4.0 : 2.0) * passes * (double)rows * (double)vocab;
+}
+
+static mc_status check_logprob(const mc_logprob_desc* d) {
+    MC_CHECK(d != nullptr, MC_ERR_NULL, "token_logprobs: descriptor is NULL");
+    mc_status s = check_vocab("token_logprobs", d->rows, d->vocab, d->dtype);
+    return s != MC_OK ? s : check_temperature("token_logprobs", d->temperature);
+}
+
+mc_status mc_token_logprobs_fwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets, float* logps,
+                                float* stats, hipStream_t stream) {
+    mc_status s = check_logprob(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && targets && logps, MC_ERR_NULL, "token_logprobs: logits, targets and logps must not be NULL");
+    if ((s = check_logits("token_logprobs", d->dtype, logits, nullptr)) != MC_OK) return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 1.0));
+    return hip_status(mc::launch_token_logprobs_fwd(*d, logits, targets, logps, stats, nullptr, stream),
+                      "token_logprobs forward");
+}
+
+mc_status mc_token_logprobs_bwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets,
+                                const float* stats, const float* dlogps, void* dlogits, hipStream_t stream) {
+    mc_status s = check_logprob(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && targets && stats && dlogps && dlogits, MC_ERR_NULL,
+             "token_logprobs backward: logits, targets, stats, dlogps and dlogits must not be NULL");
+    if ((s = check_logits("token_logprobs backward", d->dtype, logits, dlogits)) != MC_OK) return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 2.0));
+    return hip_status(mc::launch_token_logprobs_bwd(*d, logits, targets, stats, dlogps, 0, nullptr, nullptr, dlogits,
+                                                    stream),
+                      "token_logprobs backward");
+}
+
+static mc_status check_preference(const mc_preference_desc* d) {
+    MC_CHECK(d != nullptr, MC_ERR_NULL, "preference_loss: descriptor is NULL");
+    mc_status s = check_vocab("preference_loss", d->pairs >= 1 && d->pairs <= kMaxBlockRows ? seq_rows(2 * d->pairs, d->seq) : 0,
+                              d->vocab, d->dtype);
+    if (s != MC_OK) return s;
+    MC_CHECK(d->kind == MC_PREF_SIGMOID || d->kind == MC_PREF_HINGE || d->kind == MC_PREF_SQUARED, MC_ERR_VALUE,
+             "preference_loss: unknown kind %d", (int)d->kind);
+    MC_CHECK(d->average == 0 || d->average == 1, MC_ERR_VALUE, "preference_loss: average must be 0 or 1");
+    MC_CHECK(d->beta > 0.0f && std::isfinite(d->beta), MC_ERR_VALUE, "preference_loss: beta must be positive, got %g",
+             (double)d->beta);
+    MC_CHECK(d->label_smoothing >= 0.0f && d->label_smoothing < 1.0f, MC_ERR_VALUE,
+             "preference_loss: label_smoothing must be in [0, 1), got %g", (double)d->label_smoothing);
+    MC_CHECK(d->label_smoothing == 0.0f || d->kind == MC_PREF_SIGMOID, MC_ERR_VALUE,
+             "preference_loss: label_smoothing belongs to the sigmoid loss");
+    MC_CHECK(std::isfinite(d->margin), MC_ERR_VALUE, "preference_loss: margin must be finite");
+    MC_CHECK(d->margin == 0.0f || d->kind != MC_PREF_SQUARED, MC_ERR_VALUE,
+             "preference_loss: the squared loss has no margin");
+    return MC_OK;
+}
+
+size_t mc_preference_loss_workspace_size(const mc_preference_desc* d) {
+    return check_preference(d) == MC_OK ? mc::preference_ws(*d).total : 0;
+}
+
+mc_status mc_preference_loss_fwd(const mc_preference_desc* d, const void* logits, const uint32_t* targets,
+                                 const float* ref_logps, float* loss, float* rewards, float* stats, void* workspace,
+                                 size_t workspace_bytes, hipStream_t stream) {
+    mc_status s = check_preference(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && targets && loss, MC_ERR_NULL, "preference_loss: logits, targets and loss must not be NULL");
+    if ((s = check_logits("preference_loss", d->dtype, logits, nullptr)) != MC_OK) return s;
+    if ((s = check_workspace("preference_loss", workspace, workspace_bytes, mc::preference_ws(*d).total)) != MC_OK)
+        return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(2 * d->pairs * d->seq, d->vocab, d->dtype, 1.0));
+    return hip_status(mc::launch_preference_fwd(*d, logits, targets, ref_logps, loss, rewards, stats,
+                                                static_cast<char*>(workspace), stream),
+                      "preference_loss forward");
+}
+
+mc_status mc_preference_loss_bwd(const mc_preference_desc* d, const void* logits, const uint32_t* targets,
+                                 const float* stats, const float* dloss, void* dlogits, hipStream_t stream) {
+    mc_status s = check_preference(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && targets && stats && dlogits, MC_ERR_NULL,
+             "preference_loss backward: logits, targets, stats and dlogits must not be NULL");
+    if ((s = check_logits("preference_loss backward", d->dtype, logits, dlogits)) != MC_OK) return s;
+    const int64_t rows = 2 * d->pairs * d->seq;
+    const mc_logprob_desc lp{rows, d->vocab, d->ignore_index, 1.0f, d->dtype};
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(rows, d->vocab, d->dtype, 2.0));
+    return hip_status(mc::launch_token_logprobs_bwd(lp, logits, targets, stats, stats + 2 * rows, d->seq, nullptr,
+                                                    dloss, dlogits, stream),
+                      "preference_loss backward");
+}
+
+static mc_status check_policy(const mc_policy_desc* d) {
+    MC_CHECK(d != nullptr, MC_ERR_NULL, "policy_loss: descriptor is NULL");
+    mc_status s = check_vocab("policy_loss", seq_rows(d->batch, d->seq), d->vocab, d->dtype);
+    if (s != MC_OK) return s;
+    if ((s = check_temperature("policy_loss", d->temperature)) != MC_OK) return s;
+    MC_CHECK(d->per_token_advantages == 0 || d->per_token_advantages == 1, MC_ERR_VALUE,
+             "policy_loss: per_token_advantages must be 0 or 1");
+    MC_CHECK(d->reduction == MC_MEAN_TOKENS || d->reduction == MC_MEAN_SEQUENCES, MC_ERR_VALUE,
+             "policy_loss: unknown reduction %d", (int)d->reduction);
+    MC_CHECK(d->clip_low >= 0.0f && d->clip_low <= 1.0f && d->clip_high >= 0.0f && std::isfinite(d->clip_high),
+             MC_ERR_VALUE, "policy_loss: clip_low must be in [0, 1] and clip_high finite and >= 0");
+    MC_CHECK(d->kl_coef >= 0.0f && std::isfinite(d->kl_coef), MC_ERR_VALUE,
+             "policy_loss: kl_coef must be finite and >= 0");
+    return MC_OK;
+}
+
+size_t mc_policy_loss_workspace_size(const mc_policy_desc* d) {
+    return check_policy(d) == MC_OK ? mc::policy_ws(*d).total : 0;
+}
+
+size_t mc_policy_loss_fwd_bwd_workspace_size(const mc_policy_desc* d) {
+    return check_policy(d) == MC_OK ? mc::policy_fwd_bwd_ws(*d) : 0;
+}
+
+static mc_status check_policy_inputs(const mc_policy_desc* d, const void* logits, const uint32_t* targets,
+                                     const float* advantages, const float* ref_logps, const float* loss,
+                                     const float* logps) {
+    MC_CHECK(logits && targets && advantages && loss && logps, MC_ERR_NULL,
+             "policy_loss: logits, targets, advantages, loss and logps must not be NULL");
+    MC_CHECK(ref_logps || d->kl_coef == 0.0f, MC_ERR_NULL, "policy_loss: kl_coef > 0 requires ref_logps");
+    return MC_OK;
+}
+
+mc_status mc_policy_loss_fwd(const mc_policy_desc* d, const void* logits, const uint32_t* targets,
+                             const float* advantages, const float* old_logps, const float* ref_logps, float* loss,
+                             float* logps, float* metrics, float* stats, void* workspace, size_t workspace_bytes,
+                             hipStream_t stream) {
+    mc_status s = check_policy(d);
+    if (s != MC_OK) return s;
+    if ((s = check_policy_inputs(d, logits, targets, advantages, ref_logps, loss, logps)) != MC_OK) return s;
+    if ((s = check_logits("policy_loss", d->dtype, logits, nullptr)) != MC_OK) return s;
+    if ((s = check_workspace("policy_loss", workspace, workspace_bytes, mc::policy_ws(*d).total)) != MC_OK) return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->batch * d->seq, d->vocab, d->dtype, 1.0));
+    return hip_status(mc::launch_policy_fwd(*d, logits, targets, advantages, old_logps, ref_logps, loss, logps, metrics,
+                                            stats, static_cast<char*>(workspace), stream),
+                      "policy_loss forward");
+}
+
+mc_status mc_policy_loss_bwd(const mc_policy_desc* d, const void* logits, const uint32_t* targets, const float* stats,
+                             const float* dloss, void* dlogits, hipStream_t stream) {
+    mc_status s = check_policy(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && targets && stats && dlogits, MC_ERR_NULL,
+             "policy_loss backward: logits, targets, stats and dlogits must not be NULL");
+    if ((s = check_logits("policy_loss backward", d->dtype, logits, dlogits)) != MC_OK) return s;
+    const int64_t rows = d->batch * d->seq;
+    const mc_logprob_desc lp{rows, d->vocab, d->ignore_index, d->temperature, d->dtype};
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(rows, d->vocab, d->dtype, 2.0));
+    return hip_status(mc::launch_token_logprobs_bwd(lp, logits, targets, stats, stats + 2 * rows, 0, stats + 3 * rows,
+                                                    dloss, dlogits, stream),
+                      "policy_loss backward");
+}
+
+mc_status mc_policy_loss_fwd_bwd(const mc_policy_desc* d, const void* logits, const uint32_t* targets,
+                                 const float* advantages, const float* old_logps, const float* ref_logps,
+                                 const float* dloss, float* loss, float* logps, float* metrics, void* dlogits,
+                                 void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    mc_status s = check_policy(d);
+    if (s != MC_OK) return s;
+    if ((s = check_policy_inputs(d, logits, targets, advantages, ref_logps, loss, logps)) != MC_OK) return s;
+    MC_CHECK(dlogits, MC_ERR_NULL, "policy_loss: dlogits must not be NULL");
+    if ((s = check_logits("policy_loss", d->dtype, logits, dlogits)) != MC_OK) return s;
+    if ((s = check_workspace("policy_loss", workspace, workspace_bytes, mc::policy_fwd_bwd_ws(*d))) != MC_OK) return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->batch * d->seq, d->vocab, d->dtype, 2.0));
+    return hip_status(mc::launch_policy_fwd_bwd(*d, logits, targets, advantages, old_logps, ref_logps, dloss, loss,
+                                                logps, metrics, dlogits, static_cast<char*>(workspace), stream),
+                      "policy_loss forward and backward");
+}
+
+static mc_status check_distill(const mc_distill_desc* d) {
+    MC_CHECK(d != nullptr, MC_ERR_NULL, "distillation_loss: descriptor is NULL");
+    mc_status s = check_vocab("distillation_loss", d->rows, d->vocab, d->dtype);
+    if (s != MC_OK) return s;
+    MC_CHECK(d->top >= 1 && d->top <= MC_DISTILL_MAX_TOP, MC_ERR_SHAPE,
+             "distillation_loss: %d teacher entries per row, must be in [1, %d]", (int)d->top, MC_DISTILL_MAX_TOP);
+    return check_temperature("distillation_loss", d->temperature);
+}
+
+size_t mc_distill_loss_workspace_size(const mc_distill_desc* d) {
+    return check_distill(d) == MC_OK ? mc::distill_ws(*d).total : 0;
+}
+
+size_t mc_distill_loss_fwd_bwd_workspace_size(const mc_distill_desc* d) {
+    return check_distill(d) == MC_OK ? mc::distill_fwd_bwd_ws(*d) : 0;
+}
+
+mc_status mc_distill_loss_fwd(const mc_distill_desc* d, const void* logits, const int32_t* teacher_ids,
+                              const float* teacher_logits, const float* teacher_lse, const uint8_t* mask, float* loss,
+                              float* stats, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    mc_status s = check_distill(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && teacher_ids && teacher_logits && loss, MC_ERR_NULL,
+             "distillation_loss: logits, teacher_ids, teacher_logits and loss must not be NULL");
+    if ((s = check_logits("distillation_loss", d->dtype, logits, nullptr)) != MC_OK) return s;
+    if ((s = check_workspace("distillation_loss", workspace, workspace_bytes, mc::distill_ws(*d).total)) != MC_OK)
+        return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 1.0));
+    return hip_status(mc::launch_distill_fwd(*d, logits, teacher_ids, teacher_logits, teacher_lse, mask, loss, stats,
+                                             static_cast<char*>(workspace), stream),
+                      "distillation_loss forward");
+}
+
+mc_status mc_distill_loss_bwd(const mc_distill_desc* d, const void* logits, const int32_t* teacher_ids,
+                              const float* teacher_logits, const float* teacher_lse, const uint8_t* mask,
+                              const float* stats, const float* dloss, void* dlogits, hipStream_t stream) {
+    mc_status s = check_distill(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && teacher_ids && teacher_logits && stats && dlogits, MC_ERR_NULL,
+             "distillation_loss backward: logits, teacher_ids, teacher_logits, stats and dlogits must not be NULL");
+    if ((s = check_logits("distillation_loss backward", d->dtype, logits, dlogits)) != MC_OK) return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 2.0));
+    return hip_status(mc::launch_distill_bwd(*d, logits, teacher_ids, teacher_logits, teacher_lse, mask, stats, dloss,
+                                             dlogits, stream),
+                      "distillation_loss backward");
+}
+
+mc_status mc_distill_loss_fwd_bwd(const mc_distill_desc* d, const void* logits, const int32_t* teacher_ids,
+                                  const float* teacher_logits, const float* teacher_lse, const uint8_t* mask,
+                                  const float* dloss, float* loss, void* dlogits, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream) {
+    mc_status s = check_distill(d);
+    if (s != MC_OK) return s;
+    MC_CHECK(logits && teacher_ids && teacher_logits && loss && dlogits, MC_ERR_NULL,
+             "distillation_loss: logits, teacher_ids, teacher_logits, loss and dlogits must not be NULL");
+    if ((s = check_logits("distillation_loss", d->dtype, logits, dlogits)) != MC_OK) return s;
+    if ((s = check_workspace("distillation_loss", workspace, workspace_bytes, mc::distill_fwd_bwd_ws(*d))) != MC_OK)
+        return s;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 2.0));
+    return hip_status(mc::launch_distill_fwd_bwd(*d, logits, teacher_ids, teacher_logits, teacher_lse, mask, dloss,
+                                                 loss, dlogits, static_cast<char*>(workspace), stream),
+                      "distillation_loss forward and backward");
+}
+
 // Philox4x32-10 (Salmon et al., SC'11), 10 rounds of the two 32x32->64
 // multiplies 0xD2511F53 / 0xCD9E8D57 with Weyl key steps 0x9E3779B9 /
 // 0xBB67AE85.

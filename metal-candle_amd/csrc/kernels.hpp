@@ -199,4 +199,64 @@ hipError_t launch_cross_entropy_fwd(const mc_xent_desc& d, const void* logits, c
 hipError_t launch_cross_entropy_bwd(const mc_xent_desc& d, const void* logits, const uint32_t* targets,
                                     const float* stats, const float* dloss, void* dlogits, hipStream_t stream);
 
+// ----------------------------------------------- losses over log-probabilities
+// log2(e) / T as c_hi + c_lo, and 1 / T.
+struct LpScale {
+    float c_hi, c_lo, inv_t;
+};
+// What the forward keeps of a row of logits: its maximum and its sum of
+// exponentials relative to it.
+struct RowStat {
+    float m, s;
+};
+constexpr int kDistillMaxTop = MC_DISTILL_MAX_TOP;  // a teacher's entries per row: one per thread
+// counter: cleared by the kernel if not null.
+hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
+                                     float* stats, uint32_t* counter, hipStream_t stream);
+// dl: dloss/dl per row, or per sequence of seq rows where seq > 0; times scale[0] and dloss[0] (each may be null).
+hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
+                                     const float* stats, const float* dl, int64_t seq, const float* scale,
+                                     const float* dloss, void* dlogits, hipStream_t stream);
+// Workspaces (byte offsets): a counter at 0, then
+struct PreferenceWs {
+    size_t logp;   // f32 [2 pairs seq]
+    size_t score;  // f64 [2 pairs]
+    size_t inv_n;  // f32 [2 pairs]
+    size_t total;
+};
+struct PolicyWs {
+    size_t part;    // f64 [256][4] sums
+    size_t counts;  // u32 [batch] counted tokens, where the mean runs over sequences
+    size_t total;
+};
+struct DistillWs {
+    size_t part;  // f64 [256][2] sums
+    size_t kl;    // f32 [rows]
+    size_t total;
+};
+PreferenceWs preference_ws(const mc_preference_desc& d);
+PolicyWs policy_ws(const mc_policy_desc& d);
+DistillWs distill_ws(const mc_distill_desc& d);
+hipError_t launch_preference_fwd(const mc_preference_desc& d, const void* logits, const uint32_t* targets,
+                                 const float* ref, float* loss, float* rewards, float* stats, char* ws,
+                                 hipStream_t stream);
+hipError_t launch_policy_fwd(const mc_policy_desc& d, const void* logits, const uint32_t* targets, const float* adv,
+                             const float* old, const float* ref, float* loss, float* logp, float* metrics,
+                             float* stats, char* ws, hipStream_t stream);
+// fwd_bwd: the forward's buffers, then its stats.
+size_t policy_fwd_bwd_ws(const mc_policy_desc& d);
+size_t distill_fwd_bwd_ws(const mc_distill_desc& d);
+hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, const uint32_t* targets,
+                                 const float* adv, const float* old, const float* ref, const float* dloss, float* loss,
+                                 float* logp, float* metrics, void* dlogits, char* ws, hipStream_t stream);
+hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, const int32_t* ids, const float* tl,
+                              const float* tlse, const uint8_t* mask, float* loss, float* stats, char* ws,
+                              hipStream_t stream);
+hipError_t launch_distill_bwd(const mc_distill_desc& d, const void* logits, const int32_t* ids, const float* tl,
+                              const float* tlse, const uint8_t* mask, const float* stats, const float* dloss,
+                              void* dlogits, hipStream_t stream);
+hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, const int32_t* ids, const float* tl,
+                                  const float* tlse, const uint8_t* mask, const float* dloss, float* loss,
+                                  void* dlogits, char* ws, hipStream_t stream);
+
 }  // namespace mc

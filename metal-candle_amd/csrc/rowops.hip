@@ -28,6 +28,7 @@
 #include "common.hpp"
 #include "kernels.hpp"
 #include "rules.hpp"
+#include "vocab_rows.hpp"
 
 namespace mc {
 namespace {
@@ -400,26 +401,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return t;
 }
 
-// A row as aligned 16-byte vectors between up to N - 1 elements on each side,
-// for rows of any length and start: vector c holds elements head + N c ..
-template <typename T> struct RowSpan {
-    int64_t head, nvec, tail;  // elements before the vectors, vectors, first element after them
-    __device__ RowSpan(const T* p, int64_t dim) {
-        constexpr int N = Vec16<T>::N;
-        const int64_t mis = (int64_t)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-        head = mis ? N - mis : 0;
-        if (head > dim) head = dim;
-        nvec = (dim - head) / N;
-        tail = head + nvec * N;
-    }
-    // The element of an edge that thread t (of at least 2 N) takes, or -1.
-    __device__ int64_t edge(int t, int64_t dim) const {
-        constexpr int N = Vec16<T>::N;
-        if (t < N) return t < head ? t : -1;
-        return t < 2 * N && tail + t - N < dim ? tail + t - N : -1;
-    }
-};
-
 // Per-thread online (max, sum of exp, sum) over the row, NT threads. Four
 // vectors are requested and reduced at a time: one rescale to their max, then
 // one exp per element into sums of their own. (One vector at a time left a
@@ -619,14 +600,6 @@ __global__ __launch_bounds__(1024) void xent_final_k(int64_t rows, int64_t vocab
         loss[0] = l;
         if (count_out) count_out[0] = tc;
     }
-}
-
-__device__ __forceinline__ void store_nt16(float* p, const float (&v)[4]) {
-    __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4*>(p));
-}
-__device__ __forceinline__ void store_nt16(uint16_t* p, const float (&v)[8]) {
-    const u32x4 q = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-    __builtin_nontemporal_store(q, reinterpret_cast<u32x4*>(p));
 }
 
 // dlogits = dloss ((1 - s) valid (p - onehot(t)) / count + s (p - 1/V) / rows), p = exp(x - lse)

@@ -12,7 +12,8 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import AdamWConfig, AdamWTensor, AttnDesc, LoraDesc, LoraProj, McError, XentDesc, check, lib
+from ._lib import (AdamWConfig, AdamWTensor, AttnDesc, DistillDesc, LogprobDesc, LoraDesc, LoraProj, McError, PolicyDesc,
+                   PreferenceDesc, XentDesc, check, lib)
 
 _DTYPES = {torch.float32: _lib.MC_F32, torch.bfloat16: _lib.MC_BF16}
 
@@ -475,6 +476,287 @@ def cross_entropy_backward(logits, targets, stats, dloss=None, ignore_index=None
     check(lib().mc_cross_entropy_bwd(ctypes.byref(d), _ptr(logits), _ptr(targets), _ptr(stats), _ptr(dloss),
                                      _ptr(dlogits), _stream(logits)))
     return dlogits
+
+
+# --------------------------------------------------- losses over log-probabilities
+def _optional(t, name, shape, dtype, device):
+    """A device address for an optional tensor of the given shape, or None."""
+    if t is None:
+        return None
+    _expect(t, name, shape, dtype, device)
+    return t.data_ptr()
+
+
+def _launch(t, fn, *args):
+    """fn(*args, stream) on the device of t and its current stream."""
+    if t.is_cuda and t.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(t.device):
+            check(fn(*args, _stream(t)))
+    else:
+        check(fn(*args, _stream(t)))
+
+
+def _loss_inputs(logits, targets, ignore_index, seqs):
+    """(targets as the kernels read them, ignore_index, dtype code) of logits [..., V] with targets over its leading
+    dims; seqs: the logits must be [sequences, tokens, V]."""
+    if not isinstance(logits, torch.Tensor):
+        raise McError(_lib.MC_ERR_NULL, "logits must be a tensor")
+    if seqs and logits.dim() != 3:
+        raise McError(_lib.MC_ERR_SHAPE, f"logits must be [sequences, tokens, vocab], got {tuple(logits.shape)}")
+    _rows_of(logits, "logits")
+    if logits.numel() == 0:
+        raise McError(_lib.MC_ERR_SHAPE, f"logits are empty: {tuple(logits.shape)}")
+    targets = _targets(targets, logits)
+    if seqs and tuple(targets.shape) != tuple(logits.shape[:-1]):
+        raise McError(_lib.MC_ERR_SHAPE, f"targets has shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
+    return targets, -1 if ignore_index is None else int(ignore_index), _DTYPES[logits.dtype]
+
+
+def _logprob_desc(logits, ignore, temperature, code):
+    V = logits.shape[-1]
+    return LogprobDesc(logits.numel() // V, V, ignore, float(temperature), code)
+
+
+def token_logprobs_forward(logits, targets, ignore_index=None, temperature=1.0, save_stats=True):
+    """Log-probabilities of the given tokens under logits [..., V]: (logps [...] fp32, stats).
+
+    logps = logits[target] / T - logsumexp(logits / T), 0 where the target is
+    ignore_index (such rows are not read); stats [rows, 2] fp32 is what
+    token_logprobs_backward needs, or None."""
+    targets, ignore, code = _loss_inputs(logits, targets, ignore_index, False)
+    d = _logprob_desc(logits, ignore, temperature, code)
+    logps = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    stats = torch.empty(d.rows, 2, dtype=torch.float32, device=logits.device) if save_stats else None
+    _launch(logits, lib().mc_token_logprobs_fwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(),
+            logps.data_ptr(), _ptr(stats))
+    return logps, stats
+
+
+def token_logprobs_backward(logits, targets, stats, dlogps, ignore_index=None, temperature=1.0):
+    """The logits' gradient from that of their tokens' log-probabilities, dlogps [...] fp32: with it, any loss over
+    log-probabilities has its gradient in one pass over the logits."""
+    targets, ignore, code = _loss_inputs(logits, targets, ignore_index, False)
+    d = _logprob_desc(logits, ignore, temperature, code)
+    dev = logits.device
+    if stats is None or dlogps is None:
+        raise McError(_lib.MC_ERR_NULL, "token_logprobs_backward: stats and dlogps are required")
+    _expect(stats, "stats", (d.rows, 2), torch.float32, dev)
+    _expect(dlogps, "dlogps", logits.shape[:-1], torch.float32, dev)
+    dlogits = torch.empty_like(logits)
+    _launch(logits, lib().mc_token_logprobs_bwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(),
+            stats.data_ptr(), dlogps.data_ptr(), dlogits.data_ptr())
+    return dlogits
+
+
+_PREF_KINDS = {"sigmoid": _lib.MC_PREF_SIGMOID, "hinge": _lib.MC_PREF_HINGE, "squared": _lib.MC_PREF_SQUARED}
+
+
+def _choice(table, key, name):
+    try:
+        return table[key]
+    except (KeyError, TypeError):
+        raise McError(_lib.MC_ERR_VALUE, f"{name} must be one of {', '.join(table)}, got {key!r}")
+
+
+def _pairs(logits):
+    if logits.shape[0] % 2:
+        raise McError(_lib.MC_ERR_SHAPE, f"logits hold pairs of sequences: {logits.shape[0]} is odd")
+    return logits.shape[0] // 2
+
+
+def preference_loss_forward(logits, targets, ref_logps=None, beta=0.1, kind="sigmoid", label_smoothing=0.0, margin=0.0,
+                            average=False, ignore_index=None):
+    """Preference loss over pairs of sequences: (loss [1], rewards [2P], stats).
+
+    logits [2P, S, V], the P preferred answers first, then the others in the
+    same order; targets [2P, S], padding and prompts as ignore_index; ref_logps
+    [2P, S] fp32, the reference policy's token_logprobs_forward (None: no
+    reference). A sequence's score is the sum (average: the mean) of logps -
+    ref_logps, d a pair's difference of scores, z = beta d - margin; the loss
+    is the pairs' mean of -(1 - e) log sigma(z) - e log sigma(-z) with
+    e = label_smoothing ("sigmoid"), max(0, 1 - z) ("hinge") or
+    (d - 1 / (2 beta))^2 ("squared"). rewards = beta times the scores."""
+    targets, ignore, code = _loss_inputs(logits, targets, ignore_index, True)
+    P, dev = _pairs(logits), logits.device
+    _, S, V = logits.shape
+    d = PreferenceDesc(P, S, V, ignore, _choice(_PREF_KINDS, kind, "kind"), int(bool(average)), float(beta),
+                       float(label_smoothing), float(margin), code)
+    ref = _optional(ref_logps, "ref_logps", (2 * P, S), torch.float32, dev)
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    rewards = torch.empty(2 * P, dtype=torch.float32, device=dev)
+    stats = torch.empty(4 * P * S + 2 * P, dtype=torch.float32, device=dev)
+    ws_n = lib().mc_preference_loss_workspace_size(ctypes.byref(d))
+    ws = _workspace(ws_n, dev)
+    _launch(logits, lib().mc_preference_loss_fwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(), ref,
+            loss.data_ptr(), rewards.data_ptr(), stats.data_ptr(), _ptr(ws), ws_n)
+    return loss, rewards, stats
+
+
+def preference_loss_backward(logits, targets, stats, dloss=None, ignore_index=None):
+    """d loss / d logits (times dloss, a fp32 [1] device tensor; default 1); stats from preference_loss_forward."""
+    targets, ignore, code = _loss_inputs(logits, targets, ignore_index, True)
+    P, dev = _pairs(logits), logits.device
+    _, S, V = logits.shape
+    if stats is None:
+        raise McError(_lib.MC_ERR_NULL, "stats from preference_loss_forward are required")
+    _expect(stats, "stats", (4 * P * S + 2 * P,), torch.float32, dev)
+    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    # what the loss was is in stats
+    d = PreferenceDesc(P, S, V, ignore, _lib.MC_PREF_SIGMOID, 0, 1.0, 0.0, 0.0, code)
+    dlogits = torch.empty_like(logits)
+    _launch(logits, lib().mc_preference_loss_bwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(),
+            stats.data_ptr(), g, dlogits.data_ptr())
+    return dlogits
+
+
+_REDUCTIONS = {"tokens": _lib.MC_MEAN_TOKENS, "sequences": _lib.MC_MEAN_SEQUENCES}
+
+
+def _policy_call(logits, targets, advantages, old_logps, ref_logps, clip_low, clip_high, kl_coef, temperature,
+                 reduction, ignore_index):
+    targets, ignore, code = _loss_inputs(logits, targets, ignore_index, True)
+    B, S, V = logits.shape
+    dev = logits.device
+    if not isinstance(advantages, torch.Tensor):
+        raise McError(_lib.MC_ERR_NULL, "advantages must be a tensor")
+    per_token = advantages.dim() == 2
+    _expect(advantages, "advantages", (B, S) if per_token else (B,), torch.float32, dev)
+    old = _optional(old_logps, "old_logps", (B, S), torch.float32, dev)
+    ref = _optional(ref_logps, "ref_logps", (B, S), torch.float32, dev)
+    d = PolicyDesc(B, S, V, ignore, int(per_token), _choice(_REDUCTIONS, reduction, "reduction"), float(clip_low),
+                   float(clip_high), float(kl_coef), float(temperature), code)
+    out = torch.empty(3, dtype=torch.float32, device=dev)
+    logps = torch.empty(B, S, dtype=torch.float32, device=dev)
+    return d, targets, old, ref, out[:1], logps, out[1:]
+
+
+def policy_loss_forward(logits, targets, advantages, old_logps=None, ref_logps=None, clip_low=0.2, clip_high=0.2,
+                        kl_coef=0.0, temperature=1.0, reduction="tokens", ignore_index=None):
+    """Clipped policy loss over sampled tokens: (loss [1], logps [B, S], metrics [2], stats).
+
+    logits [B, S, V], targets [B, S] (padding and prompts as ignore_index),
+    advantages [B] or [B, S] fp32; old_logps and ref_logps [B, S] fp32, the
+    sampling and the reference policy's token_logprobs_forward at the same
+    temperature. With r = exp(logps - old_logps) (1 without old_logps) a token's
+    loss is -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef kl,
+    kl = exp(ref - logps) - (ref - logps) - 1; the loss is their mean over the
+    counted tokens, or with reduction="sequences" the batch's mean of the
+    sequences' means. metrics: kl and the share of clipped tokens, averaged
+    alike."""
+    d, targets, old, ref, loss, logps, metrics = _policy_call(
+        logits, targets, advantages, old_logps, ref_logps, clip_low, clip_high, kl_coef, temperature, reduction,
+        ignore_index)
+    stats = torch.empty(3 * logps.numel() + 1, dtype=torch.float32, device=logits.device)
+    ws_n = lib().mc_policy_loss_workspace_size(ctypes.byref(d))
+    ws = _workspace(ws_n, logits.device)
+    _launch(logits, lib().mc_policy_loss_fwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(),
+            advantages.data_ptr(), old, ref, loss.data_ptr(), logps.data_ptr(), metrics.data_ptr(), stats.data_ptr(),
+            _ptr(ws), ws_n)
+    return loss, logps, metrics, stats
+
+
+def policy_loss_backward(logits, targets, stats, dloss=None, temperature=1.0, ignore_index=None):
+    """d loss / d logits (times dloss, a fp32 [1] device tensor; default 1); stats from policy_loss_forward."""
+    targets, ignore, code = _loss_inputs(logits, targets, ignore_index, True)
+    B, S, V = logits.shape
+    dev = logits.device
+    if stats is None:
+        raise McError(_lib.MC_ERR_NULL, "stats from policy_loss_forward are required")
+    _expect(stats, "stats", (3 * B * S + 1,), torch.float32, dev)
+    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    d = PolicyDesc(B, S, V, ignore, 0, _lib.MC_MEAN_TOKENS, 0.0, 0.0, 0.0, float(temperature), code)
+    dlogits = torch.empty_like(logits)
+    _launch(logits, lib().mc_policy_loss_bwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(), stats.data_ptr(),
+            g, dlogits.data_ptr())
+    return dlogits
+
+
+def policy_loss_forward_backward(logits, targets, advantages, old_logps=None, ref_logps=None, clip_low=0.2,
+                                 clip_high=0.2, kl_coef=0.0, temperature=1.0, reduction="tokens", ignore_index=None,
+                                 dloss=None):
+    """policy_loss_forward and _backward in one call, for a training step: (loss, logps, metrics, dlogits). The
+    logits need not be read twice."""
+    d, targets, old, ref, loss, logps, metrics = _policy_call(
+        logits, targets, advantages, old_logps, ref_logps, clip_low, clip_high, kl_coef, temperature, reduction,
+        ignore_index)
+    g = _optional(dloss, "dloss", (1,), torch.float32, logits.device)
+    dlogits = torch.empty_like(logits)
+    ws_n = lib().mc_policy_loss_fwd_bwd_workspace_size(ctypes.byref(d))
+    ws = _workspace(ws_n, logits.device)
+    _launch(logits, lib().mc_policy_loss_fwd_bwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(),
+            advantages.data_ptr(), old, ref, g, loss.data_ptr(), logps.data_ptr(), metrics.data_ptr(),
+            dlogits.data_ptr(), _ptr(ws), ws_n)
+    return loss, logps, metrics, dlogits
+
+
+def _distill_call(logits, teacher_ids, teacher_logits, temperature, teacher_lse, mask):
+    rows, V = _rows_of(logits, "logits")
+    lead, dev = tuple(logits.shape[:-1]), logits.device
+    if not isinstance(teacher_ids, torch.Tensor) or not isinstance(teacher_logits, torch.Tensor):
+        raise McError(_lib.MC_ERR_NULL, "teacher_ids and teacher_logits must be tensors")
+    if teacher_ids.dim() != logits.dim() or tuple(teacher_ids.shape[:-1]) != lead:
+        raise McError(_lib.MC_ERR_SHAPE,
+                      f"teacher_ids has shape {tuple(teacher_ids.shape)}, expected {lead} and the number of entries")
+    K = teacher_ids.shape[-1]
+    if teacher_ids.dtype == torch.int64:
+        # ids that do not fit 32 bits stay out of every vocabulary
+        teacher_ids = teacher_ids.clamp(-1, 2**31 - 1).to(torch.int32)
+    _expect(teacher_ids, "teacher_ids", lead + (K,), torch.int32, dev)
+    _expect(teacher_logits, "teacher_logits", lead + (K,), torch.float32, dev)
+    lse = _optional(teacher_lse, "teacher_lse", lead, torch.float32, dev)
+    m = _optional(mask, "mask", lead, torch.uint8, dev)
+    return DistillDesc(rows, V, K, float(temperature), _DTYPES[logits.dtype]), teacher_ids, lse, m
+
+
+def distillation_loss_forward(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None, mask=None):
+    """Distillation from a teacher's top logits: (loss [1], stats).
+
+    logits [..., V]; teacher_ids int32 and teacher_logits fp32 [..., K], K up to
+    256, in any order (an entry of -inf is left out, whatever its id); mask
+    uint8 [...], rows of 0 are not counted. p = softmax(teacher_logits / T), or
+    exp(teacher_logits / T - teacher_lse) where teacher_lse [...] holds the
+    log-sum-exp of all the teacher's logits / T; the loss is T^2 times the
+    counted rows' mean of sum_k p_k (log p_k - log softmax(logits / T)[id_k])."""
+    d, ids, lse, m = _distill_call(logits, teacher_ids, teacher_logits, temperature, teacher_lse, mask)
+    dev = logits.device
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    stats = torch.empty(2 * d.rows + 1, dtype=torch.float32, device=dev)
+    ws_n = lib().mc_distill_loss_workspace_size(ctypes.byref(d))
+    ws = _workspace(ws_n, dev)
+    _launch(logits, lib().mc_distill_loss_fwd, ctypes.byref(d), logits.data_ptr(), ids.data_ptr(),
+            teacher_logits.data_ptr(), lse, m, loss.data_ptr(), stats.data_ptr(), _ptr(ws), ws_n)
+    return loss, stats
+
+
+def distillation_loss_backward(logits, teacher_ids, teacher_logits, stats, dloss=None, temperature=1.0,
+                               teacher_lse=None, mask=None):
+    """d loss / d logits (times dloss, a fp32 [1] device tensor; default 1); stats from distillation_loss_forward."""
+    d, ids, lse, m = _distill_call(logits, teacher_ids, teacher_logits, temperature, teacher_lse, mask)
+    dev = logits.device
+    if stats is None:
+        raise McError(_lib.MC_ERR_NULL, "stats from distillation_loss_forward are required")
+    _expect(stats, "stats", (2 * d.rows + 1,), torch.float32, dev)
+    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    dlogits = torch.empty_like(logits)
+    _launch(logits, lib().mc_distill_loss_bwd, ctypes.byref(d), logits.data_ptr(), ids.data_ptr(),
+            teacher_logits.data_ptr(), lse, m, stats.data_ptr(), g, dlogits.data_ptr())
+    return dlogits
+
+
+def distillation_loss_forward_backward(logits, teacher_ids, teacher_logits, temperature=1.0, teacher_lse=None,
+                                       mask=None, dloss=None):
+    """distillation_loss_forward and _backward in one call, for a training step: (loss, dlogits). The logits need not
+    be read twice."""
+    d, ids, lse, m = _distill_call(logits, teacher_ids, teacher_logits, temperature, teacher_lse, mask)
+    dev = logits.device
+    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    dlogits = torch.empty_like(logits)
+    ws_n = lib().mc_distill_loss_fwd_bwd_workspace_size(ctypes.byref(d))
+    ws = _workspace(ws_n, dev)
+    _launch(logits, lib().mc_distill_loss_fwd_bwd, ctypes.byref(d), logits.data_ptr(), ids.data_ptr(),
+            teacher_logits.data_ptr(), lse, m, g, loss.data_ptr(), dlogits.data_ptr(), _ptr(ws), ws_n)
+    return loss, dlogits
 
 
 def adamw_step(params, grads, ms, vs, steps, lr=1e-4, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,

@@ -774,7 +774,7 @@ mc_status mc_token_logprobs_fwd(const mc_logprob_desc* d, const void* logits, co
     MC_CHECK(logits && targets && logps, MC_ERR_NULL, "token_logprobs: logits, targets and logps must not be NULL");
     if ((s = check_logits("token_logprobs", d->dtype, logits, nullptr)) != MC_OK) return s;
     mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 1.0));
-    return hip_status(mc::launch_token_logprobs_fwd(*d, logits, targets, logps, stats, nullptr, stream),
+    return hip_status(mc::launch_token_logprobs_fwd(*d, logits, targets, logps, stats, stream),
                       "token_logprobs forward");
 }
 

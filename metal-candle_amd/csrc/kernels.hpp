@@ -203,6 +203,7 @@ hipError_t launch_cross_entropy_bwd(const mc_xent_desc& d, const void* logits, c
 // log2(e) / T as c_hi + c_lo, and 1 / T.
 struct LpScale {
     float c_hi, c_lo, inv_t;
+    double inv_t64;
 };
 // What the forward keeps of a row of logits: its maximum and its sum of
 // exponentials relative to it.
@@ -210,16 +211,15 @@ struct RowStat {
     float m, s;
 };
 constexpr int kDistillMaxTop = MC_DISTILL_MAX_TOP;  // a teacher's entries per row: one per thread
-// counter: cleared by the kernel if not null.
 hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
-                                     float* stats, uint32_t* counter, hipStream_t stream);
+                                     float* stats, hipStream_t stream);
 // dl: dloss/dl per row, or per sequence of seq rows where seq > 0; times scale[0] and dloss[0] (each may be null).
 hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
                                      const float* stats, const float* dl, int64_t seq, const float* scale,
                                      const float* dloss, void* dlogits, hipStream_t stream);
 // Workspaces (byte offsets): a counter at 0, then
 struct PreferenceWs {
-    size_t logp;   // f32 [2 pairs seq]
+    size_t logp;   // f64 [2 pairs seq]
     size_t score;  // f64 [2 pairs]
     size_t inv_n;  // f32 [2 pairs]
     size_t total;

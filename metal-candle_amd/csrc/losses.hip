@@ -28,6 +28,15 @@ namespace {
 
 constexpr float kNegInf = -__builtin_inff();
 
+// An element as its bits, to convert where it is used: a conversion waits for the load.
+template <typename T> __device__ __forceinline__ uint32_t raw_load(const T* p, int64_t i) {
+    if constexpr (std::is_same<T, float>::value) return __float_as_uint(p[i]);
+    else return p[i];
+}
+template <typename T> __device__ __forceinline__ float from_raw(uint32_t w) {
+    return std::is_same<T, float>::value ? __uint_as_float(w) : __uint_as_float(w << 16);
+}
+
 // ------------------------------------------------------------ row statistics
 // m = max x and s = sum 2^((x - m) c), c = log2(e) / T as c_hi + c_lo
 // (row_scale): with one float for c every exponent is off by up to 6e-8 of
@@ -37,21 +46,27 @@ constexpr float kNegInf = -__builtin_inff();
 // m = -inf and s = 0, a NaN in the row makes s NaN: l and the gradient are NaN in
 // both. The backward takes m and s as they are: lse as one float would cost each
 // q 2^-24 |lse| of itself.
-__device__ __forceinline__ RowStat stat_join(RowStat a, RowStat b, float c) {
+// S, the sum's type: in float one part in 2^24 of the sum is lost at every
+// addition to it, which shows in an l whose token holds nearly all of the row.
+template <typename S> struct Stat {
+    float m;
+    S s;
+};
+template <typename S> __device__ __forceinline__ Stat<S> stat_join(Stat<S> a, Stat<S> b, float c) {
     const float m = fmaxf(a.m, b.m);
     // equal maxima, -inf among them, need no factor
-    const float sa = a.m == m ? a.s : a.s * exp2_hw((a.m - m) * c);
-    const float sb = b.m == m ? b.s : b.s * exp2_hw((b.m - m) * c);
-    return RowStat{m, sa + sb};
+    const S sa = a.m == m ? a.s : a.s * (S)exp2_hw((a.m - m) * c);
+    const S sb = b.m == m ? b.s : b.s * (S)exp2_hw((b.m - m) * c);
+    return Stat<S>{m, sa + sb};
 }
 
 // Over the workgroup's NT threads in a fixed order: a butterfly over each wave,
 // then the waves in order. red: one slot per wave.
-template <int NT>
-__device__ __forceinline__ RowStat wg_stat(RowStat v, float c, RowStat* red) {
+template <int NT, typename S>
+__device__ __forceinline__ Stat<S> wg_stat(Stat<S> v, float c, Stat<S>* red) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1)
-        v = stat_join(v, RowStat{__shfl_xor(v.m, o, kWave), __shfl_xor(v.s, o, kWave)}, c);
+        v = stat_join(v, Stat<S>{__shfl_xor(v.m, o, kWave), __shfl_xor(v.s, o, kWave)}, c);
     if (lane_id() == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
@@ -67,12 +82,13 @@ __device__ __forceinline__ float term_of(float x, float base, LpScale k) {
     return exp2_hw(fmaf(d, k.c_lo, d * k.c_hi));
 }
 
-// One thread's share of a row: four vectors requested and reduced at a time,
-// one rescale to their maximum, then one exp2 per element.
-template <typename T, int NT>
-__device__ __forceinline__ RowStat row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
-    constexpr int N = Vec16<T>::N, U = 4;
-    float m = kNegInf, s = 0.f;
+// One thread's share of a row: U vectors requested and reduced at a time, one
+// rescale to their maximum, then one exp2 per element.
+template <typename T, int NT, typename S, int U = 4>
+__device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
+    constexpr int N = Vec16<T>::N;
+    float m = kNegInf;
+    S s = 0;
     const RowSpan<T> span(xr, vocab);
     const T* xv = xr + span.head;
     const int nvec = (int)span.nvec;
@@ -87,7 +103,7 @@ __device__ __forceinline__ RowStat row_stat(const T* __restrict__ xr, int vocab,
 #pragma unroll
             for (int e = 0; e < N; ++e) vm = fmaxf(vm, v[u][e]);
         if (vm > m) {
-            s *= exp2_hw((m - vm) * k.c_hi);  // 0 for the first
+            s *= (S)exp2_hw((m - vm) * k.c_hi);  // 0 for the first
             m = vm;
         }
         const float base = base_of(m);
@@ -98,8 +114,11 @@ __device__ __forceinline__ RowStat row_stat(const T* __restrict__ xr, int vocab,
 #pragma unroll
             for (int e = 0; e < N; ++e) ps[u] += term_of(v[u][e], base, k);
         }
-        if constexpr (K == 4) s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-        else s += ps[0];
+#pragma unroll
+        for (int u = K; u > 1; u /= 2)
+#pragma unroll
+            for (int i = 0; i < u / 2; ++i) ps[i] = ps[i] + ps[i + u / 2];
+        s += ps[0];
     };
     int c = threadIdx.x;
     for (; c < nvec - (U - 1) * NT; c += U * NT) group(c, std::integral_constant<int, U>{});
@@ -107,9 +126,9 @@ __device__ __forceinline__ RowStat row_stat(const T* __restrict__ xr, int vocab,
     const int64_t j = span.edge((int)threadIdx.x, vocab);
     if (j >= 0) {
         const float v = Elem<T>::load(xr, j);
-        return stat_join(RowStat{m, s}, RowStat{v, term_of(v, base_of(v), k)}, k.c_hi);
+        return stat_join(Stat<S>{m, s}, Stat<S>{v, (S)term_of(v, base_of(v), k)}, k.c_hi);
     }
-    return RowStat{m, s};
+    return Stat<S>{m, s};
 }
 
 // -------------------------------------------------- sums over many workgroups
@@ -154,60 +173,75 @@ __device__ __forceinline__ bool counted(uint32_t t, int64_t ignore_index) {
 // l (0 where the row is not counted) and the row's statistics; a counted target
 // past the vocabulary makes its l NaN. counter: cleared for the kernel that
 // follows.
-template <typename T, int NT>
+// L: float, or double for sums over answers.
+template <typename T, int NT, typename L>
 __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__ logits,
                                                 const uint32_t* __restrict__ targets, int64_t ignore_index, LpScale k,
-                                                float* __restrict__ logp, RowStat* __restrict__ stats,
+                                                L* __restrict__ logp, RowStat* __restrict__ stats,
                                                 uint32_t* __restrict__ counter) {
-    __shared__ RowStat red[NT / 64];
+    __shared__ Stat<double> red[NT / 64];
     const int64_t row = blockIdx.x;
     if (counter && row == 0 && threadIdx.x == 0) *counter = 0;
     const uint32_t t = targets[row];
     if (!counted(t, ignore_index)) {
         if (threadIdx.x == 0) {
-            logp[row] = 0.f;
+            logp[row] = 0;
             if (stats) stats[row] = RowStat{0.f, 1.f};
         }
         return;
     }
     const T* xr = logits + row * vocab;
-    const RowStat v = wg_stat<NT>(row_stat<T, NT>(xr, vocab, k), k.c_hi, red);
+    const Stat<double> v = wg_stat<NT>(row_stat<T, NT, double>(xr, vocab, k), k.c_hi, red);
     if (threadIdx.x == 0) {
-        logp[row] = t < (uint32_t)vocab ? (Elem<T>::load(xr, t) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
-        if (stats) stats[row] = v;
+        const double d = (double)(t < (uint32_t)vocab ? Elem<T>::load(xr, t) : __builtin_nanf("")) - (double)v.m;
+        logp[row] = (L)(d * k.inv_t64 - log(v.s));
+        if (stats) stats[row] = RowStat{v.m, (float)v.s};
     }
 }
 
 // ------------------------------------------------------------- preference
-// A workgroup per sequence; the last one turns the pairs' scores into the loss
-// and each sequence's dloss/dl. Scores in 64 bits: they are differences of sums
-// over whole answers.
-__global__ __launch_bounds__(256) void preference_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
-                                                    const float* __restrict__ logp, const float* __restrict__ ref,
-                                                    double* __restrict__ score, float* __restrict__ inv_n,
-                                                    uint32_t* __restrict__ counter, float* __restrict__ loss,
-                                                    float* __restrict__ rewards, float* __restrict__ dseq) {
-    __shared__ double red[4][2];
-    __shared__ uint32_t slot;
-    const int64_t q = blockIdx.x;
-    double v[2] = {0.0, 0.0};
-    for (int64_t i = threadIdx.x; i < d.seq; i += 256) {
-        const int64_t row = q * d.seq + i;
-        if (!counted(targets[row], d.ignore_index)) continue;
-        v[0] += (double)logp[row] - (ref ? (double)ref[row] : 0.0);
-        v[1] += 1.0;
+// A sequence's score and the factor of its tokens, from the sums over its
+// counted tokens.
+__device__ __forceinline__ void preference_score(const mc_preference_desc& d, int64_t q, double sum, double n,
+                                                 double* score, float* inv_n, float* rewards) {
+    const double inv = d.average && n > 0.0 ? 1.0 / n : 1.0;
+    score[q] = sum * inv;
+    inv_n[q] = (float)inv;
+    if (rewards) rewards[q] = (float)(d.beta * score[q]);
+}
+// The thread's tokens at, at + step, .. of sequence q, eight loaded together.
+__device__ __forceinline__ void preference_sum(const mc_preference_desc& d, int64_t q, int at, int step,
+                                               const uint32_t* targets, const double* logp, const float* ref,
+                                               double (&v)[2]) {
+    constexpr int U = 8;
+    const int64_t first = q * d.seq;
+    for (int64_t i0 = at; i0 < d.seq; i0 += U * step) {
+        uint32_t t[U];
+        double l[U];
+        float r[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = first + (i0 + u * step < d.seq ? i0 + u * step : i0);
+            t[u] = targets[row];
+            l[u] = logp[row];
+            r[u] = ref ? ref[row] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool on = i0 + u * step < d.seq && counted(t[u], d.ignore_index);
+            v[0] += on ? l[u] - (double)r[u] : 0.0;
+            v[1] += on ? 1.0 : 0.0;
+        }
     }
-    wg_sum_f64<2>(v, red);
-    if (threadIdx.x == 0) {
-        const double inv = d.average && v[1] > 0.0 ? 1.0 / v[1] : 1.0;
-        score[q] = v[0] * inv;
-        inv_n[q] = (float)inv;
-        if (rewards) rewards[q] = (float)(d.beta * score[q]);
-    }
-    if (!last_to_arrive(counter, &slot)) return;
+}
+
+// The pairs' losses and each sequence's dloss/dl, by the workgroup's NT threads.
+template <int NT>
+__device__ __forceinline__ void preference_pairs(const mc_preference_desc& d, const double* score, const float* inv_n,
+                                                 double (*red)[2], float* loss, float* dseq) {
     double sum[2] = {0.0, 0.0};
     const double beta = d.beta, eps = d.label_smoothing, pairs = (double)d.pairs;
-    for (int64_t i = threadIdx.x; i < d.pairs; i += 256) {
+    for (int64_t i = threadIdx.x; i < d.pairs; i += NT) {
         const double diff = score[i] - score[d.pairs + i];
         double l, dd;
         if (d.kind == MC_PREF_SQUARED) {
@@ -238,6 +272,44 @@ __global__ __launch_bounds__(256) void preference_k(mc_preference_desc d, const 
     if (threadIdx.x == 0) loss[0] = (float)(sum[0] / pairs);
 }
 
+// All in one workgroup, a wave per sequence (kOneGroupRows).
+__global__ __launch_bounds__(1024) void preference_one_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
+                                                         const double* __restrict__ logp,
+                                                         const float* __restrict__ ref, double* __restrict__ score,
+                                                         float* __restrict__ inv_n, float* __restrict__ loss,
+                                                         float* __restrict__ rewards, float* __restrict__ dseq) {
+    __shared__ double red[16][2];
+    for (int64_t q = wave_id(); q < 2 * d.pairs; q += 16) {
+        double v[2] = {0.0, 0.0};
+        preference_sum(d, q, lane_id(), kWave, targets, logp, ref, v);
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            v[0] += __shfl_xor(v[0], o, kWave);
+            v[1] += __shfl_xor(v[1], o, kWave);
+        }
+        if (lane_id() == 0) preference_score(d, q, v[0], v[1], score, inv_n, rewards);
+    }
+    __syncthreads();
+    preference_pairs<1024>(d, score, inv_n, red, loss, dseq);
+}
+
+// A workgroup per sequence; the last to arrive goes on to the pairs.
+__global__ __launch_bounds__(256) void preference_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
+                                                    const double* __restrict__ logp, const float* __restrict__ ref,
+                                                    double* score, float* inv_n, uint32_t* counter,
+                                                    float* __restrict__ loss, float* __restrict__ rewards,
+                                                    float* __restrict__ dseq) {
+    __shared__ double red[4][2];
+    __shared__ uint32_t slot;
+    const int64_t q = blockIdx.x;
+    double v[2] = {0.0, 0.0};
+    preference_sum(d, q, (int)threadIdx.x, 256, targets, logp, ref, v);
+    wg_sum_f64<2>(v, red);
+    if (threadIdx.x == 0) preference_score(d, q, v[0], v[1], score, inv_n, rewards);
+    if (!last_to_arrive(counter, &slot)) return;
+    preference_pairs<256>(d, score, inv_n, red, loss, dseq);
+}
+
 // ------------------------------------------------------------------ policy
 // Counted tokens of each sequence, a wave for each.
 __global__ __launch_bounds__(256) void seq_counts_k(int64_t batch, int64_t seq, const uint32_t* __restrict__ targets,
@@ -256,18 +328,27 @@ __global__ __launch_bounds__(256) void seq_counts_k(int64_t batch, int64_t seq, 
 struct PolicyTerm {
     float term, dl, kl, clipped;
 };
-__device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, float l, float A, const float* old,
-                                                  const float* ref, int64_t row) {
+struct PolicyInputs {
+    float A, old, ref;
+    bool has_old, has_ref;
+};
+__device__ __forceinline__ PolicyInputs policy_inputs(const mc_policy_desc& d, const float* adv, const float* old,
+                                                      const float* ref, int64_t row, uint32_t seq) {
+    return PolicyInputs{adv[d.per_token_advantages ? row : seq], old ? old[row] : 0.f, ref ? ref[row] : 0.f,
+                        old != nullptr, ref != nullptr};
+}
+__device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, float l, const PolicyInputs& in) {
     PolicyTerm p;
-    const float r = old ? expf(l - old[row]) : (l == l ? 1.f : l);
+    const float A = in.A;
+    const float r = in.has_old ? expf(l - in.old) : (l == l ? 1.f : l);
     const float held = fminf(fmaxf(r, 1.f - d.clip_low), 1.f + d.clip_high);
     const bool clipped = held * A < r * A;
     p.clipped = clipped ? 1.f : 0.f;
     p.term = -(clipped ? held * A : r * A);
     p.dl = clipped ? 0.f : -r * A;
     p.kl = 0.f;
-    if (ref) {
-        const float u = ref[row] - l, g = expm1f(u);
+    if (in.has_ref) {
+        const float u = in.ref - l, g = expm1f(u);
         p.kl = g - u;
         if (d.kl_coef != 0.f) {
             p.term = fmaf(d.kl_coef, p.kl, p.term);
@@ -281,39 +362,59 @@ __device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, float
 // and the counted ones. n: counted tokens of each sequence where the mean runs
 // over sequences. dlp: dloss/dl but for the factor at dlp[rows], which is known
 // only at the end.
-__global__ __launch_bounds__(256) void policy_k(mc_policy_desc d, int64_t chunk, const uint32_t* __restrict__ targets,
-                                                const float* __restrict__ logp, const float* __restrict__ adv,
-                                                const float* __restrict__ old, const float* __restrict__ ref,
-                                                const uint32_t* __restrict__ n, double (*part)[4],
-                                                uint32_t* __restrict__ counter, float* __restrict__ loss,
-                                                float* __restrict__ metrics, float* __restrict__ dlp) {
-    __shared__ double red[4][4];
+template <int NT>
+__global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, const uint32_t* __restrict__ targets,
+                                               const float* __restrict__ logp, const float* __restrict__ adv,
+                                               const float* __restrict__ old, const float* __restrict__ ref,
+                                               const uint32_t* __restrict__ n, double (*part)[4], uint32_t* counter,
+                                               float* __restrict__ loss, float* __restrict__ metrics,
+                                               float* __restrict__ dlp) {
+    __shared__ double red[NT / 64][4];
     __shared__ uint32_t slot;
     const int64_t rows = d.batch * d.seq, r0 = (int64_t)blockIdx.x * chunk;
     const int64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
     double v[4] = {0.0, 0.0, 0.0, 0.0};
-    for (int64_t row = r0 + threadIdx.x; row < r1; row += 256) {
-        float dl = 0.f;
-        if (counted(targets[row], d.ignore_index)) {
+    constexpr int U = 4;  // rows whose loads are in flight together
+    for (int64_t row0 = r0 + threadIdx.x; row0 < r1; row0 += U * NT) {
+        uint32_t t[U], nq[U];
+        float l[U];
+        PolicyInputs in[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = row0 + u * NT < r1 ? row0 + u * NT : row0;
             const uint32_t q = (uint32_t)row / (uint32_t)d.seq;
-            const PolicyTerm p = policy_term(d, logp[row], adv[d.per_token_advantages ? row : q], old, ref, row);
-            const double w = n ? 1.0 / (double)n[q] : 1.0;
-            v[0] += w * (double)p.term;
-            v[1] += w * (double)p.kl;
-            v[2] += w * (double)p.clipped;
-            v[3] += 1.0;
-            dl = (float)(w * (double)p.dl);
+            t[u] = targets[row];
+            l[u] = logp[row];
+            in[u] = policy_inputs(d, adv, old, ref, row, q);
+            nq[u] = n ? n[q] : 1u;
         }
-        if (dlp) dlp[row] = dl;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = row0 + u * NT;
+            if (row >= r1) break;
+            float dl = 0.f;
+            if (counted(t[u], d.ignore_index)) {
+                const PolicyTerm p = policy_term(d, l[u], in[u]);
+                const double w = n ? 1.0 / (double)nq[u] : 1.0;
+                v[0] += w * (double)p.term;
+                v[1] += w * (double)p.kl;
+                v[2] += w * (double)p.clipped;
+                v[3] += 1.0;
+                dl = (float)(w * (double)p.dl);
+            }
+            if (dlp) dlp[row] = dl;
+        }
     }
     wg_sum_f64<4>(v, red);
-    if (threadIdx.x == 0)
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) part[blockIdx.x][c] = v[c];
-    if (!last_to_arrive(counter, &slot)) return;
+            for (int c = 0; c < 4; ++c) part[blockIdx.x][c] = v[c];
+        if (!last_to_arrive(counter, &slot)) return;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
-    wg_sum_f64<4>(v, red);
+        for (int c = 0; c < 4; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
+        wg_sum_f64<4>(v, red);
+    }
     if (threadIdx.x == 0) {
         const double N = n ? (double)d.batch : v[3];  // no token at all: 0 / 0, a NaN loss
         loss[0] = (float)(v[0] / N);
@@ -326,63 +427,83 @@ __global__ __launch_bounds__(256) void policy_k(mc_policy_desc d, int64_t chunk,
 }
 
 // ------------------------------------------------------------ distillation
-// The teacher's entries of one row in LDS: ids, probabilities (0 where the entry
-// is left out: a logit of -inf), their sum P and sum p log p. bad: an entry
-// whose id is past the vocabulary.
-struct Teacher {
-    int id[kDistillMaxTop];
-    float p[kDistillMaxTop];
-};
+// A row's teacher, an entry per thread. Its softmax takes two steps with a
+// barrier of the kernel behind each: open leaves the waves' maxima and sums,
+// close forms p_k and the terms p_k (log p_k - log q_k), and sums gives their
+// totals to every thread. An entry is left out where its logit is -inf.
 struct TeacherSums {
-    float P, plogp;
-    bool bad;
+    float P, kl;
+    bool bad;  // an id past the vocabulary: the row is NaN
 };
-// All threads of the workgroup; NT >= kDistillMaxTop. red: 4 floats per wave.
-template <int NT>
-__device__ __forceinline__ TeacherSums load_teacher(Teacher& te, const mc_distill_desc& d, int64_t row,
-                                                    const int32_t* __restrict__ ids, const float* __restrict__ tl,
-                                                    const float* __restrict__ tlse, float* red) {
-    static_assert(NT >= kDistillMaxTop, "an entry per thread");
-    const int t = threadIdx.x;
-    const bool on = t < d.top;
-    const float inv_t = 1.0f / d.temperature;
-    const float z = on ? tl[row * d.top + t] * inv_t : kNegInf;
-    const int id = on ? ids[row * d.top + t] : 0;
-    float logp;
-    if (tlse) {
-        logp = z - tlse[row];
-    } else {
-        const float zm = wg_max(z, red);
-        // z != z: a NaN, which the maximum passes over, stays in the sum
-        const float e = z == kNegInf ? 0.f : expf(z - zm);
-        const float sum = wg_sum(e, red + NT / 64);
-        logp = (z - zm) - logf(sum);
+struct Teacher {
+    int id[kDistillMaxTop];                           // -1: left out
+    float p[kDistillMaxTop], x[kDistillMaxTop];       // and the student's logit
+    Stat<float> part[kDistillMaxTop / kWave];
+    float sum[kDistillMaxTop / kWave][2];
+    int bad[kDistillMaxTop / kWave];
+};
+struct TopEntry {
+    float z;
+    int id;
+    // Unconditional: see HeldRow.
+    __device__ __forceinline__ void load(const mc_distill_desc& d, int64_t row, const int32_t* __restrict__ ids,
+                                         const float* __restrict__ tl) {
+        const int64_t at = row * d.top + ((int)threadIdx.x < d.top ? (int)threadIdx.x : 0);
+        z = tl[at];
+        id = ids[at];
     }
-    const float p = z == kNegInf ? 0.f : expf(logp);
-    const float term = p == 0.f ? 0.f : p * logp;
-    const bool bad = p != 0.f && (id < 0 || id >= (int)d.vocab);
-    if (on) {
-        te.id[t] = p != 0.f ? id : -1;
-        te.p[t] = p;
+    __device__ __forceinline__ void open(const mc_distill_desc& d, float inv_t, Teacher& te) {
+        if (wave_id() * kWave >= d.top) return;
+        z = (int)threadIdx.x < d.top ? z * inv_t : kNegInf;
+        const float m = wave_max(z);  // passes over a NaN, which then stays in the sum
+        const float s = wave_sum(z == kNegInf ? 0.f : expf(z - m));
+        if (lane_id() == 0) te.part[wave_id()] = Stat<float>{m, s};
+        if (z == kNegInf) id = -1;
     }
-    TeacherSums s;
-    s.P = wg_sum(p, red + 2 * (NT / 64));
-    s.plogp = wg_sum(term, red + 3 * (NT / 64));
-    s.bad = __syncthreads_or(bad);
-    return s;
-}
-
-// sum_k p_k (log p_k - log q_k) of a row with statistics v. red: a float per wave.
-template <typename T>
-__device__ __forceinline__ float distill_row(const Teacher& te, TeacherSums s, int top, const T* __restrict__ xr,
-                                             RowStat v, LpScale k, float* red) {
-    float cross = 0.f;  // sum p log q
-    const int t = threadIdx.x;
-    const float ls = logf(v.s);
-    if (t < top && te.p[t] != 0.f && !s.bad) cross = te.p[t] * ((Elem<T>::load(xr, te.id[t]) - v.m) * k.inv_t - ls);
-    cross = wg_sum(cross, red);
-    return s.bad ? __builtin_nanf("") : s.plogp - cross;
-}
+    // x: the bits of the student's logit at id, v the row's statistics.
+    __device__ __forceinline__ void close(const mc_distill_desc& d, bool has_lse, float lse, float x, RowStat v,
+                                          LpScale k, Teacher& te) {
+        if (wave_id() * kWave >= d.top) return;
+        float m = lse, ls = 0.f;
+        if (!has_lse) {
+            m = kNegInf;
+            for (int w = 0; w * kWave < d.top; ++w) m = fmaxf(m, te.part[w].m);
+            float s = 0.f;
+            for (int w = 0; w * kWave < d.top; ++w) {
+                const Stat<float> t = te.part[w];
+                s += t.m == m ? t.s : t.s * expf(t.m - m);
+            }
+            ls = logf(s);
+        }
+        const float lp = (z - m) - ls, p = z == kNegInf ? 0.f : expf(lp);
+        const bool bad = p != 0.f && (id < 0 || id >= (int)d.vocab);
+        te.id[threadIdx.x] = id;
+        te.p[threadIdx.x] = p;
+        te.x[threadIdx.x] = x;
+        const float P = wave_sum(p);
+        const float kl = wave_sum(p == 0.f ? 0.f : p * (lp - ((x - v.m) * k.inv_t - logf(v.s))));
+        const int any = __any(bad);
+        if (lane_id() == 0) {
+            te.sum[wave_id()][0] = P;
+            te.sum[wave_id()][1] = kl;
+            te.bad[wave_id()] = any;
+        }
+    }
+    static __device__ __forceinline__ TeacherSums sums(const mc_distill_desc& d, const Teacher& te) {
+        TeacherSums s{0.f, 0.f, false};
+        for (int w = 0; w * kWave < d.top; ++w) {
+            s.P += te.sum[w][0];
+            s.kl += te.sum[w][1];
+            s.bad |= te.bad[w] != 0;
+        }
+        if (s.bad) s.kl = __builtin_nanf("");
+        return s;
+    }
+    // The bits of the student's logit at the entry.
+    template <typename T> __device__ __forceinline__ uint32_t logit(const T* __restrict__ xr, int vocab) const {
+        return raw_load(xr, (unsigned)id < (unsigned)vocab ? id : 0);
+    }
+};
 
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T* __restrict__ logits,
@@ -390,8 +511,7 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
                                                      const float* __restrict__ tlse, const uint8_t* __restrict__ mask,
                                                      LpScale k, float* __restrict__ kl, RowStat* __restrict__ stats,
                                                      uint32_t* __restrict__ counter) {
-    __shared__ RowStat red[NT / 64];
-    __shared__ float redf[5 * (NT / 64)];
+    __shared__ Stat<float> red[NT / 64];
     __shared__ Teacher te;
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
@@ -404,39 +524,58 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
         return;
     }
     const T* xr = logits + row * vocab;
-    const TeacherSums ts = load_teacher<NT>(te, d, row, ids, tl, tlse, redf);
-    const RowStat v = wg_stat<NT>(row_stat<T, NT>(xr, vocab, k), k.c_hi, red);
-    const float r = ts.P == 0.f ? 0.f : distill_row(te, ts, d.top, xr, v, k, redf + 4 * (NT / 64));
+    TopEntry entry;
+    entry.load(d, row, ids, tl);
+    entry.open(d, k.inv_t, te);
+    const uint32_t x = entry.logit(xr, vocab);
+    const Stat<float> st = wg_stat<NT>(row_stat<T, NT, float>(xr, vocab, k), k.c_hi, red);
+    const RowStat v{st.m, st.s};
+    entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
+    __syncthreads();
     if (threadIdx.x == 0) {
-        kl[row] = r;
+        kl[row] = entry.sums(d, te).kl;
         if (stats) stats[row] = v;
     }
 }
 
 // loss = T^2 sum kl / counted rows; scale = T / counted rows.
-__global__ __launch_bounds__(256) void distill_final_k(int64_t rows, int64_t chunk, float temperature,
-                                                       const uint8_t* __restrict__ mask, const float* __restrict__ kl,
-                                                       double (*part)[2], uint32_t* __restrict__ counter,
-                                                       float* __restrict__ loss, float* __restrict__ scale) {
-    __shared__ double red[4][2];
+template <int NT>
+__global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chunk, float temperature,
+                                                      const uint8_t* __restrict__ mask, const float* __restrict__ kl,
+                                                      double (*part)[2], uint32_t* counter, float* __restrict__ loss,
+                                                      float* __restrict__ scale) {
+    __shared__ double red[NT / 64][2];
     __shared__ uint32_t slot;
     const int64_t r0 = (int64_t)blockIdx.x * chunk;
     const int64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
     double v[2] = {0.0, 0.0};
-    for (int64_t row = r0 + threadIdx.x; row < r1; row += 256)
-        if (!mask || mask[row] != 0) {
-            v[0] += (double)kl[row];
-            v[1] += 1.0;
-        }
-    wg_sum_f64<2>(v, red);
-    if (threadIdx.x == 0) {
-        part[blockIdx.x][0] = v[0];
-        part[blockIdx.x][1] = v[1];
-    }
-    if (!last_to_arrive(counter, &slot)) return;
+    constexpr int U = 4;
+    for (int64_t row0 = r0 + threadIdx.x; row0 < r1; row0 += U * NT) {
+        float x[U];
+        bool on[U];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = row0 + u * NT < r1 ? row0 + u * NT : row0;
+            x[u] = kl[row];
+            on[u] = row0 + u * NT < r1 && (!mask || mask[row] != 0);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[0] += on[u] ? (double)x[u] : 0.0;
+            v[1] += on[u] ? 1.0 : 0.0;
+        }
+    }
     wg_sum_f64<2>(v, red);
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) {
+            part[blockIdx.x][0] = v[0];
+            part[blockIdx.x][1] = v[1];
+        }
+        if (!last_to_arrive(counter, &slot)) return;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
+        wg_sum_f64<2>(v, red);
+    }
     if (threadIdx.x == 0) {
         const double T = temperature;
         loss[0] = (float)(T * T * v[0] / v[1]);  // no row counted: 0 / 0, a NaN loss
@@ -445,34 +584,47 @@ __global__ __launch_bounds__(256) void distill_final_k(int64_t rows, int64_t chu
 }
 
 // ---------------------------------------------------------------- gradients
-// The row's dense part a q, q = 2^((x - m) c) / s, with `take` adding to the elements j0 ..
-// j0 + N of a vector what the loss holds there. Rows run backwards, and stream
-// stores past the caches, for the reasons of the cross entropy's backward.
-template <typename T, int NT, typename Take>
+// A row's gradient is a q, q = 2^((x - m) c) / s, but for the elements of the
+// target or of the teacher's entries. Those are stored once more by the thread
+// that stored their vector, behind it: stores of a thread stay in order, so that
+// needs no barrier, and the loop over the row no test. Rows run backwards, and
+// stream stores past the caches, for the reasons of the cross entropy's backward.
+struct RowGrad {
+    float a, m, c;  // a: with 1 / s
+    __device__ __forceinline__ float operator()(float x) const { return a * exp2_hw((x - m) * c); }
+};
+__device__ __forceinline__ RowGrad row_grad(float a, RowStat st, float c) { return RowGrad{a / st.s, st.m, c}; }
+
+template <typename T, int NT>
 __device__ __forceinline__ void write_row(const T* __restrict__ xr, T* __restrict__ dr, int vocab, bool vec,
-                                          bool stream, float a, float c, RowStat st, const Take& take) {
+                                          bool stream, RowGrad grad) {
     constexpr int N = Vec16<T>::N;
-    const float m = st.m;
-    a /= st.s;
     if (vec) {
         const RowSpan<T> span(xr, vocab);
-        const int head = (int)span.head;
         for (int cc = (int)span.nvec - 1 - (int)threadIdx.x; cc >= 0; cc -= NT) {
-            const int64_t j0 = head + (int64_t)cc * N;
+            const int64_t j0 = span.head + (int64_t)cc * N;
             float v[N];
             Vec16<T>::load(xr + j0, v);
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = a * exp2_hw((v[e] - m) * c);
-            take(cc, (int)j0, v);
+            for (int e = 0; e < N; ++e) v[e] = grad(v[e]);
             if (stream) store_nt16(dr + j0, v);
             else Vec16<T>::store(dr + j0, v);
         }
         const int64_t j = span.edge((int)threadIdx.x, vocab);
-        if (j >= 0) Elem<T>::store(dr, j, take.at((int)j, a * exp2_hw((Elem<T>::load(xr, j) - m) * c)));
+        if (j >= 0) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
     } else {
-        for (int64_t j = threadIdx.x; j < vocab; j += NT)
-            Elem<T>::store(dr, j, take.at((int)j, a * exp2_hw((Elem<T>::load(xr, j) - m) * c)));
+        for (int64_t j = threadIdx.x; j < vocab; j += NT) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
     }
+}
+// The thread that stores element j: its vector's (BACK: as write_row deals them,
+// else as a held row's), its edge's, or its own where the row goes one by one.
+template <int NT, int N, bool BACK>
+__device__ __forceinline__ int owner_of(int j, int head, int nvec, bool vec) {
+    if (!vec) return j & (NT - 1);
+    if (j < head) return j;
+    const int c = (j - head) / N;
+    if (c >= nvec) return N + (j - head - nvec * N);
+    return (BACK ? nvec - 1 - c : c) & (NT - 1);
 }
 
 template <typename T, int NT>
@@ -489,60 +641,43 @@ __device__ __forceinline__ void zero_row(T* __restrict__ dr, int vocab, bool str
     if (j >= 0) Elem<T>::store(dr, j, 0.f);
 }
 
-// One target's g.
-struct TakeOne {
-    int t;
-    float g;
-    template <int N> __device__ __forceinline__ void operator()(int, int j0, float (&v)[N]) const {
-        if ((unsigned)(t - j0) < (unsigned)N) {
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[e] += j0 + e == t ? g : 0.f;
-        }
-    }
-    __device__ __forceinline__ float at(int j, float v) const { return j == t ? v + g : v; }
-};
+// Which of a teacher's entries each thread stores: a bit for entry k in word
+// k / 32 of its owner.
+template <int NT> struct TopOwners {
+    uint32_t bits[kDistillMaxTop / 32 * NT];
 
-// A teacher's entries, w p_k each, in the order of k where an id comes twice.
-// A bit per vector says whether any entry lies in it (two vectors 2^16 apart
-// share a bit), so only those vectors go through the list.
-constexpr int kTakeBits = 1 << 16;
-struct TakeTop {
-    const Teacher& te;
-    const uint32_t* bits;
-    int top;
-    float w;
-    template <int N> __device__ __forceinline__ void operator()(int cc, int j0, float (&v)[N]) const {
-        const unsigned b = (unsigned)cc & (kTakeBits - 1);
-        if (!((bits[b >> 5] >> (b & 31)) & 1u)) return;
-        for (int k = 0; k < top; ++k) {
-            const int id = te.id[k];
-            if ((unsigned)(id - j0) < (unsigned)N) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) v[e] -= j0 + e == id ? w * te.p[k] : 0.f;
-            }
-        }
+    // Before the entries are there, with a barrier behind it.
+    __device__ __forceinline__ void clear(int top) {
+        for (int i = threadIdx.x; i < (top + 31) / 32 * NT; i += NT) bits[i] = 0;
     }
-    __device__ __forceinline__ float at(int j, float v) const {
-        for (int k = 0; k < top; ++k)
-            if (te.id[k] == j) v -= w * te.p[k];
-        return v;
+    // Thread k puts in entry k. A barrier before the patch.
+    template <int N, bool BACK>
+    __device__ __forceinline__ void insert(int id, int top, int head, int nvec, int vocab, bool vec) {
+        const int k = threadIdx.x;
+        if (k < top && (unsigned)id < (unsigned)vocab)
+            atomicOr(&bits[(k >> 5) * NT + owner_of<NT, N, BACK>(id, head, nvec, vec)], 1u << (k & 31));
+    }
+    template <typename F> __device__ __forceinline__ void each(int top, F&& fn) const {
+        for (int w = 0; w < (top + 31) / 32; ++w)
+            for (uint32_t b = bits[w * NT + threadIdx.x]; b; b &= b - 1) fn(32 * w + __ffs(b) - 1);
+    }
+    // The thread's entries' elements, once the row is stored: w p_k less, for all
+    // the entries of an id, in the order of k.
+    template <typename T>
+    __device__ __forceinline__ void patch(const Teacher& te, int top, T* __restrict__ dr, RowGrad grad, float w) const {
+        each(top, [&](int k) {
+            const int id = te.id[k];
+            float p = 0.f;
+            bool first = true;
+            each(top, [&](int o) {
+                if (te.id[o] != id) return;
+                first = first && o >= k;
+                p += te.p[o];
+            });
+            if (first) Elem<T>::store(dr, id, grad(te.x[k]) - w * p);
+        });
     }
 };
-// The bits of a row's entries (ids in range). All threads; head as in write_row.
-template <int NT, int N>
-__device__ __forceinline__ void mark_top(const Teacher& te, int top, int head, int nvec, uint32_t* bits) {
-    const int words = ((nvec < kTakeBits ? nvec : kTakeBits) + 31) / 32;
-    for (int i = threadIdx.x; i < words; i += NT) bits[i] = 0;
-    __syncthreads();
-    if ((int)threadIdx.x < top) {
-        const int id = te.id[threadIdx.x];
-        if (id >= head) {
-            const int c = (id - head) / N;
-            if (c < nvec) atomicOr(&bits[(c & (kTakeBits - 1)) >> 5], 1u << (c & 31));
-        }
-    }
-    __syncthreads();
-}
 
 // dlogits of a loss over l: g ([j = t] - q_j) / T, g = dl of the row (or of its
 // sequence) times the optional device scalars.
@@ -568,7 +703,13 @@ __global__ __launch_bounds__(NT) void lp_bwd_k(int64_t rows, int vocab, bool vec
         return;
     }
     g *= k.inv_t;
-    write_row<T, NT>(logits + row * vocab, dr, vocab, vec, stream, -g, k.c_hi, stats[row], TakeOne{(int)t, g});
+    const T* xr = logits + row * vocab;
+    const RowGrad grad = row_grad(-g, stats[row], k.c_hi);
+    write_row<T, NT>(xr, dr, vocab, vec, stream, grad);
+    const RowSpan<T> span(xr, vocab);
+    if (t < (uint32_t)vocab &&
+        owner_of<NT, Vec16<T>::N, true>((int)t, (int)span.head, (int)span.nvec, vec) == (int)threadIdx.x)
+        Elem<T>::store(dr, t, grad(Elem<T>::load(xr, t)) + g);
 }
 
 template <typename T, int NT>
@@ -578,28 +719,289 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
                                                     const uint8_t* __restrict__ mask, LpScale k,
                                                     const RowStat* __restrict__ stats, const float* __restrict__ scale,
                                                     const float* __restrict__ dloss, T* __restrict__ dlogits) {
-    __shared__ float redf[4 * (NT / 64)];
+    constexpr int N = Vec16<T>::N;
     __shared__ Teacher te;
-    __shared__ uint32_t bits[kTakeBits / 32];
+    __shared__ TopOwners<NT> owners;
     const int64_t row = d.rows - 1 - (int64_t)blockIdx.x;
     const int vocab = (int)d.vocab;
     T* dr = dlogits + row * vocab;
-    float w = 0.f;
-    TeacherSums ts{};
-    if (!mask || mask[row] != 0) {
-        ts = load_teacher<NT>(te, d, row, ids, tl, tlse, redf);
-        w = scale[0] * (dloss ? dloss[0] : 1.f);
-        if (ts.bad) w = __builtin_nanf("");
-        if (ts.P == 0.f) w = 0.f;
+    if (mask && mask[row] == 0) {
+        zero_row<T, NT>(dr, vocab, stream);
+        return;
     }
-    if (w == 0.f) {
+    owners.clear(d.top);
+    const T* xr = logits + row * vocab;
+    const RowSpan<T> span(xr, vocab);
+    const RowStat v = stats[row];
+    TopEntry entry;
+    entry.load(d, row, ids, tl);
+    entry.open(d, k.inv_t, te);
+    const uint32_t x = entry.logit(xr, vocab);
+    __syncthreads();
+    owners.template insert<N, true>(entry.id, d.top, (int)span.head, (int)span.nvec, vocab, vec);
+    entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
+    __syncthreads();
+    const TeacherSums ts = entry.sums(d, te);
+    float w = scale[0] * (dloss ? dloss[0] : 1.f);
+    if (ts.bad) w = __builtin_nanf("");
+    if (ts.P == 0.f || w == 0.f) {
+        zero_row<T, NT>(dr, vocab, stream);
+        return;
+    }
+    const RowGrad grad = row_grad(w * ts.P, v, k.c_hi);
+    write_row<T, NT>(xr, dr, vocab, vec, stream, grad);
+    owners.patch(te, d.top, dr, grad, w);
+}
+
+// ------------------------------------------- value and gradient in one read
+// A row held in registers, vector u * NT + t of it in thread t, so that the
+// statistics and the gradient come from one read: 1024 threads hold 320 KB, the
+// smaller shapes several rows per CU. All the loads are in flight at once, and
+// the statistics take them as they come, so whatever else a kernel loads comes
+// before them (loads return in order). Loads past the last vector give zeros
+// and stores there are dropped. The edges' elements are in the first 2 N
+// threads, as their bits.
+// Nothing is loaded under a condition, or every wait would be for the path with
+// the fewest loads, that is for all of them.
+template <typename T, int NT, int NV> struct HeldRow {
+    static constexpr int N = Vec16<T>::N, G = 16 / N;  // vectors reduced at a time
+    i32x4 q[NV];
+    uint32_t edge;
+    int head, nvec, j;  // j: the edge element, or -1
+
+    __device__ __forceinline__ void load(const T* __restrict__ xr, int vocab) {
+        const RowSpan<T> span(xr, vocab);
+        head = (int)span.head;
+        nvec = (int)span.nvec;
+        j = (int)span.edge((int)threadIdx.x, vocab);
+        edge = raw_load(xr, j < 0 ? 0 : j);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(xr + head, (int64_t)nvec * 16);
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            __builtin_amdgcn_sched_barrier(0);  // in the order of their use
+            q[u] = buf_load16(r, (uint32_t)(u * NT + (int)threadIdx.x) * 16u);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __forceinline__ Stat<float> stat(LpScale k) const {
+        float m = kNegInf, s = 0.f;
+#pragma unroll
+        for (int u0 = 0; u0 < NV; u0 += G) {
+            if (u0 * NT >= nvec) break;
+            float v[G][N];
+            float vm = kNegInf;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int u = u0 + g;
+                if (u < NV) BVec<T>::unpack(q[u], v[g]);
+                if (u >= NV || ((u + 1) * NT > nvec && u * NT + (int)threadIdx.x >= nvec)) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v[g][e] = kNegInf;
+                }
+#pragma unroll
+                for (int e = 0; e < N; ++e) vm = fmaxf(vm, v[g][e]);
+            }
+            if (vm > m) {
+                s *= exp2_hw((m - vm) * k.c_hi);
+                m = vm;
+            }
+            const float base = base_of(m);
+            float ps[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                ps[g] = 0.f;
+#pragma unroll
+                for (int e = 0; e < N; ++e) ps[g] += term_of(v[g][e], base, k);
+            }
+            s += G == 4 ? (ps[0] + ps[1]) + (ps[G - 2] + ps[G - 1]) : ps[0] + ps[1];
+        }
+        if (j >= 0) {
+            const float x = from_raw<T>(edge);
+            return stat_join(Stat<float>{m, s}, Stat<float>{x, term_of(x, base_of(x), k)}, k.c_hi);
+        }
+        return Stat<float>{m, s};
+    }
+    // into the gradient's row dr, which starts like the logits'
+    __device__ __forceinline__ void store(T* __restrict__ dr, bool stream, RowGrad grad) const {
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(dr + head, (int64_t)nvec * 16);
+        uint32_t at = threadIdx.x * 16u;
+        asm volatile("" : "+v"(at));  // or the loads' NV offsets are held for the stores
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            if (u * NT >= nvec) break;
+            float v[N];
+            BVec<T>::unpack(q[u], v);
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = grad(v[e]);
+            if (stream) BVec<T>::store_nt(r, at + u * NT * 16u, v);
+            else BVec<T>::store(r, at + u * NT * 16u, v);
+        }
+        if (j >= 0) Elem<T>::store(dr, j, grad(from_raw<T>(edge)));
+    }
+};
+
+// Counted tokens of 64 blocks of rows, for the weight of a token.
+constexpr int kCountBlocks = 64;
+__global__ __launch_bounds__(256) void counts_k(int64_t rows, int64_t chunk, const uint32_t* __restrict__ targets,
+                                                const uint8_t* __restrict__ mask, int64_t ignore_index,
+                                                uint32_t* __restrict__ part) {
+    __shared__ uint32_t red[4];
+    const int64_t r0 = (int64_t)blockIdx.x * chunk;
+    const int64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
+    uint32_t c = 0;
+    for (int64_t row = r0 + threadIdx.x; row < r1; row += 256)
+        c += (targets ? counted(targets[row], ignore_index) : mask[row] != 0) ? 1u : 0u;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) c += (uint32_t)__shfl_xor((int)c, o, kWave);
+    if (lane_id() == 0) red[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+// How many tokens share a row's weight: the sum of `given` counts, or where four
+// loads per thread go over the `len` targets (or the mask) themselves, those. load
+// before the row's loads, put after them, a barrier of the kernel, total.
+template <int NT> struct RowCount {
+    static constexpr int kPer = 4;
+    uint32_t w[kPer];
+    // value(i): the i-th target or mask byte; called where len is 0, too
+    template <typename F> __device__ __forceinline__ void load(int len, F&& value) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) w[i] = value(i * NT + (int)threadIdx.x < len ? i * NT + (int)threadIdx.x : 0);
+    }
+    template <typename F> __device__ __forceinline__ void put(int len, uint32_t* red, F&& on) const {
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) c += i * NT + (int)threadIdx.x < len && on(w[i]) ? 1u : 0u;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) c += (uint32_t)__shfl_xor((int)c, o, kWave);
+        if (lane_id() == 0) red[threadIdx.x >> 6] = c;
+    }
+    static __device__ __forceinline__ uint32_t total(const uint32_t* red, const uint32_t* __restrict__ given, int n) {
+        uint32_t c = 0;
+        if (given) {
+            for (int i = 0; i < n; ++i) c += given[i];
+        } else {
+#pragma unroll
+            for (int k = 0; k < NT / 64; ++k) c += red[k];
+        }
+        return c;
+    }
+};
+
+// l, and with the token's weight its gradient. given: n_given counts that add up
+// to the tokens that share the weight (by_seq: of each sequence, one number
+// each), or null: counted here over len targets. n (may be null): receives the
+// sequences' counts.
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool stream, const T* __restrict__ logits,
+                                                       const uint32_t* __restrict__ targets,
+                                                       const float* __restrict__ adv, const float* __restrict__ old,
+                                                       const float* __restrict__ ref,
+                                                       const uint32_t* __restrict__ given, int n_given, int len,
+                                                       bool by_seq,
+                                                       uint32_t* __restrict__ n, LpScale k,
+                                                       const float* __restrict__ dloss, float* __restrict__ logp,
+                                                       T* __restrict__ dlogits, uint32_t* __restrict__ counter) {
+    __shared__ Stat<float> red[NT / 64];
+    __shared__ uint32_t redc[NT / 64];
+    const int64_t row = blockIdx.x;
+    const int vocab = (int)d.vocab;
+    if (row == 0 && threadIdx.x == 0) *counter = 0;
+    T* dr = dlogits + row * vocab;
+    const uint32_t t = targets[row];
+    if (!counted(t, d.ignore_index)) {
+        if (threadIdx.x == 0) logp[row] = 0.f;
         zero_row<T, NT>(dr, vocab, stream);
         return;
     }
     const T* xr = logits + row * vocab;
-    const RowSpan<T> span(xr, vocab);
-    mark_top<NT, Vec16<T>::N>(te, d.top, (int)span.head, (int)span.nvec, bits);
-    write_row<T, NT>(xr, dr, vocab, vec, stream, w * ts.P, k.c_hi, stats[row], TakeTop{te, bits, d.top, w});
+    const bool in = t < (uint32_t)vocab;
+    const uint32_t xt = raw_load(xr, in ? t : 0);
+    const uint32_t q = (uint32_t)row / (uint32_t)d.seq;
+    const PolicyInputs pin = policy_inputs(d, adv, old, ref, row, q);
+    const float up = dloss ? dloss[0] : 1.f;
+    const uint32_t* cw = by_seq ? targets + (int64_t)q * d.seq : targets;
+    RowCount<NT> count;
+    count.load(len, [&](int i) { return cw[i]; });
+    HeldRow<T, NT, NV> held;
+    held.load(xr, vocab);
+    count.put(len, redc, [&](uint32_t w) { return counted(w, d.ignore_index); });
+    const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
+    const RowStat v{st.m, st.s};
+    const uint32_t share = count.total(redc, given ? given + (by_seq ? q : 0) : nullptr, n_given);
+    const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
+    if (threadIdx.x == 0) {
+        logp[row] = l;
+        if (n) n[q] = share;  // the same from every row of the sequence
+    }
+    float g = policy_term(d, l, pin).dl / (by_seq ? (float)d.batch * (float)share : (float)share) * up;
+    if (g == 0.f) {
+        zero_row<T, NT>(dr, vocab, stream);
+        return;
+    }
+    g *= k.inv_t;
+    const RowGrad grad = row_grad(-g, v, k.c_hi);
+    held.store(dr, stream, grad);
+    if (in && owner_of<NT, Vec16<T>::N, false>((int)t, held.head, held.nvec, true) == (int)threadIdx.x)
+        Elem<T>::store(dr, t, grad(from_raw<T>(xt)) + g);
+}
+
+// given: n_given counts of the mask, or null: counted here over len of it (0
+// without a mask).
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool stream, const T* __restrict__ logits,
+                                                        const int32_t* __restrict__ ids, const float* __restrict__ tl,
+                                                        const float* __restrict__ tlse,
+                                                        const uint8_t* __restrict__ mask,
+                                                        const uint32_t* __restrict__ given, int n_given, int len,
+                                                        LpScale k, const float* __restrict__ dloss,
+                                                        float* __restrict__ kl,
+                                                        T* __restrict__ dlogits, uint32_t* __restrict__ counter) {
+    constexpr int N = Vec16<T>::N;
+    __shared__ Stat<float> red[NT / 64];
+    __shared__ uint32_t redc[NT / 64];
+    __shared__ Teacher te;
+    __shared__ TopOwners<NT> owners;
+    const int64_t row = blockIdx.x;
+    const int vocab = (int)d.vocab;
+    if (row == 0 && threadIdx.x == 0) *counter = 0;
+    T* dr = dlogits + row * vocab;
+    if (mask && mask[row] == 0) {
+        if (threadIdx.x == 0) kl[row] = 0.f;
+        zero_row<T, NT>(dr, vocab, stream);
+        return;
+    }
+    const T* xr = logits + row * vocab;
+    TopEntry entry;
+    entry.load(d, row, ids, tl);
+    owners.clear(d.top);
+    __syncthreads();
+    const float up = dloss ? dloss[0] : 1.f;
+    const float lse = tlse ? tlse[row] : 0.f;
+    RowCount<NT> count;
+    const uint8_t* cw = mask ? mask : reinterpret_cast<const uint8_t*>(xr);
+    count.load(len, [&](int i) { return (uint32_t)cw[i]; });
+    HeldRow<T, NT, NV> held;
+    held.load(xr, vocab);
+    count.put(len, redc, [](uint32_t w) { return w != 0; });
+    entry.open(d, k.inv_t, te);
+    owners.template insert<N, false>(entry.id, d.top, held.head, held.nvec, vocab, true);
+    const uint32_t x = entry.logit(xr, vocab);
+    const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
+    const RowStat v{st.m, st.s};
+    entry.close(d, tlse != nullptr, lse, from_raw<T>(x), v, k, te);
+    float w = d.temperature / (mask ? (float)count.total(redc, given, n_given) : (float)d.rows) * up;
+    __syncthreads();
+    const TeacherSums ts = entry.sums(d, te);
+    if (threadIdx.x == 0) kl[row] = ts.kl;
+    if (ts.bad) w = __builtin_nanf("");
+    if (ts.P == 0.f || w == 0.f) {
+        zero_row<T, NT>(dr, vocab, stream);
+        return;
+    }
+    const RowGrad grad = row_grad(w * ts.P, v, k.c_hi);
+    held.store(dr, stream, grad);
+    owners.patch(te, d.top, dr, grad, w);
 }
 
 // c = log2(e) / T as a float below it and the rest: with c_lo > 0, x c_lo has the
@@ -610,7 +1012,8 @@ LpScale row_scale(float temperature) {
     k.c_hi = (float)c;
     if ((double)k.c_hi >= c) k.c_hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, k.c_hi) - 1);
     k.c_lo = (float)(c - (double)k.c_hi);
-    k.inv_t = (float)(1.0 / (double)temperature);
+    k.inv_t64 = 1.0 / (double)temperature;
+    k.inv_t = (float)k.inv_t64;
     return k;
 }
 
@@ -626,15 +1029,45 @@ hipError_t by_row_kernel(int64_t rows, int64_t vocab, int dtype, F&& fn) {
     return hipGetLastError();
 }
 
+// fn(element type, threads, vectors per thread) for the smallest shape that holds
+// a row; false where none does.
+template <typename F>
+bool by_held_shape(int64_t vocab, int dtype, F&& fn) {
+    auto go = [&](auto elem) {
+        typedef decltype(elem) T;
+        const int64_t vectors = vocab / Vec16<T>::N;
+        auto shape = [&](auto threads, auto held) {
+            if (vectors > decltype(threads)::value * decltype(held)::value) return false;
+            fn(elem, threads, held);
+            return true;
+        };
+        using std::integral_constant;
+        return shape(integral_constant<int, 256>{}, integral_constant<int, 4>{}) ||
+               shape(integral_constant<int, 256>{}, integral_constant<int, 8>{}) ||
+               shape(integral_constant<int, 512>{}, integral_constant<int, 8>{}) ||
+               shape(integral_constant<int, 512>{}, integral_constant<int, 16>{}) ||
+               shape(integral_constant<int, 1024>{}, integral_constant<int, 10>{}) ||
+               shape(integral_constant<int, 1024>{}, integral_constant<int, 13>{}) ||
+               shape(integral_constant<int, 1024>{}, integral_constant<int, 16>{}) ||
+               shape(integral_constant<int, 1024>{}, integral_constant<int, 19>{});
+    };
+    return dtype == MC_F32 ? go(float{}) : go(uint16_t{});
+}
+
 bool same_start(const void* a, const void* b) {
     return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
-// Workgroups of the kernels that sum over rows, and rows of each: at most 256
-// partial sums, which one workgroup then adds.
-int64_t sum_chunk(int64_t rows) {
-    const int64_t c = (rows + 255) / 256;
-    return c < 256 ? 256 : c;
+// Rows whose sums one workgroup of 1024 threads forms by itself; past it 256
+// workgroups, which meet in the last one.
+constexpr int64_t kOneGroupRows = 8192;
+template <typename F> void by_sum_kernel(int64_t rows, F&& fn) {
+    if (rows <= kOneGroupRows) {
+        fn(std::integral_constant<int, 1024>{}, dim3(1), rows);
+    } else {
+        const int64_t chunk = (rows + 255) / 256;
+        fn(std::integral_constant<int, 256>{}, dim3((unsigned)((rows + chunk - 1) / chunk)), chunk);
+    }
 }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -642,8 +1075,10 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace
 
 // ------------------------------------------------------------- launchers
-hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
-                                     float* stats, uint32_t* counter, hipStream_t stream) {
+namespace {
+template <typename L>
+hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, L* logp, float* stats,
+                          uint32_t* counter, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
     return by_row_kernel(d.rows, d.vocab, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
@@ -652,6 +1087,12 @@ hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logit
                                                                     targets, d.ignore_index, k, logp,
                                                                     reinterpret_cast<RowStat*>(stats), counter);
     });
+}
+}  // namespace
+
+hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
+                                     float* stats, hipStream_t stream) {
+    return launch_lp_rows(d, logits, targets, logp, stats, nullptr, stream);
 }
 
 hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
@@ -673,7 +1114,7 @@ PreferenceWs preference_ws(const mc_preference_desc& d) {
     PreferenceWs w;
     size_t at = 256;  // the counter
     w.logp = at;
-    at += align256((size_t)(2 * d.pairs * d.seq) * sizeof(float));
+    at += align256((size_t)(2 * d.pairs * d.seq) * sizeof(double));
     w.score = at;
     at += align256((size_t)(2 * d.pairs) * sizeof(double));
     w.inv_n = at;
@@ -686,14 +1127,19 @@ hipError_t launch_preference_fwd(const mc_preference_desc& d, const void* logits
                                  hipStream_t stream) {
     const PreferenceWs w = preference_ws(d);
     const int64_t rows = 2 * d.pairs * d.seq;
-    float* logp = reinterpret_cast<float*>(ws + w.logp);
+    double* logp = reinterpret_cast<double*>(ws + w.logp);
+    double* score = reinterpret_cast<double*>(ws + w.score);
+    float* inv_n = reinterpret_cast<float*>(ws + w.inv_n);
+    float* dseq = stats ? stats + 2 * rows : nullptr;
     uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, 1.0f, d.dtype};
-    hipError_t e = launch_token_logprobs_fwd(lp, logits, targets, logp, stats, counter, stream);
+    hipError_t e = launch_lp_rows(lp, logits, targets, logp, stats, counter, stream);
     if (e != hipSuccess) return e;
-    preference_k<<<dim3((unsigned)(2 * d.pairs)), 256, 0, stream>>>(
-        d, targets, logp, ref, reinterpret_cast<double*>(ws + w.score), reinterpret_cast<float*>(ws + w.inv_n), counter,
-        loss, rewards, stats ? stats + 2 * rows : nullptr);
+    if (rows <= kOneGroupRows)
+        preference_one_k<<<dim3(1), 1024, 0, stream>>>(d, targets, logp, ref, score, inv_n, loss, rewards, dseq);
+    else
+        preference_k<<<dim3((unsigned)(2 * d.pairs)), 256, 0, stream>>>(d, targets, logp, ref, score, inv_n, counter,
+                                                                         loss, rewards, dseq);
     return hipGetLastError();
 }
 
@@ -718,24 +1164,33 @@ const uint32_t* policy_counts(const mc_policy_desc& d, const uint32_t* targets, 
     e = hipGetLastError();
     return n;
 }
+
+hipError_t launch_policy_sums(const mc_policy_desc& d, const uint32_t* targets, const float* logp, const float* adv,
+                              const float* old, const float* ref, const uint32_t* n, char* ws, float* loss,
+                              float* metrics, float* dlp, hipStream_t stream) {
+    by_sum_kernel(d.batch * d.seq, [&](auto threads, dim3 grid, int64_t chunk) {
+        constexpr int NT = decltype(threads)::value;
+        policy_k<NT><<<grid, NT, 0, stream>>>(d, chunk, targets, logp, adv, old, ref, n,
+                                              reinterpret_cast<double(*)[4]>(ws + policy_ws(d).part),
+                                              reinterpret_cast<uint32_t*>(ws), loss, metrics, dlp);
+    });
+    return hipGetLastError();
+}
 }  // namespace
 
 hipError_t launch_policy_fwd(const mc_policy_desc& d, const void* logits, const uint32_t* targets, const float* adv,
                              const float* old, const float* ref, float* loss, float* logp, float* metrics,
                              float* stats, char* ws, hipStream_t stream) {
-    const PolicyWs w = policy_ws(d);
-    const int64_t rows = d.batch * d.seq, chunk = sum_chunk(rows);
+    const int64_t rows = d.batch * d.seq;
     uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, d.temperature, d.dtype};
     hipError_t e;
     const uint32_t* n = policy_counts(d, targets, ws, stream, e);
     if (e != hipSuccess) return e;
-    e = launch_token_logprobs_fwd(lp, logits, targets, logp, stats, counter, stream);
+    e = launch_lp_rows(lp, logits, targets, logp, stats, counter, stream);
     if (e != hipSuccess) return e;
-    policy_k<<<dim3((unsigned)((rows + chunk - 1) / chunk)), 256, 0, stream>>>(
-        d, chunk, targets, logp, adv, old, ref, n, reinterpret_cast<double(*)[4]>(ws + w.part), counter, loss, metrics,
-        stats ? stats + 2 * rows : nullptr);
-    return hipGetLastError();
+    return launch_policy_sums(d, targets, logp, adv, old, ref, n, ws, loss, metrics, stats ? stats + 2 * rows : nullptr,
+                              stream);
 }
 
 DistillWs distill_ws(const mc_distill_desc& d) {
@@ -747,6 +1202,19 @@ DistillWs distill_ws(const mc_distill_desc& d) {
     w.total = at + align256((size_t)d.rows * sizeof(float));
     return w;
 }
+
+namespace {
+hipError_t launch_distill_sums(const mc_distill_desc& d, const uint8_t* mask, const float* kl, char* ws, float* loss,
+                               float* scale, hipStream_t stream) {
+    by_sum_kernel(d.rows, [&](auto threads, dim3 grid, int64_t chunk) {
+        constexpr int NT = decltype(threads)::value;
+        distill_final_k<NT><<<grid, NT, 0, stream>>>(d.rows, chunk, d.temperature, mask, kl,
+                                                     reinterpret_cast<double(*)[2]>(ws + distill_ws(d).part),
+                                                     reinterpret_cast<uint32_t*>(ws), loss, scale);
+    });
+    return hipGetLastError();
+}
+}  // namespace
 
 hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, const int32_t* ids, const float* tl,
                               const float* tlse, const uint8_t* mask, float* loss, float* stats, char* ws,
@@ -763,11 +1231,7 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
                                                                          reinterpret_cast<RowStat*>(stats), counter);
     });
     if (e != hipSuccess) return e;
-    const int64_t chunk = sum_chunk(d.rows);
-    distill_final_k<<<dim3((unsigned)((d.rows + chunk - 1) / chunk)), 256, 0, stream>>>(
-        d.rows, chunk, d.temperature, mask, kl, reinterpret_cast<double(*)[2]>(ws + w.part), counter, loss,
-        stats ? stats + 2 * d.rows : nullptr);
-    return hipGetLastError();
+    return launch_distill_sums(d, mask, kl, ws, loss, stats ? stats + 2 * d.rows : nullptr, stream);
 }
 
 hipError_t launch_distill_bwd(const mc_distill_desc& d, const void* logits, const int32_t* ids, const float* tl,
@@ -784,16 +1248,55 @@ hipError_t launch_distill_bwd(const mc_distill_desc& d, const void* logits, cons
     });
 }
 
+// counts_k over rows into ws; the number of its blocks
+namespace {
+int launch_counts(int64_t rows, const uint32_t* targets, const uint8_t* mask, int64_t ignore_index, uint32_t* part,
+                  hipStream_t stream) {
+    int64_t chunk = (rows + kCountBlocks - 1) / kCountBlocks;
+    if (chunk < 256) chunk = 256;
+    const int blocks = (int)((rows + chunk - 1) / chunk);
+    counts_k<<<dim3((unsigned)blocks), 256, 0, stream>>>(rows, chunk, targets, mask, ignore_index, part);
+    return blocks;
+}
+}  // namespace
+
+// The forward's buffers, then 64 counts or, where no shape holds a row, the
+// forward's stats.
 size_t policy_fwd_bwd_ws(const mc_policy_desc& d) {
-    return policy_ws(d).total + align256((size_t)(3 * d.batch * d.seq + 1) * sizeof(float));
+    return policy_ws(d).total + align256((size_t)(3 * d.batch * d.seq + kCountBlocks) * sizeof(float));
 }
 
 hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, const uint32_t* targets,
                                  const float* adv, const float* old, const float* ref, const float* dloss, float* loss,
                                  float* logp, float* metrics, void* dlogits, char* ws, hipStream_t stream) {
-    float* stats = reinterpret_cast<float*>(ws + policy_ws(d).total);
+    const PolicyWs w = policy_ws(d);
+    float* stats = reinterpret_cast<float*>(ws + w.total);
     const int64_t rows = d.batch * d.seq;
-    hipError_t e = launch_policy_fwd(d, logits, targets, adv, old, ref, loss, logp, metrics, stats, ws, stream);
+    const LpScale k = row_scale(d.temperature);
+    hipError_t e;
+    if (same_start(logits, dlogits) && by_held_shape(d.vocab, d.dtype, [](auto, auto, auto) {})) {
+        uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
+        uint32_t* part = reinterpret_cast<uint32_t*>(stats);
+        const bool by_seq = d.reduction == MC_MEAN_SEQUENCES;
+        uint32_t* n = by_seq ? reinterpret_cast<uint32_t*>(ws + w.counts) : nullptr;
+        by_held_shape(d.vocab, d.dtype, [&](auto elem, auto threads, auto held) {
+            typedef decltype(elem) T;
+            constexpr int NT = decltype(threads)::value, NV = decltype(held)::value;
+            const int64_t span = by_seq ? d.seq : rows;
+            const bool here = span <= RowCount<NT>::kPer * NT;
+            int n_given = 1;
+            e = hipSuccess;
+            if (!here && by_seq) policy_counts(d, targets, ws, stream, e);
+            else if (!here) n_given = launch_counts(rows, targets, nullptr, d.ignore_index, part, stream);
+            policy_held_k<T, NT, NV><<<dim3((unsigned)rows), NT, 0, stream>>>(
+                d, xent_stream_gradients(rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), targets, adv, old,
+                ref, here ? nullptr : by_seq ? n : part, n_given, here ? (int)span : 0, by_seq, here ? n : nullptr, k,
+                dloss, logp, static_cast<T*>(dlogits), counter);
+        });
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        return launch_policy_sums(d, targets, logp, adv, old, ref, n, ws, loss, metrics, nullptr, stream);
+    }
+    e = launch_policy_fwd(d, logits, targets, adv, old, ref, loss, logp, metrics, stats, ws, stream);
     if (e != hipSuccess) return e;
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, d.temperature, d.dtype};
     return launch_token_logprobs_bwd(lp, logits, targets, stats, stats + 2 * rows, 0, stats + 3 * rows, dloss, dlogits,
@@ -801,14 +1304,34 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
 }
 
 size_t distill_fwd_bwd_ws(const mc_distill_desc& d) {
-    return distill_ws(d).total + align256((size_t)(2 * d.rows + 1) * sizeof(float));
+    return distill_ws(d).total + align256((size_t)(2 * d.rows + kCountBlocks) * sizeof(float));
 }
 
 hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, const int32_t* ids, const float* tl,
                                   const float* tlse, const uint8_t* mask, const float* dloss, float* loss,
                                   void* dlogits, char* ws, hipStream_t stream) {
-    float* stats = reinterpret_cast<float*>(ws + distill_ws(d).total);
-    hipError_t e = launch_distill_fwd(d, logits, ids, tl, tlse, mask, loss, stats, ws, stream);
+    const DistillWs w = distill_ws(d);
+    float* stats = reinterpret_cast<float*>(ws + w.total);
+    const LpScale k = row_scale(d.temperature);
+    hipError_t e;
+    if (same_start(logits, dlogits) && by_held_shape(d.vocab, d.dtype, [](auto, auto, auto) {})) {
+        uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
+        float* kl = reinterpret_cast<float*>(ws + w.kl);
+        uint32_t* part = reinterpret_cast<uint32_t*>(stats);
+        by_held_shape(d.vocab, d.dtype, [&](auto elem, auto threads, auto held) {
+            typedef decltype(elem) T;
+            constexpr int NT = decltype(threads)::value, NV = decltype(held)::value;
+            const bool here = !mask || d.rows <= RowCount<NT>::kPer * NT;
+            const int n_given = here ? 0 : launch_counts(d.rows, nullptr, mask, -1, part, stream);
+            distill_held_k<T, NT, NV><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
+                d, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl, tlse,
+                mask, here ? nullptr : part, n_given, mask && here ? (int)d.rows : 0, k, dloss, kl,
+                static_cast<T*>(dlogits), counter);
+        });
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        return launch_distill_sums(d, mask, kl, ws, loss, nullptr, stream);
+    }
+    e = launch_distill_fwd(d, logits, ids, tl, tlse, mask, loss, stats, ws, stream);
     if (e != hipSuccess) return e;
     return launch_distill_bwd(d, logits, ids, tl, tlse, mask, stats, dloss, dlogits, stream);
 }

@@ -82,16 +82,13 @@ __device__ __forceinline__ float term_of(float x, float base, LpScale k) {
     return exp2_hw(fmaf(d, k.c_lo, d * k.c_hi));
 }
 
-// One thread's share of a row: U vectors requested and reduced at a time, one
-// rescale to their maximum, then one exp2 per element.
-template <typename T, int NT, typename S, int U = 4>
-__device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
+// One thread's share of a row's vectors from c on: U of them requested and
+// reduced at a time, one rescale to their maximum, then one exp2 per element.
+template <typename T, int NT, typename S, int U>
+__device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int nvec, LpScale k) {
     constexpr int N = Vec16<T>::N;
     float m = kNegInf;
     S s = 0;
-    const RowSpan<T> span(xr, vocab);
-    const T* xv = xr + span.head;
-    const int nvec = (int)span.nvec;
     auto group = [&](int c, auto count) {
         constexpr int K = decltype(count)::value;
         float v[K][N];
@@ -120,15 +117,19 @@ __device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab,
             for (int i = 0; i < u / 2; ++i) ps[i] = ps[i] + ps[i + u / 2];
         s += ps[0];
     };
-    int c = threadIdx.x;
     for (; c < nvec - (U - 1) * NT; c += U * NT) group(c, std::integral_constant<int, U>{});
     for (; c < nvec; c += NT) group(c, std::integral_constant<int, 1>{});
-    const int64_t j = span.edge((int)threadIdx.x, vocab);
-    if (j >= 0) {
-        const float v = Elem<T>::load(xr, j);
-        return stat_join(Stat<S>{m, s}, Stat<S>{v, (S)term_of(v, base_of(v), k)}, k.c_hi);
-    }
     return Stat<S>{m, s};
+}
+template <typename T, int NT, typename S>
+__device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
+    const RowSpan<T> span(xr, vocab);
+    const Stat<S> st = vec_stat<T, NT, S, 4>(xr + span.head, threadIdx.x, (int)span.nvec, k);
+    static_assert(NT >= 2 * Vec16<T>::N, "a thread per edge element");
+    const int64_t j = span.edge((int)threadIdx.x, vocab);
+    if (j < 0) return st;
+    const float v = Elem<T>::load(xr, j);
+    return stat_join(st, Stat<S>{v, (S)term_of(v, base_of(v), k)}, k.c_hi);
 }
 
 // -------------------------------------------------- sums over many workgroups
@@ -595,49 +596,67 @@ struct RowGrad {
 };
 __device__ __forceinline__ RowGrad row_grad(float a, RowStat st, float c) { return RowGrad{a / st.s, st.m, c}; }
 
-template <typename T, int NT>
-__device__ __forceinline__ void write_row(const T* __restrict__ xr, T* __restrict__ dr, int vocab, bool vec,
-                                          bool stream, RowGrad grad) {
-    constexpr int N = Vec16<T>::N;
-    if (vec) {
-        const RowSpan<T> span(xr, vocab);
-        for (int cc = (int)span.nvec - 1 - (int)threadIdx.x; cc >= 0; cc -= NT) {
-            const int64_t j0 = span.head + (int64_t)cc * N;
-            float v[N];
-            Vec16<T>::load(xr + j0, v);
-#pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = grad(v[e]);
-            if (stream) store_nt16(dr + j0, v);
-            else Vec16<T>::store(dr + j0, v);
-        }
-        const int64_t j = span.edge((int)threadIdx.x, vocab);
-        if (j >= 0) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
-    } else {
-        for (int64_t j = threadIdx.x; j < vocab; j += NT) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
-    }
-}
-// The thread that stores element j: its vector's (BACK: as write_row deals them,
-// else as a held row's), its edge's, or its own where the row goes one by one.
-template <int NT, int N, bool BACK>
-__device__ __forceinline__ int owner_of(int j, int head, int nvec, bool vec) {
-    if (!vec) return j & (NT - 1);
-    if (j < head) return j;
-    const int c = (j - head) / N;
-    if (c >= nvec) return N + (j - head - nvec * N);
-    return (BACK ? nvec - 1 - c : c) & (NT - 1);
+// The threads of a row: those of the gridDim.y workgroups that share it.
+struct RowThreads {
+    int self, count;
+};
+template <int NT> __device__ __forceinline__ RowThreads row_threads() {
+    return RowThreads{(int)(blockIdx.y * NT + threadIdx.x), (int)(gridDim.y * NT)};
 }
 
-template <typename T, int NT>
-__device__ __forceinline__ void zero_row(T* __restrict__ dr, int vocab, bool stream) {
+// Vectors c, c - step, .. down to lo: U requested at a time.
+template <typename T, int U>
+__device__ __forceinline__ void write_vecs(const T* __restrict__ xv, T* __restrict__ dv, int c, int step, int lo,
+                                           bool stream, RowGrad grad) {
+    constexpr int N = Vec16<T>::N;
+    auto group = [&](int c, auto count) {
+        constexpr int K = decltype(count)::value;
+        float v[K][N];
+#pragma unroll
+        for (int u = 0; u < K; ++u) Vec16<T>::load(xv + (int64_t)(c - u * step) * N, v[u]);
+#pragma unroll
+        for (int u = 0; u < K; ++u) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[u][e] = grad(v[u][e]);
+            if (stream) store_nt16(dv + (int64_t)(c - u * step) * N, v[u]);
+            else Vec16<T>::store(dv + (int64_t)(c - u * step) * N, v[u]);
+        }
+    };
+    for (; c >= lo + (U - 1) * step; c -= U * step) group(c, std::integral_constant<int, U>{});
+    for (; c >= lo; c -= step) group(c, std::integral_constant<int, 1>{});
+}
+template <typename T>
+__device__ __forceinline__ void write_row(const T* __restrict__ xr, T* __restrict__ dr, int vocab, bool vec,
+                                          bool stream, RowThreads th, RowGrad grad) {
+    if (vec) {
+        const RowSpan<T> span(xr, vocab);
+        write_vecs<T, 4>(xr + span.head, dr + span.head, (int)span.nvec - 1 - th.self, th.count, 0, stream, grad);
+        const int64_t j = span.edge(th.self, vocab);
+        if (j >= 0) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
+    } else {
+        for (int64_t j = th.self; j < vocab; j += th.count) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
+    }
+}
+// The thread that stores element j: its vector's, its edge's, or its own where
+// the row goes one by one.
+template <int N> __device__ __forceinline__ int owner_of(int j, int head, int nvec, bool vec, int threads) {
+    if (!vec) return j % threads;
+    if (j < head) return j;
+    const int c = (j - head) / N;
+    return c < nvec ? (nvec - 1 - c) % threads : N + (j - head - nvec * N);
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_row(T* __restrict__ dr, int vocab, bool stream, RowThreads th) {
     constexpr int N = Vec16<T>::N;
     const RowSpan<T> span(dr, vocab);
     const float z[N] = {};
-    for (int c = threadIdx.x; c < (int)span.nvec; c += NT) {
+    for (int c = th.self; c < (int)span.nvec; c += th.count) {
         T* p = dr + span.head + (int64_t)c * N;
         if (stream) store_nt16(p, z);
         else Vec16<T>::store(p, z);
     }
-    const int64_t j = span.edge((int)threadIdx.x, vocab);
+    const int64_t j = span.edge(th.self, vocab);
     if (j >= 0) Elem<T>::store(dr, j, 0.f);
 }
 
@@ -650,12 +669,11 @@ template <int NT> struct TopOwners {
     __device__ __forceinline__ void clear(int top) {
         for (int i = threadIdx.x; i < (top + 31) / 32 * NT; i += NT) bits[i] = 0;
     }
-    // Thread k puts in entry k. A barrier before the patch.
-    template <int N, bool BACK>
-    __device__ __forceinline__ void insert(int id, int top, int head, int nvec, int vocab, bool vec) {
+    // Thread k puts in entry k, whose element the row's thread `owner` stores; the
+    // workgroup's own are from first on. A barrier before the patch.
+    __device__ __forceinline__ void insert(int owner, int first) {
         const int k = threadIdx.x;
-        if (k < top && (unsigned)id < (unsigned)vocab)
-            atomicOr(&bits[(k >> 5) * NT + owner_of<NT, N, BACK>(id, head, nvec, vec)], 1u << (k & 31));
+        if ((unsigned)(owner - first) < (unsigned)NT) atomicOr(&bits[(k >> 5) * NT + owner - first], 1u << (k & 31));
     }
     template <typename F> __device__ __forceinline__ void each(int top, F&& fn) const {
         for (int w = 0; w < (top + 31) / 32; ++w)
@@ -688,6 +706,7 @@ __global__ __launch_bounds__(NT) void lp_bwd_k(int64_t rows, int vocab, bool vec
                                                const float* __restrict__ dl, uint32_t seq,
                                                const float* __restrict__ scale, const float* __restrict__ dloss,
                                                T* __restrict__ dlogits) {
+    const RowThreads th = row_threads<NT>();
     const int64_t row = rows - 1 - (int64_t)blockIdx.x;
     T* dr = dlogits + row * vocab;
     const uint32_t t = targets[row];
@@ -699,16 +718,16 @@ __global__ __launch_bounds__(NT) void lp_bwd_k(int64_t rows, int vocab, bool vec
         if (t >= (uint32_t)vocab) g = __builtin_nanf("");
     }
     if (g == 0.f) {
-        zero_row<T, NT>(dr, vocab, stream);
+        zero_row(dr, vocab, stream, th);
         return;
     }
     g *= k.inv_t;
     const T* xr = logits + row * vocab;
     const RowGrad grad = row_grad(-g, stats[row], k.c_hi);
-    write_row<T, NT>(xr, dr, vocab, vec, stream, grad);
+    write_row(xr, dr, vocab, vec, stream, th, grad);
     const RowSpan<T> span(xr, vocab);
     if (t < (uint32_t)vocab &&
-        owner_of<NT, Vec16<T>::N, true>((int)t, (int)span.head, (int)span.nvec, vec) == (int)threadIdx.x)
+        owner_of<Vec16<T>::N>((int)t, (int)span.head, (int)span.nvec, vec, th.count) == th.self)
         Elem<T>::store(dr, t, grad(Elem<T>::load(xr, t)) + g);
 }
 
@@ -722,11 +741,12 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
     constexpr int N = Vec16<T>::N;
     __shared__ Teacher te;
     __shared__ TopOwners<NT> owners;
+    const RowThreads th = row_threads<NT>();
     const int64_t row = d.rows - 1 - (int64_t)blockIdx.x;
     const int vocab = (int)d.vocab;
     T* dr = dlogits + row * vocab;
     if (mask && mask[row] == 0) {
-        zero_row<T, NT>(dr, vocab, stream);
+        zero_row(dr, vocab, stream, th);
         return;
     }
     owners.clear(d.top);
@@ -738,18 +758,19 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
     entry.open(d, k.inv_t, te);
     const uint32_t x = entry.logit(xr, vocab);
     __syncthreads();
-    owners.template insert<N, true>(entry.id, d.top, (int)span.head, (int)span.nvec, vocab, vec);
+    if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab)
+        owners.insert(owner_of<N>(entry.id, (int)span.head, (int)span.nvec, vec, th.count), (int)(blockIdx.y * NT));
     entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
     __syncthreads();
     const TeacherSums ts = entry.sums(d, te);
     float w = scale[0] * (dloss ? dloss[0] : 1.f);
     if (ts.bad) w = __builtin_nanf("");
     if (ts.P == 0.f || w == 0.f) {
-        zero_row<T, NT>(dr, vocab, stream);
+        zero_row(dr, vocab, stream, th);
         return;
     }
     const RowGrad grad = row_grad(w * ts.P, v, k.c_hi);
-    write_row<T, NT>(xr, dr, vocab, vec, stream, grad);
+    write_row(xr, dr, vocab, vec, stream, th, grad);
     owners.patch(te, d.top, dr, grad, w);
 }
 
@@ -763,11 +784,20 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
 // threads, as their bits.
 // Nothing is loaded under a condition, or every wait would be for the path with
 // the fewest loads, that is for all of them.
-template <typename T, int NT, int NV> struct HeldRow {
+// REST: rows of any length. What lies past NT NV vectors is read twice, its end,
+// which the cache still has, first.
+template <typename T, int NT, int NV, bool REST> struct HeldRow {
+    // The thread whose vector, or edge, element j is in.
+    __device__ __forceinline__ int owner(int at) const {
+        if (at < head) return at;
+        const int c = (at - head) / N;
+        return c < nvec ? c & (NT - 1) : N + (at - head - nvec * N);
+    }
     static constexpr int N = Vec16<T>::N, G = 16 / N;  // vectors reduced at a time
     i32x4 q[NV];
     uint32_t edge;
     int head, nvec, j;  // j: the edge element, or -1
+    const T* xv;        // the first vector
 
     __device__ __forceinline__ void load(const T* __restrict__ xr, int vocab) {
         const RowSpan<T> span(xr, vocab);
@@ -775,7 +805,8 @@ template <typename T, int NT, int NV> struct HeldRow {
         nvec = (int)span.nvec;
         j = (int)span.edge((int)threadIdx.x, vocab);
         edge = raw_load(xr, j < 0 ? 0 : j);
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(xr + head, (int64_t)nvec * 16);
+        xv = xr + head;
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(xv, (int64_t)(REST ? NT * NV : nvec) * 16);
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
             __builtin_amdgcn_sched_barrier(0);  // in the order of their use
@@ -787,14 +818,14 @@ template <typename T, int NT, int NV> struct HeldRow {
         float m = kNegInf, s = 0.f;
 #pragma unroll
         for (int u0 = 0; u0 < NV; u0 += G) {
-            if (u0 * NT >= nvec) break;
+            if (!REST && u0 * NT >= nvec) break;
             float v[G][N];
             float vm = kNegInf;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const int u = u0 + g;
                 if (u < NV) BVec<T>::unpack(q[u], v[g]);
-                if (u >= NV || ((u + 1) * NT > nvec && u * NT + (int)threadIdx.x >= nvec)) {
+                if (u >= NV || (!REST && (u + 1) * NT > nvec && u * NT + (int)threadIdx.x >= nvec)) {
 #pragma unroll
                     for (int e = 0; e < N; ++e) v[g][e] = kNegInf;
                 }
@@ -815,20 +846,26 @@ template <typename T, int NT, int NV> struct HeldRow {
             }
             s += G == 4 ? (ps[0] + ps[1]) + (ps[G - 2] + ps[G - 1]) : ps[0] + ps[1];
         }
+        Stat<float> st{m, s};
+        if constexpr (REST)
+            st = stat_join(st, vec_stat<T, NT, float, G>(xv, NT * NV + (int)threadIdx.x, nvec, k), k.c_hi);
         if (j >= 0) {
             const float x = from_raw<T>(edge);
-            return stat_join(Stat<float>{m, s}, Stat<float>{x, term_of(x, base_of(x), k)}, k.c_hi);
+            st = stat_join(st, Stat<float>{x, term_of(x, base_of(x), k)}, k.c_hi);
         }
-        return Stat<float>{m, s};
+        return st;
     }
     // into the gradient's row dr, which starts like the logits'
     __device__ __forceinline__ void store(T* __restrict__ dr, bool stream, RowGrad grad) const {
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(dr + head, (int64_t)nvec * 16);
+        if constexpr (REST)
+            write_vecs<T, G>(xv, dr + head, (int)threadIdx.x + (nvec - 1 - (int)threadIdx.x) / NT * NT, NT, NT * NV,
+                             stream, grad);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(dr + head, (int64_t)(REST ? NT * NV : nvec) * 16);
         uint32_t at = threadIdx.x * 16u;
         asm volatile("" : "+v"(at));  // or the loads' NV offsets are held for the stores
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            if (u * NT >= nvec) break;
+            if (!REST && u * NT >= nvec) break;
             float v[N];
             BVec<T>::unpack(q[u], v);
 #pragma unroll
@@ -892,7 +929,7 @@ template <int NT> struct RowCount {
 // to the tokens that share the weight (by_seq: of each sequence, one number
 // each), or null: counted here over len targets. n (may be null): receives the
 // sequences' counts.
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool REST>
 __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool stream, const T* __restrict__ logits,
                                                        const uint32_t* __restrict__ targets,
                                                        const float* __restrict__ adv, const float* __restrict__ old,
@@ -904,6 +941,7 @@ __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool st
                                                        T* __restrict__ dlogits, uint32_t* __restrict__ counter) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ uint32_t redc[NT / 64];
+    const RowThreads th{(int)threadIdx.x, NT};
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
     if (row == 0 && threadIdx.x == 0) *counter = 0;
@@ -911,7 +949,7 @@ __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool st
     const uint32_t t = targets[row];
     if (!counted(t, d.ignore_index)) {
         if (threadIdx.x == 0) logp[row] = 0.f;
-        zero_row<T, NT>(dr, vocab, stream);
+        zero_row(dr, vocab, stream, th);
         return;
     }
     const T* xr = logits + row * vocab;
@@ -923,7 +961,7 @@ __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool st
     const uint32_t* cw = by_seq ? targets + (int64_t)q * d.seq : targets;
     RowCount<NT> count;
     count.load(len, [&](int i) { return cw[i]; });
-    HeldRow<T, NT, NV> held;
+    HeldRow<T, NT, NV, REST> held;
     held.load(xr, vocab);
     count.put(len, redc, [&](uint32_t w) { return counted(w, d.ignore_index); });
     const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
@@ -936,19 +974,19 @@ __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool st
     }
     float g = policy_term(d, l, pin).dl / (by_seq ? (float)d.batch * (float)share : (float)share) * up;
     if (g == 0.f) {
-        zero_row<T, NT>(dr, vocab, stream);
+        zero_row(dr, vocab, stream, th);
         return;
     }
     g *= k.inv_t;
     const RowGrad grad = row_grad(-g, v, k.c_hi);
     held.store(dr, stream, grad);
-    if (in && owner_of<NT, Vec16<T>::N, false>((int)t, held.head, held.nvec, true) == (int)threadIdx.x)
+    if (in && held.owner((int)t) == (int)threadIdx.x)
         Elem<T>::store(dr, t, grad(from_raw<T>(xt)) + g);
 }
 
 // given: n_given counts of the mask, or null: counted here over len of it (0
 // without a mask).
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool REST>
 __global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool stream, const T* __restrict__ logits,
                                                         const int32_t* __restrict__ ids, const float* __restrict__ tl,
                                                         const float* __restrict__ tlse,
@@ -957,18 +995,18 @@ __global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool 
                                                         LpScale k, const float* __restrict__ dloss,
                                                         float* __restrict__ kl,
                                                         T* __restrict__ dlogits, uint32_t* __restrict__ counter) {
-    constexpr int N = Vec16<T>::N;
     __shared__ Stat<float> red[NT / 64];
     __shared__ uint32_t redc[NT / 64];
     __shared__ Teacher te;
     __shared__ TopOwners<NT> owners;
+    const RowThreads th{(int)threadIdx.x, NT};
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
     if (row == 0 && threadIdx.x == 0) *counter = 0;
     T* dr = dlogits + row * vocab;
     if (mask && mask[row] == 0) {
         if (threadIdx.x == 0) kl[row] = 0.f;
-        zero_row<T, NT>(dr, vocab, stream);
+        zero_row(dr, vocab, stream, th);
         return;
     }
     const T* xr = logits + row * vocab;
@@ -981,11 +1019,11 @@ __global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool 
     RowCount<NT> count;
     const uint8_t* cw = mask ? mask : reinterpret_cast<const uint8_t*>(xr);
     count.load(len, [&](int i) { return (uint32_t)cw[i]; });
-    HeldRow<T, NT, NV> held;
+    HeldRow<T, NT, NV, REST> held;
     held.load(xr, vocab);
     count.put(len, redc, [](uint32_t w) { return w != 0; });
     entry.open(d, k.inv_t, te);
-    owners.template insert<N, false>(entry.id, d.top, held.head, held.nvec, vocab, true);
+    if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab) owners.insert(held.owner(entry.id), 0);
     const uint32_t x = entry.logit(xr, vocab);
     const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
     const RowStat v{st.m, st.s};
@@ -996,7 +1034,7 @@ __global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool 
     if (threadIdx.x == 0) kl[row] = ts.kl;
     if (ts.bad) w = __builtin_nanf("");
     if (ts.P == 0.f || w == 0.f) {
-        zero_row<T, NT>(dr, vocab, stream);
+        zero_row(dr, vocab, stream, th);
         return;
     }
     const RowGrad grad = row_grad(w * ts.P, v, k.c_hi);
@@ -1018,40 +1056,47 @@ LpScale row_scale(float temperature) {
 }
 
 // fn(element type, threads per row)
-template <typename F>
-hipError_t by_row_kernel(int64_t rows, int64_t vocab, int dtype, F&& fn) {
+template <typename F> void by_threads(int threads, int dtype, F&& fn) {
     auto by_dtype = [&](auto threads) {
         if (dtype == MC_F32) fn(float{}, threads);
         else fn(uint16_t{}, threads);
     };
-    if (xent_wide_rows(rows, vocab, dtype == MC_F32 ? 4 : 2)) by_dtype(std::integral_constant<int, 1024>{});
-    else by_dtype(std::integral_constant<int, 256>{});
-    return hipGetLastError();
+    switch (threads) {
+        case 64: return by_dtype(std::integral_constant<int, 64>{});
+        case 128: return by_dtype(std::integral_constant<int, 128>{});
+        case 512: return by_dtype(std::integral_constant<int, 512>{});
+        case 1024: return by_dtype(std::integral_constant<int, 1024>{});
+        default: return by_dtype(std::integral_constant<int, 256>{});
+    }
 }
+int64_t row_bytes(int64_t vocab, int dtype) { return vocab * (dtype == MC_F32 ? 4 : 2); }
 
-// fn(element type, threads, vectors per thread) for the smallest shape that holds
-// a row; false where none does.
-template <typename F>
-bool by_held_shape(int64_t vocab, int dtype, F&& fn) {
+// fn(element type, HeldShape) for the smallest shape of at least MIN threads that
+// holds a row, or the largest with the rest of the row read twice.
+template <int NT, int NV, bool REST> struct HeldShape {
+    static constexpr int kThreads = NT, kVectors = NV;
+    static constexpr bool kRest = REST;
+};
+template <int MIN, typename F> void by_held_shape(int64_t vocab, int dtype, F&& fn) {
     auto go = [&](auto elem) {
-        typedef decltype(elem) T;
-        const int64_t vectors = vocab / Vec16<T>::N;
-        auto shape = [&](auto threads, auto held) {
-            if (vectors > decltype(threads)::value * decltype(held)::value) return false;
-            fn(elem, threads, held);
-            return true;
+        const int64_t vectors = vocab / Vec16<decltype(elem)>::N;
+        auto shape = [&](auto s) {
+            typedef decltype(s) S;
+            if constexpr (S::kThreads >= MIN) {
+                if (!S::kRest && vectors > S::kThreads * S::kVectors) return false;
+                fn(elem, s);
+                return true;
+            }
+            return false;
         };
-        using std::integral_constant;
-        return shape(integral_constant<int, 256>{}, integral_constant<int, 4>{}) ||
-               shape(integral_constant<int, 256>{}, integral_constant<int, 8>{}) ||
-               shape(integral_constant<int, 512>{}, integral_constant<int, 8>{}) ||
-               shape(integral_constant<int, 512>{}, integral_constant<int, 16>{}) ||
-               shape(integral_constant<int, 1024>{}, integral_constant<int, 10>{}) ||
-               shape(integral_constant<int, 1024>{}, integral_constant<int, 13>{}) ||
-               shape(integral_constant<int, 1024>{}, integral_constant<int, 16>{}) ||
-               shape(integral_constant<int, 1024>{}, integral_constant<int, 19>{});
+        shape(HeldShape<64, 4, false>{}) || shape(HeldShape<128, 8, false>{}) || shape(HeldShape<256, 4, false>{}) ||
+            shape(HeldShape<512, 4, false>{}) || shape(HeldShape<512, 8, false>{}) ||
+            shape(HeldShape<512, 13, false>{}) || shape(HeldShape<512, 19, false>{}) ||
+            shape(HeldShape<1024, 13, false>{}) || shape(HeldShape<1024, 16, false>{}) ||
+            shape(HeldShape<1024, 19, false>{}) || shape(HeldShape<1024, 16, true>{});
     };
-    return dtype == MC_F32 ? go(float{}) : go(uint16_t{});
+    if (dtype == MC_F32) go(float{});
+    else go(uint16_t{});
 }
 
 bool same_start(const void* a, const void* b) {
@@ -1080,13 +1125,14 @@ template <typename L>
 hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, L* logp, float* stats,
                           uint32_t* counter, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
-    return by_row_kernel(d.rows, d.vocab, d.dtype, [&](auto elem, auto threads) {
+    by_threads(loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype)), d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
         lp_rows_k<T, NT><<<dim3((unsigned)d.rows), NT, 0, stream>>>((int)d.vocab, static_cast<const T*>(logits),
                                                                     targets, d.ignore_index, k, logp,
                                                                     reinterpret_cast<RowStat*>(stats), counter);
     });
+    return hipGetLastError();
 }
 }  // namespace
 
@@ -1100,14 +1146,16 @@ hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logit
                                      const float* dloss, void* dlogits, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
     const bool vec = same_start(logits, dlogits);
-    return by_row_kernel(d.rows, d.vocab, d.dtype, [&](auto elem, auto threads) {
+    const LossGrid grid = loss_grad_grid(d.rows, row_bytes(d.vocab, d.dtype));
+    by_threads(grid.threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
-        lp_bwd_k<T, NT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
+        lp_bwd_k<T, NT><<<dim3((unsigned)d.rows, grid.parts), NT, 0, stream>>>(
             d.rows, (int)d.vocab, vec, xent_stream_gradients(d.rows, d.vocab, sizeof(T)),
             static_cast<const T*>(logits), targets, d.ignore_index, k,
             reinterpret_cast<const RowStat*>(stats), dl, (uint32_t)seq, scale, dloss, static_cast<T*>(dlogits));
     });
+    return hipGetLastError();
 }
 
 PreferenceWs preference_ws(const mc_preference_desc& d) {
@@ -1223,13 +1271,16 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
     const LpScale k = row_scale(d.temperature);
     uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     float* kl = reinterpret_cast<float*>(ws + w.kl);
-    hipError_t e = by_row_kernel(d.rows, d.vocab, d.dtype, [&](auto elem, auto threads) {
+    const int threads = loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype));
+    by_threads(threads < kDistillMaxTop ? kDistillMaxTop : threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
-        distill_rows_k<T, NT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(d, static_cast<const T*>(logits), ids, tl,
-                                                                         tlse, mask, k, kl,
-                                                                         reinterpret_cast<RowStat*>(stats), counter);
+        if constexpr (NT >= kDistillMaxTop)  // a thread per entry
+            distill_rows_k<T, NT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
+                d, static_cast<const T*>(logits), ids, tl, tlse, mask, k, kl, reinterpret_cast<RowStat*>(stats),
+                counter);
     });
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     return launch_distill_sums(d, mask, kl, ws, loss, stats ? stats + 2 * d.rows : nullptr, stream);
 }
@@ -1239,13 +1290,17 @@ hipError_t launch_distill_bwd(const mc_distill_desc& d, const void* logits, cons
                               void* dlogits, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
     const bool vec = same_start(logits, dlogits);
-    return by_row_kernel(d.rows, d.vocab, d.dtype, [&](auto elem, auto threads) {
+    const LossGrid grid = loss_grad_grid(d.rows, row_bytes(d.vocab, d.dtype));
+    by_threads(grid.threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
-        distill_bwd_k<T, NT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
-            d, vec, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl, tlse,
-            mask, k, reinterpret_cast<const RowStat*>(stats), stats + 2 * d.rows, dloss, static_cast<T*>(dlogits));
+        if constexpr (NT >= kDistillMaxTop)
+            distill_bwd_k<T, NT><<<dim3((unsigned)d.rows, grid.parts), NT, 0, stream>>>(
+                d, vec, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl,
+                tlse, mask, k, reinterpret_cast<const RowStat*>(stats), stats + 2 * d.rows, dloss,
+                static_cast<T*>(dlogits));
     });
+    return hipGetLastError();
 }
 
 // counts_k over rows into ws; the number of its blocks
@@ -1274,21 +1329,22 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
     const int64_t rows = d.batch * d.seq;
     const LpScale k = row_scale(d.temperature);
     hipError_t e;
-    if (same_start(logits, dlogits) && by_held_shape(d.vocab, d.dtype, [](auto, auto, auto) {})) {
+    if (same_start(logits, dlogits) && loss_threads_fit(rows, 1024)) {
         uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         const bool by_seq = d.reduction == MC_MEAN_SEQUENCES;
         uint32_t* n = by_seq ? reinterpret_cast<uint32_t*>(ws + w.counts) : nullptr;
-        by_held_shape(d.vocab, d.dtype, [&](auto elem, auto threads, auto held) {
+        by_held_shape<64>(d.vocab, d.dtype, [&](auto elem, auto shape) {
             typedef decltype(elem) T;
-            constexpr int NT = decltype(threads)::value, NV = decltype(held)::value;
+            typedef decltype(shape) S;
+            constexpr int NT = S::kThreads;
             const int64_t span = by_seq ? d.seq : rows;
             const bool here = span <= RowCount<NT>::kPer * NT;
             int n_given = 1;
             e = hipSuccess;
             if (!here && by_seq) policy_counts(d, targets, ws, stream, e);
             else if (!here) n_given = launch_counts(rows, targets, nullptr, d.ignore_index, part, stream);
-            policy_held_k<T, NT, NV><<<dim3((unsigned)rows), NT, 0, stream>>>(
+            policy_held_k<T, NT, S::kVectors, S::kRest><<<dim3((unsigned)rows), NT, 0, stream>>>(
                 d, xent_stream_gradients(rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), targets, adv, old,
                 ref, here ? nullptr : by_seq ? n : part, n_given, here ? (int)span : 0, by_seq, here ? n : nullptr, k,
                 dloss, logp, static_cast<T*>(dlogits), counter);
@@ -1314,16 +1370,17 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
     float* stats = reinterpret_cast<float*>(ws + w.total);
     const LpScale k = row_scale(d.temperature);
     hipError_t e;
-    if (same_start(logits, dlogits) && by_held_shape(d.vocab, d.dtype, [](auto, auto, auto) {})) {
+    if (same_start(logits, dlogits) && loss_threads_fit(d.rows, 1024)) {
         uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
         float* kl = reinterpret_cast<float*>(ws + w.kl);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
-        by_held_shape(d.vocab, d.dtype, [&](auto elem, auto threads, auto held) {
+        by_held_shape<256>(d.vocab, d.dtype, [&](auto elem, auto shape) {
             typedef decltype(elem) T;
-            constexpr int NT = decltype(threads)::value, NV = decltype(held)::value;
+            typedef decltype(shape) S;
+            constexpr int NT = S::kThreads;
             const bool here = !mask || d.rows <= RowCount<NT>::kPer * NT;
             const int n_given = here ? 0 : launch_counts(d.rows, nullptr, mask, -1, part, stream);
-            distill_held_k<T, NT, NV><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
+            distill_held_k<T, NT, S::kVectors, S::kRest><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
                 d, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl, tlse,
                 mask, here ? nullptr : part, n_given, mask && here ? (int)d.rows : 0, k, dloss, kl,
                 static_cast<T*>(dlogits), counter);

@@ -40,6 +40,48 @@ constexpr bool xent_stream_gradients(int64_t rows, int64_t vocab, int elem_size)
     return rows * vocab * elem_size > (int64_t)64 << 20;
 }
 
+// The losses over log-probabilities (losses.hip). One launch holds at most
+// 2^32 - 1 work-items.
+constexpr bool loss_threads_fit(int64_t rows, int threads) { return rows <= (((int64_t)1 << 32) - 1) / threads; }
+
+// Threads that read a row of logits for its statistics. Short rows leave most
+// threads of a large workgroup without a vector; of long ones few large
+// workgroups keep fewer rows open, once every CU has several. us, 64 / 128 / 256 /
+// 512 / 1024 threads:
+//   2 KB rows, 16384     14.3 / 19.2 / 28.7 / 52.1
+//   8 KB rows, 16384     29.4 / 31.4 / 38.1 / 57.4
+//   16 KB rows, 8192     32.7 / 31.6 / 33.8 / 47.6
+//   32 KB rows, 4000     30.8 / 29.7 / 30.5 / 34.0
+//   64 KB rows, 2000     26.8 / 28.2 / 28.4 / 28.0
+//   98 KB rows, 3624              256 70.2 / 65.3 / 78.4
+//   201 KB rows, 1511             256 59.6 / 57.6 / 55.2
+//   304 KB rows, 64 18.2 / 13.7 / 13.6; 256 19.4 / 15.1 / 16.6; 400 28.3 / 26.7 / 28.8;
+//                1200 68.6 / 66.3 / 65.6; 3024 165 / 165 / 156
+constexpr int loss_row_threads(int64_t rows, int64_t row_bytes) {
+    if (row_bytes < 4 << 10) return 64;
+    if (row_bytes < 24 << 10) return 128;
+    if (row_bytes < 64 << 10 || !loss_threads_fit(rows, 1024)) return 256;
+    return row_bytes < 192 << 10 || rows < 768 ? 512 : 1024;
+}
+
+// Threads that write a row's gradient, and workgroups that share a row where
+// there are too few rows for the CUs. us, right behind a forward (64 rows: alone),
+// 256 / 512 / 1024 threads:
+//   8 KB rows, 16384   95.0 / 94.4 / 98.1      16 KB rows, 8192   84.4 / 82.9 / 82.3
+//   64 KB rows, 2000   68.3 / 66.7 / 65.9      98 KB rows, 4816   220 / 208 / 200
+//   201 KB rows, 2036  194 / 182 / 172         304 KB rows, 2036  294 / 278 / 267
+//   304 KB rows, 64    33.7 / 19.6 / 12.2
+struct LossGrid {
+    int threads;
+    unsigned parts;
+};
+constexpr LossGrid loss_grad_grid(int64_t rows, int64_t row_bytes) {
+    if (row_bytes < 16 << 10 || !loss_threads_fit(rows, 1024)) return LossGrid{256, 1};
+    const int64_t most = (row_bytes + (16 << 10) - 1) / (16 << 10);  // a vector per thread
+    const int64_t wanted = rows >= 256 ? 1 : (512 + rows - 1) / rows;
+    return LossGrid{1024, (unsigned)(wanted < most ? wanted : most)};
+}
+
 // Softmax rows that are not whole 16-byte vectors: the covering vectors of the
 // one-wave kernels, or for short rows a lane per element (the scalar kernels),
 // where the vectors keep only a few lanes busy and pay for the shared edges.

@@ -382,8 +382,10 @@ typedef struct mc_logprob_desc {
     int32_t dtype;         /* mc_dtype of logits and dlogits */
 } mc_logprob_desc;
 
+size_t mc_token_logprobs_workspace_size(const mc_logprob_desc* d);  /* may be 0: then workspace may be NULL */
+
 mc_status mc_token_logprobs_fwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets, float* logps,
-                                float* stats, hipStream_t stream);
+                                float* stats, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* dlogits = dlogps ([j = target] - softmax(x / T)) / T; dlogps fp32 [rows]. */
 mc_status mc_token_logprobs_bwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets,

@@ -219,7 +219,8 @@ _SIGNATURES = {
     "mc_cross_entropy_workspace_size": (_sz, [ctypes.POINTER(XentDesc)]),
     "mc_cross_entropy_fwd": (ctypes.c_int, [ctypes.POINTER(XentDesc), _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mc_cross_entropy_bwd": (ctypes.c_int, [ctypes.POINTER(XentDesc), _vp, _vp, _vp, _vp, _vp, _vp]),
-    "mc_token_logprobs_fwd": (ctypes.c_int, [_lp, _vp, _vp, _vp, _vp, _vp]),
+    "mc_token_logprobs_workspace_size": (_sz, [_lp]),
+    "mc_token_logprobs_fwd": (ctypes.c_int, [_lp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mc_token_logprobs_bwd": (ctypes.c_int, [_lp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mc_preference_loss_workspace_size": (_sz, [_rp]),
     "mc_preference_loss_fwd": (ctypes.c_int, [_rp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),

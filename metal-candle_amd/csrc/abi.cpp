@@ -767,14 +767,20 @@ static mc_status check_logprob(const mc_logprob_desc* d) {
     return s != MC_OK ? s : check_temperature("token_logprobs", d->temperature);
 }
 
+size_t mc_token_logprobs_workspace_size(const mc_logprob_desc* d) {
+    return check_logprob(d) == MC_OK ? mc::loss_parts_ws(d->rows, d->vocab, d->dtype) : 0;
+}
+
 mc_status mc_token_logprobs_fwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets, float* logps,
-                                float* stats, hipStream_t stream) {
+                                float* stats, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     mc_status s = check_logprob(d);
     if (s != MC_OK) return s;
     MC_CHECK(logits && targets && logps, MC_ERR_NULL, "token_logprobs: logits, targets and logps must not be NULL");
     if ((s = check_logits("token_logprobs", d->dtype, logits, nullptr)) != MC_OK) return s;
+    const size_t need = mc::loss_parts_ws(d->rows, d->vocab, d->dtype);
+    if (need && (s = check_workspace("token_logprobs", workspace, workspace_bytes, need)) != MC_OK) return s;
     mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 1.0));
-    return hip_status(mc::launch_token_logprobs_fwd(*d, logits, targets, logps, stats, stream),
+    return hip_status(mc::launch_token_logprobs_fwd(*d, logits, targets, logps, stats, workspace, stream),
                       "token_logprobs forward");
 }
 

@@ -211,8 +211,11 @@ struct RowStat {
     float m, s;
 };
 constexpr int kDistillMaxTop = MC_DISTILL_MAX_TOP;  // a teacher's entries per row: one per thread
+// Bytes for the statistics of rows that several workgroups share; 0 where one does.
+size_t loss_parts_ws(int64_t rows, int64_t vocab, int dtype);
+// ws: loss_parts_ws bytes
 hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
-                                     float* stats, hipStream_t stream);
+                                     float* stats, void* ws, hipStream_t stream);
 // dl: dloss/dl per row, or per sequence of seq rows where seq > 0; times scale[0] and dloss[0] (each may be null).
 hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
                                      const float* stats, const float* dl, int64_t seq, const float* scale,
@@ -222,16 +225,19 @@ struct PreferenceWs {
     size_t logp;   // f64 [2 pairs seq]
     size_t score;  // f64 [2 pairs]
     size_t inv_n;  // f32 [2 pairs]
+    size_t parts;  // loss_parts_ws
     size_t total;
 };
 struct PolicyWs {
     size_t part;    // f64 [256][4] sums
     size_t counts;  // u32 [batch] counted tokens, where the mean runs over sequences
+    size_t parts;   // loss_parts_ws
     size_t total;
 };
 struct DistillWs {
-    size_t part;  // f64 [256][2] sums
-    size_t kl;    // f32 [rows]
+    size_t part;   // f64 [256][2] sums
+    size_t kl;     // f32 [rows]
+    size_t split;  // loss_parts_ws
     size_t total;
 };
 PreferenceWs preference_ws(const mc_preference_desc& d);

@@ -121,36 +121,54 @@ __device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int
     for (; c < nvec; c += NT) group(c, std::integral_constant<int, 1>{});
     return Stat<S>{m, s};
 }
-template <typename T, int NT, typename S>
-__device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
-    const RowSpan<T> span(xr, vocab);
-    const Stat<S> st = vec_stat<T, NT, S, 4>(xr + span.head, threadIdx.x, (int)span.nvec, k);
-    static_assert(NT >= 2 * Vec16<T>::N, "a thread per edge element");
+// with the thread's element of the row's edges, if it has one
+template <typename T, typename S>
+__device__ __forceinline__ Stat<S> edge_stat(const T* __restrict__ xr, int vocab, const RowSpan<T>& span, Stat<S> st,
+                                             LpScale k) {
     const int64_t j = span.edge((int)threadIdx.x, vocab);
     if (j < 0) return st;
     const float v = Elem<T>::load(xr, j);
     return stat_join(st, Stat<S>{v, (S)term_of(v, base_of(v), k)}, k.c_hi);
 }
+template <typename T, int NT, typename S>
+__device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
+    static_assert(NT >= 2 * Vec16<T>::N, "a thread per edge element");
+    const RowSpan<T> span(xr, vocab);
+    return edge_stat(xr, vocab, span, vec_stat<T, NT, S, 4>(xr + span.head, threadIdx.x, (int)span.nvec, k), k);
+}
 
 // -------------------------------------------------- sums over many workgroups
 // Each workgroup leaves its partial sums in memory; the last one to arrive adds
 // them in workgroup order. The kernel before on the stream clears the counter.
-template <int C>
-__device__ __forceinline__ void wg_sum_f64(double (&v)[C], double (*red)[C]) {
+template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// wave_sum's steps in 64 bits
+__device__ __forceinline__ double wave_sum(double v) {
+    v += dpp64<0xB1>(v);
+    v += dpp64<0x4E>(v);
+    v += dpp64<0x141>(v);
+    v += dpp64<0x140>(v);
+    v += __shfl_xor(v, 16, kWave);
+    v += __shfl_xor(v, 32, kWave);
+    return v;
+}
+template <int NT, int C> __device__ __forceinline__ void wg_sum_f64(double (&v)[C], double (*red)[C]) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) v[c] += __shfl_xor(v[c], o, kWave);
+    for (int c = 0; c < C; ++c) v[c] = wave_sum(v[c]);
     __syncthreads();
     if (lane_id() == 0)
 #pragma unroll
         for (int c = 0; c < C; ++c) red[threadIdx.x >> 6][c] = v[c];
     __syncthreads();
-    const int nw = (int)(blockDim.x >> 6);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         v[c] = red[0][c];
-        for (int w = 1; w < nw; ++w) v[c] += red[w][c];
+#pragma unroll
+        for (int w = 1; w < NT / 64; ++w) v[c] += red[w][c];
     }
 }
 
@@ -171,15 +189,42 @@ __device__ __forceinline__ bool counted(uint32_t t, int64_t ignore_index) {
     return !(ignore_index >= 0 && (int64_t)t == ignore_index);
 }
 
-// l (0 where the row is not counted) and the row's statistics; a counted target
-// past the vocabulary makes its l NaN. counter: cleared for the kernel that
-// follows.
-// L: float, or double for sums over answers.
-template <typename T, int NT, typename L>
+// Few rows do not fill the CUs, and one CU reads about 30 bytes a ns: then
+// gridDim.y workgroups take a share of a row's vectors each, and the kernel that
+// follows joins their statistics.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void parts_k(int vocab, const T* __restrict__ logits,
+                                              const uint32_t* __restrict__ targets, int64_t ignore_index,
+                                              const uint8_t* __restrict__ mask, LpScale k,
+                                              Stat<double>* __restrict__ part) {
+    __shared__ Stat<double> red[NT / 64];
+    const int64_t row = blockIdx.x;
+    if (targets ? !counted(targets[row], ignore_index) : mask && mask[row] == 0) return;
+    const T* xr = logits + row * vocab;
+    const RowSpan<T> span(xr, vocab);
+    const int share = ((int)span.nvec + (int)gridDim.y - 1) / (int)gridDim.y, lo = (int)blockIdx.y * share;
+    const int hi = lo + share < (int)span.nvec ? lo + share : (int)span.nvec;
+    Stat<double> st = vec_stat<T, NT, double, 4>(xr + span.head, lo + (int)threadIdx.x, hi, k);
+    if (blockIdx.y == 0) st = edge_stat(xr, vocab, span, st, k);
+    st = wg_stat<NT>(st, k.c_hi, red);
+    if (threadIdx.x == 0) part[row * gridDim.y + blockIdx.y] = st;
+}
+// The thread's part of a row, for wg_stat.
+__device__ __forceinline__ Stat<double> own_part(const Stat<double>* __restrict__ part, int64_t row, int parts) {
+    return (int)threadIdx.x < parts ? part[row * parts + threadIdx.x] : Stat<double>{kNegInf, 0.0};
+}
+
+__device__ __forceinline__ Stat<float> float_stat(Stat<double> v) { return Stat<float>{v.m, (float)v.s}; }
+
+// l (0 where the row is not counted) and the row's statistics, read from the
+// logits or (SPLIT) joined from its parts; a counted target past the vocabulary
+// makes its l NaN. counter: cleared for the kernel that follows. L: float, or
+// double for sums over answers.
+template <typename T, int NT, typename L, bool SPLIT>
 __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__ logits,
                                                 const uint32_t* __restrict__ targets, int64_t ignore_index, LpScale k,
-                                                L* __restrict__ logp, RowStat* __restrict__ stats,
-                                                uint32_t* __restrict__ counter) {
+                                                const Stat<double>* __restrict__ part, int parts, L* __restrict__ logp,
+                                                RowStat* __restrict__ stats, uint32_t* __restrict__ counter) {
     __shared__ Stat<double> red[NT / 64];
     const int64_t row = blockIdx.x;
     if (counter && row == 0 && threadIdx.x == 0) *counter = 0;
@@ -192,10 +237,14 @@ __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__
         return;
     }
     const T* xr = logits + row * vocab;
-    const Stat<double> v = wg_stat<NT>(row_stat<T, NT, double>(xr, vocab, k), k.c_hi, red);
+    const uint32_t xt = raw_load(xr, t < (uint32_t)vocab ? t : 0);
+    Stat<double> v;
+    if constexpr (SPLIT) v = own_part(part, row, parts);
+    else v = row_stat<T, NT, double>(xr, vocab, k);
+    v = wg_stat<NT>(v, k.c_hi, red);
     if (threadIdx.x == 0) {
-        const double d = (double)(t < (uint32_t)vocab ? Elem<T>::load(xr, t) : __builtin_nanf("")) - (double)v.m;
-        logp[row] = (L)(d * k.inv_t64 - log(v.s));
+        const double x = t < (uint32_t)vocab ? from_raw<T>(xt) : __builtin_nanf("");
+        logp[row] = (L)((x - (double)v.m) * k.inv_t64 - log(v.s));
         if (stats) stats[row] = RowStat{v.m, (float)v.s};
     }
 }
@@ -269,29 +318,27 @@ __device__ __forceinline__ void preference_pairs(const mc_preference_desc& d, co
             dseq[d.pairs + i] = (float)(-dd / pairs * (double)inv_n[d.pairs + i]);
         }
     }
-    wg_sum_f64<2>(sum, red);
+    wg_sum_f64<NT>(sum, red);
     if (threadIdx.x == 0) loss[0] = (float)(sum[0] / pairs);
 }
 
 // All in one workgroup, a wave per sequence (kOneGroupRows).
-__global__ __launch_bounds__(1024) void preference_one_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
-                                                         const double* __restrict__ logp,
-                                                         const float* __restrict__ ref, double* __restrict__ score,
-                                                         float* __restrict__ inv_n, float* __restrict__ loss,
-                                                         float* __restrict__ rewards, float* __restrict__ dseq) {
-    __shared__ double red[16][2];
-    for (int64_t q = wave_id(); q < 2 * d.pairs; q += 16) {
+template <int NT>
+__global__ __launch_bounds__(NT) void preference_one_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
+                                                       const double* __restrict__ logp, const float* __restrict__ ref,
+                                                       double* __restrict__ score, float* __restrict__ inv_n,
+                                                       float* __restrict__ loss, float* __restrict__ rewards,
+                                                       float* __restrict__ dseq) {
+    __shared__ double red[NT / 64][2];
+    for (int64_t q = wave_id(); q < 2 * d.pairs; q += NT / 64) {
         double v[2] = {0.0, 0.0};
         preference_sum(d, q, lane_id(), kWave, targets, logp, ref, v);
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            v[0] += __shfl_xor(v[0], o, kWave);
-            v[1] += __shfl_xor(v[1], o, kWave);
-        }
+        v[0] = wave_sum(v[0]);
+        v[1] = wave_sum(v[1]);
         if (lane_id() == 0) preference_score(d, q, v[0], v[1], score, inv_n, rewards);
     }
     __syncthreads();
-    preference_pairs<1024>(d, score, inv_n, red, loss, dseq);
+    preference_pairs<NT>(d, score, inv_n, red, loss, dseq);
 }
 
 // A workgroup per sequence; the last to arrive goes on to the pairs.
@@ -305,7 +352,7 @@ __global__ __launch_bounds__(256) void preference_k(mc_preference_desc d, const 
     const int64_t q = blockIdx.x;
     double v[2] = {0.0, 0.0};
     preference_sum(d, q, (int)threadIdx.x, 256, targets, logp, ref, v);
-    wg_sum_f64<2>(v, red);
+    wg_sum_f64<256>(v, red);
     if (threadIdx.x == 0) preference_score(d, q, v[0], v[1], score, inv_n, rewards);
     if (!last_to_arrive(counter, &slot)) return;
     preference_pairs<256>(d, score, inv_n, red, loss, dseq);
@@ -406,7 +453,7 @@ __global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, 
             if (dlp) dlp[row] = dl;
         }
     }
-    wg_sum_f64<4>(v, red);
+    wg_sum_f64<NT>(v, red);
     if (gridDim.x > 1) {
         if (threadIdx.x == 0)
 #pragma unroll
@@ -414,7 +461,7 @@ __global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, 
         if (!last_to_arrive(counter, &slot)) return;
 #pragma unroll
         for (int c = 0; c < 4; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
-        wg_sum_f64<4>(v, red);
+        wg_sum_f64<NT>(v, red);
     }
     if (threadIdx.x == 0) {
         const double N = n ? (double)d.batch : v[3];  // no token at all: 0 / 0, a NaN loss
@@ -506,11 +553,12 @@ struct TopEntry {
     }
 };
 
-template <typename T, int NT>
+template <typename T, int NT, bool SPLIT>
 __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T* __restrict__ logits,
                                                      const int32_t* __restrict__ ids, const float* __restrict__ tl,
                                                      const float* __restrict__ tlse, const uint8_t* __restrict__ mask,
-                                                     LpScale k, float* __restrict__ kl, RowStat* __restrict__ stats,
+                                                     LpScale k, const Stat<double>* __restrict__ part, int parts,
+                                                     float* __restrict__ kl, RowStat* __restrict__ stats,
                                                      uint32_t* __restrict__ counter) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ Teacher te;
@@ -529,7 +577,10 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
     entry.load(d, row, ids, tl);
     entry.open(d, k.inv_t, te);
     const uint32_t x = entry.logit(xr, vocab);
-    const Stat<float> st = wg_stat<NT>(row_stat<T, NT, float>(xr, vocab, k), k.c_hi, red);
+    Stat<float> st;
+    if constexpr (SPLIT) st = float_stat(own_part(part, row, parts));
+    else st = row_stat<T, NT, float>(xr, vocab, k);
+    st = wg_stat<NT>(st, k.c_hi, red);
     const RowStat v{st.m, st.s};
     entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
     __syncthreads();
@@ -566,7 +617,7 @@ __global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chun
             v[1] += on[u] ? 1.0 : 0.0;
         }
     }
-    wg_sum_f64<2>(v, red);
+    wg_sum_f64<NT>(v, red);
     if (gridDim.x > 1) {
         if (threadIdx.x == 0) {
             part[blockIdx.x][0] = v[0];
@@ -575,7 +626,7 @@ __global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chun
         if (!last_to_arrive(counter, &slot)) return;
 #pragma unroll
         for (int c = 0; c < 2; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
-        wg_sum_f64<2>(v, red);
+        wg_sum_f64<NT>(v, red);
     }
     if (threadIdx.x == 0) {
         const double T = temperature;
@@ -787,19 +838,20 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
 // REST: rows of any length. What lies past NT NV vectors is read twice, its end,
 // which the cache still has, first.
 template <typename T, int NT, int NV, bool REST> struct HeldRow {
-    // The thread whose vector, or edge, element j is in.
-    __device__ __forceinline__ int owner(int at) const {
-        if (at < head) return at;
-        const int c = (at - head) / N;
-        return c < nvec ? c & (NT - 1) : N + (at - head - nvec * N);
-    }
     static constexpr int N = Vec16<T>::N, G = 16 / N;  // vectors reduced at a time
     i32x4 q[NV];
     uint32_t edge;
     int head, nvec, j;  // j: the edge element, or -1
     const T* xv;        // the first vector
 
-    __device__ __forceinline__ void load(const T* __restrict__ xr, int vocab) {
+    // The thread that stores element `at`: its vector's, or its edge's.
+    __device__ __forceinline__ int owner(int at) const {
+        if (at < head) return at;
+        const int c = (at - head) / N;
+        return c < nvec ? c & (NT - 1) : N + (at - head - nvec * N);
+    }
+    __device__ __forceinline__ void load(const T* __restrict__ xr, int vocab, const Stat<double>*, int64_t,
+                                         RowThreads) {
         const RowSpan<T> span(xr, vocab);
         head = (int)span.head;
         nvec = (int)span.nvec;
@@ -877,6 +929,32 @@ template <typename T, int NT, int NV, bool REST> struct HeldRow {
     }
 };
 
+// A row of few, shared by gridDim.y workgroups: its statistics from parts_k, its
+// logits read again, from the cache as a rule.
+template <typename T, int NT> struct SplitRow {
+    static constexpr int N = Vec16<T>::N;
+    const T* xr;
+    RowThreads th;
+    int vocab, head, nvec;
+    Stat<double> part;
+
+    __device__ __forceinline__ int owner(int at) const { return owner_of<N>(at, head, nvec, true, th.count); }
+    __device__ __forceinline__ void load(const T* __restrict__ xr_, int vocab_, const Stat<double>* __restrict__ parts,
+                                         int64_t row, RowThreads th_) {
+        const RowSpan<T> span(xr_, vocab_);
+        xr = xr_;
+        th = th_;
+        vocab = vocab_;
+        head = (int)span.head;
+        nvec = (int)span.nvec;
+        part = own_part(parts, row, th.count / NT);
+    }
+    __device__ __forceinline__ Stat<float> stat(LpScale) const { return float_stat(part); }
+    __device__ __forceinline__ void store(T* __restrict__ dr, bool stream, RowGrad grad) const {
+        write_row(xr, dr, vocab, true, stream, th, grad);
+    }
+};
+
 // Counted tokens of 64 blocks of rows, for the weight of a token.
 constexpr int kCountBlocks = 64;
 __global__ __launch_bounds__(256) void counts_k(int64_t rows, int64_t chunk, const uint32_t* __restrict__ targets,
@@ -925,15 +1003,17 @@ template <int NT> struct RowCount {
     }
 };
 
-// l, and with the token's weight its gradient. given: n_given counts that add up
+// l, and with the token's weight its gradient. Row: HeldRow, or SplitRow with
+// parts. given: n_given counts that add up
 // to the tokens that share the weight (by_seq: of each sequence, one number
 // each), or null: counted here over len targets. n (may be null): receives the
 // sequences' counts.
-template <typename T, int NT, int NV, bool REST>
-__global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool stream, const T* __restrict__ logits,
+template <typename T, int NT, typename Row>
+__global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool stream, const T* __restrict__ logits,
                                                        const uint32_t* __restrict__ targets,
                                                        const float* __restrict__ adv, const float* __restrict__ old,
                                                        const float* __restrict__ ref,
+                                                       const Stat<double>* __restrict__ parts,
                                                        const uint32_t* __restrict__ given, int n_given, int len,
                                                        bool by_seq,
                                                        uint32_t* __restrict__ n, LpScale k,
@@ -941,14 +1021,15 @@ __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool st
                                                        T* __restrict__ dlogits, uint32_t* __restrict__ counter) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ uint32_t redc[NT / 64];
-    const RowThreads th{(int)threadIdx.x, NT};
+    const RowThreads th = row_threads<NT>();
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
-    if (row == 0 && threadIdx.x == 0) *counter = 0;
+    const bool writer = th.self == 0;
+    if (row == 0 && writer) *counter = 0;
     T* dr = dlogits + row * vocab;
     const uint32_t t = targets[row];
     if (!counted(t, d.ignore_index)) {
-        if (threadIdx.x == 0) logp[row] = 0.f;
+        if (writer) logp[row] = 0.f;
         zero_row(dr, vocab, stream, th);
         return;
     }
@@ -961,14 +1042,14 @@ __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool st
     const uint32_t* cw = by_seq ? targets + (int64_t)q * d.seq : targets;
     RowCount<NT> count;
     count.load(len, [&](int i) { return cw[i]; });
-    HeldRow<T, NT, NV, REST> held;
-    held.load(xr, vocab);
+    Row held;
+    held.load(xr, vocab, parts, row, th);
     count.put(len, redc, [&](uint32_t w) { return counted(w, d.ignore_index); });
     const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
     const RowStat v{st.m, st.s};
     const uint32_t share = count.total(redc, given ? given + (by_seq ? q : 0) : nullptr, n_given);
     const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
-    if (threadIdx.x == 0) {
+    if (writer) {
         logp[row] = l;
         if (n) n[q] = share;  // the same from every row of the sequence
     }
@@ -980,17 +1061,18 @@ __global__ __launch_bounds__(NT, 4) void policy_held_k(mc_policy_desc d, bool st
     g *= k.inv_t;
     const RowGrad grad = row_grad(-g, v, k.c_hi);
     held.store(dr, stream, grad);
-    if (in && held.owner((int)t) == (int)threadIdx.x)
+    if (in && held.owner((int)t) == th.self)
         Elem<T>::store(dr, t, grad(from_raw<T>(xt)) + g);
 }
 
 // given: n_given counts of the mask, or null: counted here over len of it (0
 // without a mask).
-template <typename T, int NT, int NV, bool REST>
-__global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool stream, const T* __restrict__ logits,
+template <typename T, int NT, typename Row>
+__global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool stream, const T* __restrict__ logits,
                                                         const int32_t* __restrict__ ids, const float* __restrict__ tl,
                                                         const float* __restrict__ tlse,
                                                         const uint8_t* __restrict__ mask,
+                                                        const Stat<double>* __restrict__ parts,
                                                         const uint32_t* __restrict__ given, int n_given, int len,
                                                         LpScale k, const float* __restrict__ dloss,
                                                         float* __restrict__ kl,
@@ -999,13 +1081,14 @@ __global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool 
     __shared__ uint32_t redc[NT / 64];
     __shared__ Teacher te;
     __shared__ TopOwners<NT> owners;
-    const RowThreads th{(int)threadIdx.x, NT};
+    const RowThreads th = row_threads<NT>();
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
-    if (row == 0 && threadIdx.x == 0) *counter = 0;
+    const bool writer = th.self == 0;
+    if (row == 0 && writer) *counter = 0;
     T* dr = dlogits + row * vocab;
     if (mask && mask[row] == 0) {
-        if (threadIdx.x == 0) kl[row] = 0.f;
+        if (writer) kl[row] = 0.f;
         zero_row(dr, vocab, stream, th);
         return;
     }
@@ -1019,11 +1102,12 @@ __global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool 
     RowCount<NT> count;
     const uint8_t* cw = mask ? mask : reinterpret_cast<const uint8_t*>(xr);
     count.load(len, [&](int i) { return (uint32_t)cw[i]; });
-    HeldRow<T, NT, NV, REST> held;
-    held.load(xr, vocab);
+    Row held;
+    held.load(xr, vocab, parts, row, th);
     count.put(len, redc, [](uint32_t w) { return w != 0; });
     entry.open(d, k.inv_t, te);
-    if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab) owners.insert(held.owner(entry.id), 0);
+    if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab) 
+        owners.insert(held.owner(entry.id), (int)(blockIdx.y * NT));
     const uint32_t x = entry.logit(xr, vocab);
     const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
     const RowStat v{st.m, st.s};
@@ -1031,7 +1115,7 @@ __global__ __launch_bounds__(NT, 4) void distill_held_k(mc_distill_desc d, bool 
     float w = d.temperature / (mask ? (float)count.total(redc, given, n_given) : (float)d.rows) * up;
     __syncthreads();
     const TeacherSums ts = entry.sums(d, te);
-    if (threadIdx.x == 0) kl[row] = ts.kl;
+    if (writer) kl[row] = ts.kl;
     if (ts.bad) w = __builtin_nanf("");
     if (ts.P == 0.f || w == 0.f) {
         zero_row(dr, vocab, stream, th);
@@ -1071,15 +1155,30 @@ template <typename F> void by_threads(int threads, int dtype, F&& fn) {
 }
 int64_t row_bytes(int64_t vocab, int dtype) { return vocab * (dtype == MC_F32 ? 4 : 2); }
 
-// fn(element type, HeldShape) for the smallest shape of at least MIN threads that
-// holds a row, or the largest with the rest of the row read twice.
-template <int NT, int NV, bool REST> struct HeldShape {
+constexpr int kPartThreads = 256;  // of the workgroups that share a row
+// Where a fwd_bwd kernel has a row from.
+template <typename T, int NT, int NV, bool REST> struct Held {
     static constexpr int kThreads = NT, kVectors = NV;
     static constexpr bool kRest = REST;
+    typedef HeldRow<T, NT, NV, REST> Row;
 };
-template <int MIN, typename F> void by_held_shape(int64_t vocab, int dtype, F&& fn) {
+template <typename T> struct Split {
+    static constexpr int kThreads = kPartThreads;
+    typedef SplitRow<T, kPartThreads> Row;
+};
+// fn(element type, source): the parts of split rows, the smallest held shape of
+// at least MIN threads for a row, or the largest with the rest of the row read
+// twice. us of held rows alone, by threads x vectors:
+//   16 KB rows, 8192   128x8 49.5, 256x4 47.4, 512x4 58.4
+//   32 KB rows, 8192   512x4 88.9, 256x8 92.5, 512x8 87.4
+//   64 KB rows, 4000   512x8 88.9, 512x13 83.7, 1024x4 115
+//   98 KB rows, 4816   512x13 165, 1024x8 195
+//   201 KB rows, 2036  1024x13 139, 1024x16 140, 1024x19 142
+template <int MIN, typename F> void by_row_source(int parts, int64_t vocab, int dtype, F&& fn) {
     auto go = [&](auto elem) {
-        const int64_t vectors = vocab / Vec16<decltype(elem)>::N;
+        typedef decltype(elem) T;
+        if (parts > 1) return fn(elem, Split<T>{});
+        const int64_t vectors = vocab / Vec16<T>::N;
         auto shape = [&](auto s) {
             typedef decltype(s) S;
             if constexpr (S::kThreads >= MIN) {
@@ -1089,11 +1188,13 @@ template <int MIN, typename F> void by_held_shape(int64_t vocab, int dtype, F&& 
             }
             return false;
         };
-        shape(HeldShape<64, 4, false>{}) || shape(HeldShape<128, 8, false>{}) || shape(HeldShape<256, 4, false>{}) ||
-            shape(HeldShape<512, 4, false>{}) || shape(HeldShape<512, 8, false>{}) ||
-            shape(HeldShape<512, 13, false>{}) || shape(HeldShape<512, 19, false>{}) ||
-            shape(HeldShape<1024, 13, false>{}) || shape(HeldShape<1024, 16, false>{}) ||
-            shape(HeldShape<1024, 19, false>{}) || shape(HeldShape<1024, 16, true>{});
+        // a rest's vectors need registers of their own, unpacked
+        constexpr int kWithRest = Vec16<T>::N == 4 ? 16 : 8;
+        shape(Held<T, 64, 4, false>{}) || shape(Held<T, 128, 8, false>{}) || shape(Held<T, 256, 4, false>{}) ||
+            shape(Held<T, 512, 4, false>{}) || shape(Held<T, 512, 8, false>{}) || shape(Held<T, 512, 13, false>{}) ||
+            shape(Held<T, 512, 19, false>{}) || shape(Held<T, 1024, 13, false>{}) ||
+            shape(Held<T, 1024, 16, false>{}) || shape(Held<T, 1024, 19, false>{}) ||
+            shape(Held<T, 1024, kWithRest, true>{});
     };
     if (dtype == MC_F32) go(float{});
     else go(uint16_t{});
@@ -1103,12 +1204,16 @@ bool same_start(const void* a, const void* b) {
     return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
-// Rows whose sums one workgroup of 1024 threads forms by itself; past it 256
-// workgroups, which meet in the last one.
+// Rows whose sums one workgroup forms by itself; past it 256 workgroups, which
+// meet in the last one.
 constexpr int64_t kOneGroupRows = 8192;
+template <typename F> void by_group_size(int64_t rows, F&& fn) {
+    if (rows <= 1024) fn(std::integral_constant<int, 256>{});
+    else fn(std::integral_constant<int, 1024>{});
+}
 template <typename F> void by_sum_kernel(int64_t rows, F&& fn) {
     if (rows <= kOneGroupRows) {
-        fn(std::integral_constant<int, 1024>{}, dim3(1), rows);
+        by_group_size(rows, [&](auto threads) { fn(threads, dim3(1), rows); });
     } else {
         const int64_t chunk = (rows + 255) / 256;
         fn(std::integral_constant<int, 256>{}, dim3((unsigned)((rows + chunk - 1) / chunk)), chunk);
@@ -1120,25 +1225,57 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace
 
 // ------------------------------------------------------------- launchers
+size_t loss_parts_ws(int64_t rows, int64_t vocab, int dtype) {
+    const int64_t parts = loss_row_parts(rows, row_bytes(vocab, dtype));
+    return parts > 1 ? align256((size_t)(rows * parts) * sizeof(Stat<double>)) : 0;
+}
+
 namespace {
-template <typename L>
-hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, L* logp, float* stats,
-                          uint32_t* counter, hipStream_t stream) {
-    const LpScale k = row_scale(d.temperature);
-    by_threads(loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype)), d.dtype, [&](auto elem, auto threads) {
+// The statistics of a row's parts into ws (loss_parts_ws bytes) and their number,
+// or 1: not split.
+int launch_parts(int64_t rows, int64_t vocab, int dtype, const void* logits, const uint32_t* targets,
+                 int64_t ignore_index, const uint8_t* mask, LpScale k, void* ws, hipStream_t stream) {
+    const int parts = (int)loss_row_parts(rows, row_bytes(vocab, dtype));
+    if (parts == 1) return 1;
+    by_threads(kPartThreads, dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
-        lp_rows_k<T, NT><<<dim3((unsigned)d.rows), NT, 0, stream>>>((int)d.vocab, static_cast<const T*>(logits),
-                                                                    targets, d.ignore_index, k, logp,
-                                                                    reinterpret_cast<RowStat*>(stats), counter);
+        if constexpr (NT == kPartThreads)
+            parts_k<T, NT><<<dim3((unsigned)rows, (unsigned)parts), NT, 0, stream>>>(
+                (int)vocab, static_cast<const T*>(logits), targets, ignore_index, mask, k,
+                static_cast<Stat<double>*>(ws));
+    });
+    return parts;
+}
+
+template <typename L>
+hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, L* logp, float* stats,
+                          uint32_t* counter, void* parts_ws, hipStream_t stream) {
+    const LpScale k = row_scale(d.temperature);
+    const int parts =
+        launch_parts(d.rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
+    const int threads = parts > 1 ? 64 : loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype));
+    by_threads(threads, d.dtype, [&](auto elem, auto threads) {
+        typedef decltype(elem) T;
+        constexpr int NT = decltype(threads)::value;
+        auto go = [&](auto split) {
+            constexpr bool SPLIT = decltype(split)::value;
+            lp_rows_k<T, NT, L, SPLIT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
+                (int)d.vocab, static_cast<const T*>(logits), targets, d.ignore_index, k,
+                static_cast<const Stat<double>*>(parts_ws), parts, logp, reinterpret_cast<RowStat*>(stats), counter);
+        };
+        if constexpr (NT == 64) {
+            if (parts > 1) return go(std::true_type{});
+        }
+        go(std::false_type{});
     });
     return hipGetLastError();
 }
 }  // namespace
 
 hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
-                                     float* stats, hipStream_t stream) {
-    return launch_lp_rows(d, logits, targets, logp, stats, nullptr, stream);
+                                     float* stats, void* ws, hipStream_t stream) {
+    return launch_lp_rows(d, logits, targets, logp, stats, nullptr, ws, stream);
 }
 
 hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
@@ -1166,7 +1303,9 @@ PreferenceWs preference_ws(const mc_preference_desc& d) {
     w.score = at;
     at += align256((size_t)(2 * d.pairs) * sizeof(double));
     w.inv_n = at;
-    w.total = at + align256((size_t)(2 * d.pairs) * sizeof(float));
+    at += align256((size_t)(2 * d.pairs) * sizeof(float));
+    w.parts = at;
+    w.total = at + loss_parts_ws(2 * d.pairs * d.seq, d.vocab, d.dtype);
     return w;
 }
 
@@ -1181,10 +1320,13 @@ hipError_t launch_preference_fwd(const mc_preference_desc& d, const void* logits
     float* dseq = stats ? stats + 2 * rows : nullptr;
     uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, 1.0f, d.dtype};
-    hipError_t e = launch_lp_rows(lp, logits, targets, logp, stats, counter, stream);
+    hipError_t e = launch_lp_rows(lp, logits, targets, logp, stats, counter, ws + w.parts, stream);
     if (e != hipSuccess) return e;
     if (rows <= kOneGroupRows)
-        preference_one_k<<<dim3(1), 1024, 0, stream>>>(d, targets, logp, ref, score, inv_n, loss, rewards, dseq);
+        by_group_size(rows, [&](auto threads) {
+            constexpr int NT = decltype(threads)::value;
+            preference_one_k<NT><<<dim3(1), NT, 0, stream>>>(d, targets, logp, ref, score, inv_n, loss, rewards, dseq);
+        });
     else
         preference_k<<<dim3((unsigned)(2 * d.pairs)), 256, 0, stream>>>(d, targets, logp, ref, score, inv_n, counter,
                                                                          loss, rewards, dseq);
@@ -1198,7 +1340,8 @@ PolicyWs policy_ws(const mc_policy_desc& d) {
     at += 256 * 4 * sizeof(double);
     w.counts = at;
     if (d.reduction == MC_MEAN_SEQUENCES) at += align256((size_t)d.batch * sizeof(uint32_t));
-    w.total = at;
+    w.parts = at;
+    w.total = at + loss_parts_ws(d.batch * d.seq, d.vocab, d.dtype);
     return w;
 }
 
@@ -1235,7 +1378,7 @@ hipError_t launch_policy_fwd(const mc_policy_desc& d, const void* logits, const 
     hipError_t e;
     const uint32_t* n = policy_counts(d, targets, ws, stream, e);
     if (e != hipSuccess) return e;
-    e = launch_lp_rows(lp, logits, targets, logp, stats, counter, stream);
+    e = launch_lp_rows(lp, logits, targets, logp, stats, counter, ws + policy_ws(d).parts, stream);
     if (e != hipSuccess) return e;
     return launch_policy_sums(d, targets, logp, adv, old, ref, n, ws, loss, metrics, stats ? stats + 2 * rows : nullptr,
                               stream);
@@ -1247,7 +1390,9 @@ DistillWs distill_ws(const mc_distill_desc& d) {
     w.part = at;
     at += 256 * 2 * sizeof(double);
     w.kl = at;
-    w.total = at + align256((size_t)d.rows * sizeof(float));
+    at += align256((size_t)d.rows * sizeof(float));
+    w.split = at;
+    w.total = at + loss_parts_ws(d.rows, d.vocab, d.dtype);
     return w;
 }
 
@@ -1271,14 +1416,23 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
     const LpScale k = row_scale(d.temperature);
     uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     float* kl = reinterpret_cast<float*>(ws + w.kl);
-    const int threads = loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype));
-    by_threads(threads < kDistillMaxTop ? kDistillMaxTop : threads, d.dtype, [&](auto elem, auto threads) {
+    const int parts = launch_parts(d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, ws + w.split, stream);
+    int threads = parts > 1 ? kDistillMaxTop : loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype));
+    if (threads < kDistillMaxTop) threads = kDistillMaxTop;  // a thread per entry
+    by_threads(threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
-        if constexpr (NT >= kDistillMaxTop)  // a thread per entry
-            distill_rows_k<T, NT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
-                d, static_cast<const T*>(logits), ids, tl, tlse, mask, k, kl, reinterpret_cast<RowStat*>(stats),
+        auto go = [&](auto split) {
+            constexpr bool SPLIT = decltype(split)::value;
+            distill_rows_k<T, NT, SPLIT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
+                d, static_cast<const T*>(logits), ids, tl, tlse, mask, k,
+                reinterpret_cast<const Stat<double>*>(ws + w.split), parts, kl, reinterpret_cast<RowStat*>(stats),
                 counter);
+        };
+        if constexpr (NT == kDistillMaxTop) {
+            if (parts > 1) return go(std::true_type{});
+        }
+        if constexpr (NT >= kDistillMaxTop) go(std::false_type{});
     });
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1334,21 +1488,25 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         const bool by_seq = d.reduction == MC_MEAN_SEQUENCES;
         uint32_t* n = by_seq ? reinterpret_cast<uint32_t*>(ws + w.counts) : nullptr;
-        by_held_shape<64>(d.vocab, d.dtype, [&](auto elem, auto shape) {
+        void* parts_ws = ws + w.parts;
+        const int parts =
+            launch_parts(rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
+        e = hipSuccess;
+        by_row_source<64>(parts, d.vocab, d.dtype, [&](auto elem, auto source) {
             typedef decltype(elem) T;
-            typedef decltype(shape) S;
+            typedef decltype(source) S;
             constexpr int NT = S::kThreads;
             const int64_t span = by_seq ? d.seq : rows;
             const bool here = span <= RowCount<NT>::kPer * NT;
             int n_given = 1;
-            e = hipSuccess;
             if (!here && by_seq) policy_counts(d, targets, ws, stream, e);
             else if (!here) n_given = launch_counts(rows, targets, nullptr, d.ignore_index, part, stream);
-            policy_held_k<T, NT, S::kVectors, S::kRest><<<dim3((unsigned)rows), NT, 0, stream>>>(
+            policy_both_k<T, NT, typename S::Row><<<dim3((unsigned)rows, (unsigned)parts), NT, 0, stream>>>(
                 d, xent_stream_gradients(rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), targets, adv, old,
-                ref, here ? nullptr : by_seq ? n : part, n_given, here ? (int)span : 0, by_seq, here ? n : nullptr, k,
-                dloss, logp, static_cast<T*>(dlogits), counter);
+                ref, static_cast<const Stat<double>*>(parts_ws), here ? nullptr : by_seq ? n : part, n_given,
+                here ? (int)span : 0, by_seq, here ? n : nullptr, k, dloss, logp, static_cast<T*>(dlogits), counter);
         });
+        if (e != hipSuccess) return e;
         if ((e = hipGetLastError()) != hipSuccess) return e;
         return launch_policy_sums(d, targets, logp, adv, old, ref, n, ws, loss, metrics, nullptr, stream);
     }
@@ -1374,16 +1532,18 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
         uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
         float* kl = reinterpret_cast<float*>(ws + w.kl);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
-        by_held_shape<256>(d.vocab, d.dtype, [&](auto elem, auto shape) {
+        void* parts_ws = ws + w.split;
+        const int parts = launch_parts(d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, parts_ws, stream);
+        by_row_source<kDistillMaxTop>(parts, d.vocab, d.dtype, [&](auto elem, auto source) {
             typedef decltype(elem) T;
-            typedef decltype(shape) S;
+            typedef decltype(source) S;
             constexpr int NT = S::kThreads;
             const bool here = !mask || d.rows <= RowCount<NT>::kPer * NT;
             const int n_given = here ? 0 : launch_counts(d.rows, nullptr, mask, -1, part, stream);
-            distill_held_k<T, NT, S::kVectors, S::kRest><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
+            distill_both_k<T, NT, typename S::Row><<<dim3((unsigned)d.rows, (unsigned)parts), NT, 0, stream>>>(
                 d, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl, tlse,
-                mask, here ? nullptr : part, n_given, mask && here ? (int)d.rows : 0, k, dloss, kl,
-                static_cast<T*>(dlogits), counter);
+                mask, static_cast<const Stat<double>*>(parts_ws), here ? nullptr : part, n_given,
+                mask && here ? (int)d.rows : 0, k, dloss, kl, static_cast<T*>(dlogits), counter);
         });
         if ((e = hipGetLastError()) != hipSuccess) return e;
         return launch_distill_sums(d, mask, kl, ws, loss, nullptr, stream);

@@ -64,6 +64,15 @@ constexpr int loss_row_threads(int64_t rows, int64_t row_bytes) {
     return row_bytes < 192 << 10 || rows < 768 ? 512 : 1024;
 }
 
+// Workgroups of 256 threads that share a row's statistics (1: none do), where
+// there are few long rows: one CU reads about 30 bytes a ns.
+constexpr int64_t loss_row_parts(int64_t rows, int64_t row_bytes) {
+    if (rows > 128 || row_bytes < 96 << 10) return 1;
+    const int64_t wanted = (1024 + rows - 1) / rows, most = row_bytes / (8 << 10);
+    const int64_t parts = wanted < most ? wanted : most;
+    return parts < 32 ? parts : 32;
+}
+
 // Threads that write a row's gradient, and workgroups that share a row where
 // there are too few rows for the CUs. us, right behind a forward (64 rows: alone),
 // 256 / 512 / 1024 threads:

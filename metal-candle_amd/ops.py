@@ -527,8 +527,10 @@ def token_logprobs_forward(logits, targets, ignore_index=None, temperature=1.0, 
     d = _logprob_desc(logits, ignore, temperature, code)
     logps = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
     stats = torch.empty(d.rows, 2, dtype=torch.float32, device=logits.device) if save_stats else None
+    ws_n = lib().mc_token_logprobs_workspace_size(ctypes.byref(d))
+    ws = _workspace(ws_n, logits.device)
     _launch(logits, lib().mc_token_logprobs_fwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(),
-            logps.data_ptr(), _ptr(stats))
+            logps.data_ptr(), _ptr(stats), _ptr(ws), ws_n)
     return logps, stats
 
 

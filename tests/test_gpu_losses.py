@@ -526,6 +526,86 @@ def test_distillation_bad_id_and_nothing_counted(mc, dev):
     assert torch.isnan(loss).all() and not d.any()
 
 
+# ------------------------------------------------------------------- long rows
+# Rows of every way of taking them: shared by workgroups (few long rows), held in
+# registers by each number of threads, too long to be held.
+LONG = [(torch.bfloat16, 1, 151936), (torch.bfloat16, 7, 60001), (torch.float32, 128, 24577), (torch.float32, 3, 400003),
+        (torch.bfloat16, 129, 151936), (torch.float32, 131, 77823), (torch.float32, 129, 77829),
+        (torch.float32, 130, 100003), (torch.bfloat16, 129, 155651), (torch.bfloat16, 130, 200003),
+        (torch.bfloat16, 300, 20000), (torch.bfloat16, 200, 40007), (torch.bfloat16, 200, 52001),
+        (torch.bfloat16, 200, 77001), (torch.float32, 140, 50257), (torch.float32, 140, 65001),
+        (torch.float32, 400, 1021), (torch.float32, 400, 4100), (torch.float32, 300, 8193)]
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("dtype,rows,V", LONG)
+def test_rows_of_every_length(mc, dev, nan_outputs, dtype, rows, V, offset):
+    g = gen(dev, V)
+    x = logits_at(dev, g, (rows, V), dtype, offset)
+    t = some_targets(dev, g, (rows,), V, drop=0.2)
+    t[0] = min(V - 1, 5)
+    dl = torch.randn(rows, generator=g, device=dev)
+    l, stats = mc.token_logprobs_forward(x, t, ignore_index=PAD)
+    l64, tol, q = plain_logps(x, t)
+    close(l, l64, tol, "logps")
+    close_grad(mc.token_logprobs_backward(x, t, stats, dl, ignore_index=PAD), *plain_grad(q, t, dl.double()), dtype)
+    # an advantage per token: -A r is the whole of dl
+    A = torch.randn(rows, 1, generator=g, device=dev)
+    outs = mc.policy_loss_forward_backward(x[:, None], t[:, None], A, ignore_index=PAD)
+    check_policy(mc, dev, x[:, None], t[:, None], l64[:, None], tol[:, None], q[:, None], A, None, None, {}, outs, 1.0,
+                 dtype)
+    loss, logps, metrics, pstats = mc.policy_loss_forward(x[:, None], t[:, None], A, ignore_index=PAD)
+    d = mc.policy_loss_backward(x[:, None], t[:, None], pstats, ignore_index=PAD)
+    check_policy(mc, dev, x[:, None], t[:, None], l64[:, None], tol[:, None], q[:, None], A, None, None, {},
+                 (loss, logps, metrics, d), 1.0, dtype)
+    ids = torch.randint(0, V, (rows, 40), generator=g, device=dev, dtype=torch.int32)
+    ids[:, :4] = torch.tensor([0, V - 1, V // 2, V // 2], device=dev, dtype=torch.int32)
+    tl = torch.randn(rows, 40, generator=g, device=dev) * 2
+    mask = (torch.rand(rows, generator=g, device=dev) < 0.8).to(torch.uint8)
+    mask[0] = 1
+    want, tol, grad, terms = plain_distill(x, ids, tl, 1.0, None, mask)
+    loss, dstats = mc.distillation_loss_forward(x, ids, tl, mask=mask)
+    d = mc.distillation_loss_backward(x, ids, tl, dstats, mask=mask)
+    for v, dv in ((loss, d), mc.distillation_loss_forward_backward(x, ids, tl, mask=mask)):
+        assert abs(float(v) - float(want)) <= float(tol) + 2.0 ** -23 * abs(float(want))
+        close_grad(dv, grad, terms, dtype)
+    if rows % 2 == 0:
+        P = rows // 2
+        ploss, rewards, pst = mc.preference_loss_forward(x[:, None], t[:, None], beta=0.3, ignore_index=PAD)
+        l = l64[:, None].clone().requires_grad_()
+        want, _ = plain_preference(l, t[:, None], None, 0.3, "sigmoid", 0.0, 0.0, False)
+        want.backward()
+        assert abs(float(ploss) - float(want.detach())) <= 1e-5 * max(1.0, abs(float(want.detach())))
+        grad, terms = plain_grad(q, t, l.grad[:, 0])
+        pd = mc.preference_loss_backward(x[:, None], t[:, None], pst, ignore_index=PAD)
+        close_grad(pd[:, 0], grad, 1.3 * terms, dtype)
+
+
+@pytest.mark.parametrize("rows,B", [(20000, 5), (9000, 9000)])
+def test_many_rows(mc, dev, rows, B):
+    """Sums over more rows than one workgroup takes, counts by a kernel of their own."""
+    V, g = 37, gen(dev, rows)
+    x, t, l64, tol, q, old, ref, A = policy_case(dev, B, rows // B, V, torch.float32, 0, False, 1.0, rows)
+    for kw in (dict(kl_coef=0.1), dict(kl_coef=0.1, reduction="sequences")):
+        outs = mc.policy_loss_forward_backward(x, t, A, old, ref, ignore_index=PAD, **kw)
+        check_policy(mc, dev, x, t, l64, tol, q, A, old, ref, kw, outs, 1.0, torch.float32)
+        loss, logps, metrics, stats = mc.policy_loss_forward(x, t, A, old, ref, ignore_index=PAD, **kw)
+        d = mc.policy_loss_backward(x, t, stats, ignore_index=PAD)
+        check_policy(mc, dev, x, t, l64, tol, q, A, old, ref, kw, (loss, logps, metrics, d), 1.0, torch.float32)
+    ids = torch.randint(0, V, (rows, 3), generator=g, device=dev, dtype=torch.int32)
+    tl = torch.randn(rows, 3, generator=g, device=dev)
+    for mask in (None, (torch.rand(rows, generator=g, device=dev) < 0.5).to(torch.uint8)):
+        want, dtol, grad, terms = plain_distill(x.view(rows, V), ids, tl, 1.0, None, mask)
+        for loss, d in (mc.distillation_loss_forward_backward(x.view(rows, V), ids, tl, mask=mask),):
+            assert abs(float(loss) - float(want)) <= float(dtol) + 2.0 ** -23 * abs(float(want))
+            close_grad(d, grad, terms, torch.float32)
+    y, ty = (x[:-1], t[:-1]) if B % 2 else (x, t)
+    loss, rewards, _ = mc.preference_loss_forward(y.contiguous(), ty.contiguous(), beta=0.01, ignore_index=PAD)
+    want, r64 = plain_preference(l64[: y.shape[0]], ty, None, 0.01, "sigmoid", 0.0, 0.0, False)
+    close(rewards, r64, 0.01 * tol[: y.shape[0]].sum(1) + 2.0 ** -23 * r64.abs(), "rewards")
+    assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+
+
 # ------------------------------------------------------- differences, together
 def losses_of(mc, name, x, extra):
     """(loss, dlogits) of one of the losses on [4, 5, V]."""

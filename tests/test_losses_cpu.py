@@ -92,7 +92,7 @@ def test_abi_logprobs(mc, field, value, code, text):
     d = mc._lib.LogprobDesc(4, 8, -1, 1.0, 0)
     setattr(d, field, value)
     p = ctypes.byref(d)
-    assert L.mc_token_logprobs_fwd(p, FAKE, FAKE, FAKE, FAKE, None) == code and text in mc._lib.last_error()
+    assert L.mc_token_logprobs_fwd(p, FAKE, FAKE, FAKE, FAKE, None, 0, None) == code and text in mc._lib.last_error()
     assert L.mc_token_logprobs_bwd(p, FAKE, FAKE, FAKE, FAKE, FAKE, None) == code
     if field in ("rows", "vocab", "dtype", "temperature") and hasattr(mc._lib.DistillDesc, field):
         e = mc._lib.DistillDesc(4, 8, 5, 1.0, 0)
@@ -105,10 +105,14 @@ def test_abi_null_layout_and_workspace(mc):
     L, S = mc._lib.lib(), mc._lib
     odd = ctypes.c_void_p(257)
     lp = ctypes.byref(S.LogprobDesc(4, 8, -1, 1.0, 1))
-    assert L.mc_token_logprobs_fwd(None, FAKE, FAKE, FAKE, None, None) == NULL
-    assert L.mc_token_logprobs_fwd(lp, None, FAKE, FAKE, None, None) == NULL
-    assert L.mc_token_logprobs_fwd(lp, FAKE, FAKE, None, None, None) == NULL
-    assert L.mc_token_logprobs_fwd(lp, odd, FAKE, FAKE, None, None) == LAYOUT
+    assert L.mc_token_logprobs_fwd(None, FAKE, FAKE, FAKE, None, None, 0, None) == NULL
+    assert L.mc_token_logprobs_fwd(lp, None, FAKE, FAKE, None, None, 0, None) == NULL
+    assert L.mc_token_logprobs_fwd(lp, FAKE, FAKE, None, None, None, 0, None) == NULL
+    assert L.mc_token_logprobs_fwd(lp, odd, FAKE, FAKE, None, None, 0, None) == LAYOUT
+    few = S.LogprobDesc(1, 1 << 20, -1, 1.0, 1)
+    need = L.mc_token_logprobs_workspace_size(ctypes.byref(few))
+    assert need > 0 and L.mc_token_logprobs_workspace_size(lp) == 0
+    assert L.mc_token_logprobs_fwd(ctypes.byref(few), FAKE, FAKE, FAKE, None, FAKE, need - 1, None) == WORKSPACE
     assert L.mc_token_logprobs_bwd(lp, FAKE, FAKE, None, FAKE, FAKE, None) == NULL
     assert L.mc_token_logprobs_bwd(lp, FAKE, FAKE, FAKE, FAKE, odd, None) == LAYOUT
 

@@ -479,21 +479,27 @@ def cross_entropy_backward(logits, targets, stats, dloss=None, ignore_index=None
 
 
 # --------------------------------------------------- losses over log-probabilities
-def _optional(t, name, shape, dtype, device):
-    """A device address for an optional tensor of the given shape, or None."""
+def _address(t, name, shape, dtype, device):
+    """The device address of a tensor of the given shape (a tuple), or None for None."""
     if t is None:
         return None
-    _expect(t, name, shape, dtype, device)
+    if type(t) is not torch.Tensor or t.shape != shape or t.dtype is not dtype or t.device != device or \
+            not t.is_contiguous():
+        _expect(t, name, shape, dtype, device)
     return t.data_ptr()
 
 
 def _launch(t, fn, *args):
     """fn(*args, stream) on the device of t and its current stream."""
-    if t.is_cuda and t.get_device() != torch.cuda.current_device():
-        with torch.cuda.device(t.device):
-            check(fn(*args, _stream(t)))
+    if not t.is_cuda:
+        torch.cuda.current_stream(t.device)  # refuses what is not on a GPU
+    device = t.get_device()
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        check(fn(*args, _stream(t)))
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    check(status)
 
 
 def _loss_inputs(logits, targets, ignore_index, seqs):
@@ -507,7 +513,7 @@ def _loss_inputs(logits, targets, ignore_index, seqs):
     if logits.numel() == 0:
         raise McError(_lib.MC_ERR_SHAPE, f"logits are empty: {tuple(logits.shape)}")
     targets = _targets(targets, logits)
-    if seqs and tuple(targets.shape) != tuple(logits.shape[:-1]):
+    if seqs and targets.shape != logits.shape[:-1]:
         raise McError(_lib.MC_ERR_SHAPE, f"targets has shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
     return targets, -1 if ignore_index is None else int(ignore_index), _DTYPES[logits.dtype]
 
@@ -525,7 +531,10 @@ def token_logprobs_forward(logits, targets, ignore_index=None, temperature=1.0, 
     token_logprobs_backward needs, or None."""
     targets, ignore, code = _loss_inputs(logits, targets, ignore_index, False)
     d = _logprob_desc(logits, ignore, temperature, code)
-    logps = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    if targets.dim() == logits.dim() - 1:
+        logps = torch.empty_like(targets, dtype=torch.float32)  # half the time of empty with a shape
+    else:
+        logps = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
     stats = torch.empty(d.rows, 2, dtype=torch.float32, device=logits.device) if save_stats else None
     ws_n = lib().mc_token_logprobs_workspace_size(ctypes.byref(d))
     ws = _workspace(ws_n, logits.device)
@@ -542,11 +551,11 @@ def token_logprobs_backward(logits, targets, stats, dlogps, ignore_index=None, t
     dev = logits.device
     if stats is None or dlogps is None:
         raise McError(_lib.MC_ERR_NULL, "token_logprobs_backward: stats and dlogps are required")
-    _expect(stats, "stats", (d.rows, 2), torch.float32, dev)
-    _expect(dlogps, "dlogps", logits.shape[:-1], torch.float32, dev)
+    stats_at = _address(stats, "stats", (d.rows, 2), torch.float32, dev)
+    dlogps_at = _address(dlogps, "dlogps", logits.shape[:-1], torch.float32, dev)
     dlogits = torch.empty_like(logits)
-    _launch(logits, lib().mc_token_logprobs_bwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(),
-            stats.data_ptr(), dlogps.data_ptr(), dlogits.data_ptr())
+    _launch(logits, lib().mc_token_logprobs_bwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(), stats_at,
+            dlogps_at, dlogits.data_ptr())
     return dlogits
 
 
@@ -583,7 +592,7 @@ def preference_loss_forward(logits, targets, ref_logps=None, beta=0.1, kind="sig
     _, S, V = logits.shape
     d = PreferenceDesc(P, S, V, ignore, _choice(_PREF_KINDS, kind, "kind"), int(bool(average)), float(beta),
                        float(label_smoothing), float(margin), code)
-    ref = _optional(ref_logps, "ref_logps", (2 * P, S), torch.float32, dev)
+    ref = _address(ref_logps, "ref_logps", (2 * P, S), torch.float32, dev)
     loss = torch.empty(1, dtype=torch.float32, device=dev)
     rewards = torch.empty(2 * P, dtype=torch.float32, device=dev)
     stats = torch.empty(4 * P * S + 2 * P, dtype=torch.float32, device=dev)
@@ -602,7 +611,7 @@ def preference_loss_backward(logits, targets, stats, dloss=None, ignore_index=No
     if stats is None:
         raise McError(_lib.MC_ERR_NULL, "stats from preference_loss_forward are required")
     _expect(stats, "stats", (4 * P * S + 2 * P,), torch.float32, dev)
-    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    g = _address(dloss, "dloss", (1,), torch.float32, dev)
     # what the loss was is in stats
     d = PreferenceDesc(P, S, V, ignore, _lib.MC_PREF_SIGMOID, 0, 1.0, 0.0, 0.0, code)
     dlogits = torch.empty_like(logits)
@@ -622,14 +631,13 @@ def _policy_call(logits, targets, advantages, old_logps, ref_logps, clip_low, cl
     if not isinstance(advantages, torch.Tensor):
         raise McError(_lib.MC_ERR_NULL, "advantages must be a tensor")
     per_token = advantages.dim() == 2
-    _expect(advantages, "advantages", (B, S) if per_token else (B,), torch.float32, dev)
-    old = _optional(old_logps, "old_logps", (B, S), torch.float32, dev)
-    ref = _optional(ref_logps, "ref_logps", (B, S), torch.float32, dev)
+    _address(advantages, "advantages", (B, S) if per_token else (B,), torch.float32, dev)
+    old = _address(old_logps, "old_logps", (B, S), torch.float32, dev)
+    ref = _address(ref_logps, "ref_logps", (B, S), torch.float32, dev)
     d = PolicyDesc(B, S, V, ignore, int(per_token), _choice(_REDUCTIONS, reduction, "reduction"), float(clip_low),
                    float(clip_high), float(kl_coef), float(temperature), code)
-    out = torch.empty(3, dtype=torch.float32, device=dev)
-    logps = torch.empty(B, S, dtype=torch.float32, device=dev)
-    return d, targets, old, ref, out[:1], logps, out[1:]
+    loss, metrics = (torch.empty(n, dtype=torch.float32, device=dev) for n in (1, 2))
+    return d, targets, old, ref, loss, torch.empty_like(targets, dtype=torch.float32), metrics
 
 
 def policy_loss_forward(logits, targets, advantages, old_logps=None, ref_logps=None, clip_low=0.2, clip_high=0.2,
@@ -665,7 +673,7 @@ def policy_loss_backward(logits, targets, stats, dloss=None, temperature=1.0, ig
     if stats is None:
         raise McError(_lib.MC_ERR_NULL, "stats from policy_loss_forward are required")
     _expect(stats, "stats", (3 * B * S + 1,), torch.float32, dev)
-    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    g = _address(dloss, "dloss", (1,), torch.float32, dev)
     d = PolicyDesc(B, S, V, ignore, 0, _lib.MC_MEAN_TOKENS, 0.0, 0.0, 0.0, float(temperature), code)
     dlogits = torch.empty_like(logits)
     _launch(logits, lib().mc_policy_loss_bwd, ctypes.byref(d), logits.data_ptr(), targets.data_ptr(), stats.data_ptr(),
@@ -681,7 +689,7 @@ def policy_loss_forward_backward(logits, targets, advantages, old_logps=None, re
     d, targets, old, ref, loss, logps, metrics = _policy_call(
         logits, targets, advantages, old_logps, ref_logps, clip_low, clip_high, kl_coef, temperature, reduction,
         ignore_index)
-    g = _optional(dloss, "dloss", (1,), torch.float32, logits.device)
+    g = _address(dloss, "dloss", (1,), torch.float32, logits.device)
     dlogits = torch.empty_like(logits)
     ws_n = lib().mc_policy_loss_fwd_bwd_workspace_size(ctypes.byref(d))
     ws = _workspace(ws_n, logits.device)
@@ -705,8 +713,8 @@ def _distill_call(logits, teacher_ids, teacher_logits, temperature, teacher_lse,
         teacher_ids = teacher_ids.clamp(-1, 2**31 - 1).to(torch.int32)
     _expect(teacher_ids, "teacher_ids", lead + (K,), torch.int32, dev)
     _expect(teacher_logits, "teacher_logits", lead + (K,), torch.float32, dev)
-    lse = _optional(teacher_lse, "teacher_lse", lead, torch.float32, dev)
-    m = _optional(mask, "mask", lead, torch.uint8, dev)
+    lse = _address(teacher_lse, "teacher_lse", lead, torch.float32, dev)
+    m = _address(mask, "mask", lead, torch.uint8, dev)
     return DistillDesc(rows, V, K, float(temperature), _DTYPES[logits.dtype]), teacher_ids, lse, m
 
 
@@ -738,7 +746,7 @@ def distillation_loss_backward(logits, teacher_ids, teacher_logits, stats, dloss
     if stats is None:
         raise McError(_lib.MC_ERR_NULL, "stats from distillation_loss_forward are required")
     _expect(stats, "stats", (2 * d.rows + 1,), torch.float32, dev)
-    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    g = _address(dloss, "dloss", (1,), torch.float32, dev)
     dlogits = torch.empty_like(logits)
     _launch(logits, lib().mc_distill_loss_bwd, ctypes.byref(d), logits.data_ptr(), ids.data_ptr(),
             teacher_logits.data_ptr(), lse, m, stats.data_ptr(), g, dlogits.data_ptr())
@@ -751,7 +759,7 @@ def distillation_loss_forward_backward(logits, teacher_ids, teacher_logits, temp
     be read twice."""
     d, ids, lse, m = _distill_call(logits, teacher_ids, teacher_logits, temperature, teacher_lse, mask)
     dev = logits.device
-    g = _optional(dloss, "dloss", (1,), torch.float32, dev)
+    g = _address(dloss, "dloss", (1,), torch.float32, dev)
     loss = torch.empty(1, dtype=torch.float32, device=dev)
     dlogits = torch.empty_like(logits)
     ws_n = lib().mc_distill_loss_fwd_bwd_workspace_size(ctypes.byref(d))

@@ -768,7 +768,7 @@ static mc_status check_logprob(const mc_logprob_desc* d) {
 }
 
 size_t mc_token_logprobs_workspace_size(const mc_logprob_desc* d) {
-    return check_logprob(d) == MC_OK ? mc::loss_parts_ws(d->rows, d->vocab, d->dtype) : 0;
+    return check_logprob(d) == MC_OK ? mc::loss_parts_ws(d->rows, d->vocab, d->dtype, false) : 0;
 }
 
 mc_status mc_token_logprobs_fwd(const mc_logprob_desc* d, const void* logits, const uint32_t* targets, float* logps,
@@ -777,7 +777,7 @@ mc_status mc_token_logprobs_fwd(const mc_logprob_desc* d, const void* logits, co
     if (s != MC_OK) return s;
     MC_CHECK(logits && targets && logps, MC_ERR_NULL, "token_logprobs: logits, targets and logps must not be NULL");
     if ((s = check_logits("token_logprobs", d->dtype, logits, nullptr)) != MC_OK) return s;
-    const size_t need = mc::loss_parts_ws(d->rows, d->vocab, d->dtype);
+    const size_t need = mc::loss_parts_ws(d->rows, d->vocab, d->dtype, false);
     if (need && (s = check_workspace("token_logprobs", workspace, workspace_bytes, need)) != MC_OK) return s;
     mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, logit_bytes(d->rows, d->vocab, d->dtype, 1.0));
     return hip_status(mc::launch_token_logprobs_fwd(*d, logits, targets, logps, stats, workspace, stream),

@@ -200,9 +200,9 @@ hipError_t launch_cross_entropy_bwd(const mc_xent_desc& d, const void* logits, c
                                     const float* stats, const float* dloss, void* dlogits, hipStream_t stream);
 
 // ----------------------------------------------- losses over log-probabilities
-// log2(e) / T as c_hi + c_lo, and 1 / T.
+// log2(e) / T as c_hi + c_lo and as c, the nearest float, and 1 / T.
 struct LpScale {
-    float c_hi, c_lo, inv_t;
+    float c_hi, c_lo, c, inv_t;
     double inv_t64;
 };
 // What the forward keeps of a row of logits: its maximum and its sum of
@@ -211,8 +211,8 @@ struct RowStat {
     float m, s;
 };
 constexpr int kDistillMaxTop = MC_DISTILL_MAX_TOP;  // a teacher's entries per row: one per thread
-// Bytes for the statistics of rows that several workgroups share; 0 where one does.
-size_t loss_parts_ws(int64_t rows, int64_t vocab, int dtype);
+// Bytes for the statistics of rows that several workgroups share (both: in a fwd_bwd call); 0 where one does.
+size_t loss_parts_ws(int64_t rows, int64_t vocab, int dtype, bool both);
 // ws: loss_parts_ws bytes
 hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
                                      float* stats, void* ws, hipStream_t stream);

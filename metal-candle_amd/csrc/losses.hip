@@ -52,73 +52,83 @@ template <typename S> struct Stat {
     float m;
     S s;
 };
-template <typename S> __device__ __forceinline__ Stat<S> stat_join(Stat<S> a, Stat<S> b, float c) {
+// 2^(d c), d <= 0. The small product goes into the fma: added to a rounded one it
+// would be lost.
+__device__ __forceinline__ float exp_of(float d, LpScale k) { return exp2_hw(fmaf(d, k.c_hi, d * k.c_lo)); }
+
+template <typename S> __device__ __forceinline__ Stat<S> stat_join(Stat<S> a, Stat<S> b, LpScale k) {
     const float m = fmaxf(a.m, b.m);
     // equal maxima, -inf among them, need no factor
-    const S sa = a.m == m ? a.s : a.s * (S)exp2_hw((a.m - m) * c);
-    const S sb = b.m == m ? b.s : b.s * (S)exp2_hw((b.m - m) * c);
+    const S sa = a.m == m ? a.s : a.s * (S)exp_of(a.m - m, k);
+    const S sb = b.m == m ? b.s : b.s * (S)exp_of(b.m - m, k);
     return Stat<S>{m, sa + sb};
 }
 
 // Over the workgroup's NT threads in a fixed order: a butterfly over each wave,
 // then the waves in order. red: one slot per wave.
 template <int NT, typename S>
-__device__ __forceinline__ Stat<S> wg_stat(Stat<S> v, float c, Stat<S>* red) {
+__device__ __forceinline__ Stat<S> wg_stat(Stat<S> v, LpScale k, Stat<S>* red) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1)
-        v = stat_join(v, Stat<S>{__shfl_xor(v.m, o, kWave), __shfl_xor(v.s, o, kWave)}, c);
+        v = stat_join(v, Stat<S>{__shfl_xor(v.m, o, kWave), __shfl_xor(v.s, o, kWave)}, k);
     if (lane_id() == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int k = 1; k < NT / 64; ++k) v = stat_join(v, red[k], c);
+    for (int w = 1; w < NT / 64; ++w) v = stat_join(v, red[w], k);
     return v;
 }
 
 // What a share's terms are relative to: where all of it is -inf, anything finite.
 __device__ __forceinline__ float base_of(float m) { return m == kNegInf ? 0.f : m; }
-__device__ __forceinline__ float term_of(float x, float base, LpScale k) {
-    const float d = x - base;
-    return exp2_hw(fmaf(d, k.c_lo, d * k.c_hi));
-}
+__device__ __forceinline__ float term_of(float x, float base, LpScale k) { return exp_of(x - base, k); }
 
 // One thread's share of a row's vectors from c on: U of them requested and
-// reduced at a time, one rescale to their maximum, then one exp2 per element.
+// reduced at a time, one rescale to their maximum, then one exp2 per element. The
+// last of them go together, too: one by one, each would wait for its own load.
 template <typename T, int NT, typename S, int U>
 __device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int nvec, LpScale k) {
     constexpr int N = Vec16<T>::N;
     float m = kNegInf;
     S s = 0;
-    auto group = [&](int c, auto count) {
-        constexpr int K = decltype(count)::value;
-        float v[K][N];
+    auto group = [&](auto whole) {
+        float v[U][N];
 #pragma unroll
-        for (int u = 0; u < K; ++u) Vec16<T>::load(xv + (int64_t)(c + u * NT) * N, v[u]);
+        for (int u = 0; u < U; ++u) {
+            const int at = c + u * NT;
+            Vec16<T>::load(xv + (int64_t)(decltype(whole)::value || at < nvec ? at : c) * N, v[u]);
+        }
+#pragma unroll
+        for (int u = 1; u < U; ++u)
+            if (!decltype(whole)::value && c + u * NT >= nvec) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[u][e] = kNegInf;
+            }
         float vm = v[0][0];
 #pragma unroll
-        for (int u = 0; u < K; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < N; ++e) vm = fmaxf(vm, v[u][e]);
         if (vm > m) {
-            s *= (S)exp2_hw((m - vm) * k.c_hi);  // 0 for the first
+            s *= (S)exp_of(m - vm, k);  // 0 for the first
             m = vm;
         }
         const float base = base_of(m);
-        float ps[K];
+        float ps[U];
 #pragma unroll
-        for (int u = 0; u < K; ++u) {
+        for (int u = 0; u < U; ++u) {
             ps[u] = 0.f;
 #pragma unroll
             for (int e = 0; e < N; ++e) ps[u] += term_of(v[u][e], base, k);
         }
 #pragma unroll
-        for (int u = K; u > 1; u /= 2)
+        for (int u = U; u > 1; u /= 2)
 #pragma unroll
             for (int i = 0; i < u / 2; ++i) ps[i] = ps[i] + ps[i + u / 2];
         s += ps[0];
     };
-    for (; c < nvec - (U - 1) * NT; c += U * NT) group(c, std::integral_constant<int, U>{});
-    for (; c < nvec; c += NT) group(c, std::integral_constant<int, 1>{});
+    for (; c < nvec - (U - 1) * NT; c += U * NT) group(std::true_type{});
+    if (c < nvec) group(std::false_type{});
     return Stat<S>{m, s};
 }
 // with the thread's element of the row's edges, if it has one
@@ -128,7 +138,7 @@ __device__ __forceinline__ Stat<S> edge_stat(const T* __restrict__ xr, int vocab
     const int64_t j = span.edge((int)threadIdx.x, vocab);
     if (j < 0) return st;
     const float v = Elem<T>::load(xr, j);
-    return stat_join(st, Stat<S>{v, (S)term_of(v, base_of(v), k)}, k.c_hi);
+    return stat_join(st, Stat<S>{v, (S)term_of(v, base_of(v), k)}, k);
 }
 template <typename T, int NT, typename S>
 __device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
@@ -206,7 +216,7 @@ __global__ __launch_bounds__(NT) void parts_k(int vocab, const T* __restrict__ l
     const int hi = lo + share < (int)span.nvec ? lo + share : (int)span.nvec;
     Stat<double> st = vec_stat<T, NT, double, 4>(xr + span.head, lo + (int)threadIdx.x, hi, k);
     if (blockIdx.y == 0) st = edge_stat(xr, vocab, span, st, k);
-    st = wg_stat<NT>(st, k.c_hi, red);
+    st = wg_stat<NT>(st, k, red);
     if (threadIdx.x == 0) part[row * gridDim.y + blockIdx.y] = st;
 }
 // The thread's part of a row, for wg_stat.
@@ -241,7 +251,7 @@ __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__
     Stat<double> v;
     if constexpr (SPLIT) v = own_part(part, row, parts);
     else v = row_stat<T, NT, double>(xr, vocab, k);
-    v = wg_stat<NT>(v, k.c_hi, red);
+    v = wg_stat<NT>(v, k, red);
     if (threadIdx.x == 0) {
         const double x = t < (uint32_t)vocab ? from_raw<T>(xt) : __builtin_nanf("");
         logp[row] = (L)((x - (double)v.m) * k.inv_t64 - log(v.s));
@@ -257,7 +267,7 @@ __device__ __forceinline__ void preference_score(const mc_preference_desc& d, in
     const double inv = d.average && n > 0.0 ? 1.0 / n : 1.0;
     score[q] = sum * inv;
     inv_n[q] = (float)inv;
-    if (rewards) rewards[q] = (float)(d.beta * score[q]);
+    if (rewards) rewards[q] = (float)(d.beta * (sum * inv));
 }
 // The thread's tokens at, at + step, .. of sequence q, eight loaded together.
 __device__ __forceinline__ void preference_sum(const mc_preference_desc& d, int64_t q, int at, int step,
@@ -322,15 +332,41 @@ __device__ __forceinline__ void preference_pairs(const mc_preference_desc& d, co
     if (threadIdx.x == 0) loss[0] = (float)(sum[0] / pairs);
 }
 
-// All in one workgroup, a wave per sequence (kOneGroupRows).
+// All in one workgroup, a wave per sequence.
+constexpr int kOneGroupSeqs = 512;
 template <int NT>
 __global__ __launch_bounds__(NT) void preference_one_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
                                                        const double* __restrict__ logp, const float* __restrict__ ref,
-                                                       double* __restrict__ score, float* __restrict__ inv_n,
                                                        float* __restrict__ loss, float* __restrict__ rewards,
                                                        float* __restrict__ dseq) {
-    __shared__ double red[NT / 64][2];
-    for (int64_t q = wave_id(); q < 2 * d.pairs; q += NT / 64) {
+    constexpr int W = NT / 64;
+    __shared__ double red[W][2];
+    __shared__ double score[kOneGroupSeqs];
+    __shared__ float inv_n[kOneGroupSeqs];
+    if (2 * d.pairs < W) {  // the waves of a sequence, side by side
+        const int share = W / (int)(2 * d.pairs), q = wave_id() / share;
+        double v[2] = {0.0, 0.0};
+        if (q < 2 * d.pairs)
+            preference_sum(d, q, wave_id() % share * kWave + lane_id(), share * kWave, targets, logp, ref, v);
+        v[0] = wave_sum(v[0]);
+        v[1] = wave_sum(v[1]);
+        if (lane_id() == 0) {
+            red[wave_id()][0] = v[0];
+            red[wave_id()][1] = v[1];
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < 2 * d.pairs) {
+            v[0] = v[1] = 0.0;
+            for (int w = 0; w < share; ++w) {
+                v[0] += red[threadIdx.x * share + w][0];
+                v[1] += red[threadIdx.x * share + w][1];
+            }
+            preference_score(d, threadIdx.x, v[0], v[1], score, inv_n, rewards);
+        }
+        __syncthreads();
+        return preference_pairs<NT>(d, score, inv_n, red, loss, dseq);
+    }
+    for (int64_t q = wave_id(); q < 2 * d.pairs; q += W) {
         double v[2] = {0.0, 0.0};
         preference_sum(d, q, lane_id(), kWave, targets, logp, ref, v);
         v[0] = wave_sum(v[0]);
@@ -580,7 +616,7 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
     Stat<float> st;
     if constexpr (SPLIT) st = float_stat(own_part(part, row, parts));
     else st = row_stat<T, NT, float>(xr, vocab, k);
-    st = wg_stat<NT>(st, k.c_hi, red);
+    st = wg_stat<NT>(st, k, red);
     const RowStat v{st.m, st.s};
     entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
     __syncthreads();
@@ -655,26 +691,30 @@ template <int NT> __device__ __forceinline__ RowThreads row_threads() {
     return RowThreads{(int)(blockIdx.y * NT + threadIdx.x), (int)(gridDim.y * NT)};
 }
 
-// Vectors c, c - step, .. down to lo: U requested at a time.
+// Vectors c, c - step, .. down to lo: U requested at a time, the last together.
 template <typename T, int U>
 __device__ __forceinline__ void write_vecs(const T* __restrict__ xv, T* __restrict__ dv, int c, int step, int lo,
                                            bool stream, RowGrad grad) {
     constexpr int N = Vec16<T>::N;
-    auto group = [&](int c, auto count) {
-        constexpr int K = decltype(count)::value;
-        float v[K][N];
+    auto group = [&](auto whole) {
+        float v[U][N];
 #pragma unroll
-        for (int u = 0; u < K; ++u) Vec16<T>::load(xv + (int64_t)(c - u * step) * N, v[u]);
+        for (int u = 0; u < U; ++u) {
+            const int at = c - u * step;
+            Vec16<T>::load(xv + (int64_t)(decltype(whole)::value || at >= lo ? at : c) * N, v[u]);
+        }
 #pragma unroll
-        for (int u = 0; u < K; ++u) {
+        for (int u = 0; u < U; ++u) {
+            const int at = c - u * step;
+            if (!decltype(whole)::value && at < lo) break;
 #pragma unroll
             for (int e = 0; e < N; ++e) v[u][e] = grad(v[u][e]);
-            if (stream) store_nt16(dv + (int64_t)(c - u * step) * N, v[u]);
-            else Vec16<T>::store(dv + (int64_t)(c - u * step) * N, v[u]);
+            if (stream) store_nt16(dv + (int64_t)at * N, v[u]);
+            else Vec16<T>::store(dv + (int64_t)at * N, v[u]);
         }
     };
-    for (; c >= lo + (U - 1) * step; c -= U * step) group(c, std::integral_constant<int, U>{});
-    for (; c >= lo; c -= step) group(c, std::integral_constant<int, 1>{});
+    for (; c >= lo + (U - 1) * step; c -= U * step) group(std::true_type{});
+    if (c >= lo) group(std::false_type{});
 }
 template <typename T>
 __device__ __forceinline__ void write_row(const T* __restrict__ xr, T* __restrict__ dr, int vocab, bool vec,
@@ -774,7 +814,7 @@ __global__ __launch_bounds__(NT) void lp_bwd_k(int64_t rows, int vocab, bool vec
     }
     g *= k.inv_t;
     const T* xr = logits + row * vocab;
-    const RowGrad grad = row_grad(-g, stats[row], k.c_hi);
+    const RowGrad grad = row_grad(-g, stats[row], k.c);
     write_row(xr, dr, vocab, vec, stream, th, grad);
     const RowSpan<T> span(xr, vocab);
     if (t < (uint32_t)vocab &&
@@ -820,7 +860,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
         zero_row(dr, vocab, stream, th);
         return;
     }
-    const RowGrad grad = row_grad(w * ts.P, v, k.c_hi);
+    const RowGrad grad = row_grad(w * ts.P, v, k.c);
     write_row(xr, dr, vocab, vec, stream, th, grad);
     owners.patch(te, d.top, dr, grad, w);
 }
@@ -885,7 +925,7 @@ template <typename T, int NT, int NV, bool REST> struct HeldRow {
                 for (int e = 0; e < N; ++e) vm = fmaxf(vm, v[g][e]);
             }
             if (vm > m) {
-                s *= exp2_hw((m - vm) * k.c_hi);
+                s *= exp_of(m - vm, k);
                 m = vm;
             }
             const float base = base_of(m);
@@ -900,10 +940,10 @@ template <typename T, int NT, int NV, bool REST> struct HeldRow {
         }
         Stat<float> st{m, s};
         if constexpr (REST)
-            st = stat_join(st, vec_stat<T, NT, float, G>(xv, NT * NV + (int)threadIdx.x, nvec, k), k.c_hi);
+            st = stat_join(st, vec_stat<T, NT, float, G>(xv, NT * NV + (int)threadIdx.x, nvec, k), k);
         if (j >= 0) {
             const float x = from_raw<T>(edge);
-            st = stat_join(st, Stat<float>{x, term_of(x, base_of(x), k)}, k.c_hi);
+            st = stat_join(st, Stat<float>{x, term_of(x, base_of(x), k)}, k);
         }
         return st;
     }
@@ -1045,7 +1085,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool st
     Row held;
     held.load(xr, vocab, parts, row, th);
     count.put(len, redc, [&](uint32_t w) { return counted(w, d.ignore_index); });
-    const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
+    const Stat<float> st = wg_stat<NT>(held.stat(k), k, red);
     const RowStat v{st.m, st.s};
     const uint32_t share = count.total(redc, given ? given + (by_seq ? q : 0) : nullptr, n_given);
     const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
@@ -1059,7 +1099,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool st
         return;
     }
     g *= k.inv_t;
-    const RowGrad grad = row_grad(-g, v, k.c_hi);
+    const RowGrad grad = row_grad(-g, v, k.c);
     held.store(dr, stream, grad);
     if (in && held.owner((int)t) == th.self)
         Elem<T>::store(dr, t, grad(from_raw<T>(xt)) + g);
@@ -1109,7 +1149,7 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool 
     if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab) 
         owners.insert(held.owner(entry.id), (int)(blockIdx.y * NT));
     const uint32_t x = entry.logit(xr, vocab);
-    const Stat<float> st = wg_stat<NT>(held.stat(k), k.c_hi, red);
+    const Stat<float> st = wg_stat<NT>(held.stat(k), k, red);
     const RowStat v{st.m, st.s};
     entry.close(d, tlse != nullptr, lse, from_raw<T>(x), v, k, te);
     float w = d.temperature / (mask ? (float)count.total(redc, given, n_given) : (float)d.rows) * up;
@@ -1121,7 +1161,7 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool 
         zero_row(dr, vocab, stream, th);
         return;
     }
-    const RowGrad grad = row_grad(w * ts.P, v, k.c_hi);
+    const RowGrad grad = row_grad(w * ts.P, v, k.c);
     held.store(dr, stream, grad);
     owners.patch(te, d.top, dr, grad, w);
 }
@@ -1131,7 +1171,7 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool 
 LpScale row_scale(float temperature) {
     const double c = 1.4426950408889634074 / (double)temperature;
     LpScale k;
-    k.c_hi = (float)c;
+    k.c = k.c_hi = (float)c;
     if ((double)k.c_hi >= c) k.c_hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, k.c_hi) - 1);
     k.c_lo = (float)(c - (double)k.c_hi);
     k.inv_t64 = 1.0 / (double)temperature;
@@ -1167,26 +1207,23 @@ template <typename T> struct Split {
     typedef SplitRow<T, kPartThreads> Row;
 };
 // fn(element type, source): the parts of split rows, the smallest held shape of
-// at least MIN threads for a row, or the largest with the rest of the row read
+// at least `least` threads for a row, or the largest with the rest of the row read
 // twice. us of held rows alone, by threads x vectors:
 //   16 KB rows, 8192   128x8 49.5, 256x4 47.4, 512x4 58.4
 //   32 KB rows, 8192   512x4 88.9, 256x8 92.5, 512x8 87.4
 //   64 KB rows, 4000   512x8 88.9, 512x13 83.7, 1024x4 115
 //   98 KB rows, 4816   512x13 165, 1024x8 195
 //   201 KB rows, 2036  1024x13 139, 1024x16 140, 1024x19 142
-template <int MIN, typename F> void by_row_source(int parts, int64_t vocab, int dtype, F&& fn) {
+template <typename F> void by_row_source(int least, int parts, int64_t vocab, int dtype, F&& fn) {
     auto go = [&](auto elem) {
         typedef decltype(elem) T;
         if (parts > 1) return fn(elem, Split<T>{});
         const int64_t vectors = vocab / Vec16<T>::N;
         auto shape = [&](auto s) {
             typedef decltype(s) S;
-            if constexpr (S::kThreads >= MIN) {
-                if (!S::kRest && vectors > S::kThreads * S::kVectors) return false;
-                fn(elem, s);
-                return true;
-            }
-            return false;
+            if (S::kThreads < least || (!S::kRest && vectors > S::kThreads * S::kVectors)) return false;
+            fn(elem, s);
+            return true;
         };
         // a rest's vectors need registers of their own, unpacked
         constexpr int kWithRest = Vec16<T>::N == 4 ? 16 : 8;
@@ -1225,17 +1262,17 @@ size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace
 
 // ------------------------------------------------------------- launchers
-size_t loss_parts_ws(int64_t rows, int64_t vocab, int dtype) {
-    const int64_t parts = loss_row_parts(rows, row_bytes(vocab, dtype));
+size_t loss_parts_ws(int64_t rows, int64_t vocab, int dtype, bool both) {
+    const int64_t parts = loss_row_parts(rows, vocab, dtype == MC_F32 ? 4 : 2, both);
     return parts > 1 ? align256((size_t)(rows * parts) * sizeof(Stat<double>)) : 0;
 }
 
 namespace {
 // The statistics of a row's parts into ws (loss_parts_ws bytes) and their number,
 // or 1: not split.
-int launch_parts(int64_t rows, int64_t vocab, int dtype, const void* logits, const uint32_t* targets,
+int launch_parts(bool both, int64_t rows, int64_t vocab, int dtype, const void* logits, const uint32_t* targets,
                  int64_t ignore_index, const uint8_t* mask, LpScale k, void* ws, hipStream_t stream) {
-    const int parts = (int)loss_row_parts(rows, row_bytes(vocab, dtype));
+    const int parts = loss_row_parts(rows, vocab, dtype == MC_F32 ? 4 : 2, both);
     if (parts == 1) return 1;
     by_threads(kPartThreads, dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
@@ -1253,7 +1290,7 @@ hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const ui
                           uint32_t* counter, void* parts_ws, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
     const int parts =
-        launch_parts(d.rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
+        launch_parts(false, d.rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
     const int threads = parts > 1 ? 64 : loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype));
     by_threads(threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
@@ -1305,7 +1342,7 @@ PreferenceWs preference_ws(const mc_preference_desc& d) {
     w.inv_n = at;
     at += align256((size_t)(2 * d.pairs) * sizeof(float));
     w.parts = at;
-    w.total = at + loss_parts_ws(2 * d.pairs * d.seq, d.vocab, d.dtype);
+    w.total = at + loss_parts_ws(2 * d.pairs * d.seq, d.vocab, d.dtype, false);
     return w;
 }
 
@@ -1322,10 +1359,10 @@ hipError_t launch_preference_fwd(const mc_preference_desc& d, const void* logits
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, 1.0f, d.dtype};
     hipError_t e = launch_lp_rows(lp, logits, targets, logp, stats, counter, ws + w.parts, stream);
     if (e != hipSuccess) return e;
-    if (rows <= kOneGroupRows)
+    if (rows <= kOneGroupRows && 2 * d.pairs <= kOneGroupSeqs)
         by_group_size(rows, [&](auto threads) {
             constexpr int NT = decltype(threads)::value;
-            preference_one_k<NT><<<dim3(1), NT, 0, stream>>>(d, targets, logp, ref, score, inv_n, loss, rewards, dseq);
+            preference_one_k<NT><<<dim3(1), NT, 0, stream>>>(d, targets, logp, ref, loss, rewards, dseq);
         });
     else
         preference_k<<<dim3((unsigned)(2 * d.pairs)), 256, 0, stream>>>(d, targets, logp, ref, score, inv_n, counter,
@@ -1341,7 +1378,7 @@ PolicyWs policy_ws(const mc_policy_desc& d) {
     w.counts = at;
     if (d.reduction == MC_MEAN_SEQUENCES) at += align256((size_t)d.batch * sizeof(uint32_t));
     w.parts = at;
-    w.total = at + loss_parts_ws(d.batch * d.seq, d.vocab, d.dtype);
+    w.total = at + loss_parts_ws(d.batch * d.seq, d.vocab, d.dtype, false);
     return w;
 }
 
@@ -1392,7 +1429,7 @@ DistillWs distill_ws(const mc_distill_desc& d) {
     w.kl = at;
     at += align256((size_t)d.rows * sizeof(float));
     w.split = at;
-    w.total = at + loss_parts_ws(d.rows, d.vocab, d.dtype);
+    w.total = at + loss_parts_ws(d.rows, d.vocab, d.dtype, false);
     return w;
 }
 
@@ -1416,9 +1453,10 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
     const LpScale k = row_scale(d.temperature);
     uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     float* kl = reinterpret_cast<float*>(ws + w.kl);
-    const int parts = launch_parts(d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, ws + w.split, stream);
+    const int parts =
+        launch_parts(false, d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, ws + w.split, stream);
     int threads = parts > 1 ? kDistillMaxTop : loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype));
-    if (threads < kDistillMaxTop) threads = kDistillMaxTop;  // a thread per entry
+    while (threads < d.top) threads *= 2;  // a thread per entry
     by_threads(threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
@@ -1432,7 +1470,7 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
         if constexpr (NT == kDistillMaxTop) {
             if (parts > 1) return go(std::true_type{});
         }
-        if constexpr (NT >= kDistillMaxTop) go(std::false_type{});
+        go(std::false_type{});
     });
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1469,10 +1507,14 @@ int launch_counts(int64_t rows, const uint32_t* targets, const uint8_t* mask, in
 }
 }  // namespace
 
-// The forward's buffers, then 64 counts or, where no shape holds a row, the
-// forward's stats.
+// The forward's buffers, then 64 counts or, where the two run one after the
+// other, the forward's stats; then the parts of shared rows.
+namespace {
+size_t loss_stats_ws(int64_t n) { return align256((size_t)(n + kCountBlocks) * sizeof(float)); }
+}  // namespace
 size_t policy_fwd_bwd_ws(const mc_policy_desc& d) {
-    return policy_ws(d).total + align256((size_t)(3 * d.batch * d.seq + kCountBlocks) * sizeof(float));
+    const int64_t rows = d.batch * d.seq;
+    return policy_ws(d).total + loss_stats_ws(3 * rows) + loss_parts_ws(rows, d.vocab, d.dtype, true);
 }
 
 hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, const uint32_t* targets,
@@ -1488,11 +1530,11 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         const bool by_seq = d.reduction == MC_MEAN_SEQUENCES;
         uint32_t* n = by_seq ? reinterpret_cast<uint32_t*>(ws + w.counts) : nullptr;
-        void* parts_ws = ws + w.parts;
+        void* parts_ws = ws + w.total + loss_stats_ws(3 * rows);
         const int parts =
-            launch_parts(rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
+            launch_parts(true, rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
         e = hipSuccess;
-        by_row_source<64>(parts, d.vocab, d.dtype, [&](auto elem, auto source) {
+        by_row_source(1, parts, d.vocab, d.dtype, [&](auto elem, auto source) {
             typedef decltype(elem) T;
             typedef decltype(source) S;
             constexpr int NT = S::kThreads;
@@ -1518,7 +1560,7 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
 }
 
 size_t distill_fwd_bwd_ws(const mc_distill_desc& d) {
-    return distill_ws(d).total + align256((size_t)(2 * d.rows + kCountBlocks) * sizeof(float));
+    return distill_ws(d).total + loss_stats_ws(2 * d.rows) + loss_parts_ws(d.rows, d.vocab, d.dtype, true);
 }
 
 hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, const int32_t* ids, const float* tl,
@@ -1532,9 +1574,10 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
         uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
         float* kl = reinterpret_cast<float*>(ws + w.kl);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
-        void* parts_ws = ws + w.split;
-        const int parts = launch_parts(d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, parts_ws, stream);
-        by_row_source<kDistillMaxTop>(parts, d.vocab, d.dtype, [&](auto elem, auto source) {
+        void* parts_ws = ws + w.total + loss_stats_ws(2 * d.rows);
+        const int parts =
+            launch_parts(true, d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, parts_ws, stream);
+        by_row_source(d.top, parts, d.vocab, d.dtype, [&](auto elem, auto source) {
             typedef decltype(elem) T;
             typedef decltype(source) S;
             constexpr int NT = S::kThreads;

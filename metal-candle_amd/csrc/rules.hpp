@@ -45,32 +45,42 @@ constexpr bool xent_stream_gradients(int64_t rows, int64_t vocab, int elem_size)
 constexpr bool loss_threads_fit(int64_t rows, int threads) { return rows <= (((int64_t)1 << 32) - 1) / threads; }
 
 // Threads that read a row of logits for its statistics. Short rows leave most
-// threads of a large workgroup without a vector; of long ones few large
-// workgroups keep fewer rows open, once every CU has several. us, 64 / 128 / 256 /
-// 512 / 1024 threads:
-//   2 KB rows, 16384     14.3 / 19.2 / 28.7 / 52.1
-//   8 KB rows, 16384     29.4 / 31.4 / 38.1 / 57.4
-//   16 KB rows, 8192     32.7 / 31.6 / 33.8 / 47.6
-//   32 KB rows, 4000     30.8 / 29.7 / 30.5 / 34.0
-//   64 KB rows, 2000     26.8 / 28.2 / 28.4 / 28.0
-//   98 KB rows, 3624              256 70.2 / 65.3 / 78.4
-//   201 KB rows, 1511             256 59.6 / 57.6 / 55.2
-//   304 KB rows, 64 18.2 / 13.7 / 13.6; 256 19.4 / 15.1 / 16.6; 400 28.3 / 26.7 / 28.8;
-//                1200 68.6 / 66.3 / 65.6; 3024 165 / 165 / 156
+// threads of a large workgroup without a vector; long ones are read fastest by
+// few large workgroups, but where a CU gets two or three rows these come in
+// rounds. us, 64 / 128 / 256 / 512 / 1024 threads:
+//   2 KB rows, 16384  14.3 / 19.2 / 28.7 / 52.1     8 KB, 16384  29.4 / 31.4 / 38.1 / 57.4
+//   16 KB, 8192       32.7 / 31.6 / 33.8 / 47.6     32 KB, 4000  30.8 / 29.7 / 30.5 / 34.0
+// 256 / 512 / 1024 threads:
+//   98 KB, 300   10.9 / 10.9 / 13.1   98 KB, 3624  70.2 / 65.3 / 78.4
+//   201 KB, 600  25.1 / 26.5 / 25.5   201 KB, 1511 59.6 / 57.6 / 55.2
+//   304 KB, 200  18.3 / 14.6 / 14.5   304 KB, 300  25.2 / 24.0 / 25.8   304 KB, 520 34.9 / 41.0 / 38.6
+//   304 KB, 777  51.7 / 52.0 / 50.7   304 KB, 1200 68.2 / 68.1 / 65.4   304 KB, 3024 165 / 165 / 156
+//   608 KB, 700  73.8 / 75.4 / 73.3
 constexpr int loss_row_threads(int64_t rows, int64_t row_bytes) {
     if (row_bytes < 4 << 10) return 64;
     if (row_bytes < 24 << 10) return 128;
     if (row_bytes < 64 << 10 || !loss_threads_fit(rows, 1024)) return 256;
-    return row_bytes < 192 << 10 || rows < 768 ? 512 : 1024;
+    if (rows <= 256) return 512;
+    if (rows < 768) return 256;
+    return row_bytes < 192 << 10 ? 512 : 1024;
 }
 
 // Workgroups of 256 threads that share a row's statistics (1: none do), where
-// there are few long rows: one CU reads about 30 bytes a ns.
-constexpr int64_t loss_row_parts(int64_t rows, int64_t row_bytes) {
-    if (rows > 128 || row_bytes < 96 << 10) return 1;
-    const int64_t wanted = (1024 + rows - 1) / rows, most = row_bytes / (8 << 10);
-    const int64_t parts = wanted < most ? wanted : most;
-    return parts < 32 ? parts : 32;
+// there are few long rows and one CU would read each (about 30 bytes a ns). They
+// cost a launch. us, one / shared by 512 / rows, at most 32:
+//   forward   304 KB rows, 1 12.0 / 7.5, 64 13.1 / 9.7, 128 13.6 / 12.3
+//             201 KB rows, 50 7.5 / 7.9   98 KB rows, 20 6.8 / 7.2
+//   forward and backward, whose held rows a CU also takes one by one
+//             bf16 of 151936, 4 22.1 / 9.4, 32 23.1 / 12.0, 64 24.2 / 15.8, 100 24.9 / 22.5
+//             f32 of 151936, 4 22.4 / 9.1, 32 25.7 / 14.4, 64 28.1 / 22.7, 100 31.2 / 33.7
+//             bf16 of 100000, 64 18.5 / 12.8   f32 of 50257, 16 11.5 / 8.5, 32 12.0 / 9.9, 64 13.0 / 12.0
+//             bf16 of 50257, 32 10.7 / 8.9, 64 11.1 / 10.5   of 32000, 4 7.9 / 8.2
+constexpr int loss_row_parts(int64_t rows, int64_t vocab, int elem_size, bool both) {
+    const int most = !both ? (vocab * elem_size >= 256 << 10 ? 128 : 0)
+                     : vocab >= 96000 ? (elem_size == 2 ? 128 : 64) : vocab >= 48000 ? 32 : 0;
+    if (rows > most) return 1;
+    const int64_t parts = 512 / rows;
+    return parts < 32 ? (int)parts : 32;
 }
 
 // Threads that write a row's gradient, and workgroups that share a row where

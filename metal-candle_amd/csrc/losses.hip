@@ -766,25 +766,48 @@ template <int NT> struct TopOwners {
         const int k = threadIdx.x;
         if ((unsigned)(owner - first) < (unsigned)NT) atomicOr(&bits[(k >> 5) * NT + owner - first], 1u << (k & 31));
     }
-    template <typename F> __device__ __forceinline__ void each(int top, F&& fn) const {
-        for (int w = 0; w < (top + 31) / 32; ++w)
-            for (uint32_t b = bits[w * NT + threadIdx.x]; b; b &= b - 1) fn(32 * w + __ffs(b) - 1);
-    }
-    // The thread's entries' elements, once the row is stored: w p_k less, for all
-    // the entries of an id, in the order of k.
+    // The thread's entries' elements, once the row is stored: w times the entry's p
+    // less. Entries of one id come in the order of k, each with the sum so far, so
+    // that the last one leaves the whole: of up to four entries the sums before are
+    // in registers, more than that (several in one thread's vectors, or one id many
+    // times) are searched. Searching for every thread took 108 us in place of 97 for
+    // 2000 rows of 50257 bf16 logits and 256 entries, 63 in place of 43 for 4000 of
+    // 8000.
     template <typename T>
     __device__ __forceinline__ void patch(const Teacher& te, int top, T* __restrict__ dr, RowGrad grad, float w) const {
-        each(top, [&](int k) {
-            const int id = te.id[k];
-            float p = 0.f;
-            bool first = true;
-            each(top, [&](int o) {
-                if (te.id[o] != id) return;
-                first = first && o >= k;
-                p += te.p[o];
-            });
-            if (first) Elem<T>::store(dr, id, grad(te.x[k]) - w * p);
-        });
+        constexpr int W = kDistillMaxTop / 32, kKept = 3;
+        uint32_t own[W];
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            own[i] = 32 * i < top ? bits[i * NT + threadIdx.x] : 0;
+            count += __popc(own[i]);
+        }
+        int ids[kKept] = {-1, -1, -1};
+        float sums[kKept] = {};
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            for (uint32_t b = own[i]; b; b &= b - 1) {
+                const int k = 32 * i + __ffs(b) - 1, id = te.id[k];
+                float p = te.p[k];
+                if (count <= kKept + 1) {
+                    float before = 0.f;
+#pragma unroll
+                    for (int o = kKept - 1; o >= 0; --o) before = ids[o] == id ? sums[o] : before;
+                    p += before;
+#pragma unroll
+                    for (int o = kKept - 1; o > 0; --o) {
+                        ids[o] = ids[o - 1];
+                        sums[o] = sums[o - 1];
+                    }
+                    ids[0] = id;
+                    sums[0] = p;
+                } else {
+                    p = 0.f;
+                    for (int o = 0; o <= k; ++o) p += te.id[o] == id ? te.p[o] : 0.f;
+                }
+                Elem<T>::store(dr, id, grad(te.x[k]) - w * p);
+            }
     }
 };
 

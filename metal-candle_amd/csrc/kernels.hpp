@@ -220,7 +220,7 @@ hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logit
 hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
                                      const float* stats, const float* dl, int64_t seq, const float* scale,
                                      const float* dloss, void* dlogits, hipStream_t stream);
-// Workspaces (byte offsets): a counter at 0, then
+// Workspaces (byte offsets).
 struct PreferenceWs {
     size_t logp;   // f64 [2 pairs seq]
     size_t score;  // f64 [2 pairs]

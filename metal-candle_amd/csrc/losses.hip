@@ -147,9 +147,7 @@ __device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab,
     return edge_stat(xr, vocab, span, vec_stat<T, NT, S, 4>(xr + span.head, threadIdx.x, (int)span.nvec, k), k);
 }
 
-// -------------------------------------------------- sums over many workgroups
-// Each workgroup leaves its partial sums in memory; the last one to arrive adds
-// them in workgroup order. The kernel before on the stream clears the counter.
+// ------------------------------------------------- sums over a workgroup
 template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
@@ -180,18 +178,6 @@ template <int NT, int C> __device__ __forceinline__ void wg_sum_f64(double (&v)[
 #pragma unroll
         for (int w = 1; w < NT / 64; ++w) v[c] += red[w][c];
     }
-}
-
-// True in every thread of the workgroup that arrives last; what the others wrote
-// before is visible to it.
-__device__ __forceinline__ bool last_to_arrive(uint32_t* counter, uint32_t* slot) {
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) *slot = atomicAdd(counter, 1u);
-    __syncthreads();
-    const bool last = *slot == gridDim.x - 1;
-    if (last) __threadfence();
-    return last;
 }
 
 // ------------------------------------------------------------- row kernels
@@ -228,16 +214,14 @@ __device__ __forceinline__ Stat<float> float_stat(Stat<double> v) { return Stat<
 
 // l (0 where the row is not counted) and the row's statistics, read from the
 // logits or (SPLIT) joined from its parts; a counted target past the vocabulary
-// makes its l NaN. counter: cleared for the kernel that follows. L: float, or
-// double for sums over answers.
+// makes its l NaN. L: float, or double for sums over answers.
 template <typename T, int NT, typename L, bool SPLIT>
 __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__ logits,
                                                 const uint32_t* __restrict__ targets, int64_t ignore_index, LpScale k,
                                                 const Stat<double>* __restrict__ part, int parts, L* __restrict__ logp,
-                                                RowStat* __restrict__ stats, uint32_t* __restrict__ counter) {
+                                                RowStat* __restrict__ stats) {
     __shared__ Stat<double> red[NT / 64];
     const int64_t row = blockIdx.x;
-    if (counter && row == 0 && threadIdx.x == 0) *counter = 0;
     const uint32_t t = targets[row];
     if (!counted(t, ignore_index)) {
         if (threadIdx.x == 0) {
@@ -332,8 +316,11 @@ __device__ __forceinline__ void preference_pairs(const mc_preference_desc& d, co
     if (threadIdx.x == 0) loss[0] = (float)(sum[0] / pairs);
 }
 
-// All in one workgroup, a wave per sequence.
-constexpr int kOneGroupSeqs = 512;
+// All in one workgroup, a wave per sequence or several: for few sequences, whose
+// tokens it would walk in rounds else. The whole forward over 64 logits, us, so /
+// as scores and pairs: 2 sequences of 128 tokens 7.0 / 8.2, 4 of 500 9.4 / 9.6, 40
+// of 50 11.4 / 9.7, 100 of 20 18.5 / 9.8.
+constexpr int kOneGroupSeqs = 16;
 template <int NT>
 __global__ __launch_bounds__(NT) void preference_one_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
                                                        const double* __restrict__ logp, const float* __restrict__ ref,
@@ -377,21 +364,24 @@ __global__ __launch_bounds__(NT) void preference_one_k(mc_preference_desc d, con
     preference_pairs<NT>(d, score, inv_n, red, loss, dseq);
 }
 
-// A workgroup per sequence; the last to arrive goes on to the pairs.
-__global__ __launch_bounds__(256) void preference_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
-                                                    const double* __restrict__ logp, const float* __restrict__ ref,
-                                                    double* score, float* inv_n, uint32_t* counter,
-                                                    float* __restrict__ loss, float* __restrict__ rewards,
-                                                    float* __restrict__ dseq) {
+// The scores alone, a workgroup per sequence, and the pairs.
+__global__ __launch_bounds__(256) void preference_scores_k(mc_preference_desc d, const uint32_t* __restrict__ targets,
+                                                           const double* __restrict__ logp,
+                                                           const float* __restrict__ ref, double* __restrict__ score,
+                                                           float* __restrict__ inv_n, float* __restrict__ rewards) {
     __shared__ double red[4][2];
-    __shared__ uint32_t slot;
     const int64_t q = blockIdx.x;
     double v[2] = {0.0, 0.0};
     preference_sum(d, q, (int)threadIdx.x, 256, targets, logp, ref, v);
     wg_sum_f64<256>(v, red);
     if (threadIdx.x == 0) preference_score(d, q, v[0], v[1], score, inv_n, rewards);
-    if (!last_to_arrive(counter, &slot)) return;
-    preference_pairs<256>(d, score, inv_n, red, loss, dseq);
+}
+template <int NT>
+__global__ __launch_bounds__(NT) void preference_pairs_k(mc_preference_desc d, const double* __restrict__ score,
+                                                         const float* __restrict__ inv_n, float* __restrict__ loss,
+                                                         float* __restrict__ dseq) {
+    __shared__ double red[NT / 64][2];
+    preference_pairs<NT>(d, score, inv_n, red, loss, dseq);
 }
 
 // ------------------------------------------------------------------ policy
@@ -442,19 +432,30 @@ __device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, float
     return p;
 }
 
+__device__ __forceinline__ void policy_finish(const mc_policy_desc& d, bool by_seq, const double (&v)[4],
+                                              float* __restrict__ loss, float* __restrict__ metrics,
+                                              float* __restrict__ dlp) {
+    const double N = by_seq ? (double)d.batch : v[3];  // no token at all: 0 / 0, a NaN loss
+    loss[0] = (float)(v[0] / N);
+    if (metrics) {
+        metrics[0] = (float)(v[1] / N);
+        metrics[1] = (float)(v[2] / N);
+    }
+    if (dlp) dlp[d.batch * d.seq] = (float)(1.0 / N);
+}
 // Workgroup b: rows b * chunk ..; sums of the terms, the KL, the clipped tokens
 // and the counted ones. n: counted tokens of each sequence where the mean runs
 // over sequences. dlp: dloss/dl but for the factor at dlp[rows], which is known
-// only at the end.
+// only at the end. One workgroup ends here; of several, policy_join_k adds the
+// sums in order.
 template <int NT>
 __global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, const uint32_t* __restrict__ targets,
                                                const float* __restrict__ logp, const float* __restrict__ adv,
                                                const float* __restrict__ old, const float* __restrict__ ref,
-                                               const uint32_t* __restrict__ n, double (*part)[4], uint32_t* counter,
+                                               const uint32_t* __restrict__ n, double (*part)[4],
                                                float* __restrict__ loss, float* __restrict__ metrics,
                                                float* __restrict__ dlp) {
     __shared__ double red[NT / 64][4];
-    __shared__ uint32_t slot;
     const int64_t rows = d.batch * d.seq, r0 = (int64_t)blockIdx.x * chunk;
     const int64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
     double v[4] = {0.0, 0.0, 0.0, 0.0};
@@ -490,24 +491,21 @@ __global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, 
         }
     }
     wg_sum_f64<NT>(v, red);
-    if (gridDim.x > 1) {
-        if (threadIdx.x == 0)
+    if (threadIdx.x != 0) return;
+    if (gridDim.x == 1) return policy_finish(d, n != nullptr, v, loss, metrics, dlp);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) part[blockIdx.x][c] = v[c];
-        if (!last_to_arrive(counter, &slot)) return;
+    for (int c = 0; c < 4; ++c) part[blockIdx.x][c] = v[c];
+}
+constexpr int kSumGroups = 256;  // at most, a thread of the join for each
+__global__ __launch_bounds__(kSumGroups) void policy_join_k(mc_policy_desc d, bool by_seq, int groups,
+                                                            const double (*part)[4], float* __restrict__ loss,
+                                                            float* __restrict__ metrics, float* __restrict__ dlp) {
+    __shared__ double red[kSumGroups / 64][4];
+    double v[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
-        wg_sum_f64<NT>(v, red);
-    }
-    if (threadIdx.x == 0) {
-        const double N = n ? (double)d.batch : v[3];  // no token at all: 0 / 0, a NaN loss
-        loss[0] = (float)(v[0] / N);
-        if (metrics) {
-            metrics[0] = (float)(v[1] / N);
-            metrics[1] = (float)(v[2] / N);
-        }
-        if (dlp) dlp[rows] = (float)(1.0 / N);
-    }
+    for (int c = 0; c < 4; ++c) v[c] = (int)threadIdx.x < groups ? part[threadIdx.x][c] : 0.0;
+    wg_sum_f64<kSumGroups>(v, red);
+    if (threadIdx.x == 0) policy_finish(d, by_seq, v, loss, metrics, dlp);
 }
 
 // ------------------------------------------------------------ distillation
@@ -594,13 +592,11 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
                                                      const int32_t* __restrict__ ids, const float* __restrict__ tl,
                                                      const float* __restrict__ tlse, const uint8_t* __restrict__ mask,
                                                      LpScale k, const Stat<double>* __restrict__ part, int parts,
-                                                     float* __restrict__ kl, RowStat* __restrict__ stats,
-                                                     uint32_t* __restrict__ counter) {
+                                                     float* __restrict__ kl, RowStat* __restrict__ stats) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ Teacher te;
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
-    if (row == 0 && threadIdx.x == 0) *counter = 0;
     if (mask && mask[row] == 0) {
         if (threadIdx.x == 0) {
             kl[row] = 0.f;
@@ -626,14 +622,19 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
     }
 }
 
-// loss = T^2 sum kl / counted rows; scale = T / counted rows.
+// loss = T^2 sum kl / counted rows; scale = T / counted rows. Workgroups as
+// policy_k's.
+__device__ __forceinline__ void distill_finish(double T, const double (&v)[2], float* __restrict__ loss,
+                                               float* __restrict__ scale) {
+    loss[0] = (float)(T * T * v[0] / v[1]);  // no row counted: 0 / 0, a NaN loss
+    if (scale) scale[0] = (float)(T / v[1]);
+}
 template <int NT>
 __global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chunk, float temperature,
                                                       const uint8_t* __restrict__ mask, const float* __restrict__ kl,
-                                                      double (*part)[2], uint32_t* counter, float* __restrict__ loss,
+                                                      double (*part)[2], float* __restrict__ loss,
                                                       float* __restrict__ scale) {
     __shared__ double red[NT / 64][2];
-    __shared__ uint32_t slot;
     const int64_t r0 = (int64_t)blockIdx.x * chunk;
     const int64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
     double v[2] = {0.0, 0.0};
@@ -654,21 +655,19 @@ __global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chun
         }
     }
     wg_sum_f64<NT>(v, red);
-    if (gridDim.x > 1) {
-        if (threadIdx.x == 0) {
-            part[blockIdx.x][0] = v[0];
-            part[blockIdx.x][1] = v[1];
-        }
-        if (!last_to_arrive(counter, &slot)) return;
+    if (threadIdx.x != 0) return;
+    if (gridDim.x == 1) return distill_finish(temperature, v, loss, scale);
+    part[blockIdx.x][0] = v[0];
+    part[blockIdx.x][1] = v[1];
+}
+__global__ __launch_bounds__(kSumGroups) void distill_join_k(float temperature, int groups, const double (*part)[2],
+                                                             float* __restrict__ loss, float* __restrict__ scale) {
+    __shared__ double red[kSumGroups / 64][2];
+    double v[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) v[c] = threadIdx.x < gridDim.x ? part[threadIdx.x][c] : 0.0;
-        wg_sum_f64<NT>(v, red);
-    }
-    if (threadIdx.x == 0) {
-        const double T = temperature;
-        loss[0] = (float)(T * T * v[0] / v[1]);  // no row counted: 0 / 0, a NaN loss
-        if (scale) scale[0] = (float)(T / v[1]);
-    }
+    for (int c = 0; c < 2; ++c) v[c] = (int)threadIdx.x < groups ? part[threadIdx.x][c] : 0.0;
+    wg_sum_f64<kSumGroups>(v, red);
+    if (threadIdx.x == 0) distill_finish(temperature, v, loss, scale);
 }
 
 // ---------------------------------------------------------------- gradients
@@ -1081,14 +1080,13 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool st
                                                        bool by_seq,
                                                        uint32_t* __restrict__ n, LpScale k,
                                                        const float* __restrict__ dloss, float* __restrict__ logp,
-                                                       T* __restrict__ dlogits, uint32_t* __restrict__ counter) {
+                                                       T* __restrict__ dlogits) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ uint32_t redc[NT / 64];
     const RowThreads th = row_threads<NT>();
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
     const bool writer = th.self == 0;
-    if (row == 0 && writer) *counter = 0;
     T* dr = dlogits + row * vocab;
     const uint32_t t = targets[row];
     if (!counted(t, d.ignore_index)) {
@@ -1139,7 +1137,7 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool 
                                                         const uint32_t* __restrict__ given, int n_given, int len,
                                                         LpScale k, const float* __restrict__ dloss,
                                                         float* __restrict__ kl,
-                                                        T* __restrict__ dlogits, uint32_t* __restrict__ counter) {
+                                                        T* __restrict__ dlogits) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ uint32_t redc[NT / 64];
     __shared__ Teacher te;
@@ -1148,7 +1146,6 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool 
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
     const bool writer = th.self == 0;
-    if (row == 0 && writer) *counter = 0;
     T* dr = dlogits + row * vocab;
     if (mask && mask[row] == 0) {
         if (writer) kl[row] = 0.f;
@@ -1264,19 +1261,24 @@ bool same_start(const void* a, const void* b) {
     return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
-// Rows whose sums one workgroup forms by itself; past it 256 workgroups, which
-// meet in the last one.
-constexpr int64_t kOneGroupRows = 8192;
+// Rows whose sums one workgroup forms by itself; past it up to 256 of them, and a
+// launch that joins theirs. A forward over 64 logits, us, one / more and the join:
+// policy 2000 rows 8.9 / 10.0, 4000 11.0 / 11.3, 8192 16.2 / 14.0, 16384 26.2 /
+// 19.8; distillation 4000 10.3 / 11.5, 16000 23.5 / 21.2. The join as the work of
+// whichever workgroup ends last took 35.3 at 16384: its fences cost more than a
+// launch. Threads of the one workgroup, 256 / 1024: 256 rows 6.4 / 7.0, 4000 13.4
+// / 11.4.
+constexpr int64_t kOneGroupRows = 4096;
 template <typename F> void by_group_size(int64_t rows, F&& fn) {
     if (rows <= 1024) fn(std::integral_constant<int, 256>{});
     else fn(std::integral_constant<int, 1024>{});
 }
 template <typename F> void by_sum_kernel(int64_t rows, F&& fn) {
     if (rows <= kOneGroupRows) {
-        by_group_size(rows, [&](auto threads) { fn(threads, dim3(1), rows); });
+        by_group_size(rows, [&](auto threads) { fn(threads, 1, rows); });
     } else {
-        const int64_t chunk = (rows + 255) / 256;
-        fn(std::integral_constant<int, 256>{}, dim3((unsigned)((rows + chunk - 1) / chunk)), chunk);
+        const int64_t even = (rows + kSumGroups - 1) / kSumGroups, chunk = even < 1024 ? 1024 : even;
+        fn(std::integral_constant<int, 256>{}, (int)((rows + chunk - 1) / chunk), chunk);
     }
 }
 
@@ -1310,7 +1312,7 @@ int launch_parts(bool both, int64_t rows, int64_t vocab, int dtype, const void* 
 
 template <typename L>
 hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, L* logp, float* stats,
-                          uint32_t* counter, void* parts_ws, hipStream_t stream) {
+                          void* parts_ws, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
     const int parts =
         launch_parts(false, d.rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
@@ -1322,7 +1324,7 @@ hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const ui
             constexpr bool SPLIT = decltype(split)::value;
             lp_rows_k<T, NT, L, SPLIT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
                 (int)d.vocab, static_cast<const T*>(logits), targets, d.ignore_index, k,
-                static_cast<const Stat<double>*>(parts_ws), parts, logp, reinterpret_cast<RowStat*>(stats), counter);
+                static_cast<const Stat<double>*>(parts_ws), parts, logp, reinterpret_cast<RowStat*>(stats));
         };
         if constexpr (NT == 64) {
             if (parts > 1) return go(std::true_type{});
@@ -1335,7 +1337,7 @@ hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const ui
 
 hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
                                      float* stats, void* ws, hipStream_t stream) {
-    return launch_lp_rows(d, logits, targets, logp, stats, nullptr, ws, stream);
+    return launch_lp_rows(d, logits, targets, logp, stats, ws, stream);
 }
 
 hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
@@ -1357,7 +1359,7 @@ hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logit
 
 PreferenceWs preference_ws(const mc_preference_desc& d) {
     PreferenceWs w;
-    size_t at = 256;  // the counter
+    size_t at = 0;
     w.logp = at;
     at += align256((size_t)(2 * d.pairs * d.seq) * sizeof(double));
     w.score = at;
@@ -1378,26 +1380,30 @@ hipError_t launch_preference_fwd(const mc_preference_desc& d, const void* logits
     double* score = reinterpret_cast<double*>(ws + w.score);
     float* inv_n = reinterpret_cast<float*>(ws + w.inv_n);
     float* dseq = stats ? stats + 2 * rows : nullptr;
-    uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, 1.0f, d.dtype};
-    hipError_t e = launch_lp_rows(lp, logits, targets, logp, stats, counter, ws + w.parts, stream);
+    hipError_t e = launch_lp_rows(lp, logits, targets, logp, stats, ws + w.parts, stream);
     if (e != hipSuccess) return e;
-    if (rows <= kOneGroupRows && 2 * d.pairs <= kOneGroupSeqs)
+    if (rows <= kOneGroupRows && 2 * d.pairs <= kOneGroupSeqs) {
         by_group_size(rows, [&](auto threads) {
             constexpr int NT = decltype(threads)::value;
             preference_one_k<NT><<<dim3(1), NT, 0, stream>>>(d, targets, logp, ref, loss, rewards, dseq);
         });
-    else
-        preference_k<<<dim3((unsigned)(2 * d.pairs)), 256, 0, stream>>>(d, targets, logp, ref, score, inv_n, counter,
-                                                                         loss, rewards, dseq);
+        return hipGetLastError();
+    }
+    preference_scores_k<<<dim3((unsigned)(2 * d.pairs)), 256, 0, stream>>>(d, targets, logp, ref, score, inv_n,
+                                                                          rewards);
+    by_group_size(d.pairs, [&](auto threads) {
+        constexpr int NT = decltype(threads)::value;
+        preference_pairs_k<NT><<<dim3(1), NT, 0, stream>>>(d, score, inv_n, loss, dseq);
+    });
     return hipGetLastError();
 }
 
 PolicyWs policy_ws(const mc_policy_desc& d) {
     PolicyWs w;
-    size_t at = 256;  // the counter
+    size_t at = 0;
     w.part = at;
-    at += 256 * 4 * sizeof(double);
+    at += kSumGroups * 4 * sizeof(double);
     w.counts = at;
     if (d.reduction == MC_MEAN_SEQUENCES) at += align256((size_t)d.batch * sizeof(uint32_t));
     w.parts = at;
@@ -1419,11 +1425,13 @@ const uint32_t* policy_counts(const mc_policy_desc& d, const uint32_t* targets, 
 hipError_t launch_policy_sums(const mc_policy_desc& d, const uint32_t* targets, const float* logp, const float* adv,
                               const float* old, const float* ref, const uint32_t* n, char* ws, float* loss,
                               float* metrics, float* dlp, hipStream_t stream) {
-    by_sum_kernel(d.batch * d.seq, [&](auto threads, dim3 grid, int64_t chunk) {
+    auto* part = reinterpret_cast<double(*)[4]>(ws + policy_ws(d).part);
+    by_sum_kernel(d.batch * d.seq, [&](auto threads, int groups, int64_t chunk) {
         constexpr int NT = decltype(threads)::value;
-        policy_k<NT><<<grid, NT, 0, stream>>>(d, chunk, targets, logp, adv, old, ref, n,
-                                              reinterpret_cast<double(*)[4]>(ws + policy_ws(d).part),
-                                              reinterpret_cast<uint32_t*>(ws), loss, metrics, dlp);
+        policy_k<NT><<<dim3((unsigned)groups), NT, 0, stream>>>(d, chunk, targets, logp, adv, old, ref, n, part, loss,
+                                                                metrics, dlp);
+        if (groups > 1)
+            policy_join_k<<<dim3(1), kSumGroups, 0, stream>>>(d, n != nullptr, groups, part, loss, metrics, dlp);
     });
     return hipGetLastError();
 }
@@ -1433,12 +1441,11 @@ hipError_t launch_policy_fwd(const mc_policy_desc& d, const void* logits, const 
                              const float* old, const float* ref, float* loss, float* logp, float* metrics,
                              float* stats, char* ws, hipStream_t stream) {
     const int64_t rows = d.batch * d.seq;
-    uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, d.temperature, d.dtype};
     hipError_t e;
     const uint32_t* n = policy_counts(d, targets, ws, stream, e);
     if (e != hipSuccess) return e;
-    e = launch_lp_rows(lp, logits, targets, logp, stats, counter, ws + policy_ws(d).parts, stream);
+    e = launch_lp_rows(lp, logits, targets, logp, stats, ws + policy_ws(d).parts, stream);
     if (e != hipSuccess) return e;
     return launch_policy_sums(d, targets, logp, adv, old, ref, n, ws, loss, metrics, stats ? stats + 2 * rows : nullptr,
                               stream);
@@ -1446,9 +1453,9 @@ hipError_t launch_policy_fwd(const mc_policy_desc& d, const void* logits, const 
 
 DistillWs distill_ws(const mc_distill_desc& d) {
     DistillWs w;
-    size_t at = 256;  // the counter
+    size_t at = 0;
     w.part = at;
-    at += 256 * 2 * sizeof(double);
+    at += kSumGroups * 2 * sizeof(double);
     w.kl = at;
     at += align256((size_t)d.rows * sizeof(float));
     w.split = at;
@@ -1459,11 +1466,13 @@ DistillWs distill_ws(const mc_distill_desc& d) {
 namespace {
 hipError_t launch_distill_sums(const mc_distill_desc& d, const uint8_t* mask, const float* kl, char* ws, float* loss,
                                float* scale, hipStream_t stream) {
-    by_sum_kernel(d.rows, [&](auto threads, dim3 grid, int64_t chunk) {
+    auto* part = reinterpret_cast<double(*)[2]>(ws + distill_ws(d).part);
+    by_sum_kernel(d.rows, [&](auto threads, int groups, int64_t chunk) {
         constexpr int NT = decltype(threads)::value;
-        distill_final_k<NT><<<grid, NT, 0, stream>>>(d.rows, chunk, d.temperature, mask, kl,
-                                                     reinterpret_cast<double(*)[2]>(ws + distill_ws(d).part),
-                                                     reinterpret_cast<uint32_t*>(ws), loss, scale);
+        distill_final_k<NT><<<dim3((unsigned)groups), NT, 0, stream>>>(d.rows, chunk, d.temperature, mask, kl, part,
+                                                                       loss, scale);
+        if (groups > 1)
+            distill_join_k<<<dim3(1), kSumGroups, 0, stream>>>(d.temperature, groups, part, loss, scale);
     });
     return hipGetLastError();
 }
@@ -1474,7 +1483,6 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
                               hipStream_t stream) {
     const DistillWs w = distill_ws(d);
     const LpScale k = row_scale(d.temperature);
-    uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
     float* kl = reinterpret_cast<float*>(ws + w.kl);
     const int parts =
         launch_parts(false, d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, ws + w.split, stream);
@@ -1487,8 +1495,7 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
             constexpr bool SPLIT = decltype(split)::value;
             distill_rows_k<T, NT, SPLIT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
                 d, static_cast<const T*>(logits), ids, tl, tlse, mask, k,
-                reinterpret_cast<const Stat<double>*>(ws + w.split), parts, kl, reinterpret_cast<RowStat*>(stats),
-                counter);
+                reinterpret_cast<const Stat<double>*>(ws + w.split), parts, kl, reinterpret_cast<RowStat*>(stats));
         };
         if constexpr (NT == kDistillMaxTop) {
             if (parts > 1) return go(std::true_type{});
@@ -1549,7 +1556,6 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
     const LpScale k = row_scale(d.temperature);
     hipError_t e;
     if (same_start(logits, dlogits) && loss_threads_fit(rows, 1024)) {
-        uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         const bool by_seq = d.reduction == MC_MEAN_SEQUENCES;
         uint32_t* n = by_seq ? reinterpret_cast<uint32_t*>(ws + w.counts) : nullptr;
@@ -1569,7 +1575,7 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
             policy_both_k<T, NT, typename S::Row><<<dim3((unsigned)rows, (unsigned)parts), NT, 0, stream>>>(
                 d, xent_stream_gradients(rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), targets, adv, old,
                 ref, static_cast<const Stat<double>*>(parts_ws), here ? nullptr : by_seq ? n : part, n_given,
-                here ? (int)span : 0, by_seq, here ? n : nullptr, k, dloss, logp, static_cast<T*>(dlogits), counter);
+                here ? (int)span : 0, by_seq, here ? n : nullptr, k, dloss, logp, static_cast<T*>(dlogits));
         });
         if (e != hipSuccess) return e;
         if ((e = hipGetLastError()) != hipSuccess) return e;
@@ -1594,7 +1600,6 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
     const LpScale k = row_scale(d.temperature);
     hipError_t e;
     if (same_start(logits, dlogits) && loss_threads_fit(d.rows, 1024)) {
-        uint32_t* counter = reinterpret_cast<uint32_t*>(ws);
         float* kl = reinterpret_cast<float*>(ws + w.kl);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         void* parts_ws = ws + w.total + loss_stats_ws(2 * d.rows);
@@ -1609,7 +1614,7 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
             distill_both_k<T, NT, typename S::Row><<<dim3((unsigned)d.rows, (unsigned)parts), NT, 0, stream>>>(
                 d, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl, tlse,
                 mask, static_cast<const Stat<double>*>(parts_ws), here ? nullptr : part, n_given,
-                mask && here ? (int)d.rows : 0, k, dloss, kl, static_cast<T*>(dlogits), counter);
+                mask && here ? (int)d.rows : 0, k, dloss, kl, static_cast<T*>(dlogits));
         });
         if ((e = hipGetLastError()) != hipSuccess) return e;
         return launch_distill_sums(d, mask, kl, ws, loss, nullptr, stream);

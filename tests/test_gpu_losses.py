@@ -606,6 +606,25 @@ def test_many_rows(mc, dev, rows, B):
     assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
 
 
+@pytest.mark.parametrize("rows", [1 << 22, (1 << 24) - 1])
+def test_rows_past_a_launch_of_large_workgroups(mc, dev, rows):
+    """2^32 work-items: rows that 1024 threads each no longer launch, and the most rows there may be."""
+    V = 3
+    x, t, l64, tol, q, old, ref, A = policy_case(dev, rows // 5 if rows % 5 == 0 else 1, 5 if rows % 5 == 0 else rows,
+                                                 V, torch.bfloat16, 0, True, 1.0, rows)
+    kw = dict(kl_coef=0.1, reduction="sequences")
+    outs = mc.policy_loss_forward_backward(x, t, A, old, ref, ignore_index=PAD, **kw)
+    check_policy(mc, dev, x, t, l64, tol, q, A, old, ref, kw, outs, 1.0, torch.bfloat16)
+    del outs, l64, tol, q, old, ref
+    flat, g = x.view(rows, V), gen(dev, 1)
+    ids = torch.randint(0, V, (rows, 2), generator=g, device=dev, dtype=torch.int32)
+    tl = torch.randn(rows, 2, generator=g, device=dev)
+    loss, d = mc.distillation_loss_forward_backward(flat, ids, tl)
+    want, dtol, grad, terms = plain_distill(flat, ids, tl, 1.0, None, None)
+    assert abs(float(loss) - float(want)) <= float(dtol) + 2.0 ** -23 * abs(float(want))
+    close_grad(d, grad, terms, torch.bfloat16)
+
+
 # ------------------------------------------------------- differences, together
 def losses_of(mc, name, x, extra):
     """(loss, dlogits) of one of the losses on [4, 5, V]."""
@@ -732,3 +751,20 @@ def test_results_repeat_and_replay(mc, dev):
         for i, (a, b, e) in enumerate(zip(outs, between, eager)):
             assert torch.equal(a, e), f"replay {rep}: output {i}"
             assert torch.equal(b, e), f"eager call between replays: output {i}"
+
+
+def test_calls_at_once_on_two_streams(mc, dev):
+    """Calls that overlap share nothing."""
+    c = sequence_case(dev)
+    eager = [o.clone() for o in sequence(mc, c)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(sequence(mc, c))
+    torch.cuda.synchronize()
+    for n, got in enumerate(outs):
+        for i, (a, e) in enumerate(zip(got, eager)):
+            assert torch.equal(a, e), f"call {n}: output {i}"

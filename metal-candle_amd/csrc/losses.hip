@@ -1513,7 +1513,7 @@ hipError_t launch_distill_bwd(const mc_distill_desc& d, const void* logits, cons
     const LpScale k = row_scale(d.temperature);
     const bool vec = same_start(logits, dlogits);
     const LossGrid grid = loss_grad_grid(d.rows, row_bytes(d.vocab, d.dtype));
-    by_threads(grid.threads, d.dtype, [&](auto elem, auto threads) {
+    by_threads(grid.threads < kDistillMaxTop ? kDistillMaxTop : grid.threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
         if constexpr (NT >= kDistillMaxTop)

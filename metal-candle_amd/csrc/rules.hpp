@@ -48,21 +48,23 @@ constexpr bool loss_threads_fit(int64_t rows, int threads) { return rows <= (((i
 // threads of a large workgroup without a vector; long ones are read fastest by
 // few large workgroups, but where a CU gets two or three rows these come in
 // rounds. us, 64 / 128 / 256 / 512 / 1024 threads:
-//   2 KB rows, 16384  14.3 / 19.2 / 28.7 / 52.1     8 KB, 16384  29.4 / 31.4 / 38.1 / 57.4
-//   16 KB, 8192       32.7 / 31.6 / 33.8 / 47.6     32 KB, 4000  30.8 / 29.7 / 30.5 / 34.0
+//   4 KB rows, 400    5.4 / 5.4 / 5.6 / 6.4 / 8.3     4 KB, 16384   17.6 / 26.0 / 42.8 / 67.3 / 132
+//   12 KB, 400        6.1 / 6.3 / 5.7 / 7.3 / 9.5     12 KB, 4096   13.7 / 15.3 / 15.1 / 24.7 / 42.8
+//   24 KB, 1000       9.8 / 9.5 / 10.4 / 10.5 / 16.5  24 KB, 2000   12.8 / 13.5 / 15.0 / 15.2 / 26.8
+//   32 KB, 4096       30.5 / 29.2 / 28.1 / 30.7 / 52.1
 // 256 / 512 / 1024 threads:
-//   98 KB, 300   10.9 / 10.9 / 13.1   98 KB, 3624  70.2 / 65.3 / 78.4
+//   98 KB, 300   10.9 / 10.9 / 13.1   98 KB, 3624  70.2 / 65.3 / 78.4   128 KB, 4096 98.8 / 97.3 / 89.2
 //   201 KB, 600  25.1 / 26.5 / 25.5   201 KB, 1511 59.6 / 57.6 / 55.2
 //   304 KB, 200  18.3 / 14.6 / 14.5   304 KB, 300  25.2 / 24.0 / 25.8   304 KB, 520 34.9 / 41.0 / 38.6
 //   304 KB, 777  51.7 / 52.0 / 50.7   304 KB, 1200 68.2 / 68.1 / 65.4   304 KB, 3024 165 / 165 / 156
 //   608 KB, 700  73.8 / 75.4 / 73.3
 constexpr int loss_row_threads(int64_t rows, int64_t row_bytes) {
-    if (row_bytes < 4 << 10) return 64;
-    if (row_bytes < 24 << 10) return 128;
+    if (row_bytes < 10 << 10) return 64;
+    if (row_bytes < 28 << 10) return rows < 768 ? 256 : rows < 1536 ? 128 : 64;
     if (row_bytes < 64 << 10 || !loss_threads_fit(rows, 1024)) return 256;
     if (rows <= 256) return 512;
     if (rows < 768) return 256;
-    return row_bytes < 192 << 10 ? 512 : 1024;
+    return row_bytes < 112 << 10 ? 512 : 1024;
 }
 
 // Workgroups of 256 threads that share a row's statistics (1: none do), where
@@ -84,21 +86,25 @@ constexpr int loss_row_parts(int64_t rows, int64_t vocab, int elem_size, bool bo
 }
 
 // Threads that write a row's gradient, and workgroups that share a row where
-// there are too few rows for the CUs. us, right behind a forward (64 rows: alone),
-// 256 / 512 / 1024 threads:
-//   8 KB rows, 16384   95.0 / 94.4 / 98.1      16 KB rows, 8192   84.4 / 82.9 / 82.3
+// there are too few rows for the CUs. us, 64 / 256 / 512 / 1024 threads:
+//   2 KB rows, 8192   9.5 / 14.5 / 22.6 / 38.8     4 KB, 1000   5.1 / 5.2 / 5.9 / 7.9
+//   12 KB, 4096       19.5 / 18.4 / 19.9 / 26.9    16 KB, 8192  55.0 / 50.2 / 47.3 / 64.0
+//   24 KB, 2000       19.8 / 18.3 / 18.3 / 20.1    32 KB, 8192  107 / 97.6 / 96.7 / 93.1
+// 256 / 512 / 1024 threads, right behind a forward:
 //   64 KB rows, 2000   68.3 / 66.7 / 65.9      98 KB rows, 4816   220 / 208 / 200
 //   201 KB rows, 2036  194 / 182 / 172         304 KB rows, 2036  294 / 278 / 267
-//   304 KB rows, 64    33.7 / 19.6 / 12.2
+// 64 rows of 304 KB take 34 with a workgroup each and 12 with 8 of 1024 threads; 32
+// shared rows, 512 / 1024: 32 KB 4.7 / 5.3, 96 KB 4.8 / 5.5, 304 KB 6.8 / 7.4.
 struct LossGrid {
     int threads;
     unsigned parts;
 };
 constexpr LossGrid loss_grad_grid(int64_t rows, int64_t row_bytes) {
+    if (row_bytes < 6 << 10 && rows >= 1536) return LossGrid{64, 1};
     if (row_bytes < 16 << 10 || !loss_threads_fit(rows, 1024)) return LossGrid{256, 1};
-    const int64_t most = (row_bytes + (16 << 10) - 1) / (16 << 10);  // a vector per thread
+    const int64_t most = (row_bytes + (16 << 10) - 1) / (16 << 10);  // a vector or two per thread
     const int64_t wanted = rows >= 256 ? 1 : (512 + rows - 1) / rows;
-    return LossGrid{1024, (unsigned)(wanted < most ? wanted : most)};
+    return LossGrid{row_bytes < 28 << 10 || rows <= 64 ? 512 : 1024, (unsigned)(wanted < most ? wanted : most)};
 }
 
 // Softmax rows that are not whole 16-byte vectors: the covering vectors of the

@@ -1228,13 +1228,23 @@ template <typename T> struct Split {
 };
 // fn(element type, source): the parts of split rows, the smallest held shape of
 // at least `least` threads for a row, or the largest with the rest of the row read
-// twice. us of held rows alone, by threads x vectors:
-//   16 KB rows, 8192   128x8 49.5, 256x4 47.4, 512x4 58.4
-//   32 KB rows, 8192   512x4 88.9, 256x8 92.5, 512x8 87.4
-//   64 KB rows, 4000   512x8 88.9, 512x13 83.7, 1024x4 115
-//   98 KB rows, 4816   512x13 165, 1024x8 195
-//   201 KB rows, 2036  1024x13 139, 1024x16 140, 1024x19 142
-template <typename F> void by_row_source(int least, int parts, int64_t vocab, int dtype, F&& fn) {
+// twice. Policy loss, us, by threads x vectors, bf16:
+//   4 KB rows, 400     64x4 11.3, 256x2 8.7        4 KB, 16384   64x4 39.8, 128x4 50.3, 256x2 80.3
+//   8 KB rows, 1000    64x8 14.1, 128x8 13.4, 256x4 11.8
+//   6 KB rows, 16384   64x8 44.9, 64x16 49.3, 128x8 55.0
+//   16 KB rows, 1000   64x16 19.6, 128x8 18.1, 256x4 15.4, 512x2 17.2
+//   16 KB rows, 4096   64x16 33.8, 128x8 34.4, 256x4 36.6, 512x2 44.8
+//   24 KB rows, 4096   128x16 44.8, 256x8 43.0, 512x4 53.7
+//   32 KB rows, 1000   128x16 25.0, 256x8 21.1, 512x4 22.3
+//   64 KB rows, 1000   512x8 31.1, 512x13 32.5, 1024x4 41.0
+// f32: 64 KB rows, 4000 512x8 113, 512x13 104; 98 KB, 4096 512x13 155, 1024x8 172.
+// The kernel alone, bf16: 201 KB rows, 2036 1024x13 139, 1024x16 140, 1024x19 142.
+// Without the last shape, by a forward and a backward: 600 rows of 256000 bf16
+// 161 / 169, 300 of 256000 f32 156 / 190.
+constexpr int64_t kManyRows = 1536;  // past it a CU's rows fill it whatever their threads
+template <typename F>
+void by_row_source(int64_t rows, int least, int parts, int64_t vocab, int dtype, F&& fn) {
+    if (rows < kManyRows && least < 256) least = 256;
     auto go = [&](auto elem) {
         typedef decltype(elem) T;
         if (parts > 1) return fn(elem, Split<T>{});
@@ -1247,9 +1257,9 @@ template <typename F> void by_row_source(int least, int parts, int64_t vocab, in
         };
         // a rest's vectors need registers of their own, unpacked
         constexpr int kWithRest = Vec16<T>::N == 4 ? 16 : 8;
-        shape(Held<T, 64, 4, false>{}) || shape(Held<T, 128, 8, false>{}) || shape(Held<T, 256, 4, false>{}) ||
-            shape(Held<T, 512, 4, false>{}) || shape(Held<T, 512, 8, false>{}) || shape(Held<T, 512, 13, false>{}) ||
-            shape(Held<T, 512, 19, false>{}) || shape(Held<T, 1024, 13, false>{}) ||
+        shape(Held<T, 64, 4, false>{}) || shape(Held<T, 64, 8, false>{}) || shape(Held<T, 128, 8, false>{}) ||
+            shape(Held<T, 256, 4, false>{}) || shape(Held<T, 256, 8, false>{}) || shape(Held<T, 512, 8, false>{}) ||
+            shape(Held<T, 512, 13, false>{}) || shape(Held<T, 512, 19, false>{}) || shape(Held<T, 1024, 13, false>{}) ||
             shape(Held<T, 1024, 16, false>{}) || shape(Held<T, 1024, 19, false>{}) ||
             shape(Held<T, 1024, kWithRest, true>{});
     };
@@ -1563,7 +1573,7 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
         const int parts =
             launch_parts(true, rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
         e = hipSuccess;
-        by_row_source(1, parts, d.vocab, d.dtype, [&](auto elem, auto source) {
+        by_row_source(rows, 1, parts, d.vocab, d.dtype, [&](auto elem, auto source) {
             typedef decltype(elem) T;
             typedef decltype(source) S;
             constexpr int NT = S::kThreads;
@@ -1605,7 +1615,7 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
         void* parts_ws = ws + w.total + loss_stats_ws(2 * d.rows);
         const int parts =
             launch_parts(true, d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, parts_ws, stream);
-        by_row_source(d.top, parts, d.vocab, d.dtype, [&](auto elem, auto source) {
+        by_row_source(d.rows, d.top, parts, d.vocab, d.dtype, [&](auto elem, auto source) {
             typedef decltype(elem) T;
             typedef decltype(source) S;
             constexpr int NT = S::kThreads;

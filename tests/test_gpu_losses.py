@@ -534,7 +534,10 @@ LONG = [(torch.bfloat16, 1, 151936), (torch.bfloat16, 7, 60001), (torch.float32,
         (torch.float32, 130, 100003), (torch.bfloat16, 129, 155651), (torch.bfloat16, 130, 200003),
         (torch.bfloat16, 300, 20000), (torch.bfloat16, 200, 40007), (torch.bfloat16, 200, 52001),
         (torch.bfloat16, 200, 77001), (torch.float32, 140, 50257), (torch.float32, 140, 65001),
-        (torch.float32, 400, 1021), (torch.float32, 400, 4100), (torch.float32, 300, 8193)]
+        (torch.float32, 400, 1021), (torch.float32, 400, 4100), (torch.float32, 300, 8193),
+        (torch.bfloat16, 1600, 1501), (torch.float32, 1600, 1023), (torch.bfloat16, 1700, 4003),
+        (torch.float32, 1536, 2047), (torch.bfloat16, 1600, 8195), (torch.float32, 1600, 4099),
+        (torch.bfloat16, 1540, 16387)]
 
 
 @pytest.mark.parametrize("offset", [0, 3])

@@ -363,14 +363,15 @@ mc_status mc_cross_entropy_bwd(const mc_xent_desc* d, const void* logits, const 
 /* Losses over the logits [rows, vocab] for what comes after supervised
  * fine-tuning. No counterpart in the reference, whose only loss is the cross
  * entropy; targets and ignore_index are as there, T is a temperature in
- * [1e-6, 1e6], vocab < 2^31 and rows <= 16777215. logits may start at any element.
- * A row whose target is ignore_index (distillation: whose mask is 0) is not
- * counted: it is not read, whatever it holds, and its gradient is zero, as is
- * that of a row whose loss has no gradient. A counted id past the vocabulary
- * makes the loss NaN and the gradients that depend on it. Sums run in a fixed
- * order: results are bitwise reproducible. dloss: fp32 [1] on the device, the
- * gradient of the loss, or NULL for 1. stats of a forward, which its backward
- * needs, start with each row's maximum and sum of exponentials [rows, 2].
+ * [1e-6, 1e6], vocab < 2^31 and rows <= 16777215. logits and dlogits may start at
+ * any element and must not overlap. A row whose target is ignore_index
+ * (distillation: whose mask is 0) is not counted: it is not read, whatever it
+ * holds, and its gradient is zero, as is that of a row whose loss has no gradient.
+ * A counted id past the vocabulary makes the loss NaN and the gradients that depend
+ * on it. Sums run in a fixed order: results are bitwise reproducible. dloss: fp32
+ * [1] on the device, the gradient of the loss, or NULL for 1. stats of a forward,
+ * which its backward needs, start with each row's maximum and sum of exponentials
+ * [rows, 2]. A workspace holds nothing between calls.
  *
  * Log-probabilities of given tokens, l = x[t] / T - log sum exp(x / T), fp32
  * [rows]; 0 where the row is not counted. stats fp32 [rows, 2] may be NULL. */

@@ -799,8 +799,8 @@ mc_status mc_token_logprobs_bwd(const mc_logprob_desc* d, const void* logits, co
 
 static mc_status check_preference(const mc_preference_desc* d) {
     MC_CHECK(d != nullptr, MC_ERR_NULL, "preference_loss: descriptor is NULL");
-    mc_status s = check_vocab("preference_loss", d->pairs >= 1 && d->pairs <= kMaxBlockRows ? seq_rows(2 * d->pairs, d->seq) : 0,
-                              d->vocab, d->dtype);
+    const int64_t rows = d->pairs >= 1 && d->pairs <= kMaxBlockRows ? seq_rows(2 * d->pairs, d->seq) : 0;
+    mc_status s = check_vocab("preference_loss", rows, d->vocab, d->dtype);
     if (s != MC_OK) return s;
     MC_CHECK(d->kind == MC_PREF_SIGMOID || d->kind == MC_PREF_HINGE || d->kind == MC_PREF_SQUARED, MC_ERR_VALUE,
              "preference_loss: unknown kind %d", (int)d->kind);

@@ -514,7 +514,8 @@ def _loss_inputs(logits, targets, ignore_index, seqs):
         raise McError(_lib.MC_ERR_SHAPE, f"logits are empty: {tuple(logits.shape)}")
     targets = _targets(targets, logits)
     if seqs and targets.shape != logits.shape[:-1]:
-        raise McError(_lib.MC_ERR_SHAPE, f"targets has shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
+        raise McError(_lib.MC_ERR_SHAPE,
+                      f"targets has shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
     return targets, -1 if ignore_index is None else int(ignore_index), _DTYPES[logits.dtype]
 
 

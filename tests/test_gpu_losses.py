@@ -584,6 +584,169 @@ def test_rows_of_every_length(mc, dev, nan_outputs, dtype, rows, V, offset):
         close_grad(pd[:, 0], grad, 1.3 * terms, dtype)
 
 
+# rows held by each way: alone, shared, with a rest read twice
+WAYS = [(16, 300), (40, 1003), (1600, 301), (300, 20001), (14, 100003), (140, 200003)]
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", WAYS)
+def test_one_read_with_masked_logits(mc, dev, nan_outputs, dtype, rows, V, offset):
+    """-inf, the type's lowest value and NaN in the rows that the policy and distillation losses read once."""
+    g = gen(dev, V)
+    x = logits_at(dev, g, (rows, V), dtype, offset)
+    t = some_targets(dev, g, (rows,), V, drop=0.0)
+    low = torch.finfo(dtype).min
+    x[2, 1:], t[2] = -math.inf, 0
+    x[3, : V // 2], t[3] = -math.inf, V - 1
+    x[4, V // 3:], t[4] = low, 1
+    x[5] = low
+    x[6, : V - 7], t[6] = low, V - 3
+    x[8] = -1e30
+    x[9], t[9] = math.nan, -1
+    x[10], t[10] = -math.inf, -1
+    on = t != -1
+    l64, tol, q = plain_logps(x, t)
+    A = torch.randn(rows, 1, generator=g, device=dev)
+    l64, tol, q = torch.where(on, l64, 0.0), torch.where(on, tol, 0.0), torch.where(on[:, None], q, 0.0)
+    outs = mc.policy_loss_forward_backward(x[:, None], t[:, None], A, ignore_index=PAD)
+    check_policy(mc, dev, x[:, None], t[:, None], l64[:, None], tol[:, None], q[:, None], A, None, None, {}, outs, 1.0,
+                 dtype)
+    # the teacher's entries where the student's are finite
+    ids = torch.randint(0, V, (rows, 6), generator=g, device=dev, dtype=torch.int32)
+    ids[2], ids[3], ids[4], ids[6], ids[9:11] = 0, V - 2, ids[4] % (V // 3), V - 1, 2**31 - 1
+    tl = torch.randn(rows, 6, generator=g, device=dev)
+    tl[9:11] = math.nan
+    mask = on.to(torch.uint8)
+    clean = torch.where(on[:, None], x, 0.0)
+    want, dtol, grad, terms = plain_distill(clean, ids, torch.where(on[:, None], tl, 0.0), 1.0, None, mask)
+    for loss, d in (mc.distillation_loss_forward_backward(x, ids, tl, mask=mask),):
+        assert abs(float(loss) - float(want)) <= float(dtol) + 2.0 ** -23 * abs(float(want))
+        close_grad(d, grad, terms, dtype)
+        assert not d[~on].any()
+    # NaN and infinities in counted rows stay in them
+    z, u = x.clone(), t.clone()
+    u[9:11] = 0
+    z[11, V // 2], z[12, 0] = math.inf, math.nan
+    _, logps, _, d = mc.policy_loss_forward_backward(z[:, None], u[:, None], A, ignore_index=PAD)
+    bad = torch.zeros(rows, dtype=torch.bool, device=dev)
+    bad[9:13] = True
+    assert torch.isnan(logps[bad]).all() and torch.isfinite(logps[~bad]).all()
+    assert torch.isnan(d[bad]).all() and torch.isfinite(d[~bad]).all()
+
+
+@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", WAYS)
+def test_repeated_ids_in_rows_of_every_way(mc, dev, nan_outputs, dtype, rows, V, offset):
+    """256 entries: all the same, all of a few vectors, pairs, the edges; in one call and in two."""
+    K, g = 256, gen(dev, rows)
+    x = logits_at(dev, g, (rows, V), dtype, offset)
+    ids = torch.randint(0, V, (rows, K), generator=g, device=dev, dtype=torch.int32)
+    near = torch.arange(K, device=dev, dtype=torch.int32)
+    ids[0], ids[1], ids[2] = 0, V - 1, V // 2
+    ids[3], ids[4], ids[5], ids[6] = near % 20, V - 1 - near % 17, near // 2, 40 + near // 3
+    ids[7, ::2] = 17
+    ids[8] = ids[8].sort().values // 4 * 4 % V
+    tl = torch.randn(rows, K, generator=g, device=dev) * 2
+    want, tol, grad, terms = plain_distill(x, ids, tl, 1.0, None, None)
+    loss, stats = mc.distillation_loss_forward(x, ids, tl)
+    for v, d in ((loss, mc.distillation_loss_backward(x, ids, tl, stats)),
+                 mc.distillation_loss_forward_backward(x, ids, tl)):
+        assert abs(float(v) - float(want)) <= float(tol) + 2.0 ** -23 * abs(float(want))
+        close_grad(d, grad, terms, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_the_longest_row(mc, dev, dtype):
+    """2^31 - 1 logits: 4 or 8 GiB in one row."""
+    V, step = 2**31 - 1, 1 << 27
+    x = torch.empty(1, V, dtype=dtype, device=dev)
+    g = gen(dev, 12)
+    for i in range(0, V, step):
+        x[0, i: i + step].normal_(0.0, 3.0, generator=g)
+    t = torch.tensor([V - 2], device=dev, dtype=torch.int32)
+    x[0, V - 2], x[0, 1 << 30] = 20.0, 19.0
+    m = float(x.max())
+    s = sum(float((x[0, i: i + step].double() - m).exp().sum()) for i in range(0, V, step))
+    z = float(x[0, V - 2]) - m
+    l, stats = mc.token_logprobs_forward(x, t)
+    assert abs(float(l) - (z - math.log(s))) <= 2.0 ** -20 + 2.0 ** -22 * (abs(z) + math.log(s))
+
+    def gradient(d, a, taken):
+        """d against a q less what is taken out of single elements."""
+        for i in range(0, V, step):
+            q = (x[0, i: i + step].double() - m).exp() / s
+            want, terms = a * q, abs(a) * q
+            for j, p in taken.items():
+                if i <= j < i + step:
+                    want[j - i] -= p
+                    terms[j - i] += abs(p)
+            close_grad(d[0, i: i + step], want, terms, dtype)
+
+    one = torch.ones(1, device=dev)
+    gradient(mc.token_logprobs_backward(x, t, stats, one), -1.0, {V - 2: -1.0})
+    loss, logps, _, d = mc.policy_loss_forward_backward(x[None], t[None], one)
+    assert abs(float(logps) - float(l)) <= 2.0 ** -20 + 2.0 ** -22 * (abs(z) + math.log(s))
+    gradient(d.view(1, V), 1.0, {V - 2: 1.0})
+    del d
+    ids = torch.tensor([[0, V - 1, 1 << 30, V - 2]], device=dev, dtype=torch.int32)
+    tl = torch.zeros(1, 4, device=dev)
+    loss, d = mc.distillation_loss_forward_backward(x, ids, tl)
+    lq = [float(x[0, j]) - m - math.log(s) for j in ids[0].tolist()]
+    want = sum(0.25 * (math.log(0.25) - v) for v in lq)
+    assert abs(float(loss) - want) <= 2.0 ** -19 + 2.0 ** -21 * (2.0 + max(abs(v) for v in lq))
+    gradient(d, 1.0, {j: 0.25 for j in ids[0].tolist()})
+
+
+def test_dloss_and_optional_outputs(mc, dev):
+    """A dloss of 0 and of NaN; outputs that may be NULL."""
+    import ctypes
+
+    g = gen(dev, 13)
+    x = logits_at(dev, g, (4, 5, 77), torch.float32)
+    t = some_targets(dev, g, (4, 5), 77)
+    A = torch.randn(4, generator=g, device=dev)
+    ids = torch.randint(0, 77, (4, 5, 3), generator=g, device=dev, dtype=torch.int32)
+    tl = torch.randn(4, 5, 3, generator=g, device=dev)
+    ploss, rewards, pstats = mc.preference_loss_forward(x, t, ignore_index=PAD)
+    loss, logps, metrics, stats = mc.policy_loss_forward(x, t, A, ignore_index=PAD)
+    kl, kstats = mc.distillation_loss_forward(x, ids, tl)
+    for v in (0.0, math.nan):
+        dloss = torch.full((1,), v, device=dev)
+        for d, on in ((mc.preference_loss_backward(x, t, pstats, dloss, ignore_index=PAD), t != -1),
+                      (mc.policy_loss_backward(x, t, stats, dloss, ignore_index=PAD), t != -1),
+                      (mc.policy_loss_forward_backward(x, t, A, ignore_index=PAD, dloss=dloss)[3], t != -1),
+                      (mc.distillation_loss_backward(x, ids, tl, kstats, dloss), None),
+                      (mc.distillation_loss_forward_backward(x, ids, tl, dloss=dloss)[1], None)):
+            if v == 0.0:
+                assert not d.any()
+            else:
+                assert torch.isnan(d if on is None else d[on]).all() and (on is None or not d[~on].any())
+    L, lib = mc.ops._lib, mc.ops.lib()
+    s = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device=dev)
+    p = lambda v: v.data_ptr()  # noqa: E731
+    d = L.PreferenceDesc(2, 5, 77, PAD, L.MC_PREF_SIGMOID, 0, 0.1, 0.0, 0.0, L.MC_F32)
+    out = torch.empty(1, device=dev)
+    assert lib.mc_preference_loss_fwd(ctypes.byref(d), p(x), p(t), None, p(out), None, None, p(ws), ws.numel(), s) == 0
+    assert torch.equal(out, ploss)
+    d = L.PolicyDesc(4, 5, 77, PAD, 0, L.MC_MEAN_TOKENS, 0.2, 0.2, 0.0, 1.0, L.MC_F32)
+    l = torch.empty(4, 5, device=dev)
+    assert lib.mc_policy_loss_fwd(ctypes.byref(d), p(x), p(t), p(A), None, None, p(out), p(l), None, None, p(ws),
+                                  ws.numel(), s) == 0
+    assert torch.equal(out, loss) and torch.equal(l, logps)
+    dx, out2 = torch.empty_like(x), torch.empty(1, device=dev)
+    assert lib.mc_policy_loss_fwd_bwd(ctypes.byref(d), p(x), p(t), p(A), None, None, None, p(out2), p(l), None, p(dx),
+                                      p(ws), ws.numel(), s) == 0
+    got = mc.policy_loss_forward_backward(x, t, A, ignore_index=PAD)
+    assert torch.equal(out2, got[0]) and torch.equal(dx, got[3])
+    d = L.DistillDesc(20, 77, 3, 1.0, L.MC_F32)
+    assert lib.mc_distill_loss_fwd(ctypes.byref(d), p(x), p(ids), p(tl), None, None, p(out), None, p(ws), ws.numel(),
+                                   s) == 0
+    assert torch.equal(out, kl)
+
+
 @pytest.mark.parametrize("rows,B", [(20000, 5), (9000, 9000)])
 def test_many_rows(mc, dev, rows, B):
     """Sums over more rows than one workgroup takes, counts by a kernel of their own."""

@@ -692,6 +692,18 @@ struct RowGrad {
 };
 __device__ __forceinline__ RowGrad row_grad(float a, RowStat st, float c) { return RowGrad{a / st.s, st.m, c}; }
 
+// How vectors are stored: in the caches, past them, or at any element, where the
+// gradients do not start at the logits' place in a vector. Then the fwd_bwd calls
+// run as a forward and a backward (as a second way to store a held row this cost
+// the longest 60 registers): 2036 bf16 rows of 151936 backward 251 us, element by
+// element 456, aligned 238; policy 362, 550, 242.
+enum class Store { kCached, kStream, kAny };
+template <typename T, int N> __device__ __forceinline__ void store16(T* p, const float (&v)[N], Store how) {
+    if (how == Store::kStream) store_nt16(p, v);
+    else if (how == Store::kAny) store_any16(p, v);
+    else Vec16<T>::store(p, v);
+}
+
 // The threads of a row: those of the gridDim.y workgroups that share it.
 struct RowThreads {
     int self, count;
@@ -703,7 +715,7 @@ template <int NT> __device__ __forceinline__ RowThreads row_threads() {
 // Vectors c, c - step, .. down to lo: U requested at a time, the last together.
 template <typename T, int U>
 __device__ __forceinline__ void write_vecs(const T* __restrict__ xv, T* __restrict__ dv, int c, int step, int lo,
-                                           bool stream, RowGrad grad) {
+                                           Store how, RowGrad grad) {
     constexpr int N = Vec16<T>::N;
     auto group = [&](auto whole) {
         float v[U][N];
@@ -718,42 +730,35 @@ __device__ __forceinline__ void write_vecs(const T* __restrict__ xv, T* __restri
             if (!decltype(whole)::value && at < lo) break;
 #pragma unroll
             for (int e = 0; e < N; ++e) v[u][e] = grad(v[u][e]);
-            if (stream) store_nt16(dv + (int64_t)at * N, v[u]);
-            else Vec16<T>::store(dv + (int64_t)at * N, v[u]);
+            store16(dv + (int64_t)at * N, v[u], how);
         }
     };
     for (; c >= lo + (U - 1) * step; c -= U * step) group(std::true_type{});
     if (c >= lo) group(std::false_type{});
 }
 template <typename T>
-__device__ __forceinline__ void write_row(const T* __restrict__ xr, T* __restrict__ dr, int vocab, bool vec,
-                                          bool stream, RowThreads th, RowGrad grad) {
-    if (vec) {
-        const RowSpan<T> span(xr, vocab);
-        write_vecs<T, 4>(xr + span.head, dr + span.head, (int)span.nvec - 1 - th.self, th.count, 0, stream, grad);
-        const int64_t j = span.edge(th.self, vocab);
-        if (j >= 0) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
-    } else {
-        for (int64_t j = th.self; j < vocab; j += th.count) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
-    }
+__device__ __forceinline__ void write_row(const T* __restrict__ xr, T* __restrict__ dr, int vocab, Store how,
+                                          RowThreads th, RowGrad grad) {
+    const RowSpan<T> span(xr, vocab);
+    write_vecs<T, 4>(xr + span.head, dr + span.head, (int)span.nvec - 1 - th.self, th.count, 0, how, grad);
+    const int64_t j = span.edge(th.self, vocab);
+    if (j >= 0) Elem<T>::store(dr, j, grad(Elem<T>::load(xr, j)));
 }
-// The thread that stores element j: its vector's, its edge's, or its own where
-// the row goes one by one.
-template <int N> __device__ __forceinline__ int owner_of(int j, int head, int nvec, bool vec, int threads) {
-    if (!vec) return j % threads;
+// The thread that stores element j: its vector's, or its edge's.
+template <int N> __device__ __forceinline__ int owner_of(int j, int head, int nvec, int threads) {
     if (j < head) return j;
     const int c = (j - head) / N;
     return c < nvec ? (nvec - 1 - c) % threads : N + (j - head - nvec * N);
 }
 
 template <typename T>
-__device__ __forceinline__ void zero_row(T* __restrict__ dr, int vocab, bool stream, RowThreads th) {
+__device__ __forceinline__ void zero_row(T* __restrict__ dr, int vocab, Store how, RowThreads th) {
     constexpr int N = Vec16<T>::N;
-    const RowSpan<T> span(dr, vocab);
+    const RowSpan<T> span(dr, vocab);  // its own vectors
     const float z[N] = {};
     for (int c = th.self; c < (int)span.nvec; c += th.count) {
         T* p = dr + span.head + (int64_t)c * N;
-        if (stream) store_nt16(p, z);
+        if (how == Store::kStream) store_nt16(p, z);
         else Vec16<T>::store(p, z);
     }
     const int64_t j = span.edge(th.self, vocab);
@@ -823,7 +828,7 @@ template <int NT> struct TopOwners {
 // dlogits of a loss over l: g ([j = t] - q_j) / T, g = dl of the row (or of its
 // sequence) times the optional device scalars.
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void lp_bwd_k(int64_t rows, int vocab, bool vec, bool stream,
+__global__ __launch_bounds__(NT) void lp_bwd_k(int64_t rows, int vocab, Store how,
                                                const T* __restrict__ logits, const uint32_t* __restrict__ targets,
                                                int64_t ignore_index, LpScale k, const RowStat* __restrict__ stats,
                                                const float* __restrict__ dl, uint32_t seq,
@@ -841,21 +846,21 @@ __global__ __launch_bounds__(NT) void lp_bwd_k(int64_t rows, int vocab, bool vec
         if (t >= (uint32_t)vocab) g = __builtin_nanf("");
     }
     if (g == 0.f) {
-        zero_row(dr, vocab, stream, th);
+        zero_row(dr, vocab, how, th);
         return;
     }
     g *= k.inv_t;
     const T* xr = logits + row * vocab;
     const RowGrad grad = row_grad(-g, stats[row], k.c);
-    write_row(xr, dr, vocab, vec, stream, th, grad);
+    write_row(xr, dr, vocab, how, th, grad);
     const RowSpan<T> span(xr, vocab);
     if (t < (uint32_t)vocab &&
-        owner_of<Vec16<T>::N>((int)t, (int)span.head, (int)span.nvec, vec, th.count) == th.self)
+        owner_of<Vec16<T>::N>((int)t, (int)span.head, (int)span.nvec, th.count) == th.self)
         Elem<T>::store(dr, t, grad(Elem<T>::load(xr, t)) + g);
 }
 
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec, bool stream,
+__global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, Store how,
                                                     const T* __restrict__ logits, const int32_t* __restrict__ ids,
                                                     const float* __restrict__ tl, const float* __restrict__ tlse,
                                                     const uint8_t* __restrict__ mask, LpScale k,
@@ -869,7 +874,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
     const int vocab = (int)d.vocab;
     T* dr = dlogits + row * vocab;
     if (mask && mask[row] == 0) {
-        zero_row(dr, vocab, stream, th);
+        zero_row(dr, vocab, how, th);
         return;
     }
     owners.clear(d.top);
@@ -882,18 +887,18 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, bool vec,
     const uint32_t x = entry.logit(xr, vocab);
     __syncthreads();
     if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab)
-        owners.insert(owner_of<N>(entry.id, (int)span.head, (int)span.nvec, vec, th.count), (int)(blockIdx.y * NT));
+        owners.insert(owner_of<N>(entry.id, (int)span.head, (int)span.nvec, th.count), (int)(blockIdx.y * NT));
     entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
     __syncthreads();
     const TeacherSums ts = entry.sums(d, te);
     float w = scale[0] * (dloss ? dloss[0] : 1.f);
     if (ts.bad) w = __builtin_nanf("");
     if (ts.P == 0.f || w == 0.f) {
-        zero_row(dr, vocab, stream, th);
+        zero_row(dr, vocab, how, th);
         return;
     }
     const RowGrad grad = row_grad(w * ts.P, v, k.c);
-    write_row(xr, dr, vocab, vec, stream, th, grad);
+    write_row(xr, dr, vocab, how, th, grad);
     owners.patch(te, d.top, dr, grad, w);
 }
 
@@ -983,10 +988,10 @@ template <typename T, int NT, int NV, bool REST> struct HeldRow {
         return st;
     }
     // into the gradient's row dr, which starts like the logits'
-    __device__ __forceinline__ void store(T* __restrict__ dr, bool stream, RowGrad grad) const {
+    __device__ __forceinline__ void store(T* __restrict__ dr, Store how, RowGrad grad) const {
         if constexpr (REST)
             write_vecs<T, G>(xv, dr + head, (int)threadIdx.x + (nvec - 1 - (int)threadIdx.x) / NT * NT, NT, NT * NV,
-                             stream, grad);
+                             how, grad);
         const __amdgpu_buffer_rsrc_t r = make_rsrc(dr + head, (int64_t)(REST ? NT * NV : nvec) * 16);
         uint32_t at = threadIdx.x * 16u;
         asm volatile("" : "+v"(at));  // or the loads' NV offsets are held for the stores
@@ -997,7 +1002,7 @@ template <typename T, int NT, int NV, bool REST> struct HeldRow {
             BVec<T>::unpack(q[u], v);
 #pragma unroll
             for (int e = 0; e < N; ++e) v[e] = grad(v[e]);
-            if (stream) BVec<T>::store_nt(r, at + u * NT * 16u, v);
+            if (how == Store::kStream) BVec<T>::store_nt(r, at + u * NT * 16u, v);
             else BVec<T>::store(r, at + u * NT * 16u, v);
         }
         if (j >= 0) Elem<T>::store(dr, j, grad(from_raw<T>(edge)));
@@ -1013,7 +1018,7 @@ template <typename T, int NT> struct SplitRow {
     int vocab, head, nvec;
     Stat<double> part;
 
-    __device__ __forceinline__ int owner(int at) const { return owner_of<N>(at, head, nvec, true, th.count); }
+    __device__ __forceinline__ int owner(int at) const { return owner_of<N>(at, head, nvec, th.count); }
     __device__ __forceinline__ void load(const T* __restrict__ xr_, int vocab_, const Stat<double>* __restrict__ parts,
                                          int64_t row, RowThreads th_) {
         const RowSpan<T> span(xr_, vocab_);
@@ -1025,8 +1030,8 @@ template <typename T, int NT> struct SplitRow {
         part = own_part(parts, row, th.count / NT);
     }
     __device__ __forceinline__ Stat<float> stat(LpScale) const { return float_stat(part); }
-    __device__ __forceinline__ void store(T* __restrict__ dr, bool stream, RowGrad grad) const {
-        write_row(xr, dr, vocab, true, stream, th, grad);
+    __device__ __forceinline__ void store(T* __restrict__ dr, Store how, RowGrad grad) const {
+        write_row(xr, dr, vocab, how, th, grad);
     }
 };
 
@@ -1084,7 +1089,7 @@ template <int NT> struct RowCount {
 // (by_seq: of each sequence, one number each), or null: counted here over len
 // targets. n (may be null): receives the sequences' counts.
 template <typename T, int NT, typename Row>
-__global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool stream, const T* __restrict__ logits,
+__global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store how, const T* __restrict__ logits,
                                                        const uint32_t* __restrict__ targets,
                                                        const float* __restrict__ adv, const float* __restrict__ old,
                                                        const float* __restrict__ ref,
@@ -1104,7 +1109,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool st
     const uint32_t t = targets[row];
     if (!counted(t, d.ignore_index)) {
         if (writer) logp[row] = 0.f;
-        zero_row(dr, vocab, stream, th);
+        zero_row(dr, vocab, how, th);
         return;
     }
     const T* xr = logits + row * vocab;
@@ -1129,12 +1134,12 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool st
     }
     float g = policy_term(d, l, pin).dl / (by_seq ? (float)d.batch * (float)share : (float)share) * up;
     if (g == 0.f) {
-        zero_row(dr, vocab, stream, th);
+        zero_row(dr, vocab, how, th);
         return;
     }
     g *= k.inv_t;
     const RowGrad grad = row_grad(-g, v, k.c);
-    held.store(dr, stream, grad);
+    held.store(dr, how, grad);
     if (in && held.owner((int)t) == th.self)
         Elem<T>::store(dr, t, grad(from_raw<T>(xt)) + g);
 }
@@ -1142,7 +1147,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, bool st
 // given: n_given counts of the mask, or null: counted here over len of it (0
 // without a mask).
 template <typename T, int NT, typename Row>
-__global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool stream, const T* __restrict__ logits,
+__global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store how, const T* __restrict__ logits,
                                                         const int32_t* __restrict__ ids, const float* __restrict__ tl,
                                                         const float* __restrict__ tlse,
                                                         const uint8_t* __restrict__ mask,
@@ -1162,7 +1167,7 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool 
     T* dr = dlogits + row * vocab;
     if (mask && mask[row] == 0) {
         if (writer) kl[row] = 0.f;
-        zero_row(dr, vocab, stream, th);
+        zero_row(dr, vocab, how, th);
         return;
     }
     const T* xr = logits + row * vocab;
@@ -1191,11 +1196,11 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, bool 
     if (writer) kl[row] = ts.kl;
     if (ts.bad) w = __builtin_nanf("");
     if (ts.P == 0.f || w == 0.f) {
-        zero_row(dr, vocab, stream, th);
+        zero_row(dr, vocab, how, th);
         return;
     }
     const RowGrad grad = row_grad(w * ts.P, v, k.c);
-    held.store(dr, stream, grad);
+    held.store(dr, how, grad);
     owners.patch(te, d.top, dr, grad, w);
 }
 
@@ -1280,8 +1285,9 @@ void by_row_source(int64_t rows, int least, int parts, int64_t vocab, int dtype,
     else go(uint16_t{});
 }
 
-bool same_start(const void* a, const void* b) {
-    return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+Store store_of(const void* logits, const void* dlogits, int64_t rows, int64_t vocab, int dtype) {
+    if ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(dlogits)) & 15) return Store::kAny;
+    return xent_stream_gradients(rows, vocab, dtype == MC_F32 ? 4 : 2) ? Store::kStream : Store::kCached;
 }
 
 // Rows whose sums one workgroup forms by itself; past it up to 256 of them, and a
@@ -1367,13 +1373,12 @@ hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logit
                                      const float* stats, const float* dl, int64_t seq, const float* scale,
                                      const float* dloss, void* dlogits, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
-    const bool vec = same_start(logits, dlogits);
     const LossGrid grid = loss_grad_grid(d.rows, row_bytes(d.vocab, d.dtype));
     by_threads(grid.threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
         lp_bwd_k<T, NT><<<dim3((unsigned)d.rows, grid.parts), NT, 0, stream>>>(
-            d.rows, (int)d.vocab, vec, xent_stream_gradients(d.rows, d.vocab, sizeof(T)),
+            d.rows, (int)d.vocab, store_of(logits, dlogits, d.rows, d.vocab, d.dtype),
             static_cast<const T*>(logits), targets, d.ignore_index, k,
             reinterpret_cast<const RowStat*>(stats), dl, (uint32_t)seq, scale, dloss, static_cast<T*>(dlogits));
     });
@@ -1534,14 +1539,13 @@ hipError_t launch_distill_bwd(const mc_distill_desc& d, const void* logits, cons
                               const float* tlse, const uint8_t* mask, const float* stats, const float* dloss,
                               void* dlogits, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
-    const bool vec = same_start(logits, dlogits);
     const LossGrid grid = loss_grad_grid(d.rows, row_bytes(d.vocab, d.dtype));
     by_threads(grid.threads < kDistillMaxTop ? kDistillMaxTop : grid.threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
         if constexpr (NT >= kDistillMaxTop)
             distill_bwd_k<T, NT><<<dim3((unsigned)d.rows, grid.parts), NT, 0, stream>>>(
-                d, vec, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl,
+                d, store_of(logits, dlogits, d.rows, d.vocab, d.dtype), static_cast<const T*>(logits), ids, tl,
                 tlse, mask, k, reinterpret_cast<const RowStat*>(stats), stats + 2 * d.rows, dloss,
                 static_cast<T*>(dlogits));
     });
@@ -1577,8 +1581,9 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
     float* stats = reinterpret_cast<float*>(ws + w.total);
     const int64_t rows = d.batch * d.seq;
     const LpScale k = row_scale(d.temperature);
+    const Store how = store_of(logits, dlogits, rows, d.vocab, d.dtype);
     hipError_t e;
-    if (same_start(logits, dlogits) && loss_threads_fit(rows, 1024)) {
+    if (how != Store::kAny && loss_threads_fit(rows, 1024)) {
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         const bool by_seq = d.reduction == MC_MEAN_SEQUENCES;
         uint32_t* n = by_seq ? reinterpret_cast<uint32_t*>(ws + w.counts) : nullptr;
@@ -1596,7 +1601,7 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
             if (!here && by_seq) policy_counts(d, targets, ws, stream, e);
             else if (!here) n_given = launch_counts(rows, targets, nullptr, d.ignore_index, part, stream);
             policy_both_k<T, NT, typename S::Row><<<dim3((unsigned)rows, (unsigned)parts), NT, 0, stream>>>(
-                d, xent_stream_gradients(rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), targets, adv, old,
+                d, how, static_cast<const T*>(logits), targets, adv, old,
                 ref, static_cast<const Stat<double>*>(parts_ws), here ? nullptr : by_seq ? n : part, n_given,
                 here ? (int)span : 0, by_seq, here ? n : nullptr, k, dloss, logp, static_cast<T*>(dlogits));
         });
@@ -1621,8 +1626,9 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
     const DistillWs w = distill_ws(d);
     float* stats = reinterpret_cast<float*>(ws + w.total);
     const LpScale k = row_scale(d.temperature);
+    const Store how = store_of(logits, dlogits, d.rows, d.vocab, d.dtype);
     hipError_t e;
-    if (same_start(logits, dlogits) && loss_threads_fit(d.rows, 1024)) {
+    if (how != Store::kAny && loss_threads_fit(d.rows, 1024)) {
         float* kl = reinterpret_cast<float*>(ws + w.kl);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         void* parts_ws = ws + w.total + loss_stats_ws(2 * d.rows);
@@ -1635,7 +1641,7 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
             const bool here = !mask || d.rows <= RowCount<NT>::kPer * NT;
             const int n_given = here ? 0 : launch_counts(d.rows, nullptr, mask, -1, part, stream);
             distill_both_k<T, NT, typename S::Row><<<dim3((unsigned)d.rows, (unsigned)parts), NT, 0, stream>>>(
-                d, xent_stream_gradients(d.rows, d.vocab, sizeof(T)), static_cast<const T*>(logits), ids, tl, tlse,
+                d, how, static_cast<const T*>(logits), ids, tl, tlse,
                 mask, static_cast<const Stat<double>*>(parts_ws), here ? nullptr : part, n_given,
                 mask && here ? (int)d.rows : 0, k, dloss, kl, static_cast<T*>(dlogits));
         });

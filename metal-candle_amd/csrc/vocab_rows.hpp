@@ -33,5 +33,15 @@ __device__ __forceinline__ void store_nt16(uint16_t* p, const float (&v)[8]) {
     const u32x4 q = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
     __builtin_nontemporal_store(q, reinterpret_cast<u32x4*>(p));
 }
+// Sixteen bytes at any element.
+__device__ __forceinline__ void store_any16(float* p, const float (&v)[4]) {
+    typedef f32x4 __attribute__((aligned(4))) any;
+    *reinterpret_cast<any*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ void store_any16(uint16_t* p, const float (&v)[8]) {
+    typedef u32x4 __attribute__((aligned(2))) any;
+    *reinterpret_cast<any*>(p) =
+        u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+}
 
 }  // namespace mc

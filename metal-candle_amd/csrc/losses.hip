@@ -1377,10 +1377,11 @@ hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logit
     by_threads(grid.threads, d.dtype, [&](auto elem, auto threads) {
         typedef decltype(elem) T;
         constexpr int NT = decltype(threads)::value;
-        lp_bwd_k<T, NT><<<dim3((unsigned)d.rows, grid.parts), NT, 0, stream>>>(
-            d.rows, (int)d.vocab, store_of(logits, dlogits, d.rows, d.vocab, d.dtype),
-            static_cast<const T*>(logits), targets, d.ignore_index, k,
-            reinterpret_cast<const RowStat*>(stats), dl, (uint32_t)seq, scale, dloss, static_cast<T*>(dlogits));
+        if constexpr (NT != 128)  // loss_grad_grid has no such rows
+            lp_bwd_k<T, NT><<<dim3((unsigned)d.rows, grid.parts), NT, 0, stream>>>(
+                d.rows, (int)d.vocab, store_of(logits, dlogits, d.rows, d.vocab, d.dtype),
+                static_cast<const T*>(logits), targets, d.ignore_index, k,
+                reinterpret_cast<const RowStat*>(stats), dl, (uint32_t)seq, scale, dloss, static_cast<T*>(dlogits));
     });
     return hipGetLastError();
 }

@@ -122,6 +122,7 @@ def test_limits(rules):
             for threads, parts in ((rules.row_threads(*i64(rows, b)), 1),
                                    (rules.grad_threads(*i64(rows, b)), rules.grad_parts(*i64(rows, b)))):
                 assert threads in (64, 128, 256, 512, 1024) and parts >= 1
+                assert rules.grad_threads(*i64(rows, b)) != 128  # not compiled
                 assert rows * threads <= most and (parts == 1 or rows < 256) and parts <= 512
             for size in (2, 4):
                 for both in (0, 1):

@@ -230,6 +230,7 @@ struct PreferenceWs {
 };
 struct PolicyWs {
     size_t part;    // f64 [256][4] sums
+    size_t logp;    // f64 [batch seq]
     size_t counts;  // u32 [batch] counted tokens, where the mean runs over sequences
     size_t parts;   // loss_parts_ws
     size_t total;

@@ -75,18 +75,19 @@ template <typename S> __device__ __forceinline__ Stat<S> stat_join(Stat<S> a, St
 }
 
 // Over the workgroup's NT threads in a fixed order: a butterfly over each wave,
-// then the waves in order. red: one slot per wave.
-template <int NT, typename S>
-__device__ __forceinline__ Stat<S> wg_stat(Stat<S> v, LpScale k, Stat<S>* red) {
+// then the waves in order, with a sum of type R: of floats, this last chain loses
+// the most, and it alone is short enough for doubles. red: one slot per wave.
+template <int NT, typename R, typename S>
+__device__ __forceinline__ Stat<R> wg_stat(Stat<S> v, LpScale k, Stat<S>* red) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1)
         v = stat_join(v, Stat<S>{__shfl_xor(v.m, o, kWave), __shfl_xor(v.s, o, kWave)}, k);
     if (lane_id() == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = red[0];
+    Stat<R> r{red[0].m, (R)red[0].s};
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) v = stat_join(v, red[w], k);
-    return v;
+    for (int w = 1; w < NT / 64; ++w) r = stat_join(r, Stat<R>{red[w].m, (R)red[w].s}, k);
+    return r;
 }
 
 // What a share's terms are relative to: where all of it is -inf, anything finite.
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(NT) void parts_k(int vocab, const T* __restrict__ l
     const int hi = lo + share < (int)span.nvec ? lo + share : (int)span.nvec;
     Stat<double> st = vec_stat<T, NT, double, 4>(xr + span.head, lo + (int)threadIdx.x, hi, k);
     if (blockIdx.y == 0) st = edge_stat(xr, vocab, span, st, k);
-    st = wg_stat<NT>(st, k, red);
+    st = wg_stat<NT, double>(st, k, red);
     if (threadIdx.x == 0) part[row * gridDim.y + blockIdx.y] = st;
 }
 // The thread's part of a row, for wg_stat.
@@ -224,18 +225,20 @@ __device__ __forceinline__ Stat<float> float_stat(Stat<double> v) { return Stat<
 
 // l (0 where the row is not counted) and the row's statistics, read from the
 // logits or (SPLIT) joined from its parts; a counted target past the vocabulary
-// makes its l NaN. L: float, or double for sums over answers.
+// makes its l NaN. L: float, or double for sums over answers; logp32 (may be null):
+// those as floats, too.
 template <typename T, int NT, typename L, bool SPLIT>
 __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__ logits,
                                                 const uint32_t* __restrict__ targets, int64_t ignore_index, LpScale k,
                                                 const Stat<double>* __restrict__ part, int parts, L* __restrict__ logp,
-                                                RowStat* __restrict__ stats) {
+                                                float* __restrict__ logp32, RowStat* __restrict__ stats) {
     __shared__ Stat<double> red[NT / 64];
     const int64_t row = blockIdx.x;
     const uint32_t t = targets[row];
     if (!counted(t, ignore_index)) {
         if (threadIdx.x == 0) {
             logp[row] = 0;
+            if (logp32) logp32[row] = 0.f;
             if (stats) stats[row] = RowStat{0.f, 1.f};
         }
         return;
@@ -245,10 +248,12 @@ __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__
     Stat<double> v;
     if constexpr (SPLIT) v = own_part(part, row, parts);
     else v = row_stat<T, NT, double>(xr, vocab, k);
-    v = wg_stat<NT>(v, k, red);
+    v = wg_stat<NT, double>(v, k, red);
     if (threadIdx.x == 0) {
         const double x = t < (uint32_t)vocab ? from_raw<T>(xt) : __builtin_nanf("");
-        logp[row] = (L)((x - (double)v.m) * k.inv_t64 - log(v.s));
+        const double l = (x - (double)v.m) * k.inv_t64 - log(v.s);
+        logp[row] = (L)l;
+        if (logp32) logp32[row] = (float)l;
         if (stats) stats[row] = RowStat{v.m, (float)v.s};
     }
 }
@@ -416,15 +421,22 @@ struct PolicyInputs {
     float A, old, ref;
     bool has_old, has_ref;
 };
-__device__ __forceinline__ PolicyInputs policy_inputs(const mc_policy_desc& d, const float* adv, const float* old,
-                                                      const float* ref, int64_t row, uint32_t seq) {
-    return PolicyInputs{adv[d.per_token_advantages ? row : seq], old ? old[row] : 0.f, ref ? ref[row] : 0.f,
+// Unconditional, from the targets where there are none: a load under a condition is
+// waited for at its end.
+__device__ __forceinline__ PolicyInputs policy_inputs(const mc_policy_desc& d, const uint32_t* targets,
+                                                      const float* adv, const float* old, const float* ref,
+                                                      int64_t row, uint32_t seq) {
+    const float* spare = reinterpret_cast<const float*>(targets);
+    return PolicyInputs{adv[d.per_token_advantages ? row : seq], (old ? old : spare)[row], (ref ? ref : spare)[row],
                         old != nullptr, ref != nullptr};
 }
-__device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, float l, const PolicyInputs& in) {
+// L: float for the gradient. The loss takes l in double: its differences to the other
+// policies' are small against it, and terms of both signs cancel in the sum.
+template <typename L>
+__device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, L l, const PolicyInputs& in) {
     PolicyTerm p;
     const float A = in.A;
-    const float r = in.has_old ? expf(l - in.old) : (l == l ? 1.f : l);
+    const float r = in.has_old ? expf((float)(l - (L)in.old)) : l == l ? 1.f : (float)l;
     const float held = fminf(fmaxf(r, 1.f - d.clip_low), 1.f + d.clip_high);
     const bool clipped = held * A < r * A;
     p.clipped = clipped ? 1.f : 0.f;
@@ -432,7 +444,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, float
     p.dl = clipped ? 0.f : -r * A;
     p.kl = 0.f;
     if (in.has_ref) {
-        const float u = in.ref - l, g = expm1f(u);
+        const float u = (float)((L)in.ref - l), g = expm1f(u);
         p.kl = g - u;
         if (d.kl_coef != 0.f) {
             p.term = fmaf(d.kl_coef, p.kl, p.term);
@@ -460,7 +472,7 @@ __device__ __forceinline__ void policy_finish(const mc_policy_desc& d, bool by_s
 // sums in order.
 template <int NT>
 __global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, const uint32_t* __restrict__ targets,
-                                               const float* __restrict__ logp, const float* __restrict__ adv,
+                                               const double* __restrict__ logp, const float* __restrict__ adv,
                                                const float* __restrict__ old, const float* __restrict__ ref,
                                                const uint32_t* __restrict__ n, double (*part)[4],
                                                float* __restrict__ loss, float* __restrict__ metrics,
@@ -472,7 +484,7 @@ __global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, 
     constexpr int U = 4;  // rows whose loads are in flight together
     for (int64_t row0 = r0 + threadIdx.x; row0 < r1; row0 += U * NT) {
         uint32_t t[U], nq[U];
-        float l[U];
+        double l[U];
         PolicyInputs in[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -480,8 +492,8 @@ __global__ __launch_bounds__(NT) void policy_k(mc_policy_desc d, int64_t chunk, 
             const uint32_t q = (uint32_t)row / (uint32_t)d.seq;
             t[u] = targets[row];
             l[u] = logp[row];
-            in[u] = policy_inputs(d, adv, old, ref, row, q);
-            nq[u] = n ? n[q] : 1u;
+            in[u] = policy_inputs(d, targets, adv, old, ref, row, q);
+            nq[u] = (n ? n : targets)[q];
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -622,7 +634,7 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
     Stat<float> st;
     if constexpr (SPLIT) st = float_stat(own_part(part, row, parts));
     else st = row_stat<T, NT, float>(xr, vocab, k);
-    st = wg_stat<NT>(st, k, red);
+    st = wg_stat<NT, float>(st, k, red);
     const RowStat v{st.m, st.s};
     entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
     __syncthreads();
@@ -1084,6 +1096,19 @@ template <int NT> struct RowCount {
     }
 };
 
+// log s to 1e-8: s = 2^e f with f in [0.7, 1.4], whose log is small enough for a
+// float, and what the float f has lost.
+__device__ __forceinline__ double log_of(double s) {
+    int e;
+    float f = frexpf((float)s, &e);
+    if (f < 0.70710678f) {
+        f *= 2.f;
+        e -= 1;
+    }
+    const float rest = (float)(ldexp(s, -e) - (double)f);
+    return fma((double)e, 0.69314718055994530942, (double)(logf(f) + rest));
+}
+
 // l, and with the token's weight its gradient. Row: HeldRow, or SplitRow with
 // parts. given: n_given counts that add up to the tokens that share the weight
 // (by_seq: of each sequence, one number each), or null: counted here over len
@@ -1097,8 +1122,8 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
                                                        const uint32_t* __restrict__ given, int n_given, int len,
                                                        bool by_seq,
                                                        uint32_t* __restrict__ n, LpScale k,
-                                                       const float* __restrict__ dloss, float* __restrict__ logp,
-                                                       T* __restrict__ dlogits) {
+                                                       const float* __restrict__ dloss, double* __restrict__ logp,
+                                                       float* __restrict__ logp32, T* __restrict__ dlogits) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ uint32_t redc[NT / 64];
     const RowThreads th = row_threads<NT>();
@@ -1108,7 +1133,10 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     T* dr = dlogits + row * vocab;
     const uint32_t t = targets[row];
     if (!counted(t, d.ignore_index)) {
-        if (writer) logp[row] = 0.f;
+        if (writer) {
+            logp[row] = 0.0;
+            logp32[row] = 0.f;
+        }
         zero_row(dr, vocab, how, th);
         return;
     }
@@ -1116,7 +1144,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     const bool in = t < (uint32_t)vocab;
     const uint32_t xt = raw_load(xr, in ? t : 0);
     const uint32_t q = (uint32_t)row / (uint32_t)d.seq;
-    const PolicyInputs pin = policy_inputs(d, adv, old, ref, row, q);
+    const PolicyInputs pin = policy_inputs(d, targets, adv, old, ref, row, q);
     const float up = dloss ? dloss[0] : 1.f;
     const uint32_t* cw = by_seq ? targets + (int64_t)q * d.seq : targets;
     RowCount<NT> count;
@@ -1124,24 +1152,25 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     Row held;
     held.load(xr, vocab, parts, row, th);
     count.put(len, redc, [&](uint32_t w) { return counted(w, d.ignore_index); });
-    const Stat<float> st = wg_stat<NT>(held.stat(k), k, red);
-    const RowStat v{st.m, st.s};
+    const Stat<double> st = wg_stat<NT, double>(held.stat(k), k, red);
+    const RowStat v{st.m, (float)st.s};
     const uint32_t share = count.total(redc, given ? given + (by_seq ? q : 0) : nullptr, n_given);
     const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
     if (writer) {
-        logp[row] = l;
+        const double l64 = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s) : (double)l;
+        logp[row] = l64;
+        logp32[row] = (float)l64;
         if (n) n[q] = share;  // the same from every row of the sequence
     }
     float g = policy_term(d, l, pin).dl / (by_seq ? (float)d.batch * (float)share : (float)share) * up;
     if (g == 0.f) {
         zero_row(dr, vocab, how, th);
-        return;
+    } else {
+        g *= k.inv_t;
+        const RowGrad grad = row_grad(-g, v, k.c);
+        held.store(dr, how, grad);
+        if (in && held.owner((int)t) == th.self) Elem<T>::store(dr, t, grad(from_raw<T>(xt)) + g);
     }
-    g *= k.inv_t;
-    const RowGrad grad = row_grad(-g, v, k.c);
-    held.store(dr, how, grad);
-    if (in && held.owner((int)t) == th.self)
-        Elem<T>::store(dr, t, grad(from_raw<T>(xt)) + g);
 }
 
 // given: n_given counts of the mask, or null: counted here over len of it (0
@@ -1187,7 +1216,7 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store
     if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab)
         owners.insert(held.owner(entry.id), (int)(blockIdx.y * NT));
     const uint32_t x = entry.logit(xr, vocab);
-    const Stat<float> st = wg_stat<NT>(held.stat(k), k, red);
+    const Stat<float> st = wg_stat<NT, float>(held.stat(k), k, red);
     const RowStat v{st.m, st.s};
     entry.close(d, tlse != nullptr, lse, from_raw<T>(x), v, k, te);
     float w = d.temperature / (mask ? (float)count.total(redc, given, n_given) : (float)d.rows) * up;
@@ -1340,8 +1369,8 @@ int launch_parts(bool both, int64_t rows, int64_t vocab, int dtype, const void* 
 }
 
 template <typename L>
-hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, L* logp, float* stats,
-                          void* parts_ws, hipStream_t stream) {
+hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, L* logp,
+                          float* logp32, float* stats, void* parts_ws, hipStream_t stream) {
     const LpScale k = row_scale(d.temperature);
     const int parts =
         launch_parts(false, d.rows, d.vocab, d.dtype, logits, targets, d.ignore_index, nullptr, k, parts_ws, stream);
@@ -1353,7 +1382,8 @@ hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const ui
             constexpr bool SPLIT = decltype(split)::value;
             lp_rows_k<T, NT, L, SPLIT><<<dim3((unsigned)d.rows), NT, 0, stream>>>(
                 (int)d.vocab, static_cast<const T*>(logits), targets, d.ignore_index, k,
-                static_cast<const Stat<double>*>(parts_ws), parts, logp, reinterpret_cast<RowStat*>(stats));
+                static_cast<const Stat<double>*>(parts_ws), parts, logp, logp32,
+                reinterpret_cast<RowStat*>(stats));
         };
         if constexpr (NT == 64) {
             if (parts > 1) return go(std::true_type{});
@@ -1366,7 +1396,7 @@ hipError_t launch_lp_rows(const mc_logprob_desc& d, const void* logits, const ui
 
 hipError_t launch_token_logprobs_fwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets, float* logp,
                                      float* stats, void* ws, hipStream_t stream) {
-    return launch_lp_rows(d, logits, targets, logp, stats, ws, stream);
+    return launch_lp_rows(d, logits, targets, logp, nullptr, stats, ws, stream);
 }
 
 hipError_t launch_token_logprobs_bwd(const mc_logprob_desc& d, const void* logits, const uint32_t* targets,
@@ -1410,7 +1440,7 @@ hipError_t launch_preference_fwd(const mc_preference_desc& d, const void* logits
     float* inv_n = reinterpret_cast<float*>(ws + w.inv_n);
     float* dseq = stats ? stats + 2 * rows : nullptr;
     const mc_logprob_desc lp{rows, d.vocab, d.ignore_index, 1.0f, d.dtype};
-    hipError_t e = launch_lp_rows(lp, logits, targets, logp, stats, ws + w.parts, stream);
+    hipError_t e = launch_lp_rows(lp, logits, targets, logp, nullptr, stats, ws + w.parts, stream);
     if (e != hipSuccess) return e;
     if (rows <= kOneGroupRows && 2 * d.pairs <= kOneGroupSeqs) {
         by_group_size(rows, [&](auto threads) {
@@ -1433,6 +1463,8 @@ PolicyWs policy_ws(const mc_policy_desc& d) {
     size_t at = 0;
     w.part = at;
     at += kSumGroups * 4 * sizeof(double);
+    w.logp = at;
+    at += align256((size_t)(d.batch * d.seq) * sizeof(double));
     w.counts = at;
     if (d.reduction == MC_MEAN_SEQUENCES) at += align256((size_t)d.batch * sizeof(uint32_t));
     w.parts = at;
@@ -1451,10 +1483,11 @@ const uint32_t* policy_counts(const mc_policy_desc& d, const uint32_t* targets, 
     return n;
 }
 
-hipError_t launch_policy_sums(const mc_policy_desc& d, const uint32_t* targets, const float* logp, const float* adv,
-                              const float* old, const float* ref, const uint32_t* n, char* ws, float* loss,
-                              float* metrics, float* dlp, hipStream_t stream) {
+hipError_t launch_policy_sums(const mc_policy_desc& d, const uint32_t* targets, const float* adv, const float* old,
+                              const float* ref, const uint32_t* n, char* ws, float* loss, float* metrics, float* dlp,
+                              hipStream_t stream) {
     auto* part = reinterpret_cast<double(*)[4]>(ws + policy_ws(d).part);
+    const double* logp = reinterpret_cast<const double*>(ws + policy_ws(d).logp);
     by_sum_kernel(d.batch * d.seq, [&](auto threads, int groups, int64_t chunk) {
         constexpr int NT = decltype(threads)::value;
         policy_k<NT><<<dim3((unsigned)groups), NT, 0, stream>>>(d, chunk, targets, logp, adv, old, ref, n, part, loss,
@@ -1474,10 +1507,10 @@ hipError_t launch_policy_fwd(const mc_policy_desc& d, const void* logits, const 
     hipError_t e;
     const uint32_t* n = policy_counts(d, targets, ws, stream, e);
     if (e != hipSuccess) return e;
-    e = launch_lp_rows(lp, logits, targets, logp, stats, ws + policy_ws(d).parts, stream);
+    const PolicyWs w = policy_ws(d);
+    e = launch_lp_rows(lp, logits, targets, reinterpret_cast<double*>(ws + w.logp), logp, stats, ws + w.parts, stream);
     if (e != hipSuccess) return e;
-    return launch_policy_sums(d, targets, logp, adv, old, ref, n, ws, loss, metrics, stats ? stats + 2 * rows : nullptr,
-                              stream);
+    return launch_policy_sums(d, targets, adv, old, ref, n, ws, loss, metrics, stats ? stats + 2 * rows : nullptr, stream);
 }
 
 DistillWs distill_ws(const mc_distill_desc& d) {
@@ -1604,11 +1637,12 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
             policy_both_k<T, NT, typename S::Row><<<dim3((unsigned)rows, (unsigned)parts), NT, 0, stream>>>(
                 d, how, static_cast<const T*>(logits), targets, adv, old,
                 ref, static_cast<const Stat<double>*>(parts_ws), here ? nullptr : by_seq ? n : part, n_given,
-                here ? (int)span : 0, by_seq, here ? n : nullptr, k, dloss, logp, static_cast<T*>(dlogits));
+                here ? (int)span : 0, by_seq, here ? n : nullptr, k, dloss,
+                reinterpret_cast<double*>(ws + w.logp), logp, static_cast<T*>(dlogits));
         });
         if (e != hipSuccess) return e;
         if ((e = hipGetLastError()) != hipSuccess) return e;
-        return launch_policy_sums(d, targets, logp, adv, old, ref, n, ws, loss, metrics, nullptr, stream);
+        return launch_policy_sums(d, targets, adv, old, ref, n, ws, loss, metrics, nullptr, stream);
     }
     e = launch_policy_fwd(d, logits, targets, adv, old, ref, loss, logp, metrics, stats, ws, stream);
     if (e != hipSuccess) return e;

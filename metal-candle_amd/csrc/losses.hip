@@ -47,6 +47,22 @@ template <typename T> __device__ __forceinline__ float from_raw(uint32_t w) {
     return std::is_same<T, float>::value ? __uint_as_float(w) : __uint_as_float(w << 16);
 }
 
+template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// wave_sum's steps in 64 bits
+__device__ __forceinline__ double wave_sum(double v) {
+    v += dpp64<0xB1>(v);
+    v += dpp64<0x4E>(v);
+    v += dpp64<0x141>(v);
+    v += dpp64<0x140>(v);
+    v += __shfl_xor(v, 16, kWave);
+    v += __shfl_xor(v, 32, kWave);
+    return v;
+}
 // ------------------------------------------------------------ row statistics
 // m = max x and s = sum 2^((x - m) c), c = log2(e) / T as c_hi + c_lo
 // (row_scale): with one float for c every exponent is off by up to 6e-8 of
@@ -66,27 +82,38 @@ template <typename S> struct Stat {
 // would be lost.
 __device__ __forceinline__ float exp_of(float d, LpScale k) { return exp2_hw(fmaf(d, k.c_hi, d * k.c_lo)); }
 
+// exp2_hw is low by 3.4e-9 of itself on the average of any stretch (2.6e-8 rms): what
+// sums of doubles scale their terms with, once more and more once each, is put right
+// by that.
+constexpr double kExpMean = 1.0 + 3.4e-9;
+// A sum relative to `from` as one relative to m >= from; equal ones, -inf among them,
+// need no factor.
+template <typename S> __device__ __forceinline__ S rescaled(S s, float from, float m, LpScale k) {
+    if (from == m) return s;
+    const S f = exp_of(from - m, k);
+    return std::is_same<S, double>::value ? s * (f * (S)kExpMean) : s * f;
+}
 template <typename S> __device__ __forceinline__ Stat<S> stat_join(Stat<S> a, Stat<S> b, LpScale k) {
     const float m = fmaxf(a.m, b.m);
-    // equal maxima, -inf among them, need no factor
-    const S sa = a.m == m ? a.s : a.s * (S)exp_of(a.m - m, k);
-    const S sb = b.m == m ? b.s : b.s * (S)exp_of(b.m - m, k);
-    return Stat<S>{m, sa + sb};
+    return Stat<S>{m, rescaled(a.s, a.m, m, k) + rescaled(b.s, b.m, m, k)};
 }
 
-// Over the workgroup's NT threads in a fixed order: a butterfly over each wave,
-// then the waves in order, with a sum of type R: of floats, this last chain loses
-// the most, and it alone is short enough for doubles. red: one slot per wave.
+// Over the workgroup's NT threads in a fixed order: the maximum of each wave, its
+// sums relative to that, then the same of the waves with sums of type R (of floats,
+// that chain loses the most, and it alone is short enough for doubles). One factor
+// per step: joined in pairs, a share would collect the errors of one at every level.
+// red: one slot per wave.
 template <int NT, typename R, typename S>
 __device__ __forceinline__ Stat<R> wg_stat(Stat<S> v, LpScale k, Stat<S>* red) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1)
-        v = stat_join(v, Stat<S>{__shfl_xor(v.m, o, kWave), __shfl_xor(v.s, o, kWave)}, k);
-    if (lane_id() == 0) red[threadIdx.x >> 6] = v;
+    const float wm = wave_max(v.m);
+    const S ws = wave_sum(rescaled(v.s, v.m, wm, k));
+    if (lane_id() == 0) red[threadIdx.x >> 6] = Stat<S>{wm, ws};
     __syncthreads();
-    Stat<R> r{red[0].m, (R)red[0].s};
+    Stat<R> r{red[0].m, 0};
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) r = stat_join(r, Stat<R>{red[w].m, (R)red[w].s}, k);
+    for (int w = 1; w < NT / 64; ++w) r.m = fmaxf(r.m, red[w].m);
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) r.s += rescaled((R)red[w].s, red[w].m, r.m, k);
     return r;
 }
 
@@ -121,7 +148,7 @@ __device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int
 #pragma unroll
             for (int e = 0; e < N; ++e) vm = fmaxf(vm, v[u][e]);
         if (vm > m) {
-            s *= (S)exp_of(m - vm, k);  // 0 for the first
+            s = rescaled(s, m, vm, k);  // 0 for the first
             m = vm;
         }
         const float base = base_of(m);
@@ -159,22 +186,6 @@ __device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab,
 }
 
 // ------------------------------------------------- sums over a workgroup
-template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-// wave_sum's steps in 64 bits
-__device__ __forceinline__ double wave_sum(double v) {
-    v += dpp64<0xB1>(v);
-    v += dpp64<0x4E>(v);
-    v += dpp64<0x141>(v);
-    v += dpp64<0x140>(v);
-    v += __shfl_xor(v, 16, kWave);
-    v += __shfl_xor(v, 32, kWave);
-    return v;
-}
 template <int NT, int C> __device__ __forceinline__ void wg_sum_f64(double (&v)[C], double (*red)[C]) {
 #pragma unroll
     for (int c = 0; c < C; ++c) v[c] = wave_sum(v[c]);
@@ -251,7 +262,7 @@ __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__
     v = wg_stat<NT, double>(v, k, red);
     if (threadIdx.x == 0) {
         const double x = t < (uint32_t)vocab ? from_raw<T>(xt) : __builtin_nanf("");
-        const double l = (x - (double)v.m) * k.inv_t64 - log(v.s);
+        const double l = (x - (double)v.m) * k.inv_t64 - log(v.s * kExpMean);
         logp[row] = (L)l;
         if (logp32) logp32[row] = (float)l;
         if (stats) stats[row] = RowStat{v.m, (float)v.s};
@@ -1157,7 +1168,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     const uint32_t share = count.total(redc, given ? given + (by_seq ? q : 0) : nullptr, n_given);
     const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
     if (writer) {
-        const double l64 = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s) : (double)l;
+        const double l64 = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s * kExpMean) : (double)l;
         logp[row] = l64;
         logp32[row] = (float)l64;
         if (n) n[q] = share;  // the same from every row of the sequence

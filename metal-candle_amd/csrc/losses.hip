@@ -82,9 +82,8 @@ template <typename S> struct Stat {
 // would be lost.
 __device__ __forceinline__ float exp_of(float d, LpScale k) { return exp2_hw(fmaf(d, k.c_hi, d * k.c_lo)); }
 
-// exp2_hw is low by 3.4e-9 of itself on the average of any stretch (2.6e-8 rms): what
-// sums of doubles scale their terms with, once more and more once each, is put right
-// by that.
+// exp2_hw is low by 3.4e-9 of itself on the average of any stretch (2.6e-8 rms); what
+// rescales a sum of doubles is put right by that.
 constexpr double kExpMean = 1.0 + 3.4e-9;
 // A sum relative to `from` as one relative to m >= from; equal ones, -inf among them,
 // need no factor.
@@ -124,7 +123,12 @@ __device__ __forceinline__ float term_of(float x, float base, LpScale k) { retur
 // One thread's share of a row's vectors from c on: U of them requested and
 // reduced at a time, one rescale to their maximum, then one exp2 per element. The
 // last of them go together, too: one by one, each would wait for its own load.
-template <typename T, int NT, typename S, int U>
+// P: of the sums of U vectors. With floats the thread that holds a row's largest
+// term, 1, rounds at 2^-24 of it for each term it adds there, and l is off by 4e-8
+// (rms) where that term is most of the row; a score of 110 tokens by 5e-7. Doubles
+// cost 2.7% of a preference step on 4072 bf16 rows of 151936 (555 / 570 us) and 10%
+// of 777 rows alone (51.4 / 56.5), so they are for l that are summed.
+template <typename T, int NT, typename S, int U, typename P = float>
 __device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int nvec, LpScale k) {
     constexpr int N = Vec16<T>::N;
     float m = kNegInf;
@@ -152,12 +156,12 @@ __device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int
             m = vm;
         }
         const float base = base_of(m);
-        float ps[U];
+        P ps[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            ps[u] = 0.f;
+            ps[u] = 0;
 #pragma unroll
-            for (int e = 0; e < N; ++e) ps[u] += term_of(v[u][e], base, k);
+            for (int e = 0; e < N; ++e) ps[u] += (P)term_of(v[u][e], base, k);
         }
 #pragma unroll
         for (int u = U; u > 1; u /= 2)
@@ -178,11 +182,11 @@ __device__ __forceinline__ Stat<S> edge_stat(const T* __restrict__ xr, int vocab
     const float v = Elem<T>::load(xr, j);
     return stat_join(st, Stat<S>{v, (S)term_of(v, base_of(v), k)}, k);
 }
-template <typename T, int NT, typename S>
+template <typename T, int NT, typename S, typename P>
 __device__ __forceinline__ Stat<S> row_stat(const T* __restrict__ xr, int vocab, LpScale k) {
     static_assert(NT >= 2 * Vec16<T>::N, "a thread per edge element");
     const RowSpan<T> span(xr, vocab);
-    return edge_stat(xr, vocab, span, vec_stat<T, NT, S, 4>(xr + span.head, threadIdx.x, (int)span.nvec, k), k);
+    return edge_stat(xr, vocab, span, vec_stat<T, NT, S, 4, P>(xr + span.head, threadIdx.x, (int)span.nvec, k), k);
 }
 
 // ------------------------------------------------- sums over a workgroup
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(NT) void parts_k(int vocab, const T* __restrict__ l
     const RowSpan<T> span(xr, vocab);
     const int share = ((int)span.nvec + (int)gridDim.y - 1) / (int)gridDim.y, lo = (int)blockIdx.y * share;
     const int hi = lo + share < (int)span.nvec ? lo + share : (int)span.nvec;
-    Stat<double> st = vec_stat<T, NT, double, 4>(xr + span.head, lo + (int)threadIdx.x, hi, k);
+    Stat<double> st = vec_stat<T, NT, double, 4, double>(xr + span.head, lo + (int)threadIdx.x, hi, k);
     if (blockIdx.y == 0) st = edge_stat(xr, vocab, span, st, k);
     st = wg_stat<NT, double>(st, k, red);
     if (threadIdx.x == 0) part[row * gridDim.y + blockIdx.y] = st;
@@ -258,11 +262,11 @@ __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__
     const uint32_t xt = raw_load(xr, t < (uint32_t)vocab ? t : 0);
     Stat<double> v;
     if constexpr (SPLIT) v = own_part(part, row, parts);
-    else v = row_stat<T, NT, double>(xr, vocab, k);
+    else v = row_stat<T, NT, double, L>(xr, vocab, k);
     v = wg_stat<NT, double>(v, k, red);
     if (threadIdx.x == 0) {
         const double x = t < (uint32_t)vocab ? from_raw<T>(xt) : __builtin_nanf("");
-        const double l = (x - (double)v.m) * k.inv_t64 - log(v.s * kExpMean);
+        const double l = (x - (double)v.m) * k.inv_t64 - log(v.s);
         logp[row] = (L)l;
         if (logp32) logp32[row] = (float)l;
         if (stats) stats[row] = RowStat{v.m, (float)v.s};
@@ -644,7 +648,7 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
     const uint32_t x = entry.logit(xr, vocab);
     Stat<float> st;
     if constexpr (SPLIT) st = float_stat(own_part(part, row, parts));
-    else st = row_stat<T, NT, float>(xr, vocab, k);
+    else st = row_stat<T, NT, float, float>(xr, vocab, k);
     st = wg_stat<NT, float>(st, k, red);
     const RowStat v{st.m, st.s};
     entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
@@ -1168,7 +1172,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     const uint32_t share = count.total(redc, given ? given + (by_seq ? q : 0) : nullptr, n_given);
     const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
     if (writer) {
-        const double l64 = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s * kExpMean) : (double)l;
+        const double l64 = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s) : (double)l;
         logp[row] = l64;
         logp32[row] = (float)l64;
         if (n) n[q] = share;  // the same from every row of the sequence

@@ -22,10 +22,10 @@
 // Bound by HBM throughout: 2 or 4 bytes per logit and pass against about ten
 // operations. A copy of 1 GiB runs at 5.0 TB/s here; kernels, three of four rows
 // counted:
-//   lp_rows_k       bf16 4072 x 151936 157 us, 6.0 TB/s; f32 2036 x 50257 54.5, 5.7
-//   lp_bwd_k        the same 388, 5.6; 115, 6.2
-//   policy_both_k   bf16 4096 x 151936 412, 5.3; f32 2036 x 50257 140, 5.1
-//   distill_both_k  bf16 2036 x 151936, 64 entries, 220, 4.9; f32 1500 x 50257, 8 entries, 110, 4.9
+//   lp_rows_k       f32 2036 x 50257 54.0 us, 5.7 TB/s; bf16, for sums of l, 4072 x 151936 179, 5.2
+//   lp_bwd_k        the same 116, 6.2; 380, 5.7
+//   policy_both_k   bf16 4096 x 151936 401, 5.4; f32 2036 x 50257 133, 5.4
+//   distill_both_k  bf16 2036 x 151936, 64 entries, 217, 5.0; f32 1500 x 50257, 8 entries, 108, 5.0
 #include <type_traits>
 
 #include "common.hpp"

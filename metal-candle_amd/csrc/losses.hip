@@ -415,16 +415,34 @@ __global__ __launch_bounds__(NT) void preference_pairs_k(mc_preference_desc d, c
 }
 
 // ------------------------------------------------------------------ policy
-// Counted tokens of each sequence, a wave for each.
-__global__ __launch_bounds__(256) void seq_counts_k(int64_t batch, int64_t seq, const uint32_t* __restrict__ targets,
-                                                    int64_t ignore_index, uint32_t* __restrict__ n) {
-    const int64_t q = (int64_t)blockIdx.x * 4 + wave_id();
+// Counted tokens of each sequence: NT = 64, a wave for each, or a workgroup of NT
+// threads, which keep eight loads each in flight.
+template <int NT>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void seq_counts_k(int64_t batch, int64_t seq,
+                                                                    const uint32_t* __restrict__ targets,
+                                                                    int64_t ignore_index, uint32_t* __restrict__ n) {
+    constexpr int U = 8;
+    __shared__ uint32_t red[NT / 64];
+    const int64_t q = NT == 64 ? (int64_t)blockIdx.x * 4 + wave_id() : (int64_t)blockIdx.x;
     if (q >= batch) return;
+    const uint32_t* t = targets + q * seq;
     uint32_t c = 0;
-    for (int64_t i = lane_id(); i < seq; i += kWave) c += counted(targets[q * seq + i], ignore_index) ? 1u : 0u;
+    for (int64_t i = NT == 64 ? lane_id() : (int)threadIdx.x; i < seq; i += U * NT) {
+        uint32_t v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = t[i + u * NT < seq ? i + u * NT : i];
+#pragma unroll
+        for (int u = 0; u < U; ++u) c += i + u * NT < seq && counted(v[u], ignore_index) ? 1u : 0u;
+    }
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) c += (uint32_t)__shfl_xor((int)c, o, kWave);
-    if (lane_id() == 0) n[q] = c;
+    if constexpr (NT > 64) {
+        if (lane_id() == 0) red[wave_id()] = c;
+        __syncthreads();
+        c = 0;
+        for (int w = 0; w < NT / 64; ++w) c += red[w];
+    }
+    if (NT == 64 ? lane_id() == 0 : threadIdx.x == 0) n[q] = c;
 }
 
 // A token's terms: -min(r A, clip(r) A) + kl_coef kl, dl, kl and whether the
@@ -1085,28 +1103,28 @@ __global__ __launch_bounds__(256) void counts_k(int64_t rows, int64_t chunk, con
 // row's loads, put after them, a barrier of the kernel, total.
 template <int NT> struct RowCount {
     static constexpr int kPer = 4;
-    uint32_t w[kPer];
-    // value(i): the i-th target or mask byte; called where len is 0, too
-    template <typename F> __device__ __forceinline__ void load(int len, F&& value) {
+    static_assert(NT >= kCountBlocks, "a thread for each count");
+    uint32_t w[kPer], part;
+    // value(i): the i-th target or mask byte; called where len is 0, too. given: where
+    // n_given is 0, any address.
+    template <typename F>
+    __device__ __forceinline__ void load(int len, F&& value, const uint32_t* __restrict__ given, int n_given) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) w[i] = value(i * NT + (int)threadIdx.x < len ? i * NT + (int)threadIdx.x : 0);
+        part = given[(int)threadIdx.x < n_given ? (int)threadIdx.x : 0];
     }
-    template <typename F> __device__ __forceinline__ void put(int len, uint32_t* red, F&& on) const {
-        uint32_t c = 0;
+    template <typename F> __device__ __forceinline__ void put(int len, int n_given, uint32_t* red, F&& on) const {
+        uint32_t c = (int)threadIdx.x < n_given ? part : 0u;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) c += i * NT + (int)threadIdx.x < len && on(w[i]) ? 1u : 0u;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) c += (uint32_t)__shfl_xor((int)c, o, kWave);
         if (lane_id() == 0) red[threadIdx.x >> 6] = c;
     }
-    static __device__ __forceinline__ uint32_t total(const uint32_t* red, const uint32_t* __restrict__ given, int n) {
+    static __device__ __forceinline__ uint32_t total(const uint32_t* red) {
         uint32_t c = 0;
-        if (given) {
-            for (int i = 0; i < n; ++i) c += given[i];
-        } else {
 #pragma unroll
-            for (int k = 0; k < NT / 64; ++k) c += red[k];
-        }
+        for (int k = 0; k < NT / 64; ++k) c += red[k];
         return c;
     }
 };
@@ -1126,7 +1144,7 @@ __device__ __forceinline__ double log_of(double s) {
 
 // l, and with the token's weight its gradient. Row: HeldRow, or SplitRow with
 // parts. given: n_given counts that add up to the tokens that share the weight
-// (by_seq: of each sequence, one number each), or null: counted here over len
+// (by_seq: of each sequence, one number each), or n_given 0: counted here over len
 // targets. n (may be null): receives the sequences' counts.
 template <typename T, int NT, typename Row>
 __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store how, const T* __restrict__ logits,
@@ -1163,13 +1181,13 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     const float up = dloss ? dloss[0] : 1.f;
     const uint32_t* cw = by_seq ? targets + (int64_t)q * d.seq : targets;
     RowCount<NT> count;
-    count.load(len, [&](int i) { return cw[i]; });
+    count.load(len, [&](int i) { return cw[i]; }, n_given ? given + (by_seq ? q : 0) : targets, n_given);
     Row held;
     held.load(xr, vocab, parts, row, th);
-    count.put(len, redc, [&](uint32_t w) { return counted(w, d.ignore_index); });
+    count.put(len, n_given, redc, [&](uint32_t w) { return counted(w, d.ignore_index); });
     const Stat<double> st = wg_stat<NT, double>(held.stat(k), k, red);
     const RowStat v{st.m, (float)st.s};
-    const uint32_t share = count.total(redc, given ? given + (by_seq ? q : 0) : nullptr, n_given);
+    const uint32_t share = count.total(redc);
     const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
     if (writer) {
         const double l64 = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s) : (double)l;
@@ -1188,7 +1206,7 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     }
 }
 
-// given: n_given counts of the mask, or null: counted here over len of it (0
+// given: n_given counts of the mask, or n_given 0: counted here over len of it (0
 // without a mask).
 template <typename T, int NT, typename Row>
 __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store how, const T* __restrict__ logits,
@@ -1223,10 +1241,11 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store
     const float lse = tlse ? tlse[row] : 0.f;
     RowCount<NT> count;
     const uint8_t* cw = mask ? mask : reinterpret_cast<const uint8_t*>(xr);
-    count.load(len, [&](int i) { return (uint32_t)cw[i]; });
+    count.load(len, [&](int i) { return (uint32_t)cw[i]; },
+               n_given ? given : reinterpret_cast<const uint32_t*>(ids), n_given);
     Row held;
     held.load(xr, vocab, parts, row, th);
-    count.put(len, redc, [](uint32_t w) { return w != 0; });
+    count.put(len, n_given, redc, [](uint32_t w) { return w != 0; });
     entry.open(d, k.inv_t, te);
     if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab)
         owners.insert(held.owner(entry.id), (int)(blockIdx.y * NT));
@@ -1234,7 +1253,7 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store
     const Stat<float> st = wg_stat<NT, float>(held.stat(k), k, red);
     const RowStat v{st.m, st.s};
     entry.close(d, tlse != nullptr, lse, from_raw<T>(x), v, k, te);
-    float w = d.temperature / (mask ? (float)count.total(redc, given, n_given) : (float)d.rows) * up;
+    float w = d.temperature / (mask ? (float)count.total(redc) : (float)d.rows) * up;
     __syncthreads();
     const TeacherSums ts = entry.sums(d, te);
     if (writer) kl[row] = ts.kl;
@@ -1493,7 +1512,13 @@ const uint32_t* policy_counts(const mc_policy_desc& d, const uint32_t* targets, 
     e = hipSuccess;
     if (d.reduction != MC_MEAN_SEQUENCES) return nullptr;
     uint32_t* n = reinterpret_cast<uint32_t*>(ws + policy_ws(d).counts);
-    seq_counts_k<<<dim3((unsigned)((d.batch + 3) / 4)), 256, 0, stream>>>(d.batch, d.seq, targets, d.ignore_index, n);
+    // us of a forward over 64 logits, a wave per sequence / a workgroup: 20000 of one
+    // token 27.1 / 56.6, 8 of 1024 16.7 / 17.1, 2 of 8192 25.4 / 22.3, 1 of 200000 260 / 148
+    if (d.seq <= 1024)
+        seq_counts_k<64><<<dim3((unsigned)((d.batch + 3) / 4)), 256, 0, stream>>>(d.batch, d.seq, targets,
+                                                                                  d.ignore_index, n);
+    else
+        seq_counts_k<1024><<<dim3((unsigned)d.batch), 1024, 0, stream>>>(d.batch, d.seq, targets, d.ignore_index, n);
     e = hipGetLastError();
     return n;
 }
@@ -1646,7 +1671,7 @@ hipError_t launch_policy_fwd_bwd(const mc_policy_desc& d, const void* logits, co
             constexpr int NT = S::kThreads;
             const int64_t span = by_seq ? d.seq : rows;
             const bool here = span <= RowCount<NT>::kPer * NT;
-            int n_given = 1;
+            int n_given = here ? 0 : 1;
             if (!here && by_seq) policy_counts(d, targets, ws, stream, e);
             else if (!here) n_given = launch_counts(rows, targets, nullptr, d.ignore_index, part, stream);
             policy_both_k<T, NT, typename S::Row><<<dim3((unsigned)rows, (unsigned)parts), NT, 0, stream>>>(

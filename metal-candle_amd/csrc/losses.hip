@@ -47,13 +47,13 @@ template <typename T> __device__ __forceinline__ float from_raw(uint32_t w) {
     return std::is_same<T, float>::value ? __uint_as_float(w) : __uint_as_float(w << 16);
 }
 
+// The float wave_sum's steps in 64 bits.
 template <int CTRL> __device__ __forceinline__ double dpp64(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
     const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// wave_sum's steps in 64 bits
 __device__ __forceinline__ double wave_sum(double v) {
     v += dpp64<0xB1>(v);
     v += dpp64<0x4E>(v);
@@ -63,6 +63,7 @@ __device__ __forceinline__ double wave_sum(double v) {
     v += __shfl_xor(v, 32, kWave);
     return v;
 }
+
 // ------------------------------------------------------------ row statistics
 // m = max x and s = sum 2^((x - m) c), c = log2(e) / T as c_hi + c_lo
 // (row_scale): with one float for c every exponent is off by up to 6e-8 of

@@ -128,7 +128,8 @@ __device__ __forceinline__ float term_of(float x, float base, LpScale k) { retur
 // term, 1, rounds at 2^-24 of it for each term it adds there, and l is off by 4e-8
 // (rms) where that term is most of the row; a score of 110 tokens by 5e-7. Doubles
 // cost 2.7% of a preference step on 4072 bf16 rows of 151936 (555 / 570 us) and 10%
-// of 777 rows alone (51.4 / 56.5), so they are for l that are summed.
+// of 777 rows alone (51.4 / 56.5), so of bf16 logits they are for l that are summed;
+// of f32 ones, half as many per byte, they cost nothing.
 template <typename T, int NT, typename S, int U, typename P = float>
 __device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int nvec, LpScale k) {
     constexpr int N = Vec16<T>::N;
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(NT) void lp_rows_k(int vocab, const T* __restrict__
     const uint32_t xt = raw_load(xr, t < (uint32_t)vocab ? t : 0);
     Stat<double> v;
     if constexpr (SPLIT) v = own_part(part, row, parts);
-    else v = row_stat<T, NT, double, L>(xr, vocab, k);
+    else v = row_stat<T, NT, double, typename std::conditional<sizeof(T) == 4, double, L>::type>(xr, vocab, k);
     v = wg_stat<NT, double>(v, k, red);
     if (threadIdx.x == 0) {
         const double x = t < (uint32_t)vocab ? from_raw<T>(xt) : __builtin_nanf("");

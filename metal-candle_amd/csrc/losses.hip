@@ -30,6 +30,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "log_of.hpp"
 #include "rules.hpp"
 #include "vocab_rows.hpp"
 
@@ -1130,19 +1131,6 @@ template <int NT> struct RowCount {
         return c;
     }
 };
-
-// log s to 1e-8: s = 2^e f with f in [0.7, 1.4], whose log is small enough for a
-// float, and what the float f has lost.
-__device__ __forceinline__ double log_of(double s) {
-    int e;
-    float f = frexpf((float)s, &e);
-    if (f < 0.70710678f) {
-        f *= 2.f;
-        e -= 1;
-    }
-    const float rest = (float)(ldexp(s, -e) - (double)f);
-    return fma((double)e, 0.69314718055994530942, (double)(logf(f) + rest));
-}
 
 // l, and with the token's weight its gradient. Row: HeldRow, or SplitRow with
 // parts. given: n_given counts that add up to the tokens that share the weight

@@ -486,12 +486,15 @@ mc_status mc_policy_loss_fwd_bwd(const mc_policy_desc* d, const void* logits, co
  * teacher_logits fp32 [rows, top], in any order; an entry of -inf is left out,
  * whatever its id (rows of fewer entries), and an id that comes twice counts
  * twice. p = softmax over the row's entries of teacher_logits / T, or with
- * teacher_lse fp32 [rows] (the log-sum-exp of all the teacher's logits / T)
- * p = exp(teacher_logits / T - teacher_lse). With q = softmax(logits / T)
+ * teacher_lse fp32 [rows] (the log-sum-exp of all the teacher's logits / T, with
+ * T as the float that it is here) p = exp(teacher_logits / T - teacher_lse). With q = softmax(logits / T)
  *   loss = T^2 mean over the counted rows of sum_k p_k (log p_k - log q_{id k})
  *   dlogits = dloss (T / counted rows) (q_j sum_k p_k - sum_{k: id k = j} p_k)
  * mask uint8 [rows] (NULL: every row is counted); no row counted: NaN. A row
- * whose entries are all left out counts and adds 0. stats fp32 [rows * 2 + 1]. */
+ * whose entries are all left out counts and adds 0. The logarithms are formed in
+ * 64 bits from sums of float exponentials: a row's value is off by about 1e-7, as a
+ * log-probability is, however small it is and wherever the teacher's logits lie.
+ * stats fp32 [rows * 2 + 1]. */
 #define MC_DISTILL_MAX_TOP 256
 typedef struct mc_distill_desc {
     int64_t rows;       /* 1 .. 16777215 */

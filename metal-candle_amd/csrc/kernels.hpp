@@ -237,7 +237,7 @@ struct PolicyWs {
 };
 struct DistillWs {
     size_t part;   // f64 [256][2] sums
-    size_t kl;     // f32 [rows]
+    size_t kl;     // f64 [rows]
     size_t split;  // loss_parts_ws
     size_t total;
 };

@@ -567,97 +567,157 @@ __global__ __launch_bounds__(kSumGroups) void policy_join_k(mc_policy_desc d, bo
 }
 
 // ------------------------------------------------------------ distillation
-// A row's teacher, an entry per thread. Its softmax takes two steps with a
-// barrier of the kernel behind each: open leaves the waves' maxima and sums,
-// close forms p_k and the terms p_k (log p_k - log q_k), and sums gives their
-// totals to every thread. An entry is left out where its logit is -inf.
-struct TeacherSums {
-    float P, kl;
-    bool bad;  // an id past the vocabulary: the row is NaN
+// A row's teacher. One wave forms p_k = e_k / s and their sum (Top), a thread per
+// entry adds its id and the student's logit (TopEntry), and behind a barrier of the
+// kernel one wave forms sum p_k (log p_k - log q_k) from those and the row's
+// statistics (teacher_value). Before that barrier the teacher needs no other: one
+// behind the loads of a held row would have every wave wait until the last has issued
+// its own, which is most of the time that they take (2036 bf16 rows of 151936, 283 us
+// in place of 248). An entry is left out where its logit is -inf.
+// The logarithms are in double: their difference is small against them, the terms
+// cancel until about its square is left, and 1 / T as a float has an error of one
+// sign. With floats the loss of 2000 rows 5e-3 from a teacher of logits near 110 at
+// T = 1.5 was 1.7e-5 in place of 1.2e-5.
+// N: as many entries as the workgroup has threads, and all that there may be at most.
+template <int NT> struct Teacher {
+    static constexpr int N = NT < kDistillMaxTop ? NT : kDistillMaxTop;
+    int id[N];               // -1: left out
+    float p[N], t[N], x[N];  // t: the teacher's logit, x the student's
+    double s;                // log p_k = (t_k - m) / T - lse - log s
+    float m, lse, P;         // P: sum p
+    int bad;                 // an id past the vocabulary: the row is NaN
 };
-struct Teacher {
-    int id[kDistillMaxTop];                           // -1: left out
-    float p[kDistillMaxTop], x[kDistillMaxTop];       // and the student's logit
-    Stat<float> part[kDistillMaxTop / kWave];
-    float sum[kDistillMaxTop / kWave][2];
-    int bad[kDistillMaxTop / kWave];
-};
+// 2^y to a float: of y's leading part, and the rest as a factor.
+__device__ __forceinline__ float exp2_of(double y) {
+    const float hi = (float)y, e = exp2_hw(hi);
+    return hi > -200.f ? fmaf(e, (float)(y - (double)hi) * 0.693147181f, e) : e;  // far below, the rest may be infinite
+}
 struct TopEntry {
-    float z;
+    float t;
     int id;
     // Unconditional: see HeldRow.
     __device__ __forceinline__ void load(const mc_distill_desc& d, int64_t row, const int32_t* __restrict__ ids,
                                          const float* __restrict__ tl) {
         const int64_t at = row * d.top + ((int)threadIdx.x < d.top ? (int)threadIdx.x : 0);
-        z = tl[at];
+        t = tl[at];
         id = ids[at];
     }
-    __device__ __forceinline__ void open(const mc_distill_desc& d, float inv_t, Teacher& te) {
-        if (wave_id() * kWave >= d.top) return;
-        z = (int)threadIdx.x < d.top ? z * inv_t : kNegInf;
-        const float m = wave_max(z);  // passes over a NaN, which then stays in the sum
-        const float s = wave_sum(z == kNegInf ? 0.f : expf(z - m));
-        if (lane_id() == 0) te.part[wave_id()] = Stat<float>{m, s};
-        if (z == kNegInf) id = -1;
-    }
-    // x: the bits of the student's logit at id, v the row's statistics.
-    __device__ __forceinline__ void close(const mc_distill_desc& d, bool has_lse, float lse, float x, RowStat v,
-                                          LpScale k, Teacher& te) {
-        if (wave_id() * kWave >= d.top) return;
-        float m = lse, ls = 0.f;
-        if (!has_lse) {
-            m = kNegInf;
-            for (int w = 0; w * kWave < d.top; ++w) m = fmaxf(m, te.part[w].m);
-            float s = 0.f;
-            for (int w = 0; w * kWave < d.top; ++w) {
-                const Stat<float> t = te.part[w];
-                s += t.m == m ? t.s : t.s * expf(t.m - m);
-            }
-            ls = logf(s);
-        }
-        const float lp = (z - m) - ls, p = z == kNegInf ? 0.f : expf(lp);
-        const bool bad = p != 0.f && (id < 0 || id >= (int)d.vocab);
-        te.id[threadIdx.x] = id;
-        te.p[threadIdx.x] = p;
-        te.x[threadIdx.x] = x;
-        const float P = wave_sum(p);
-        const float kl = wave_sum(p == 0.f ? 0.f : p * (lp - ((x - v.m) * k.inv_t - logf(v.s))));
-        const int any = __any(bad);
-        if (lane_id() == 0) {
-            te.sum[wave_id()][0] = P;
-            te.sum[wave_id()][1] = kl;
-            te.bad[wave_id()] = any;
-        }
-    }
-    static __device__ __forceinline__ TeacherSums sums(const mc_distill_desc& d, const Teacher& te) {
-        TeacherSums s{0.f, 0.f, false};
-        for (int w = 0; w * kWave < d.top; ++w) {
-            s.P += te.sum[w][0];
-            s.kl += te.sum[w][1];
-            s.bad |= te.bad[w] != 0;
-        }
-        if (s.bad) s.kl = __builtin_nanf("");
-        return s;
+    __device__ __forceinline__ void open() {
+        if (t == kNegInf) id = -1;
     }
     // The bits of the student's logit at the entry.
     template <typename T> __device__ __forceinline__ uint32_t logit(const T* __restrict__ xr, int vocab) const {
         return raw_load(xr, (unsigned)id < (unsigned)vocab ? id : 0);
     }
+    template <typename Te> __device__ __forceinline__ void put(const mc_distill_desc& d, float x, Te& te) const {
+        if ((int)threadIdx.x >= d.top) return;
+        te.id[threadIdx.x] = id;
+        te.x[threadIdx.x] = x;
+    }
 };
+// The entries lane, lane + 64, .. for the first wave; the others have none.
+template <int NT> struct Top {
+    typedef Teacher<NT> Te;
+    static constexpr int C = Te::N / kWave;
+    float t[C];
+    int id[C];
+    // All past 64 or none of them: without a branch between them they overlap.
+    static __device__ __forceinline__ bool here(const mc_distill_desc& d, int c) {
+        return c != 1 || (wave_id() == 0 && d.top > kWave);
+    }
+    // Before the row's loads; the first 64 are the wave's own.
+    __device__ __forceinline__ void load(const mc_distill_desc& d, int64_t row, const int32_t* __restrict__ ids,
+                                         const float* __restrict__ tl, const TopEntry& own) {
+        t[0] = own.t;
+        id[0] = own.id;
+#pragma unroll
+        for (int c = 1; c < C; ++c) {
+            if (!here(d, c)) break;
+            const int i = c * kWave + lane_id();
+            const int64_t at = row * d.top + (i < d.top ? i : 0);
+            t[c] = tl[at];
+            id[c] = ids[at];
+        }
+    }
+    // lse: the teacher's log-sum-exp, or NULL: over these entries.
+    __device__ __forceinline__ void form(const mc_distill_desc& d, const float* lse, int64_t row, LpScale k, Te& te) {
+        if (wave_id() != 0) return;
+        const double log2e = 1.4426950408889634074, c64 = k.inv_t64 * log2e;
+        float m = kNegInf, P = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (!here(d, c)) break;
+            if (c * kWave + lane_id() >= d.top) t[c] = kNegInf;
+            m = fmaxf(m, t[c]);  // passes over a NaN, which then stays in the sum
+        }
+        m = lse ? 0.f : wave_max(m);
+        const float l = lse ? lse[row] : 0.f;
+        double s = 0.0;
+        float e[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (!here(d, c)) break;
+            e[c] = exp2_of(fma((double)t[c] - (double)m, c64, -(double)l * log2e));
+            if (t[c] == kNegInf) e[c] = 0.f;
+            s += (double)e[c];
+        }
+        s = lse ? 1.0 : wave_sum(s);
+        const float r = 1.f / (float)s;  // its rounding scales every p alike
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            if (!here(d, c)) break;
+            const int i = c * kWave + lane_id();
+            const float p = t[c] == kNegInf ? 0.f : e[c] * r;  // without an entry r is infinite
+            te.t[i] = t[c];
+            te.p[i] = p;
+            P += p;
+            bad |= p != 0.f && (id[c] < 0 || id[c] >= (int)d.vocab);
+        }
+        P = wave_sum(P);
+        const int any = __any(bad);
+        if (lane_id() == 0) {
+            te.s = s;
+            te.m = m;
+            te.lse = l;
+            te.P = P;
+            te.bad = any;
+        }
+    }
+};
+// By one wave; both differences to a maximum come first, as in the rows' own sums.
+template <typename Te>
+__device__ __forceinline__ double teacher_value(const mc_distill_desc& d, const Te& te, Stat<double> st, LpScale k) {
+    const double rest = log_ratio(te.s, st.s) + (double)te.lse;
+    double v = 0.0;
+#pragma unroll
+    for (int c = 0; c < Te::N / kWave; ++c) {
+        const int i = c * kWave + lane_id();
+        if (c * kWave >= d.top) break;
+        const double p = te.p[i];  // 0 past the last
+        const double dt = (double)te.t[i] - (double)te.m, dx = (double)te.x[i] - (double)st.m;
+        v += p == 0.0 ? 0.0 : p * fma(dt - dx, k.inv_t64, -rest);
+    }
+    v = wave_sum(v);
+    return te.bad ? __builtin_nan("") : v;
+}
 
+// At most 64 registers: a CU then holds two rows of 1024 threads.
 template <typename T, int NT, bool SPLIT>
-__global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T* __restrict__ logits,
-                                                     const int32_t* __restrict__ ids, const float* __restrict__ tl,
-                                                     const float* __restrict__ tlse, const uint8_t* __restrict__ mask,
-                                                     LpScale k, const Stat<double>* __restrict__ part, int parts,
-                                                     float* __restrict__ kl, RowStat* __restrict__ stats) {
-    __shared__ Stat<float> red[NT / 64];
-    __shared__ Teacher te;
+__global__ __launch_bounds__(NT, 8) void distill_rows_k(mc_distill_desc d, const T* __restrict__ logits,
+                                                        const int32_t* __restrict__ ids, const float* __restrict__ tl,
+                                                        const float* __restrict__ tlse,
+                                                        const uint8_t* __restrict__ mask, LpScale k,
+                                                        const Stat<double>* __restrict__ part, int parts,
+                                                        double* __restrict__ kl, RowStat* __restrict__ stats) {
+    typedef typename std::conditional<SPLIT, double, float>::type Sum;
+    __shared__ Stat<Sum> red[NT / 64];
+    __shared__ Teacher<NT> te;
     const int64_t row = blockIdx.x;
     const int vocab = (int)d.vocab;
     if (mask && mask[row] == 0) {
         if (threadIdx.x == 0) {
-            kl[row] = 0.f;
+            kl[row] = 0.0;
             if (stats) stats[row] = RowStat{0.f, 1.f};
         }
         return;
@@ -665,18 +725,22 @@ __global__ __launch_bounds__(NT) void distill_rows_k(mc_distill_desc d, const T*
     const T* xr = logits + row * vocab;
     TopEntry entry;
     entry.load(d, row, ids, tl);
-    entry.open(d, k.inv_t, te);
+    Top<NT> top;
+    top.load(d, row, ids, tl, entry);
+    Stat<Sum> own;
+    if constexpr (SPLIT) own = own_part(part, row, parts);
+    else own = row_stat<T, NT, float, float>(xr, vocab, k);
+    entry.open();
     const uint32_t x = entry.logit(xr, vocab);
-    Stat<float> st;
-    if constexpr (SPLIT) st = float_stat(own_part(part, row, parts));
-    else st = row_stat<T, NT, float, float>(xr, vocab, k);
-    st = wg_stat<NT, float>(st, k, red);
-    const RowStat v{st.m, st.s};
-    entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
-    __syncthreads();
+    top.form(d, tlse, row, k, te);
+    entry.put(d, from_raw<T>(x), te);
+    Stat<double> st = wg_stat<NT, double>(own, k, red);  // its barrier is the teacher's, too
+    if (wave_id() != 0) return;
+    asm volatile("" : "+v"(st.s), "+v"(st.m) : : "memory");  // or the next reads are made among wg_stat's
+    const double v = teacher_value(d, te, st, k);
     if (threadIdx.x == 0) {
-        kl[row] = entry.sums(d, te).kl;
-        if (stats) stats[row] = v;
+        kl[row] = v;
+        if (stats) stats[row] = RowStat{st.m, (float)st.s};
     }
 }
 
@@ -689,7 +753,7 @@ __device__ __forceinline__ void distill_finish(double T, const double (&v)[2], f
 }
 template <int NT>
 __global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chunk, float temperature,
-                                                      const uint8_t* __restrict__ mask, const float* __restrict__ kl,
+                                                      const uint8_t* __restrict__ mask, const double* __restrict__ kl,
                                                       double (*part)[2], float* __restrict__ loss,
                                                       float* __restrict__ scale) {
     __shared__ double red[NT / 64][2];
@@ -698,7 +762,7 @@ __global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chun
     double v[2] = {0.0, 0.0};
     constexpr int U = 4;
     for (int64_t row0 = r0 + threadIdx.x; row0 < r1; row0 += U * NT) {
-        float x[U];
+        double x[U];
         bool on[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -708,7 +772,7 @@ __global__ __launch_bounds__(NT) void distill_final_k(int64_t rows, int64_t chun
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            v[0] += on[u] ? (double)x[u] : 0.0;
+            v[0] += on[u] ? x[u] : 0.0;
             v[1] += on[u] ? 1.0 : 0.0;
         }
     }
@@ -816,7 +880,9 @@ __device__ __forceinline__ void zero_row(T* __restrict__ dr, int vocab, Store ho
 // Which of a teacher's entries each thread stores: a bit for entry k in word
 // k / 32 of its owner.
 template <int NT> struct TopOwners {
-    uint32_t bits[kDistillMaxTop / 32 * NT];
+    typedef Teacher<NT> Te;
+    static constexpr int W = Te::N / 32;
+    uint32_t bits[W * NT];
 
     // Before the entries are there, with a barrier behind it.
     __device__ __forceinline__ void clear(int top) {
@@ -836,8 +902,8 @@ template <int NT> struct TopOwners {
     // 2000 rows of 50257 bf16 logits and 256 entries, 63 in place of 43 for 4000 of
     // 8000.
     template <typename T>
-    __device__ __forceinline__ void patch(const Teacher& te, int top, T* __restrict__ dr, RowGrad grad, float w) const {
-        constexpr int W = kDistillMaxTop / 32, kKept = 3;
+    __device__ __forceinline__ void patch(const Te& te, int top, T* __restrict__ dr, RowGrad grad, float w) const {
+        constexpr int kKept = 3;
         uint32_t own[W];
         int count = 0;
 #pragma unroll
@@ -915,7 +981,7 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, Store how
                                                     const RowStat* __restrict__ stats, const float* __restrict__ scale,
                                                     const float* __restrict__ dloss, T* __restrict__ dlogits) {
     constexpr int N = Vec16<T>::N;
-    __shared__ Teacher te;
+    __shared__ Teacher<NT> te;
     __shared__ TopOwners<NT> owners;
     const RowThreads th = row_threads<NT>();
     const int64_t row = d.rows - 1 - (int64_t)blockIdx.x;
@@ -931,21 +997,23 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, Store how
     const RowStat v = stats[row];
     TopEntry entry;
     entry.load(d, row, ids, tl);
-    entry.open(d, k.inv_t, te);
+    Top<NT> top;
+    top.load(d, row, ids, tl, entry);
+    entry.open();
     const uint32_t x = entry.logit(xr, vocab);
     __syncthreads();
     if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab)
         owners.insert(owner_of<N>(entry.id, (int)span.head, (int)span.nvec, th.count), (int)(blockIdx.y * NT));
-    entry.close(d, tlse != nullptr, tlse ? tlse[row] : 0.f, from_raw<T>(x), v, k, te);
+    top.form(d, tlse, row, k, te);
+    entry.put(d, from_raw<T>(x), te);
     __syncthreads();
-    const TeacherSums ts = entry.sums(d, te);
     float w = scale[0] * (dloss ? dloss[0] : 1.f);
-    if (ts.bad) w = __builtin_nanf("");
-    if (ts.P == 0.f || w == 0.f) {
+    if (te.bad) w = __builtin_nanf("");
+    if (te.P == 0.f || w == 0.f) {
         zero_row(dr, vocab, how, th);
         return;
     }
-    const RowGrad grad = row_grad(w * ts.P, v, k.c);
+    const RowGrad grad = row_grad(w * te.P, v, k.c);
     write_row(xr, dr, vocab, how, th, grad);
     owners.patch(te, d.top, dr, grad, w);
 }
@@ -1206,11 +1274,11 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store
                                                         const Stat<double>* __restrict__ parts,
                                                         const uint32_t* __restrict__ given, int n_given, int len,
                                                         LpScale k, const float* __restrict__ dloss,
-                                                        float* __restrict__ kl,
+                                                        double* __restrict__ kl,
                                                         T* __restrict__ dlogits) {
     __shared__ Stat<float> red[NT / 64];
     __shared__ uint32_t redc[NT / 64];
-    __shared__ Teacher te;
+    __shared__ Teacher<NT> te;
     __shared__ TopOwners<NT> owners;
     const RowThreads th = row_threads<NT>();
     const int64_t row = blockIdx.x;
@@ -1218,17 +1286,18 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store
     const bool writer = th.self == 0;
     T* dr = dlogits + row * vocab;
     if (mask && mask[row] == 0) {
-        if (writer) kl[row] = 0.f;
+        if (writer) kl[row] = 0.0;
         zero_row(dr, vocab, how, th);
         return;
     }
     const T* xr = logits + row * vocab;
     TopEntry entry;
     entry.load(d, row, ids, tl);
+    Top<NT> top;
+    top.load(d, row, ids, tl, entry);
     owners.clear(d.top);
     __syncthreads();
     const float up = dloss ? dloss[0] : 1.f;
-    const float lse = tlse ? tlse[row] : 0.f;
     RowCount<NT> count;
     const uint8_t* cw = mask ? mask : reinterpret_cast<const uint8_t*>(xr);
     count.load(len, [&](int i) { return (uint32_t)cw[i]; },
@@ -1236,23 +1305,27 @@ __global__ __launch_bounds__(NT, 4) void distill_both_k(mc_distill_desc d, Store
     Row held;
     held.load(xr, vocab, parts, row, th);
     count.put(len, n_given, redc, [](uint32_t w) { return w != 0; });
-    entry.open(d, k.inv_t, te);
+    entry.open();
     if ((int)threadIdx.x < d.top && (unsigned)entry.id < (unsigned)vocab)
         owners.insert(held.owner(entry.id), (int)(blockIdx.y * NT));
     const uint32_t x = entry.logit(xr, vocab);
-    const Stat<float> st = wg_stat<NT, float>(held.stat(k), k, red);
-    const RowStat v{st.m, st.s};
-    entry.close(d, tlse != nullptr, lse, from_raw<T>(x), v, k, te);
+    top.form(d, tlse, row, k, te);
+    const Stat<float> own = held.stat(k);
+    entry.put(d, from_raw<T>(x), te);
+    Stat<double> st = wg_stat<NT, double>(own, k, red);  // its barrier is the teacher's, too
+    // or the next reads are made among wg_stat's, for which there are no registers
+    asm volatile("" : "+v"(st.s), "+v"(st.m) : : "memory");
     float w = d.temperature / (mask ? (float)count.total(redc) : (float)d.rows) * up;
-    __syncthreads();
-    const TeacherSums ts = entry.sums(d, te);
-    if (writer) kl[row] = ts.kl;
-    if (ts.bad) w = __builtin_nanf("");
-    if (ts.P == 0.f || w == 0.f) {
+    if (blockIdx.y == 0 && wave_id() == 0) {  // while the others store
+        const double value = teacher_value(d, te, st, k);
+        if (writer) kl[row] = value;
+    }
+    if (te.bad) w = __builtin_nanf("");
+    if (te.P == 0.f || w == 0.f) {
         zero_row(dr, vocab, how, th);
         return;
     }
-    const RowGrad grad = row_grad(w * ts.P, v, k.c);
+    const RowGrad grad = row_grad(w * te.P, RowStat{st.m, (float)st.s}, k.c);
     held.store(dr, how, grad);
     owners.patch(te, d.top, dr, grad, w);
 }
@@ -1549,14 +1622,14 @@ DistillWs distill_ws(const mc_distill_desc& d) {
     w.part = at;
     at += kSumGroups * 2 * sizeof(double);
     w.kl = at;
-    at += align256((size_t)d.rows * sizeof(float));
+    at += align256((size_t)d.rows * sizeof(double));
     w.split = at;
     w.total = at + loss_parts_ws(d.rows, d.vocab, d.dtype, false);
     return w;
 }
 
 namespace {
-hipError_t launch_distill_sums(const mc_distill_desc& d, const uint8_t* mask, const float* kl, char* ws, float* loss,
+hipError_t launch_distill_sums(const mc_distill_desc& d, const uint8_t* mask, const double* kl, char* ws, float* loss,
                                float* scale, hipStream_t stream) {
     auto* part = reinterpret_cast<double(*)[2]>(ws + distill_ws(d).part);
     by_sum_kernel(d.rows, [&](auto threads, int groups, int64_t chunk) {
@@ -1575,7 +1648,7 @@ hipError_t launch_distill_fwd(const mc_distill_desc& d, const void* logits, cons
                               hipStream_t stream) {
     const DistillWs w = distill_ws(d);
     const LpScale k = row_scale(d.temperature);
-    float* kl = reinterpret_cast<float*>(ws + w.kl);
+    double* kl = reinterpret_cast<double*>(ws + w.kl);
     const int parts =
         launch_parts(false, d.rows, d.vocab, d.dtype, logits, nullptr, -1, mask, k, ws + w.split, stream);
     int threads = parts > 1 ? kDistillMaxTop : loss_row_threads(d.rows, row_bytes(d.vocab, d.dtype));
@@ -1694,7 +1767,7 @@ hipError_t launch_distill_fwd_bwd(const mc_distill_desc& d, const void* logits, 
     const Store how = store_of(logits, dlogits, d.rows, d.vocab, d.dtype);
     hipError_t e;
     if (how != Store::kAny && loss_threads_fit(d.rows, 1024)) {
-        float* kl = reinterpret_cast<float*>(ws + w.kl);
+        double* kl = reinterpret_cast<double*>(ws + w.kl);
         uint32_t* part = reinterpret_cast<uint32_t*>(stats);
         void* parts_ws = ws + w.total + loss_stats_ws(2 * d.rows);
         const int parts =

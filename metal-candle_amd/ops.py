@@ -726,8 +726,8 @@ def distillation_loss_forward(logits, teacher_ids, teacher_logits, temperature=1
     256, in any order (an entry of -inf is left out, whatever its id); mask
     uint8 [...], rows of 0 are not counted. p = softmax(teacher_logits / T), or
     exp(teacher_logits / T - teacher_lse) where teacher_lse [...] holds the
-    log-sum-exp of all the teacher's logits / T; the loss is T^2 times the
-    counted rows' mean of sum_k p_k (log p_k - log softmax(logits / T)[id_k])."""
+    log-sum-exp of all the teacher's logits / T (T as a float32); the loss is T^2
+    times the counted rows' mean of sum_k p_k (log p_k - log softmax(logits / T)[id_k])."""
     d, ids, lse, m = _distill_call(logits, teacher_ids, teacher_logits, temperature, teacher_lse, mask)
     dev = logits.device
     loss = torch.empty(1, dtype=torch.float32, device=dev)

@@ -934,3 +934,39 @@ def test_calls_at_once_on_two_streams(mc, dev):
     for n, got in enumerate(outs):
         for i, (a, e) in enumerate(zip(got, eager)):
             assert torch.equal(a, e), f"call {n}: output {i}"
+            assert torch.equal(a, e), f"call {n}: output {i}"
+
+
+# ------------------------------------------------------- small differences
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_lse", [False, True])
+@pytest.mark.parametrize("T,shift", [(0.7, 0.0), (0.7, 100.0), (1.5, 100.0), (3.0, 0.0), (1.0, 100.0)])
+def test_distillation_near_its_teacher(mc, dev, nan_outputs, dtype, with_lse, T, shift):
+    """A student within 5e-3 of its teacher's logits, whose own lie anywhere: the KL is about 1e-5 of a log-probability,
+    and the loss is held to that.
+
+    The value has two roundings: the float sums of a row's exponentials, at most 32 in a chain, each of at most 2^-24
+    of the sum and of either sign, so 2^-24 sqrt(32 / 3) < 2^-22 (rms) for a row and 6 times that over sqrt(rows) for
+    their mean; and the mean error of the hardware exponential, below 2^-28. An element of the gradient is
+    w (P q - p), in units of 2^-24: q = exp2((x - m) c) / s has three roundings of its argument, 3 |z|, 2 of the
+    exponential, 32 of s and at most 6 of the factors; p and w p have 6."""
+    rows, V, K = 2000, 4096, 64
+    T = float(torch.tensor(T))  # as the call takes it
+    g = gen(dev, 21)
+    x = torch.randn(rows, V, generator=g, device=dev).mul_(2.0).add_(8.0 - 30.0 * T)
+    ids = (torch.randint(0, V, (rows, 1), generator=g, device=dev) + V // K * torch.arange(K, device=dev)) % V
+    best = 8.0 - 1.5 * torch.arange(1, K + 1, device=dev).log() + 0.5 * torch.randn(rows, K, generator=g, device=dev)
+    x = x.scatter_(1, ids, best).to(dtype)
+    t = x.float().gather(1, ids) + shift + 5e-3 * torch.randn(rows, K, generator=g, device=dev)
+    lse = torch.logsumexp(t.double() / T, 1).float() if with_lse else None
+    want, _, grad, terms = plain_distill(x, ids, t, T, lse, None)
+    z = plain_rows(x, T)[0].abs()
+    dense, taken = (terms + grad) / 2, (terms - grad) / 2
+    gtol = 2.0 ** -24 * ((3 * z + 40) * dense + 6 * taken) + torch.finfo(dtype).eps / 2 * grad.abs() + 1e-37
+    ids = ids.to(torch.int32)
+    loss, stats = mc.distillation_loss_forward(x, ids, t, T, lse)
+    d = mc.distillation_loss_backward(x, ids, t, stats, None, T, lse)
+    for name, v, dv in (("two calls", loss, d), ("one call", *mc.distillation_loss_forward_backward(x, ids, t, T, lse))):
+        assert abs(float(v) - float(want)) <= T * T * (6 * 2.0 ** -22 / rows ** 0.5 + 2.0 ** -28) + \
+            2.0 ** -24 * abs(float(want)), (name, float(v), float(want))
+        close(dv, grad, gtol, name)

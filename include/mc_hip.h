@@ -445,7 +445,10 @@ mc_status mc_preference_loss_bwd(const mc_preference_desc* d, const void* logits
  * sequence without counted tokens. MC_MEAN_TOKENS without a counted token gives
  * NaN, as the cross entropy. logps fp32 [batch, seq] receives l; metrics fp32
  * [2] (may be NULL) kl and the clipped share, averaged as the loss is; stats
- * fp32 [rows * 3 + 1] (may be NULL) what the backward needs. */
+ * fp32 [rows * 3 + 1] (may be NULL) what the backward needs. The gradient and the
+ * loss of a call clip by the same l. Other calls sum a row's exponentials in another
+ * order: their l of the same logits may differ by about 1e-7, so r of a policy's own
+ * tokens is that near 1, and which side of a border a token on it takes may differ. */
 typedef enum mc_mean {
     MC_MEAN_TOKENS = 0,
     MC_MEAN_SEQUENCES = 1,

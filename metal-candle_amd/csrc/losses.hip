@@ -466,13 +466,14 @@ __device__ __forceinline__ PolicyInputs policy_inputs(const mc_policy_desc& d, c
     return PolicyInputs{adv[d.per_token_advantages ? row : seq], (old ? old : spare)[row], (ref ? ref : spare)[row],
                         old != nullptr, ref != nullptr};
 }
-// L: float for the gradient. The loss takes l in double: its differences to the other
-// policies' are small against it, and terms of both signs cancel in the sum.
-template <typename L>
-__device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, L l, const PolicyInputs& in) {
+// l in double: its differences to the other policies' are small against it, the KL
+// term's gradient is one of them, and terms of both signs cancel in the loss. The
+// kernels for the loss and for the gradient take the same l, or at a border the one
+// would clip a token and the other not.
+__device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, double l, const PolicyInputs& in) {
     PolicyTerm p;
     const float A = in.A;
-    const float r = in.has_old ? expf((float)(l - (L)in.old)) : l == l ? 1.f : (float)l;
+    const float r = in.has_old ? expf((float)(l - (double)in.old)) : l == l ? 1.f : (float)l;
     const float held = fminf(fmaxf(r, 1.f - d.clip_low), 1.f + d.clip_high);
     const bool clipped = held * A < r * A;
     p.clipped = clipped ? 1.f : 0.f;
@@ -480,7 +481,7 @@ __device__ __forceinline__ PolicyTerm policy_term(const mc_policy_desc& d, L l, 
     p.dl = clipped ? 0.f : -r * A;
     p.kl = 0.f;
     if (in.has_ref) {
-        const float u = (float)((L)in.ref - l), g = expm1f(u);
+        const float u = (float)((double)in.ref - l), g = expm1f(u);
         p.kl = g - u;
         if (d.kl_coef != 0.f) {
             p.term = fmaf(d.kl_coef, p.kl, p.term);
@@ -1246,11 +1247,10 @@ __global__ __launch_bounds__(NT, 4) void policy_both_k(mc_policy_desc d, Store h
     const Stat<double> st = wg_stat<NT, double>(held.stat(k), k, red);
     const RowStat v{st.m, (float)st.s};
     const uint32_t share = count.total(redc);
-    const float l = in ? (from_raw<T>(xt) - v.m) * k.inv_t - logf(v.s) : __builtin_nanf("");
+    const double l = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s) : __builtin_nan("");
     if (writer) {
-        const double l64 = in ? (from_raw<T>(xt) - (double)v.m) * k.inv_t64 - log_of(st.s) : (double)l;
-        logp[row] = l64;
-        logp32[row] = (float)l64;
+        logp[row] = l;
+        logp32[row] = (float)l;
         if (n) n[q] = share;  // the same from every row of the sequence
     }
     float g = policy_term(d, l, pin).dl / (by_seq ? (float)d.batch * (float)share : (float)share) * up;

@@ -970,3 +970,49 @@ def test_distillation_near_its_teacher(mc, dev, nan_outputs, dtype, with_lse, T,
         assert abs(float(v) - float(want)) <= T * T * (6 * 2.0 ** -22 / rows ** 0.5 + 2.0 ** -28) + \
             2.0 ** -24 * abs(float(want)), (name, float(v), float(want))
         close(dv, grad, gtol, name)
+
+
+@pytest.mark.parametrize("B,S,V", [(4, 256, 2000), (2, 16, 60001)])
+def test_policy_near_its_reference(mc, dev, nan_outputs, B, S, V):
+    """A group without advantages, 1e-3 from its reference: the KL term is the whole gradient, -kl_coef expm1(ref - l),
+    and as exact as l is in 64 bits but for the float sums of a row's exponentials, below 2^-22 (rms: 32 roundings of
+    at most 2^-24 of the sum and of either sign)."""
+    g = gen(dev, 22)
+    T, kc = 0.5, 0.1
+    x = logits_at(dev, g, (B, S, V), torch.float32, std=4.0)
+    t = some_targets(dev, g, (B, S), V)
+    l64, _, q = plain_logps(x, t, T)
+    ref = (l64 + 1e-3 * torch.randn(B, S, generator=g, device=dev)).float()
+    A, on = torch.zeros(B, device=dev), t != -1
+    kw = dict(ref_logps=ref, kl_coef=kc, temperature=T, ignore_index=PAD)
+    stats = mc.policy_loss_forward(x, t, A, **kw)[3]
+    at = t.long().clamp(min=0)[..., None]
+    want = torch.expm1(ref.double() - l64) * (1.0 - q.gather(2, at)[..., 0])
+    for name, d in (("two calls", mc.policy_loss_backward(x, t, stats, temperature=T, ignore_index=PAD)),
+                    ("one call", mc.policy_loss_forward_backward(x, t, A, **kw)[3])):
+        got = d.gather(2, at)[..., 0].double() * (-T * float(on.sum()) / kc)
+        rms = float((got - want)[on].square().mean().sqrt())
+        assert rms <= 2.0 ** -22, (name, rms)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,S,V", [(4, 256, 2000), (2, 16, 60001)])
+def test_policy_clips_its_gradient_and_its_value_alike(mc, dev, nan_outputs, dtype, B, S, V):
+    """Ratios within a rounding of the borders: the tokens without a gradient are those that the metric counts."""
+    g = gen(dev, 23)
+    x = logits_at(dev, g, (B, S, V), dtype, std=4.0)
+    t = some_targets(dev, g, (B, S), V)
+    T, on = 0.5, t != -1
+    l64, _, _ = plain_logps(x, t, T)
+    up = torch.rand(B, S, generator=g, device=dev) < 0.5
+    old = (l64 - torch.where(up, math.log1p(0.2), math.log1p(-0.2))).float()
+    A = torch.where(up, 1.0, -1.0)
+    kw = dict(old_logps=old, temperature=T, ignore_index=PAD)
+    _, _, metrics2, stats = mc.policy_loss_forward(x, t, A, **kw)
+    _, _, metrics, d = mc.policy_loss_forward_backward(x, t, A, **kw)
+    n = int(on.sum())
+    for name, dv, m in (("two calls", mc.policy_loss_backward(x, t, stats, temperature=T, ignore_index=PAD), metrics2),
+                        ("one call", d, metrics)):
+        held = int((on & ~(dv != 0).any(-1)).sum())
+        assert held == round(float(m[1]) * n), (name, held, float(m[1]) * n)
+        assert B * S < 64 or 0 < held < n

@@ -525,14 +525,15 @@ def _logprob_desc(logits, ignore, temperature, code):
 
 
 def token_logprobs_forward(logits, targets, ignore_index=None, temperature=1.0, save_stats=True):
-    """Log-probabilities of the given tokens under logits [..., V]: (logps [...] fp32, stats).
+    """Log-probabilities of the given tokens under logits [..., V]: (logps [...] fp32, stats). targets hold one id per
+    row of logits, in any shape.
 
     logps = logits[target] / T - logsumexp(logits / T), 0 where the target is
     ignore_index (such rows are not read); stats [rows, 2] fp32 is what
     token_logprobs_backward needs, or None."""
     targets, ignore, code = _loss_inputs(logits, targets, ignore_index, False)
     d = _logprob_desc(logits, ignore, temperature, code)
-    if targets.dim() == logits.dim() - 1:
+    if targets.shape == logits.shape[:-1]:
         logps = torch.empty_like(targets, dtype=torch.float32)  # half the time of empty with a shape
     else:
         logps = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)

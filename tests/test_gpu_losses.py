@@ -1016,3 +1016,17 @@ def test_policy_clips_its_gradient_and_its_value_alike(mc, dev, nan_outputs, dty
         held = int((on & ~(dv != 0).any(-1)).sum())
         assert held == round(float(m[1]) * n), (name, held, float(m[1]) * n)
         assert B * S < 64 or 0 < held < n
+
+
+def test_token_logprobs_of_targets_in_another_shape(mc, dev):
+    """Targets may come flat or folded in another way: the log-probabilities have the logits' leading dims."""
+    g = gen(dev, 24)
+    x = logits_at(dev, g, (2, 3, 101), torch.float32)
+    t = torch.randint(0, 101, (2, 3), generator=g, device=dev, dtype=torch.int32)
+    want, stats = mc.token_logprobs_forward(x, t)
+    dl = torch.randn(2, 3, generator=g, device=dev)
+    d = mc.token_logprobs_backward(x, t, stats, dl)
+    for shape in ((6,), (3, 2), (1, 6), (6, 1)):
+        got, _ = mc.token_logprobs_forward(x, t.view(shape))
+        assert got.shape == (2, 3) and torch.equal(got, want), shape
+        assert torch.equal(mc.token_logprobs_backward(x, t.view(shape), stats, dl), d), shape

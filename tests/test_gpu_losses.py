@@ -1030,3 +1030,56 @@ def test_token_logprobs_of_targets_in_another_shape(mc, dev):
         got, _ = mc.token_logprobs_forward(x, t.view(shape))
         assert got.shape == (2, 3) and torch.equal(got, want), shape
         assert torch.equal(mc.token_logprobs_backward(x, t.view(shape), stats, dl), d), shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", WAYS)
+@pytest.mark.parametrize("K", [1, 64, 65, 256])
+def test_near_teachers_of_every_size_and_way(mc, dev, nan_outputs, dtype, rows, V, K):
+    """As test_distillation_near_its_teacher, for every way of taking a row, with the teacher's log-sum-exp and
+    without. Without it, and of one entry, p is 1 and the value -log q: held to the chain's worst case, 32 roundings of
+    2^-24."""
+    g = gen(dev, rows + K)
+    T, shift = 0.5, -50.0
+    x = torch.randn(rows, V, generator=g, device=dev).mul_(2.0).add_(-12.0)
+    ids = (torch.randint(0, V, (rows, 1), generator=g, device=dev) + max(1, V // K) * torch.arange(K, device=dev)) % V
+    best = 8.0 - 1.5 * torch.arange(1, K + 1, device=dev).log() + 0.5 * torch.randn(rows, K, generator=g, device=dev)
+    x = x.scatter_(1, ids, best).to(dtype)
+    t = x.float().gather(1, ids) + shift + 5e-3 * torch.randn(rows, K, generator=g, device=dev)
+    t[rows // 2, K // 2:] = -math.inf
+    full = (torch.logsumexp(t.double() / T, 1)).float()
+    full[rows // 2] = 0.0
+    z = plain_rows(x, T)[0].abs()
+    for lse in (None, full):
+        want, _, grad, terms = plain_distill(x, ids, t, T, lse, None)
+        dense, taken = (terms + grad) / 2, (terms - grad) / 2
+        gtol = 2.0 ** -24 * ((3 * z + 40) * dense + 6 * taken) + torch.finfo(dtype).eps / 2 * grad.abs() + 1e-37
+        loss, stats = mc.distillation_loss_forward(x, ids, t, T, lse)
+        d = mc.distillation_loss_backward(x, ids, t, stats, None, T, lse)
+        for name, v, dv in (("two calls", loss, d),
+                            ("one call", *mc.distillation_loss_forward_backward(x, ids, t, T, lse))):
+            assert abs(float(v) - float(want)) <= T * T * (32 * 2.0 ** -24 + 2.0 ** -28) + \
+                2.0 ** -24 * abs(float(want)), (name, float(v), float(want))
+            close(dv, grad, gtol, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_entries_of_no_weight(mc, dev, nan_outputs, dtype):
+    """Teacher entries at the type's lowest value, whose p underflows to 0: as left out, whatever their id. A teacher
+    whose entries are all that low is uniform."""
+    V, K, g = 300, 70, gen(dev, 25)
+    low = torch.finfo(torch.float32).min
+    x = logits_at(dev, g, (5, V), dtype)
+    ids = torch.stack([torch.randperm(V, generator=g, device=dev)[:K] for _ in range(5)]).to(torch.int32)
+    t = torch.randn(5, K, generator=g, device=dev)
+    t[1, 3:], t[2, ::2], t[3] = low, low, low
+    clean = torch.where((t == low) & (t != low).any(1, keepdim=True), -math.inf, t)
+    want, tol, grad, terms = plain_distill(x, ids, torch.where(clean == low, 0.0, clean), 1.0, None, None)
+    bad = ids.clone()
+    bad[1, 3:], bad[2, ::2] = 2**31 - 1, -1
+    for i in (ids, bad):
+        loss, stats = mc.distillation_loss_forward(x, i, t)
+        for v, d in ((loss, mc.distillation_loss_backward(x, i, t, stats)),
+                     mc.distillation_loss_forward_backward(x, i, t)):
+            assert abs(float(v) - float(want)) <= float(tol) + 2.0 ** -23 * abs(float(want))
+            close_grad(d, grad, terms, dtype)

@@ -22,10 +22,13 @@
 // Bound by HBM throughout: 2 or 4 bytes per logit and pass against about ten
 // operations. A copy of 1 GiB runs at 5.0 TB/s here; kernels, three of four rows
 // counted:
-//   lp_rows_k       f32 2036 x 50257 54.0 us, 5.7 TB/s; bf16, for sums of l, 4072 x 151936 179, 5.2
-//   lp_bwd_k        the same 116, 6.2; 380, 5.7
-//   policy_both_k   bf16 4096 x 151936 401, 5.4; f32 2036 x 50257 133, 5.4
-//   distill_both_k  bf16 2036 x 151936, 64 entries, 217, 5.0; f32 1500 x 50257, 8 entries, 108, 5.0
+//   lp_rows_k       f32 2036 x 50257 54.8 us, 5.6 TB/s; bf16, for sums of l, 4072 x 151936 182, 5.1
+//   lp_bwd_k        the same 116, 6.2; 386, 5.6
+//   policy_both_k   bf16 4096 x 151936 410, 5.3; f32 2036 x 50257 143, 5.0
+//   distill_both_k  bf16 2036 x 151936, 64 entries, 219, 5.0; f32 1500 x 50257, 8 entries, 108, 4.9
+//   distill_rows_k, distill_bwd_k, nearly all rows counted: bf16 2036 x 151936, 64 entries, 104, 5.6
+//                   and 234, 5.1 (gradients elsewhere in a vector 252, 4.7); f32 1500 x 50257, 8
+//                   entries, 44.9, 5.6 and 113, 4.9 (112, 4.9)
 #include <type_traits>
 
 #include "common.hpp"
@@ -129,8 +132,9 @@ __device__ __forceinline__ float term_of(float x, float base, LpScale k) { retur
 // term, 1, rounds at 2^-24 of it for each term it adds there, and l is off by 4e-8
 // (rms) where that term is most of the row; a score of 110 tokens by 5e-7. Doubles
 // cost 2.7% of a preference step on 4072 bf16 rows of 151936 (555 / 570 us) and 10%
-// of 777 rows alone (51.4 / 56.5), so of bf16 logits they are for l that are summed;
-// of f32 ones, half as many per byte, they cost nothing.
+// of 777 rows alone (51.4 / 56.5), so of bf16 logits they are for l that are summed
+// (preference, policy forward) and for shared rows (parts_k); for l of f32 ones, half
+// as many per byte, they cost nothing. Distillation's rows and the held ones have floats.
 template <typename T, int NT, typename S, int U, typename P = float>
 __device__ __forceinline__ Stat<S> vec_stat(const T* __restrict__ xv, int c, int nvec, LpScale k) {
     constexpr int N = Vec16<T>::N;
@@ -1021,9 +1025,9 @@ __global__ __launch_bounds__(NT) void distill_bwd_k(mc_distill_desc d, Store how
 
 // ------------------------------------------- value and gradient in one read
 // A row held in registers, vector u * NT + t of it in thread t, so that the
-// statistics and the gradient come from one read: 1024 threads hold 320 KB, the
-// smaller shapes several rows per CU. Bound by HBM, with the reads of one row
-// beside the writes of another on each CU: 2036 bf16 rows of 151936 take 246 us, 325
+// statistics and the gradient come from one read: 1024 threads hold up to 304 KiB, a
+// row per CU, the smaller shapes several rows. Bound by HBM, with the reads of some
+// CUs beside the writes of others: 2036 bf16 rows of 151936 take 246 us, 325
 // as lp_rows_k and lp_bwd_k, whose second read the cache meets in part. All the
 // loads are in flight at once, and
 // the statistics take them as they come, so whatever else a kernel loads comes
@@ -1381,7 +1385,8 @@ template <typename T> struct Split {
 //   24 KB rows, 4096   128x16 44.8, 256x8 43.0, 512x4 53.7
 //   32 KB rows, 1000   128x16 25.0, 256x8 21.1, 512x4 22.3
 //   64 KB rows, 1000   512x8 31.1, 512x13 32.5, 1024x4 41.0
-// f32: 64 KB rows, 4000 512x8 113, 512x13 104; 98 KB, 4096 512x13 155, 1024x8 172.
+// f32: 98 KB rows, 4096 512x13 155, 1024x8 172. Not the fastest: 64 KB rows, 4000,
+// which take 512x8 at 113, 512x13 104.
 // The kernel alone, bf16: 201 KB rows, 2036 1024x13 139, 1024x16 140, 1024x19 142.
 // Without the last shape, by a forward and a backward: 600 rows of 256000 bf16
 // 161 / 169, 300 of 256000 f32 156 / 190.

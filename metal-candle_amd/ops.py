@@ -504,7 +504,8 @@ def _launch(t, fn, *args):
 
 def _loss_inputs(logits, targets, ignore_index, seqs):
     """(targets as the kernels read them, ignore_index, dtype code) of logits [..., V] with targets over its leading
-    dims; seqs: the logits must be [sequences, tokens, V]."""
+    dims; seqs: the logits must be [sequences, tokens, V]. Targets are unsigned: an ignore_index below 0 is none, as
+    for the cross entropy, and padding of -100 is 2**32 - 100 there."""
     if not isinstance(logits, torch.Tensor):
         raise McError(_lib.MC_ERR_NULL, "logits must be a tensor")
     if seqs and logits.dim() != 3:
@@ -530,7 +531,9 @@ def token_logprobs_forward(logits, targets, ignore_index=None, temperature=1.0, 
 
     logps = logits[target] / T - logsumexp(logits / T), 0 where the target is
     ignore_index (such rows are not read); stats [rows, 2] fp32 is what
-    token_logprobs_backward needs, or None."""
+    token_logprobs_backward needs, or None. Here and in the other losses
+    targets are read as 32-bit unsigned ids and an ignore_index below 0 is
+    none: padding of -100 takes ignore_index=2**32 - 100, or its rows are NaN."""
     targets, ignore, code = _loss_inputs(logits, targets, ignore_index, False)
     d = _logprob_desc(logits, ignore, temperature, code)
     if targets.shape == logits.shape[:-1]:

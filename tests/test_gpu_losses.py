@@ -1083,3 +1083,19 @@ def test_distillation_entries_of_no_weight(mc, dev, nan_outputs, dtype):
                      mc.distillation_loss_forward_backward(x, i, t)):
             assert abs(float(v) - float(want)) <= float(tol) + 2.0 ** -23 * abs(float(want))
             close_grad(d, grad, terms, dtype)
+
+
+@pytest.mark.parametrize("ids", [torch.int32, torch.int64])
+def test_padding_of_minus_100(mc, dev, ids):
+    """Ids are unsigned: -100 is 2^32 - 100, and an ignore_index below 0 is none. (x_t - m) / T and log s are below 14
+    each: 2^-20 + 2^-22 28 = 2^-17."""
+    g = gen(dev, 26)
+    x = logits_at(dev, g, (2, 5, 33), torch.float32)
+    t = torch.randint(0, 33, (2, 5), generator=g, device=dev)
+    t[0, :2], t[1, 4] = -100, -100
+    l, _ = mc.token_logprobs_forward(x, t.to(ids), ignore_index=2**32 - 100)
+    want = torch.log_softmax(x.double(), -1).gather(-1, t.clamp(min=0)[..., None])[..., 0]
+    on = t != -100
+    assert torch.allclose(l.double()[on], want[on], rtol=0.0, atol=2.0 ** -17) and not l[~on].any()
+    l, _ = mc.token_logprobs_forward(x, t.to(ids), ignore_index=-100)
+    assert torch.isnan(l[~on]).all() and torch.isfinite(l[on]).all()

@@ -1099,3 +1099,20 @@ def test_padding_of_minus_100(mc, dev, ids):
     assert torch.allclose(l.double()[on], want[on], rtol=0.0, atol=2.0 ** -17) and not l[~on].any()
     l, _ = mc.token_logprobs_forward(x, t.to(ids), ignore_index=-100)
     assert torch.isnan(l[~on]).all() and torch.isfinite(l[on]).all()
+
+
+@pytest.mark.parametrize("with_lse", [False, True])
+@pytest.mark.parametrize("K", [5, 130])
+def test_a_teacher_that_is_nan(mc, dev, nan_outputs, K, with_lse):
+    """A NaN among a row's teacher logits, or an infinity without their log-sum-exp: the loss and that row are NaN."""
+    V, g = 700, gen(dev, 27)
+    x = logits_at(dev, g, (4, V), torch.bfloat16)
+    ids = torch.stack([torch.randperm(V, generator=g, device=dev)[:K] for _ in range(4)]).to(torch.int32)
+    t = torch.randn(4, K, generator=g, device=dev)
+    lse = torch.logsumexp(t, 1) + 0.1 if with_lse else None
+    t[1, K - 1] = math.nan if with_lse else math.inf
+    t[2, 0] = math.nan
+    loss, stats = mc.distillation_loss_forward(x, ids, t, teacher_lse=lse)
+    for v, d in ((loss, mc.distillation_loss_backward(x, ids, t, stats, teacher_lse=lse)),
+                 mc.distillation_loss_forward_backward(x, ids, t, teacher_lse=lse)):
+        assert torch.isnan(v).all() and torch.isnan(d[1:3]).all() and torch.isfinite(d[[0, 3]]).all()

@@ -32,6 +32,9 @@
  *                    bias of MetalLayerNorm (src/embeddings/metal_bert.rs).
  *   mc_log_softmax_*, mc_cross_entropy_*  cross_entropy_loss and its label
  *                    smoothing (src/training/loss.rs:58-245).
+ *   mc_gradient_norm, mc_scale_gradients, mc_clip_gradients,
+ *   mc_embedding_*   no counterpart in the reference: clipping by the gradients'
+ *                    global norm; the scaled token embedding and its gradient.
  *   mc_token_logprobs_*, mc_preference_loss_*, mc_policy_loss_*,
  *   mc_distill_loss_*  no counterpart in the reference: losses over the same
  *                    logits for preferences, rewards and teachers.
@@ -298,6 +301,69 @@ typedef struct mc_adamw_tensor {
 mc_status mc_adamw_step(const mc_adamw_config* cfg, const mc_adamw_tensor* tensors, int32_t count,
                         hipStream_t stream);
 
+/* mc_adamw_step on gradients multiplied by *grad_scale (fp32 [1] on the device,
+ * as mc_gradient_norm writes it; 16-byte alignment is not needed; NULL: as
+ * mc_adamw_step). Equal bit for bit to mc_scale_gradients before mc_adamw_step,
+ * without writing the scaled gradients. No counterpart in the reference. */
+mc_status mc_adamw_scaled_step(const mc_adamw_config* cfg, const mc_adamw_tensor* tensors, int32_t count,
+                               const float* grad_scale, hipStream_t stream);
+
+/* Global norm of many gradients and clipping by it. No counterpart in the
+ * reference, whose optimizer takes its gradients as they are.
+ *   norm  = sqrt(sum over all elements of all tensors of grad^2), summed in 64 bits
+ *   scale = 1 where norm <= max_norm, else max_norm / norm   (NaN where norm is NaN)
+ *   out   = scale * grad, rounded once to out_dtype
+ * norm, scale: fp32 [1] on the device. max_norm > 0, infinity for none. A norm past
+ * fp32's range is stored as infinity, its scale is still max_norm / norm. Gradients
+ * and outputs may start at any element; an output is its own gradient (of the same
+ * dtype: in place) or apart from every gradient. The table is read on the host.
+ * Sums run in a fixed order: results are bitwise reproducible. The workspace holds
+ * nothing between calls. */
+typedef struct mc_grad_tensor {
+    const void* grad;   /* [numel] */
+    void* out;          /* [numel]; not read by mc_gradient_norm */
+    int64_t numel;      /* 0 .. 2^40 - 1 */
+    int32_t dtype;      /* mc_dtype of grad */
+    int32_t out_dtype;  /* mc_dtype of out */
+} mc_grad_tensor;
+
+size_t mc_gradient_norm_workspace_size(const mc_grad_tensor* tensors, int32_t count);
+
+/* scale may be NULL; then max_norm is not used. */
+mc_status mc_gradient_norm(const mc_grad_tensor* tensors, int32_t count, float max_norm, float* norm, float* scale,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream);
+mc_status mc_scale_gradients(const mc_grad_tensor* tensors, int32_t count, const float* scale, hipStream_t stream);
+
+/* Both in one call, with one launch less (workspace: mc_gradient_norm_workspace_size). */
+mc_status mc_clip_gradients(const mc_grad_tensor* tensors, int32_t count, float max_norm, float* norm, float* scale,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* Token embedding, with the scaling that some models give it, and its gradient.
+ * No entry point of the reference: its models look tokens up with
+ * candle_nn::Embedding (src/models/qwen.rs). table [vocab, dim], ids int32 [tokens]:
+ *   out[t] = scale * table[ids[t]], rounded once; 0 where ids[t] is padding_id; NaN
+ *            where ids[t] is not in [0, vocab) (the table is not read there)
+ *   dtable[v] = scale * sum over t with ids[t] = v of dout[t], fp32 [vocab, dim], 0
+ *            for ids that do not occur and for padding_id; with accumulate added to
+ *            what dtable holds (a table that is also the output projection's weight).
+ * Tokens without a row of the table are left out of the gradient, whatever dout
+ * holds there. Each row's sum runs in an order that the sizes and ids alone fix:
+ * results are bitwise reproducible. */
+typedef struct mc_embedding_desc {
+    int64_t tokens;      /* 1 .. 2^31 - 65 */
+    int64_t vocab;       /* 1 .. 2^31 - 1 */
+    int64_t dim;         /* >= 1; vocab * dim and tokens * dim < 2^40 */
+    int64_t padding_id;  /* < 0: none */
+    float scale;         /* finite */
+    int32_t dtype;       /* mc_dtype of table, out and dout */
+} mc_embedding_desc;
+
+mc_status mc_embedding_fwd(const mc_embedding_desc* d, const void* table, const int32_t* ids, void* out,
+                           hipStream_t stream);
+size_t mc_embedding_bwd_workspace_size(const mc_embedding_desc* d);
+mc_status mc_embedding_bwd(const mc_embedding_desc* d, const int32_t* ids, const void* dout, float* dtable,
+                           int32_t accumulate, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* LayerNorm over the last dim of x [rows, dim] (LayerNormOp,
  * src/backend/custom_ops.rs:826-1079; its CPU path cpu_fwd and
  * TensorExt::layer_norm, src/backend/tensor.rs:100-109; the weight and bias
@@ -539,8 +605,8 @@ mc_status mc_dropout_mask(uint64_t seed, float p, int64_t rows, int32_t rank, ui
  * returns the totals of one class. Classes: 0 = MFMA GEMM (FLOPs count the
  * base x.W^T / dY.W product only), 1 = rank-r kernels, 2 = RMSNorm,
  * 3 = softmax, 4 = attention (FLOPs of the unmasked score and P.V products),
- * 5 = AdamW (bytes: 28 per element), 6 = LayerNorm / log-softmax /
- * cross-entropy and the other losses.
+ * 5 = AdamW (bytes: 28 per element) and the gradients' norm and clipping,
+ * 6 = LayerNorm / log-softmax / cross-entropy, the other losses and the embedding.
  * Enabling allocates hipEvents (not for allocation-free use). */
 mc_status mc_profile_enable(int32_t on);
 mc_status mc_profile_collect(void);

@@ -12,12 +12,16 @@ from .ops import (  # noqa: F401
     adamw_step,
     attention_backward,
     attention_forward,
+    clip_gradients,
     cross_entropy_backward,
     cross_entropy_forward,
     distillation_loss_backward,
     distillation_loss_forward,
     distillation_loss_forward_backward,
     dropout_mask,
+    embedding_backward,
+    embedding_forward,
+    gradient_norm,
     layer_norm_backward,
     layer_norm_forward,
     log_softmax_backward,
@@ -33,6 +37,7 @@ from .ops import (  # noqa: F401
     preference_loss_forward,
     rms_norm_backward,
     rms_norm_forward,
+    scale_gradients,
     softmax_backward,
     softmax_forward,
     token_logprobs_backward,

@@ -151,6 +151,27 @@ class DistillDesc(ctypes.Structure):
     ]
 
 
+class GradTensor(ctypes.Structure):
+    _fields_ = [
+        ("grad", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("numel", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+    ]
+
+
+class EmbeddingDesc(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("dim", ctypes.c_int64),
+        ("padding_id", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 class AdamWConfig(ctypes.Structure):
     _fields_ = [
         ("learning_rate", ctypes.c_float),
@@ -184,6 +205,7 @@ _lp = ctypes.POINTER(LogprobDesc)
 _rp = ctypes.POINTER(PreferenceDesc)
 _pp = ctypes.POINTER(PolicyDesc)
 _tp = ctypes.POINTER(DistillDesc)
+_ep = ctypes.POINTER(EmbeddingDesc)
 
 _SIGNATURES = {
     "mc_version": (ctypes.c_char_p, []),
@@ -235,6 +257,14 @@ _SIGNATURES = {
     "mc_distill_loss_bwd": (ctypes.c_int, [_tp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mc_distill_loss_fwd_bwd_workspace_size": (_sz, [_tp]),
     "mc_distill_loss_fwd_bwd": (ctypes.c_int, [_tp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_adamw_scaled_step": (ctypes.c_int, [ctypes.POINTER(AdamWConfig), ctypes.POINTER(AdamWTensor), _i32, _vp, _vp]),
+    "mc_gradient_norm_workspace_size": (_sz, [_vp, _i32]),
+    "mc_gradient_norm": (ctypes.c_int, [_vp, _i32, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "mc_scale_gradients": (ctypes.c_int, [_vp, _i32, _vp, _vp]),
+    "mc_clip_gradients": (ctypes.c_int, [_vp, _i32, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "mc_embedding_fwd": (ctypes.c_int, [_ep, _vp, _vp, _vp, _vp]),
+    "mc_embedding_bwd_workspace_size": (_sz, [_ep]),
+    "mc_embedding_bwd": (ctypes.c_int, [_ep, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
     "mc_adamw_step": (ctypes.c_int, [ctypes.POINTER(AdamWConfig), ctypes.POINTER(AdamWTensor), _i32, _vp]),
     "mc_dropout_mask": (ctypes.c_int, [ctypes.c_uint64, _f32, _i64, _i32, _vp]),
     "mc_profile_enable": (ctypes.c_int, [_i32]),

@@ -547,6 +547,11 @@ static float powi_f32(float base, int32_t t) {
 
 mc_status mc_adamw_step(const mc_adamw_config* cfg, const mc_adamw_tensor* tensors, int32_t count,
                         hipStream_t stream) {
+    return mc_adamw_scaled_step(cfg, tensors, count, nullptr, stream);
+}
+
+mc_status mc_adamw_scaled_step(const mc_adamw_config* cfg, const mc_adamw_tensor* tensors, int32_t count,
+                               const float* grad_scale, hipStream_t stream) {
     MC_CHECK(cfg != nullptr, MC_ERR_NULL, "AdamW: config is NULL");
     // AdamWConfig::validate (optimizer.rs:67-103), with its comparisons
     MC_CHECK(!(cfg->learning_rate <= 0.0f), MC_ERR_VALUE, "learning rate must be positive");
@@ -598,17 +603,171 @@ mc_status mc_adamw_step(const mc_adamw_config* cfg, const mc_adamw_tensor* tenso
         sl.blk0 = blocks;
         blocks += mc::adamw_blocks(t.numel);
         if (b.count == mc::kAdamWSlots || i == count - 1) {
-            hipError_t e = mc::launch_adamw(b, blocks, stream);
+            hipError_t e = mc::launch_adamw(b, blocks, grad_scale, stream);
             if (e != hipSuccess) return hip_status(e, "AdamW");
             b.count = 0;
             blocks = 0;
         }
     }
     if (b.count > 0) {
-        hipError_t e = mc::launch_adamw(b, blocks, stream);
+        hipError_t e = mc::launch_adamw(b, blocks, grad_scale, stream);
         if (e != hipSuccess) return hip_status(e, "AdamW");
     }
     return ok();
+}
+
+static mc_status check_grads(const char* op, const mc_grad_tensor* tensors, int32_t count, bool outs, double* elems) {
+    MC_CHECK(count >= 0, MC_ERR_SHAPE, "%s: tensor count must be >= 0, got %d", op, (int)count);
+    MC_CHECK(count == 0 || tensors, MC_ERR_NULL, "%s: tensor table is NULL", op);
+    double total = 0.0;
+    for (int32_t i = 0; i < count; ++i) {
+        const mc_grad_tensor& t = tensors[i];
+        MC_CHECK(t.numel >= 0 && t.numel < ((int64_t)1 << 40), MC_ERR_SHAPE, "%s: tensor %d: numel %lld out of range",
+                 op, (int)i, (long long)t.numel);
+        if (t.numel == 0) continue;
+        MC_CHECK(t.dtype == MC_F32 || t.dtype == MC_BF16, MC_ERR_DTYPE,
+                 "%s: tensor %d: unsupported dtype code %d (supported: 0 = f32, 1 = bf16)", op, (int)i, (int)t.dtype);
+        MC_CHECK(t.grad, MC_ERR_NULL, "%s: tensor %d: grad must not be NULL", op, (int)i);
+        const uintptr_t g = reinterpret_cast<uintptr_t>(t.grad), o = reinterpret_cast<uintptr_t>(t.out);
+        const size_t gs = t.dtype == MC_F32 ? 4 : 2, os = t.out_dtype == MC_F32 ? 4 : 2;
+        MC_CHECK(g % gs == 0, MC_ERR_LAYOUT, "%s: tensor %d: grad must be aligned to its elements", op, (int)i);
+        if (outs) {
+            MC_CHECK(t.out_dtype == MC_F32 || t.out_dtype == MC_BF16, MC_ERR_DTYPE,
+                     "%s: tensor %d: unsupported out_dtype code %d (supported: 0 = f32, 1 = bf16)", op, (int)i,
+                     (int)t.out_dtype);
+            MC_CHECK(t.out, MC_ERR_NULL, "%s: tensor %d: out must not be NULL", op, (int)i);
+            MC_CHECK(o % os == 0, MC_ERR_LAYOUT, "%s: tensor %d: out must be aligned to its elements", op, (int)i);
+            const size_t n = (size_t)t.numel;
+            MC_CHECK((g == o && t.dtype == t.out_dtype) || o + n * os <= g || g + n * gs <= o, MC_ERR_LAYOUT,
+                     "%s: tensor %d: out must be grad itself or must not overlap it", op, (int)i);
+        }
+        total += (double)t.numel;
+    }
+    MC_CHECK(total < 1.0e15, MC_ERR_SHAPE, "%s: %g elements are too many", op, total);
+    *elems = total;
+    return MC_OK;
+}
+
+static mc_status check_max_norm(const char* op, float max_norm) {
+    MC_CHECK(max_norm > 0.0f, MC_ERR_VALUE, "%s: max_norm must be positive, got %g", op, (double)max_norm);
+    return MC_OK;
+}
+
+static mc_status check_workspace(const char* op, const void* workspace, size_t have, size_t need);
+
+static double grad_bytes(const mc_grad_tensor* t, int32_t count, bool read, bool outs) {
+    double b = 0.0;
+    for (int32_t i = 0; i < count; ++i)
+        b += (double)t[i].numel * ((read ? (t[i].dtype == MC_F32 ? 4.0 : 2.0) : 0.0) +
+                                   (outs ? (t[i].out_dtype == MC_F32 ? 4.0 : 2.0) : 0.0));
+    return b;
+}
+
+size_t mc_gradient_norm_workspace_size(const mc_grad_tensor* tensors, int32_t count) {
+    double n = 0.0;
+    if (check_grads("gradient_norm", tensors, count, false, &n) != MC_OK || n == 0.0) return 0;
+    return (size_t)mc::gradient_parts(tensors, count) * sizeof(double);
+}
+
+mc_status mc_gradient_norm(const mc_grad_tensor* tensors, int32_t count, float max_norm, float* norm, float* scale,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    double n = 0.0;
+    mc_status s = check_grads("gradient_norm", tensors, count, false, &n);
+    if (s != MC_OK) return s;
+    MC_CHECK(norm, MC_ERR_NULL, "gradient_norm: norm must not be NULL");
+    if (scale && (s = check_max_norm("gradient_norm", max_norm)) != MC_OK) return s;
+    const size_t need = n == 0.0 ? 0 : (size_t)mc::gradient_parts(tensors, count) * sizeof(double);
+    if (need && (s = check_workspace("gradient_norm", workspace, workspace_bytes, need)) != MC_OK) return s;
+    mc::prof::Scope sc(mc::prof::kAdamW, stream, 0.0, grad_bytes(tensors, count, true, false));
+    return hip_status(mc::launch_gradient_norm(tensors, count, max_norm, norm, scale, static_cast<double*>(workspace),
+                                               stream),
+                      "gradient_norm");
+}
+
+mc_status mc_scale_gradients(const mc_grad_tensor* tensors, int32_t count, const float* scale, hipStream_t stream) {
+    double n = 0.0;
+    mc_status s = check_grads("scale_gradients", tensors, count, true, &n);
+    if (s != MC_OK) return s;
+    MC_CHECK(scale, MC_ERR_NULL, "scale_gradients: scale must not be NULL");
+    if (n == 0.0) return ok();
+    mc::prof::Scope sc(mc::prof::kAdamW, stream, 0.0, grad_bytes(tensors, count, true, true));
+    return hip_status(mc::launch_scale_gradients(tensors, count, scale, stream), "scale_gradients");
+}
+
+mc_status mc_clip_gradients(const mc_grad_tensor* tensors, int32_t count, float max_norm, float* norm, float* scale,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    double n = 0.0;
+    mc_status s = check_grads("clip_gradients", tensors, count, true, &n);
+    if (s != MC_OK) return s;
+    MC_CHECK(norm && scale, MC_ERR_NULL, "clip_gradients: norm and scale must not be NULL");
+    if ((s = check_max_norm("clip_gradients", max_norm)) != MC_OK) return s;
+    const size_t need = n == 0.0 ? 0 : (size_t)mc::gradient_parts(tensors, count) * sizeof(double);
+    if (need && (s = check_workspace("clip_gradients", workspace, workspace_bytes, need)) != MC_OK) return s;
+    mc::prof::Scope sc(mc::prof::kAdamW, stream, 0.0, 2.0 * grad_bytes(tensors, count, true, false) +
+                                                          grad_bytes(tensors, count, false, true));
+    if (n == 0.0) return hip_status(mc::launch_gradient_norm(tensors, count, max_norm, norm, scale, nullptr, stream),
+                                    "clip_gradients");
+    return hip_status(mc::launch_clip_gradients(tensors, count, max_norm, norm, scale,
+                                                static_cast<double*>(workspace), stream),
+                      "clip_gradients");
+}
+
+static mc_status check_embedding(const char* op, const mc_embedding_desc* d) {
+    MC_CHECK(d != nullptr, MC_ERR_NULL, "%s: descriptor is NULL", op);
+    mc_status s = check_dtype(d->dtype, op);
+    if (s != MC_OK) return s;
+    MC_CHECK(d->tokens >= 1 && d->vocab >= 1 && d->dim >= 1, MC_ERR_SHAPE,
+             "%s: tokens, vocab and dim must be >= 1, got %lld, %lld, %lld", op, (long long)d->tokens,
+             (long long)d->vocab, (long long)d->dim);
+    MC_CHECK(d->tokens <= 2147483647 - 64 && d->vocab <= 2147483647, MC_ERR_SHAPE,
+             "%s: tokens must stay below 2^31 - 64 and vocab below 2^31, got %lld, %lld", op, (long long)d->tokens,
+             (long long)d->vocab);
+    MC_CHECK((double)d->vocab * (double)d->dim < 1099511627776.0 && (double)d->tokens * (double)d->dim < 1099511627776.0,
+             MC_ERR_SHAPE, "%s: vocab * dim and tokens * dim must stay below 2^40", op);
+    MC_CHECK(std::isfinite(d->scale), MC_ERR_VALUE, "%s: scale must be finite", op);
+    return MC_OK;
+}
+
+mc_status mc_embedding_fwd(const mc_embedding_desc* d, const void* table, const int32_t* ids, void* out,
+                           hipStream_t stream) {
+    mc_status s = check_embedding("embedding", d);
+    if (s != MC_OK) return s;
+    MC_CHECK(table && ids && out, MC_ERR_NULL, "embedding: table, ids and out must not be NULL");
+    // a wave per token, 256-thread workgroups: a launch holds at most 2^32 - 1 work-items
+    MC_CHECK(d->tokens <= 67108860, MC_ERR_SHAPE, "embedding: tokens must be <= 67108860, got %lld",
+             (long long)d->tokens);
+    MC_CHECK(aligned16(table) && aligned16(out), MC_ERR_LAYOUT, "embedding: table and out must be 16-byte aligned");
+    MC_CHECK(reinterpret_cast<uintptr_t>(ids) % 4 == 0, MC_ERR_LAYOUT, "embedding: ids must be 4-byte aligned");
+    const double es = d->dtype == MC_F32 ? 4.0 : 2.0;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0, (double)d->tokens * (4.0 + 2.0 * es * d->dim));
+    return hip_status(mc::launch_embedding_fwd(*d, table, ids, out, stream), "embedding forward");
+}
+
+size_t mc_embedding_bwd_workspace_size(const mc_embedding_desc* d) {
+    return check_embedding("embedding backward", d) == MC_OK ? mc::embedding_bwd_ws(*d).total : 0;
+}
+
+mc_status mc_embedding_bwd(const mc_embedding_desc* d, const int32_t* ids, const void* dout, float* dtable,
+                           int32_t accumulate, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    mc_status s = check_embedding("embedding backward", d);
+    if (s != MC_OK) return s;
+    MC_CHECK(ids && dout && dtable, MC_ERR_NULL, "embedding backward: ids, dout and dtable must not be NULL");
+    MC_CHECK(accumulate == 0 || accumulate == 1, MC_ERR_VALUE, "embedding backward: accumulate must be 0 or 1");
+    // a launch holds at most 2^32 - 1 work-items: 256 per 8 ids, 64 per 256 columns of a unit of 64 tokens or more
+    MC_CHECK(d->vocab <= 134217720 && (double)((d->tokens + 63) / 64 < 1024 ? (d->tokens + 63) / 64 : 1024) *
+                                              (double)((d->dim + 255) / 256) < 6.0e7,
+             MC_ERR_SHAPE, "embedding backward: vocab must be <= 134217720 and dim <= 15000000");
+    MC_CHECK(aligned16(dout) && aligned16(dtable), MC_ERR_LAYOUT,
+             "embedding backward: dout and dtable must be 16-byte aligned");
+    MC_CHECK(reinterpret_cast<uintptr_t>(ids) % 4 == 0, MC_ERR_LAYOUT, "embedding backward: ids must be 4-byte aligned");
+    if ((s = check_workspace("embedding backward", workspace, workspace_bytes, mc::embedding_bwd_ws(*d).total)) != MC_OK)
+        return s;
+    const double es = d->dtype == MC_F32 ? 4.0 : 2.0;
+    mc::prof::Scope sc(mc::prof::kRowOps, stream, 0.0,
+                       (double)d->tokens * (4.0 + es * d->dim) + (accumulate ? 0.0 : 4.0 * d->vocab * d->dim));
+    return hip_status(mc::launch_embedding_bwd(*d, ids, dout, dtable, accumulate != 0, static_cast<char*>(workspace),
+                                               stream),
+                      "embedding backward");
 }
 
 size_t mc_layernorm_bwd_workspace_size(int64_t rows, int64_t dim) {

@@ -47,7 +47,11 @@ __device__ __forceinline__ void adamw_elem(float& p, float g, float& m, float& v
     v = v1;
 }
 
-__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWBatch bt) {
+// SCALED: every gradient is multiplied by *grad_scale first (rounded to fp32, as
+// a clipping of its own would), so that clipped gradients are never written.
+template <bool SCALED>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWBatch bt, const float* __restrict__ grad_scale) {
+    const float f = SCALED ? *grad_scale : 1.0f;
     int s = 0;
     for (int i = 1; i < bt.count; ++i)
         if ((int)blockIdx.x >= bt.slot[i].blk0) s = i;
@@ -57,7 +61,13 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWBatch bt) {
         const int64_t e = base + (int64_t)threadIdx.x * 4;
         if (e + 4 <= t.n) {
             float4 p = *reinterpret_cast<const float4*>(t.p + e);
-            const float4 g = *reinterpret_cast<const float4*>(t.g + e);
+            float4 g = *reinterpret_cast<const float4*>(t.g + e);
+            if constexpr (SCALED) {
+                g.x *= f;
+                g.y *= f;
+                g.z *= f;
+                g.w *= f;
+            }
             float4 m = *reinterpret_cast<const float4*>(t.m + e);
             float4 v = *reinterpret_cast<const float4*>(t.v + e);
             adamw_elem(p.x, g.x, m.x, v.x, t.c1, t.c2, bt);
@@ -70,7 +80,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWBatch bt) {
         } else {
             for (int64_t i = e; i < t.n; ++i) {
                 float p = t.p[i], m = t.m[i], v = t.v[i];
-                adamw_elem(p, t.g[i], m, v, t.c1, t.c2, bt);
+                adamw_elem(p, SCALED ? t.g[i] * f : t.g[i], m, v, t.c1, t.c2, bt);
                 t.po[i] = p;
                 t.m[i] = m;
                 t.v[i] = v;
@@ -83,9 +93,10 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWBatch bt) {
 
 int adamw_blocks(int64_t n) { return (int)((n + kPerBlock - 1) / kPerBlock); }
 
-hipError_t launch_adamw(const AdamWBatch& batch, int blocks, hipStream_t stream) {
+hipError_t launch_adamw(const AdamWBatch& batch, int blocks, const float* grad_scale, hipStream_t stream) {
     if (blocks <= 0) return hipSuccess;
-    adamw_kernel<<<dim3((unsigned)blocks), kThreads, 0, stream>>>(batch);
+    if (grad_scale) adamw_kernel<true><<<dim3((unsigned)blocks), kThreads, 0, stream>>>(batch, grad_scale);
+    else adamw_kernel<false><<<dim3((unsigned)blocks), kThreads, 0, stream>>>(batch, nullptr);
     return hipGetLastError();
 }
 

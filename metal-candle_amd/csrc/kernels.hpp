@@ -182,7 +182,54 @@ struct AdamWBatch {
     float b1, b2, omb1, omb2, eps, lr, wdlr;
 };
 int adamw_blocks(int64_t n);  // workgroups one tensor of n elements takes
-hipError_t launch_adamw(const AdamWBatch& batch, int blocks, hipStream_t stream);
+// grad_scale: device factor of every gradient, or null for none.
+hipError_t launch_adamw(const AdamWBatch& batch, int blocks, const float* grad_scale, hipStream_t stream);
+
+// ------------------------------------------------------ gradients' norm
+// The tables travel by value as kernel arguments (under 4 KB); blk0: first
+// workgroup of the slot, each of `chunk` elements.
+constexpr int kGradNormSlots = 160, kGradScaleSlots = 120;
+struct GradNormSlot {
+    const void* g;
+    int64_t n;
+    int blk0, dtype;
+};
+struct GradNormBatch {
+    GradNormSlot slot[kGradNormSlots];
+    int64_t chunk;
+    int count, pad;
+};
+struct GradScaleSlot {
+    const void* g;
+    void* out;
+    int64_t n;
+    int blk0;
+    int16_t dtype, out_dtype;
+};
+struct GradScaleBatch {
+    GradScaleSlot slot[kGradScaleSlots];
+    int64_t chunk;
+    int count, pad;
+};
+int64_t gradient_parts(const mc_grad_tensor* t, int32_t count);  // f64 partial sums in the workspace
+hipError_t launch_gradient_norm(const mc_grad_tensor* t, int32_t count, float max_norm, float* norm, float* scale,
+                                double* parts, hipStream_t stream);
+hipError_t launch_scale_gradients(const mc_grad_tensor* t, int32_t count, const float* scale, hipStream_t stream);
+hipError_t launch_clip_gradients(const mc_grad_tensor* t, int32_t count, float max_norm, float* norm, float* scale,
+                                 double* parts, hipStream_t stream);
+
+// -------------------------------------------------------------- embedding
+struct EmbeddingWs {
+    size_t order;  // int32 [tokens]
+    size_t start;  // int32 [vocab + 1]
+    size_t part;   // f32 [units][2][dim], where a run can be longer than two units
+    size_t total;
+};
+EmbeddingWs embedding_bwd_ws(const mc_embedding_desc& d);
+hipError_t launch_embedding_fwd(const mc_embedding_desc& d, const void* table, const int32_t* ids, void* out,
+                                hipStream_t stream);
+hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, const void* dout, float* dtable,
+                                bool accumulate, char* ws, hipStream_t stream);
 
 // ------------------------------------------------ LayerNorm, log-softmax, CE
 int layernorm_bwd_blocks(int64_t rows);  // dw / db partial rows in the workspace

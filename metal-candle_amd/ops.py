@@ -7,13 +7,15 @@ does (src/backend/custom_ops.rs:254-270). Activations are float32 or bfloat16;
 A, B and their gradients are float32. Every call enqueues on torch's current
 stream of the tensors' device and does not synchronise.
 """
+import array
 import ctypes
+import itertools
 
 import torch
 
 from . import _lib
-from ._lib import (AdamWConfig, AdamWTensor, AttnDesc, DistillDesc, LogprobDesc, LoraDesc, LoraProj, McError, PolicyDesc,
-                   PreferenceDesc, XentDesc, check, lib)
+from ._lib import (AdamWConfig, AdamWTensor, AttnDesc, DistillDesc, EmbeddingDesc, LogprobDesc, LoraDesc, LoraProj,
+                   McError, PolicyDesc, PreferenceDesc, XentDesc, check, lib)
 
 _DTYPES = {torch.float32: _lib.MC_F32, torch.bfloat16: _lib.MC_BF16}
 
@@ -774,12 +776,152 @@ def distillation_loss_forward_backward(logits, teacher_ids, teacher_logits, temp
     return loss, dlogits
 
 
+# ------------------------------------------------------------------ embedding
+def _ids(ids, device):
+    """int32 ids, as the kernels read them; int64 ids are converted (a copy), those that do not fit to one that is in
+    no table."""
+    if not isinstance(ids, torch.Tensor):
+        raise McError(_lib.MC_ERR_NULL, "ids must be a tensor")
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, 2**31 - 1).to(torch.int32)
+    _expect(ids, "ids", dtype=torch.int32, device=device)
+    if ids.numel() == 0:
+        raise McError(_lib.MC_ERR_SHAPE, "ids are empty")
+    return ids
+
+
+def embedding_forward(table, ids, scale=1.0, padding_id=None):
+    """scale * table[ids] for table [V, D] and ids int32 (or int64) [...]: [..., D] in the table's dtype, rounded once.
+
+    A token of padding_id gets zeros, one whose id is not in the table NaN."""
+    if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.numel() == 0:
+        raise McError(_lib.MC_ERR_SHAPE, "table must be [vocab, dim]")
+    _contig(table, "table")
+    code = _dtype_code(table)
+    ids = _ids(ids, table.device)
+    V, D = table.shape
+    d = EmbeddingDesc(ids.numel(), V, D, -1 if padding_id is None else int(padding_id), float(scale), code)
+    out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
+    _launch(table, lib().mc_embedding_fwd, ctypes.byref(d), table.data_ptr(), ids.data_ptr(), out.data_ptr())
+    return out
+
+
+def embedding_backward(dout, ids, vocab, scale=1.0, padding_id=None, dtable=None):
+    """The table's gradient [vocab, D] fp32: scale times the sum of dout [..., D] over the tokens of each id.
+
+    Without dtable a new one, zero for ids that do not occur; with it (fp32 [vocab, D]) the sums are added to it, as
+    where the table is the output projection's weight as well. Padding, and ids that are not in the table, are left
+    out. The sums run in a fixed order."""
+    if not isinstance(dout, torch.Tensor) or dout.dim() < 2 or dout.numel() == 0:
+        raise McError(_lib.MC_ERR_SHAPE, "dout must be [..., dim], one row per id")
+    _contig(dout, "dout")
+    code = _dtype_code(dout)
+    ids = _ids(ids, dout.device)
+    if ids.shape != dout.shape[:-1]:
+        raise McError(_lib.MC_ERR_SHAPE, f"ids has shape {tuple(ids.shape)}, expected {tuple(dout.shape[:-1])}")
+    D, V = dout.shape[-1], int(vocab)
+    d = EmbeddingDesc(ids.numel(), V, D, -1 if padding_id is None else int(padding_id), float(scale), code)
+    into = _address(dtable, "dtable", (V, D), torch.float32, dout.device)
+    ws_n = lib().mc_embedding_bwd_workspace_size(ctypes.byref(d))
+    if dtable is None and ws_n:
+        dtable = torch.empty(V, D, dtype=torch.float32, device=dout.device)
+    ws = _workspace(ws_n, dout.device)
+    _launch(dout, lib().mc_embedding_bwd, ctypes.byref(d), ids.data_ptr(), dout.data_ptr(), _ptr(dtable),
+            int(into is not None), _ptr(ws), ws_n)
+    return dtable
+
+
+# ------------------------------------------------------- gradients' norm, AdamW
+def _tensors(group, name):
+    """(dtypes, sizes, addresses, device) of a list of contiguous tensors of one device. One pass over the list per
+    property: a model's adapters are hundreds of small tensors, and their checks take longer than their kernels."""
+    if not isinstance(group, (list, tuple)) or not group:
+        raise McError(_lib.MC_ERR_SHAPE, f"{name} must be a list of at least one tensor")
+    try:
+        whole = all(map(torch.Tensor.is_contiguous, group))
+    except TypeError:
+        raise McError(_lib.MC_ERR_NULL, f"{name} must hold tensors only")
+    if not whole:
+        raise McError(_lib.MC_ERR_LAYOUT, f"every tensor of {name} must be contiguous")
+    dtypes = [t.dtype for t in group]
+    devices = {t.device for t in group}
+    if len(devices) > 1:
+        raise McError(_lib.MC_ERR_LAYOUT, f"{name} are on {len(devices)} devices, expected one")
+    for dtype in set(dtypes):
+        if dtype not in _DTYPES:
+            raise McError(_lib.MC_ERR_DTYPE, f"unsupported dtype {dtype} in {name} (float32 or bfloat16)")
+    return dtypes, list(map(torch.Tensor.numel, group)), list(map(torch.Tensor.data_ptr, group)), devices.pop()
+
+
+def _grad_table(grads, outs):
+    """(address of the mc_grad_tensor table, its length, what keeps it alive) of gradients and where they go."""
+    dtypes, sizes, at, device = _tensors(grads, "grads")
+    codes = [_DTYPES[t] for t in dtypes] if len(set(dtypes)) > 1 else [_DTYPES[dtypes[0]]] * len(dtypes)
+    to = at
+    if outs is not None and outs is not grads:
+        if len(outs) != len(grads):
+            raise McError(_lib.MC_ERR_SHAPE, f"outs list has {len(outs)} entries, expected {len(grads)}")
+        out_dtypes, out_sizes, to, out_device = _tensors(outs, "outs")
+        if out_sizes != sizes:
+            i = next(i for i, (a, b) in enumerate(zip(sizes, out_sizes)) if a != b)
+            raise McError(_lib.MC_ERR_SHAPE, f"outs[{i}] has {out_sizes[i]} elements, expected {sizes[i]}")
+        if out_device != device:
+            raise McError(_lib.MC_ERR_LAYOUT, f"outs are on {out_device}, expected {device}")
+        codes = [c | _DTYPES[t] << 32 for c, t in zip(codes, out_dtypes)]
+    else:
+        codes = [c | c << 32 for c in codes]
+    table = array.array("Q", itertools.chain.from_iterable(zip(at, to, sizes, codes)))
+    return table.buffer_info()[0], len(sizes), table
+
+
+def gradient_norm(grads, max_norm=None):
+    """The global norm of a list of fp32 or bf16 gradients, and the factor that brings it to max_norm: (norm [1],
+    scale [1]), fp32 on the device; scale is None without max_norm.
+
+    norm = sqrt(sum of all squares), summed in 64 bits in a fixed order; scale = 1 where norm <= max_norm, else
+    max_norm / norm. Pass scale to scale_gradients, or to adamw_step, which then clips as it reads."""
+    at, n, table = _grad_table(grads, None)
+    dev = grads[0].device
+    norm = torch.empty(1, dtype=torch.float32, device=dev)
+    scale = None if max_norm is None else torch.empty(1, dtype=torch.float32, device=dev)
+    ws_n = lib().mc_gradient_norm_workspace_size(at, n)
+    ws = _workspace(ws_n, dev)
+    _launch(grads[0], lib().mc_gradient_norm, at, n, 1.0 if max_norm is None else float(max_norm), norm.data_ptr(),
+            _ptr(scale), _ptr(ws), ws_n)
+    return norm, scale
+
+
+def scale_gradients(grads, scale, outs=None):
+    """Every gradient times scale (fp32 [1] on the device) into outs (fp32 or bf16 tensors of the same sizes; default:
+    in place), one rounding each. Returns outs."""
+    at, n, table = _grad_table(grads, outs)
+    if scale is None:
+        raise McError(_lib.MC_ERR_NULL, "scale must be a tensor")
+    _expect(scale, "scale", (1,), torch.float32, grads[0].device)
+    _launch(grads[0], lib().mc_scale_gradients, at, n, scale.data_ptr())
+    return grads if outs is None else outs
+
+
+def clip_gradients(grads, max_norm, outs=None):
+    """gradient_norm and scale_gradients in one call: (norm [1], scale [1]). outs may have another dtype than the
+    gradients, as fp32 ones for adamw_step from bf16 ones."""
+    at, n, table = _grad_table(grads, outs)
+    dev = grads[0].device
+    norm, scale = (torch.empty(1, dtype=torch.float32, device=dev) for _ in range(2))
+    ws_n = lib().mc_gradient_norm_workspace_size(at, n)
+    ws = _workspace(ws_n, dev)
+    _launch(grads[0], lib().mc_clip_gradients, at, n, float(max_norm), norm.data_ptr(), scale.data_ptr(), _ptr(ws), ws_n)
+    return norm, scale
+
+
 def adamw_step(params, grads, ms, vs, steps, lr=1e-4, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
-               outs=None):
+               outs=None, grad_scale=None):
     """AdamW::step (src/training/optimizer.rs:227-281) for a list of fp32
     tensors in one call: m and v are updated in place; the new parameters go
     to outs (default: the params themselves, in place). steps: one step count
-    per tensor (or one int for all)."""
+    per tensor (or one int for all). grad_scale: gradient_norm's scale (fp32 [1]
+    on the device), by which every gradient is multiplied first, as
+    scale_gradients would, without writing it."""
     n = len(params)
     if isinstance(steps, int):
         steps = [steps] * n
@@ -800,6 +942,10 @@ def adamw_step(params, grads, ms, vs, steps, lr=1e-4, beta1=0.9, beta2=0.999, ep
         table[i] = AdamWTensor(params[i].data_ptr(), grads[i].data_ptr(), ms[i].data_ptr(), vs[i].data_ptr(),
                                outs[i].data_ptr(), numel, int(steps[i]))
     cfg = AdamWConfig(lr, beta1, beta2, eps, weight_decay)
+    if grad_scale is not None and n:
+        _expect(grad_scale, "grad_scale", (1,), torch.float32, params[0].device)
+        _launch(params[0], lib().mc_adamw_scaled_step, ctypes.byref(cfg), table, n, grad_scale.data_ptr())
+        return outs
     stream = _stream(params[0]) if n else None
     check(lib().mc_adamw_step(ctypes.byref(cfg), table, n, stream))
     return outs

@@ -32,6 +32,9 @@
  *                    bias of MetalLayerNorm (src/embeddings/metal_bert.rs).
  *   mc_log_softmax_*, mc_cross_entropy_*  cross_entropy_loss and its label
  *                    smoothing (src/training/loss.rs:58-245).
+ *   mc_attention_spans, mc_packed_attention_*  no counterpart in the reference:
+ *                    attention over packed documents, capped scores, a bias by
+ *                    distance.
  *   mc_gradient_norm, mc_scale_gradients, mc_clip_gradients,
  *   mc_embedding_*   no counterpart in the reference: clipping by the gradients'
  *                    global norm; the scaled token embedding and its gradient.
@@ -269,6 +272,54 @@ mc_status mc_attention_bwd(const mc_attn_desc* d, const void* q, const void* k, 
                            const float* mask, const void* o, const float* lse, const void* dout,
                            void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                            hipStream_t stream);
+
+/* Attention over rows that hold several documents, with what some models add to
+ * their scores. No counterpart in the reference, whose rows hold one sequence.
+ * q, k, v, o, lse, head repetition and layouts as for mc_attention_fwd; per query
+ * head h, with x = scale q.k^T,
+ *   x = cap tanh(x / cap)          (cap > 0)
+ *   x = x - slopes[h] |i - j|      (slopes fp32 [H], not NULL)
+ *   o_i = softmax of x over the keys that query i sees, times their v
+ * A query that sees no key has o = 0 and lse = -inf, and no gradient comes from
+ * it. What a pair hides is not read into any result, whatever is stored there:
+ * infinities and NaN in padding, in other documents or in later tokens included.
+ *
+ * mc_attention_spans writes who sees whom, once for all layers: spans int32
+ * [B, S, 4], for each token the queries' side [0], [1] (the keys that it sees, from
+ * and to) and the keys' side [2], [3] (the queries that see it).
+ *   documents int32 [B, S] (NULL: a row is one document): a document is a run of
+ *     equal ids, tokens see inside theirs only; ids below 0 are padding, which
+ *     sees nothing and is not seen.
+ *   causal: a token sees those up to itself; prefix uint8 [B, S] (NULL: none;
+ *     causal only): a document's leading tokens of non-zero prefix, its prompt, also
+ *     see each other. Non-zero tokens behind the first zero of a document are none.
+ * The entry points below take the spans, or with spans NULL attn.causal (which is
+ * 0 with spans). Spans of another origin are kept inside the row, but a query and a
+ * key must agree on whether they meet, and both sides must be intervals.
+ *
+ * The slopes are constants: they get no gradient. lse of a query whose q holds an
+ * infinity or NaN is NaN under a cap. */
+mc_status mc_attention_spans(int64_t batch, int64_t seq, const int32_t* documents, const uint8_t* prefix,
+                             int32_t causal, int32_t* spans, hipStream_t stream);
+
+typedef struct mc_packed_attn_desc {
+    mc_attn_desc attn;  /* scale > 0 */
+    float cap;          /* 0: none, or in [0.01, 1000] */
+    int32_t reserved;   /* 0 */
+} mc_packed_attn_desc;
+
+size_t mc_packed_attention_fwd_workspace_size(const mc_packed_attn_desc* d);
+mc_status mc_packed_attention_fwd(const mc_packed_attn_desc* d, const void* q, const void* k, const void* v,
+                                  const int32_t* spans, const float* slopes, void* o, float* lse, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream);
+
+/* As mc_attention_bwd, with the score's derivative 1 - tanh^2 in dS under a cap.
+ * with_spans: whether the call will have spans. Results are bitwise reproducible. */
+size_t mc_packed_attention_bwd_workspace_size(const mc_packed_attn_desc* d, int32_t with_spans);
+mc_status mc_packed_attention_bwd(const mc_packed_attn_desc* d, const void* q, const void* k, const void* v,
+                                  const int32_t* spans, const float* slopes, const void* o, const float* lse,
+                                  const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream);
 
 /* AdamW (src/training/optimizer.rs:33-48 config, 227-281 step) over fp32
  * parameter tensors, typically the LoRA A and B of every projection. */

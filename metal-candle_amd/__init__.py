@@ -12,6 +12,7 @@ from .ops import (  # noqa: F401
     adamw_step,
     attention_backward,
     attention_forward,
+    attention_spans,
     clip_gradients,
     cross_entropy_backward,
     cross_entropy_forward,
@@ -30,6 +31,8 @@ from .ops import (  # noqa: F401
     lora_forward,
     lora_group_backward,
     lora_group_forward,
+    packed_attention_backward,
+    packed_attention_forward,
     policy_loss_backward,
     policy_loss_forward,
     policy_loss_forward_backward,

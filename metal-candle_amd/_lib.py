@@ -78,6 +78,14 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class PackedAttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("attn", AttnDesc),
+        ("cap", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 class XentDesc(ctypes.Structure):
     _fields_ = [
         ("rows", ctypes.c_int64),
@@ -201,6 +209,7 @@ _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
 _dp = ctypes.POINTER(LoraDesc)
 _ap = ctypes.POINTER(AttnDesc)
+_kp = ctypes.POINTER(PackedAttnDesc)
 _lp = ctypes.POINTER(LogprobDesc)
 _rp = ctypes.POINTER(PreferenceDesc)
 _pp = ctypes.POINTER(PolicyDesc)
@@ -232,6 +241,12 @@ _SIGNATURES = {
     "mc_attention_fwd": (ctypes.c_int, [_ap, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "mc_attention_bwd_workspace_size": (_sz, [_ap]),
     "mc_attention_bwd": (ctypes.c_int, [_ap, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_attention_spans": (ctypes.c_int, [_i64, _i64, _vp, _vp, _i32, _vp, _vp]),
+    "mc_packed_attention_fwd_workspace_size": (_sz, [_kp]),
+    "mc_packed_attention_fwd": (ctypes.c_int, [_kp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mc_packed_attention_bwd_workspace_size": (_sz, [_kp, _i32]),
+    "mc_packed_attention_bwd": (ctypes.c_int, [_kp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                               _vp]),
     "mc_layernorm_fwd": (ctypes.c_int, [_i64, _i64, _f32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "mc_layernorm_bwd_workspace_size": (_sz, [_i64, _i64]),
     "mc_layernorm_bwd": (ctypes.c_int, [_i64, _i64, _f32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,

@@ -148,6 +148,8 @@ double attn_pairs(const mc_attn_desc* d) {
 
 extern "C" {
 
+static mc_status check_workspace(const char* op, const void* workspace, size_t bytes, size_t need);
+
 const char* mc_version(void) { return "mc_hip 0.1.0 (gfx950)"; }
 
 mc_status mc_profile_enable(int32_t on) {
@@ -531,6 +533,95 @@ mc_status mc_attention_bwd(const mc_attn_desc* d, const void* q, const void* k, 
                       "Attention backward");
 }
 
+mc_status mc_attention_spans(int64_t batch, int64_t seq, const int32_t* documents, const uint8_t* prefix,
+                             int32_t causal, int32_t* spans, hipStream_t stream) {
+    // a workgroup per row; a launch holds at most 2^32 - 1 work-items
+    MC_CHECK(batch >= 1 && batch <= 4194303 && seq >= 1 && seq < 2147483647 - 4096, MC_ERR_SHAPE,
+             "attention_spans: batch must be in [1, 4194303] and seq in [1, 2^31 - 4097), got %lld, %lld",
+             (long long)batch, (long long)seq);
+    MC_CHECK(causal == 0 || causal == 1, MC_ERR_VALUE, "attention_spans: causal must be 0 or 1");
+    MC_CHECK(!prefix || causal, MC_ERR_VALUE, "attention_spans: a prefix needs causal rows");
+    MC_CHECK(spans, MC_ERR_NULL, "attention_spans: spans must not be NULL");
+    MC_CHECK(aligned16(spans), MC_ERR_LAYOUT, "attention_spans: spans must be 16-byte aligned");
+    MC_CHECK(reinterpret_cast<uintptr_t>(documents) % 4 == 0, MC_ERR_LAYOUT,
+             "attention_spans: documents must be 4-byte aligned");
+    mc::prof::Scope sc(mc::prof::kAttention, stream, 0.0, 21.0 * (double)batch * (double)seq);
+    return hip_status(mc::launch_attention_spans(documents, prefix, batch, seq, causal, spans, stream),
+                      "attention_spans");
+}
+
+static mc_status check_packed(const char* op, const mc_packed_attn_desc* d, bool spans) {
+    MC_CHECK(d != nullptr, MC_ERR_NULL, "%s: descriptor is NULL", op);
+    const mc_status s = check_attn_desc(&d->attn, op);
+    if (s != MC_OK) return s;
+    MC_CHECK(d->attn.scale > 0.0f, MC_ERR_VALUE, "%s: scale must be positive, got %g", op, (double)d->attn.scale);
+    MC_CHECK(d->cap == 0.0f || (d->cap >= 0.01f && d->cap <= 1000.0f), MC_ERR_VALUE,
+             "%s: cap must be 0 (none) or in [0.01, 1000], got %g", op, (double)d->cap);
+    MC_CHECK(d->attn.scale < 1.0e30f, MC_ERR_VALUE, "%s: scale %g is too large", op, (double)d->attn.scale);
+    MC_CHECK(d->reserved == 0, MC_ERR_VALUE, "%s: reserved must be 0", op);
+    MC_CHECK(!spans || !d->attn.causal, MC_ERR_VALUE, "%s: causal must be 0 with spans, which hold it", op);
+    // workgroups of 256 threads per 64 rows of a head (or more), per 32 (float32 tiles) or per four; a launch
+    // holds at most 2^32 - 1 work-items, 65535 heads in its second dimension
+    const bool mfma = mc::attention_uses_mfma(d->attn);
+    const bool tiles = mc::attention_f32_mfma_fwd(d->attn) && mc::attention_f32_mfma_bwd(d->attn);
+    const double S = (double)d->attn.seq, bh = (double)d->attn.batch * d->attn.heads;
+    MC_CHECK((!mfma || bh <= 65535.0) && bh * std::ceil(S / (mfma ? 64.0 : tiles ? 32.0 : 4.0)) < 16777215.0, MC_ERR_SHAPE,
+             "%s: B * H * S (%lld x %d x %lld) too large for a launch", op, (long long)d->attn.batch,
+             (int)d->attn.heads, (long long)d->attn.seq);
+    return MC_OK;
+}
+
+size_t mc_packed_attention_fwd_workspace_size(const mc_packed_attn_desc* d) {
+    return check_packed("Packed attention", d, false) == MC_OK ? mc::packed_fwd_ws(*d).total : 0;
+}
+
+mc_status mc_packed_attention_fwd(const mc_packed_attn_desc* d, const void* q, const void* k, const void* v,
+                                  const int32_t* spans, const float* slopes, void* o, float* lse, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream) {
+    mc_status s = check_packed("Packed attention", d, spans != nullptr);
+    if (s != MC_OK) return s;
+    MC_CHECK(q && k && v && o, MC_ERR_NULL, "Packed attention: q, k, v and o must not be NULL");
+    MC_CHECK(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(spans), MC_ERR_LAYOUT,
+             "Packed attention: q, k, v, o and spans must be 16-byte aligned");
+    const size_t need = mc::packed_fwd_ws(*d).total;
+    if (need && (s = check_workspace("Packed attention", workspace, workspace_bytes, need)) != MC_OK) return s;
+    const mc_attn_desc& t = d->attn;
+    const double es = t.dtype == MC_F32 ? 4.0 : 2.0;
+    const double qo = (double)t.batch * t.heads * t.seq * t.head_dim, kv = qo / t.heads * t.kv_heads;
+    // the pairs of rows without documents: what the spans hide is not known on the host
+    mc::prof::Scope sc(mc::prof::kAttention, stream, 4.0 * attn_pairs(&t) * t.head_dim, es * (2.0 * qo + 2.0 * kv));
+    return hip_status(mc::launch_packed_fwd(*d, q, k, v, spans, slopes, o, lse, static_cast<char*>(workspace), stream),
+                      "Packed attention forward");
+}
+
+size_t mc_packed_attention_bwd_workspace_size(const mc_packed_attn_desc* d, int32_t with_spans) {
+    if (check_packed("Packed attention backward", d, with_spans != 0) != MC_OK) return 0;
+    return mc::packed_bwd_ws(*d, with_spans != 0).total;
+}
+
+mc_status mc_packed_attention_bwd(const mc_packed_attn_desc* d, const void* q, const void* k, const void* v,
+                                  const int32_t* spans, const float* slopes, const void* o, const float* lse,
+                                  const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream) {
+    mc_status s = check_packed("Packed attention backward", d, spans != nullptr);
+    if (s != MC_OK) return s;
+    MC_CHECK(q && k && v && o && lse && dout && dq && dk && dv, MC_ERR_NULL,
+             "Packed attention backward: q, k, v, o, lse, dout, dq, dk and dv must not be NULL");
+    MC_CHECK(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && aligned16(dout) && aligned16(dq) &&
+                 aligned16(dk) && aligned16(dv) && aligned16(spans),
+             MC_ERR_LAYOUT, "Packed attention backward: q, k, v, spans, o, dout, dq, dk and dv must be 16-byte aligned");
+    if ((s = check_workspace("Packed attention backward", workspace, workspace_bytes,
+                             mc::packed_bwd_ws(*d, spans != nullptr).total)) != MC_OK)
+        return s;
+    const mc_attn_desc& t = d->attn;
+    const double es = t.dtype == MC_F32 ? 4.0 : 2.0;
+    const double qo = (double)t.batch * t.heads * t.seq * t.head_dim, kv = qo / t.heads * t.kv_heads;
+    mc::prof::Scope sc(mc::prof::kAttention, stream, 8.0 * attn_pairs(&t) * t.head_dim, es * (4.0 * qo + 4.0 * kv));
+    return hip_status(mc::launch_packed_bwd(*d, q, k, v, spans, slopes, o, lse, dout, dq, dk, dv,
+                                            static_cast<char*>(workspace), stream),
+                      "Packed attention backward");
+}
+
 // b^t as Rust's f32::powi lowers it for a run-time exponent: right-to-left
 // binary exponentiation in fp32 (square the base, multiply the result in at
 // every set bit of t).
@@ -652,8 +743,6 @@ static mc_status check_max_norm(const char* op, float max_norm) {
     MC_CHECK(max_norm > 0.0f, MC_ERR_VALUE, "%s: max_norm must be positive, got %g", op, (double)max_norm);
     return MC_OK;
 }
-
-static mc_status check_workspace(const char* op, const void* workspace, size_t have, size_t need);
 
 static double grad_bytes(const mc_grad_tensor* t, int32_t count, bool read, bool outs) {
     double b = 0.0;

@@ -160,6 +160,40 @@ hipError_t launch_attention_f32_bwd(const mc_attn_desc& d, const void* q, const 
                                     void* dk, void* dv, float* delta, float* dk_part, float* dv_part,
                                     hipStream_t stream);
 
+// Attention over packed rows (attention_packed.hip; float32 and row kernels in
+// attention_packed_f32.hip). spans: int32 [B, S, 4] or null (d.attn.causal).
+bool attention_dq_from_ds(const mc_attn_desc& d);  // the dQ pass reads a stored dS^T
+struct PackedWs {
+    size_t vt, flags;  // bf16 [B, Hkv, D, Sp]; int32 [B, Hkv, Sp / 64]
+    size_t total;
+};
+struct PackedBwdWs {
+    size_t lsd, dk_part, dv_part, dst;  // as AttnBwdWs
+    size_t qflags, kflags;              // int32 [B, H, Sp / 64], [B, Hkv, S rounded up to 128 / 128]
+    size_t total;
+};
+PackedWs packed_fwd_ws(const mc_packed_attn_desc& d);
+PackedBwdWs packed_bwd_ws(const mc_packed_attn_desc& d, bool spans);
+hipError_t launch_attention_spans(const int32_t* documents, const uint8_t* prefix, int64_t batch, int64_t seq,
+                                  int causal, int32_t* spans, hipStream_t stream);
+hipError_t launch_packed_fwd(const mc_packed_attn_desc& d, const void* q, const void* k, const void* v,
+                             const int32_t* spans, const float* slopes, void* o, float* lse, char* ws,
+                             hipStream_t stream);
+hipError_t launch_packed_bwd(const mc_packed_attn_desc& d, const void* q, const void* k, const void* v,
+                             const int32_t* spans, const float* slopes, const void* o, const float* lse,
+                             const void* dout, void* dq, void* dk, void* dv, char* ws, hipStream_t stream);
+hipError_t launch_packed_f32_fwd(const mc_packed_attn_desc& d, const void* q, const void* k, const void* v,
+                                 const int32_t* spans, const float* slopes, void* o, float* lse, hipStream_t stream);
+hipError_t launch_packed_f32_bwd(const mc_packed_attn_desc& d, const void* q, const void* k, const void* v,
+                                 const int32_t* spans, const float* slopes, const void* o, const float* lse,
+                                 const void* dout, void* dq, void* dk, void* dv, float* delta, float* dk_part,
+                                 float* dv_part, hipStream_t stream);
+hipError_t launch_packed_rows_fwd(const mc_packed_attn_desc& d, const void* q, const void* k, const void* v,
+                                  const int32_t* spans, const float* slopes, void* o, float* lse, hipStream_t stream);
+hipError_t launch_packed_rows_bwd(const mc_packed_attn_desc& d, const void* q, const void* k, const void* v,
+                                  const int32_t* spans, const float* slopes, const void* o, const float* lse,
+                                  const void* dout, void* dq, void* dk, void* dv, float* delta, hipStream_t stream);
+
 // --------------------------------------------------------------- AdamW
 // One launch of the AdamW kernel updates up to kAdamWSlots tensors; the
 // table travels by value as a kernel argument (no device allocation).

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import (AdamWConfig, AdamWTensor, AttnDesc, DistillDesc, EmbeddingDesc, LogprobDesc, LoraDesc, LoraProj,
-                   McError, PolicyDesc, PreferenceDesc, XentDesc, check, lib)
+                   McError, PackedAttnDesc, PolicyDesc, PreferenceDesc, XentDesc, check, lib)
 
 _DTYPES = {torch.float32: _lib.MC_F32, torch.bfloat16: _lib.MC_BF16}
 
@@ -379,6 +379,77 @@ def attention_backward(q, k, v, o, lse, dout, causal=False, scale=None, mask=Non
     ws = _workspace(ws_n, q.device)
     check(lib().mc_attention_bwd(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(o), _ptr(lse),
                                  _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), ws_n, _stream(q)))
+    return dq, dk, dv
+
+
+def attention_spans(documents=None, prefix=None, causal=True):
+    """Who sees whom in rows that hold several documents: int32 [B, S, 4], made once for every layer's
+    packed_attention_forward and _backward.
+
+    documents int32 [B, S]: a document is a run of equal ids, whose tokens see each other only; ids below 0 are
+    padding, which sees nothing and is not seen (None: a row is one document). causal: a token sees those up to
+    itself; prefix uint8 or bool [B, S] then marks prompts, a document's leading tokens, which also see each other
+    (non-zero tokens behind a document's first zero are no prompt). A token's entry holds the keys that it sees as a
+    query, from and to, then the queries that see it as a key."""
+    ref = documents if documents is not None else prefix
+    if ref is None:
+        raise McError(_lib.MC_ERR_NULL, "attention_spans: documents or prefix is required (without either, call the "
+                      "attention with causal)")
+    if not isinstance(ref, torch.Tensor) or ref.dim() != 2 or ref.numel() == 0:
+        raise McError(_lib.MC_ERR_SHAPE, "documents and prefix must be [batch, seq]")
+    dev, shape = ref.device, tuple(ref.shape)
+    ids = _address(documents, "documents", shape, torch.int32, dev)
+    if isinstance(prefix, torch.Tensor) and prefix.dtype == torch.bool:
+        prefix = prefix.view(torch.uint8)
+    flags = _address(prefix, "prefix", shape, torch.uint8, dev)
+    spans = torch.empty(*shape, 4, dtype=torch.int32, device=dev)
+    _launch(ref, lib().mc_attention_spans, *shape, ids, flags, int(bool(causal)), spans.data_ptr())
+    return spans
+
+
+def _packed_call(q, k, v, spans, causal, scale, cap, slopes):
+    B, H, S, D = _attn_inputs(q, k, v, None)
+    if spans is not None and causal:
+        raise McError(_lib.MC_ERR_VALUE, "causal must be False with spans, which hold it")
+    at = _address(spans, "spans", (B, S, 4), torch.int32, q.device)
+    by = _address(slopes, "slopes", (H,), torch.float32, q.device)
+    d = PackedAttnDesc(attention_desc(q, k, causal, D ** -0.5 if scale is None else scale),
+                       0.0 if cap is None else float(cap), 0)
+    return d, at, by
+
+
+def packed_attention_forward(q, k, v, spans=None, causal=False, scale=None, cap=None, slopes=None, save_lse=True):
+    """Attention over packed rows, with capped scores and a bias by distance: (o [B, S, H*D], lse [B, H, S]).
+
+    q [B, H, S, D], k and v [B, Hkv, S, D]. spans from attention_spans say who sees whom; without them causal does.
+    The scores are x = scale q.k, then cap * tanh(x / cap) (cap in [0.01, 1000]; None: uncapped), then
+    x - slopes[h] * |i - j| (slopes fp32 [H], constants; None: none). A query that sees nothing has o = 0 and
+    lse = -inf. What is hidden may hold anything, NaN included. scale > 0, default 1 / sqrt(D)."""
+    d, at, by = _packed_call(q, k, v, spans, causal, scale, cap, slopes)
+    B, H, S, D = q.shape
+    o = torch.empty(B, S, H * D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if save_lse else None
+    ws_n = lib().mc_packed_attention_fwd_workspace_size(ctypes.byref(d))
+    ws = _workspace(ws_n, q.device)
+    _launch(q, lib().mc_packed_attention_fwd, ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), at, by,
+            o.data_ptr(), _ptr(lse), _ptr(ws), ws_n)
+    return o, lse
+
+
+def packed_attention_backward(q, k, v, o, lse, dout, spans=None, causal=False, scale=None, cap=None, slopes=None):
+    """(dq, dk, dv) of packed_attention_forward, called as it was; o and lse come from it. Padding gets zeros."""
+    d, at, by = _packed_call(q, k, v, spans, causal, scale, cap, slopes)
+    B, H, S, D = q.shape
+    if o is None or lse is None or dout is None:
+        raise McError(_lib.MC_ERR_NULL, "packed attention backward: o, lse and dout are required")
+    o_at = _address(o, "o", (B, S, H * D), q.dtype, q.device)
+    g_at = _address(dout, "dout", (B, S, H * D), q.dtype, q.device)
+    lse_at = _address(lse, "lse", (B, H, S), torch.float32, q.device)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    ws_n = lib().mc_packed_attention_bwd_workspace_size(ctypes.byref(d), int(at is not None))
+    ws = _workspace(ws_n, q.device)
+    _launch(q, lib().mc_packed_attention_bwd, ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), at, by, o_at,
+            lse_at, g_at, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(ws), ws_n)
     return dq, dk, dv
 
 

@@ -20,8 +20,8 @@
 //               would be NaN in every row of a tile that shares it. The forward
 //               adds them afterwards to the rows that see them.
 //  packed_fwd   one workgroup per (b, h, 128 queries).
-//  packed_prep  Delta and lse per 64 queries; blocks noted whose Q or dO must
-//               be cleared of infinities and NaN before hidden pairs meet them.
+//  packed_prep  Delta and lse per query; blocks of 64 noted whose Q or dO must be
+//               cleared of infinities and NaN before hidden pairs meet them.
 //  packed_dkdv  one workgroup per (b, K/V head, group of query heads, 128 keys);
 //               stores dS^T of the queries that its keys meet, in blocks of 128.
 //  packed_dq    dQ from the stored dS^T, one workgroup per (b, h, 128 queries);
@@ -417,33 +417,31 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
         }
 
         // Accumulator j of tile t is key key0 + 32 t + 8 (j/4) + 4 half + j%4.
-        // Without a cap or a bias the scores stay unscaled: the maximum is scaled
-        // once and the scale goes into the exponent's fma.
+        // Without a bias x stays a product until the exponent's fma, since the
+        // largest product is the largest score: its score is formed once.
         const int key0 = kb * KB;
-        constexpr bool RAW = !CAP && !BIAS;
-        const float cx = RAW ? a.scale_log2 : 1.f;
         float x[2][16];
         const float dist = (float)((int)my_q - key0 - 4 * half);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                x[t][j] = RAW ? sacc[t][j] : score_log2<CAP>(sacc[t][j], a);
+                x[t][j] = BIAS ? score_log2<CAP>(sacc[t][j], a) : sacc[t][j];
                 if constexpr (BIAS)
                     x[t][j] = __builtin_fmaf(__builtin_fabsf(dist - (float)(32 * t + 8 * (j >> 2) + (j & 3))), -slope2,
                                              x[t][j]);
             }
-        if (!(key0 >= ws.all_lo && key0 + KB <= ws.all_hi)) {
-            // key offsets in the block against this lane's span; its 4 half
-            // moves to the bounds, so each test compares a constant
-            const int lo = mine.lo - key0 - 4 * half, hi = mine.hi - key0 - 4 * half;
+        // key offsets in the block against this lane's span; its 4 half moves to
+        // the bound, so each test is one subtraction and one unsigned comparison
+        const bool edge = !(key0 >= ws.all_lo && key0 + KB <= ws.all_hi);
+        const int lo = mine.lo - key0 - 4 * half;
+        const uint32_t width = (uint32_t)(mine.hi - mine.lo);
+        if (edge) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int ko = 32 * t + 8 * (j >> 2) + (j & 3);
-                    if (ko < lo || ko >= hi) x[t][j] = kNegInf;
-                }
+                for (int j = 0; j < 16; ++j)
+                    if ((uint32_t)(32 * t + 8 * (j >> 2) + (j & 3) - lo) >= width) x[t][j] = kNegInf;
         }
 
         // online softmax over this block's 64 keys (32 here, 32 in lane ^ 32);
@@ -453,19 +451,35 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 16; ++j) mx = fmaxf(mx, x[t][j]);
-        mx = half_pair_max(mx) * cx;  // cx > 0: -inf stays -inf
+        mx = half_pair_max(mx);
+        if constexpr (!BIAS) mx = mx == kNegInf ? mx : score_log2<CAP>(mx, a);  // scale > 0
         float alpha = 1.f;
         if (mx > m_run + kMaxSlack) {
             alpha = exp2_hw(m_run - mx);  // m_run = -inf: 0 (O and l are 0 then)
             m_run = mx;
         }
         const float m_use = m_run == kNegInf ? 0.f : m_run;  // a row with no key yet keeps p = 0
+        if constexpr (CAP && !BIAS) {
+            // x -> r = (1 - tanh) / 2; a hidden score's is +inf, not that of -inf
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[t][j] = __builtin_amdgcn_rcpf(1.f + exp2_hw(x[t][j] * a.cap_in));
+            if (edge) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if ((uint32_t)(32 * t + 8 * (j >> 2) + (j & 3) - lo) >= width) x[t][j] = __builtin_inff();
+            }
+        }
+        const float mul = CAP ? -2.f * a.cap_log2 : a.scale_log2, add = (CAP ? a.cap_log2 : 0.f) - m_use;
         float ps = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                x[t][j] = exp2_hw(RAW ? __builtin_fmaf(x[t][j], cx, -m_use) : x[t][j] - m_use);
+                x[t][j] = exp2_hw(BIAS ? x[t][j] - m_use : __builtin_fmaf(x[t][j], mul, add));
                 ps += x[t][j];
             }
         l_run = l_run * alpha + ps;
@@ -555,69 +569,147 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
 }
 
 // --------------------------------------------------------- backward prep
-// Per (b, h, 64 queries): Delta = rowsum(dO (.) O) and lse * log2 e into one
-// [2][64] fp32 block, and whether the block's Q or dO may hold infinities or NaN:
-// dO does, or a row's lse is not finite (its Q or a key that it sees holds one, or
-// it sees nothing and may hold anything). A row that sees nothing gets lse = +inf,
-// which makes its P 0; one whose dO is not finite NaN, which reaches every
-// gradient that depends on it.
-template <int D>
-__global__ __launch_bounds__(256) void packed_prep(const uint16_t* __restrict__ o, const uint16_t* __restrict__ dout,
-                                                   const float* __restrict__ lse, int H, int64_t S, int64_t Sp,
-                                                   float* __restrict__ lsd, int32_t* __restrict__ flags) {
-    constexpr int CPR = D / 8;
-    const int64_t bh = blockIdx.y;
-    const int64_t b = bh / H, h = bh % H;
-    const int64_t q0 = (int64_t)blockIdx.x * 64;
-    const int64_t ldo = (int64_t)H * D;
-    const __amdgpu_buffer_rsrc_t ro = make_rsrc(o + (b * S * H + h) * D, (S * H - h) * D * 2);
-    const __amdgpu_buffer_rsrc_t rd = make_rsrc(dout + (b * S * H + h) * D, (S * H - h) * D * 2);
-    // Each wave takes 16 rows; one load instruction covers RPI whole rows.
-    constexpr int RPI = 64 / CPR, NI = 16 / RPI;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int ch = lane % CPR, rsub = lane / CPR;
-    float acc[NI];
-    int bad[NI];
+// Per (b, h, 128 queries): Delta and lse * log2 e into a [2][64] fp32 block per 64
+// queries, and whether the block's Q or dO may hold infinities or NaN: dO does, or
+// a row's lse is not finite (its Q or a key that it sees holds one, or it sees
+// nothing and may hold anything). A row that sees nothing gets lse = +inf, which
+// makes its P 0; one whose dO is not finite NaN, which reaches every gradient that
+// depends on it.
+//
+// Delta_i = sum_d dO_id O_id carries o's rounding and that of P (bf16 both), which
+// dS = P (dP - Delta) does not average away where few keys share it: dq and dk of
+// 4 causal tokens were 6e-2 of their size off, of 30 9e-3, of 1021 4.9e-3, of 4096
+// 3.6e-3 (their own roundings and dS's to bf16 make 2.4e-3). Where a workgroup's
+// queries span at most kExactKeys keys it is formed as sum_j P_ij dP_ij instead,
+// S^T = K.Q^T and dP^T = V.dO^T once more, shaped as the forward. Both the error
+// and what that costs end there: with 128 / 256 / 512 keys 8 rows of 2048 tokens
+// in documents of 340 are 4.1e-3 / 3.5e-3 / 2.9e-3 off.
+constexpr int kExactKeys = 256;
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16_t* __restrict__ o,
+                                                      const float* __restrict__ lse, float* __restrict__ lsd,
+                                                      int32_t* __restrict__ flags) {
+    constexpr int KB = 64, QB = 128, KS = D / 16;
+    constexpr int TILE = 64 * D, STAGE = 2 * TILE;  // K, V [64][D]
+    __shared__ __attribute__((aligned(1024))) uint16_t smem[2 * STAGE];
+    __shared__ int slots[4][2];
+    __shared__ int noted[4];
+    const uint32_t smem_byte = (uint32_t)reinterpret_cast<uintptr_t>(smem);
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const int col = lane & 31, half = lane >> 5;
+    const int nbh = a.B * a.H;
+    const int qb = (int)(blockIdx.x / nbh);
+    const int bh = xcd_head_order((int)(blockIdx.x % nbh), nbh);
+    const int b = bh / a.H, h = bh % a.H;
+    const int64_t bhk = (int64_t)b * a.Hkv + h / (a.H / a.Hkv);
+    const int64_t S = a.S;
+    const int64_t qw = (int64_t)qb * QB + 32 * wave;
+    const int64_t my_q = qw + col;
+
+    // dO^T fragments (B operand of dP^T = V.dO^T): query my_q, dims 16 s + 8 half .. +7
+    const int64_t ldo = (int64_t)a.H * D;
+    const __amdgpu_buffer_rsrc_t rdo = make_rsrc(a.dout + ((int64_t)b * S * a.H + h) * D, (S * a.H - h) * D * 2);
+    bf16x8 gf[KS];
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int row = wave * 16 + i * RPI + rsub;
-        const uint32_t off = q0 + row < S ? (uint32_t)(((q0 + row) * ldo + 8 * ch) * 2) : kOOB;
-        float x[8], g[8];
-        const i32x4 gv = buf_load16(rd, off);
-        BVec<uint16_t>::unpack(buf_load16(ro, off), x);
-        BVec<uint16_t>::unpack(gv, g);
-        bad[i] = any_nonfinite(__builtin_bit_cast(uint4, gv));
-        acc[i] = 0.f;
+    for (int s = 0; s < KS; ++s)
+        gf[s] = __builtin_bit_cast(
+            bf16x8, buf_load16(rdo, my_q < S ? (uint32_t)((my_q * ldo + 16 * s + 8 * half) * 2) : kOOB));
+    const float x = my_q < S ? lse[(int64_t)bh * S + my_q] : kNegInf;
+    const Span mine = query_span(a.spans, b, my_q, (int)S, a.causal);
+    const WaveSpan ws = wave_span(mine);
+    const Span wg = workgroup_span(ws, slots);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[i] += x[e] * g[e];
-    }
+    for (int s = 0; s < KS; ++s) bad |= any_nonfinite(__builtin_bit_cast(uint4, gf[s]));
+    bad |= __shfl_xor((int)bad, 32, kWave) != 0;
+    const bool empty = x == kNegInf;
+    const float lse2 = empty ? __builtin_inff() : bad ? __builtin_nanf("") : x * kLog2e;
+    const bool note = __any(my_q < S && (bad || !(__builtin_fabsf(x) < __builtin_inff())));
+
+    float delta = 0.f;
+    if (wg.hi - wg.lo > kExactKeys) {  // alike in every wave
+        const __amdgpu_buffer_rsrc_t ro = make_rsrc(o + ((int64_t)b * S * a.H + h) * D, (S * a.H - h) * D * 2);
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+        for (int s = 0; s < KS; ++s) {
+            float u[8], g[8];
+            BVec<uint16_t>::unpack(
+                buf_load16(ro, my_q < S ? (uint32_t)((my_q * ldo + 16 * s + 8 * half) * 2) : kOOB), u);
+            BVec<uint16_t>::unpack(__builtin_bit_cast(i32x4, gf[s]), g);
 #pragma unroll
-        for (int m = 1; m < CPR; m <<= 1) {
-            acc[i] += __shfl_xor(acc[i], m, kWave);
-            bad[i] |= __shfl_xor(bad[i], m, kWave);
+            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(u[e], g[e], delta);
         }
-    bool note = false;
-    if (ch == 0) {
-        float* blk = lsd + (bh * (Sp / 64) + blockIdx.x) * 128;
+    } else if (wg.lo < wg.hi) {
+        const __amdgpu_buffer_rsrc_t rq = make_rsrc(a.q + (int64_t)bh * S * D, S * D * 2);
+        bf16x8 qf[KS];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int row = wave * 16 + i * RPI + rsub;
-            float l = __builtin_inff(), delta = 0.f;  // queries past S: P = 0
-            if (q0 + row < S) {
-                const float x = lse[bh * S + q0 + row];
-                const bool empty = x == kNegInf;
-                note |= bad[i] || !(__builtin_fabsf(x) < __builtin_inff());
-                l = empty ? __builtin_inff() : bad[i] ? __builtin_nanf("") : x * kLog2e;
-                delta = empty ? 0.f : acc[i];
+        for (int s = 0; s < KS; ++s)
+            qf[s] = __builtin_bit_cast(
+                bf16x8, buf_load16(rq, my_q < S ? (uint32_t)((my_q * D + 16 * s + 8 * half) * 2) : kOOB));
+        const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+        uint32_t roff[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) roff[s] = rows_off<D>(lane, 2 * s + half);
+        const i32x4 rk = rsrc_words(a.k + bhk * S * D, S * D * 2);
+        const i32x4 rv = rsrc_words(a.v + bhk * S * D, S * D * 2);
+        auto issue = [&](int kb, int stage) {
+            const uint32_t base = smem_byte + (uint32_t)(stage * STAGE * 2);
+            dma_rows<D>(rk, base, (uint32_t)kb * KB, D, wave, lane);
+            dma_rows<D>(rv, base + TILE * 2, (uint32_t)kb * KB, D, wave, lane);
+        };
+        const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
+        issue(kb0, 0);
+        for (int kb = kb0; kb < kb1; ++kb) {
+            wait_vmcnt<0>();
+            __syncthreads();
+            if (kb + 1 < kb1) issue(kb + 1, (kb + 1 - kb0) & 1);
+            const int key0 = kb * KB;
+            if (key0 >= ws.hi || key0 + KB <= ws.lo) continue;  // wave-uniform: no query of this wave sees the block
+            const uint16_t* sk = smem + ((kb - kb0) & 1) * STAGE;
+            const uint16_t* sv = sk + TILE;
+            const bool edge = !(key0 >= ws.all_lo && key0 + KB <= ws.all_hi);
+            const float dist = (float)((int)my_q - key0 - 4 * half);
+            const int lo = mine.lo - key0 - 4 * half;
+            const uint32_t width = (uint32_t)(mine.hi - mine.lo);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                f32x16 sacc, dpacc;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sacc[j] = dpacc[j] = 0.f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_at(sk + 32 * t * D, roff[s]), qf[s], sacc, 0, 0, 0);
+                    dpacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_at(sv + 32 * t * D, roff[s]), gf[s], dpacc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int ko = 32 * t + 8 * (j >> 2) + (j & 3);
+                    float y = score_log2<CAP>(sacc[j], a);
+                    if constexpr (BIAS) y = __builtin_fmaf(__builtin_fabsf(dist - (float)ko), -slope2, y);
+                    dpacc[j] *= exp2_hw(y - lse2);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if ((uint32_t)(32 * t + 8 * (j >> 2) + (j & 3) - lo) >= width) dpacc[j] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) delta += dpacc[j];
             }
-            blk[row] = l;
-            blk[64 + row] = delta;
         }
+        wait_vmcnt<0>();
     }
-    note = __syncthreads_or(note);
-    if (threadIdx.x == 0) flags[bh * (Sp / 64) + blockIdx.x] = note;
+    delta += __shfl_xor(delta, 32, kWave);
+    // queries past S have lse = +inf too
+    if (half == 0 && my_q < a.Sp) {
+        float* blk = lsd + ((int64_t)bh * (a.Sp / 64) + my_q / 64) * 128 + my_q % 64;
+        blk[0] = lse2;
+        blk[64] = empty ? 0.f : delta;
+    }
+    if (lane == 0) noted[wave] = note;
+    __syncthreads();
+    const int64_t blk = (int64_t)qb * 2 + threadIdx.x;
+    if (threadIdx.x < 2 && blk < a.Sp / 64)
+        flags[(int64_t)bh * (a.Sp / 64) + blk] = noted[2 * threadIdx.x] | noted[2 * threadIdx.x + 1];
 }
 
 // ------------------------------------------------------------ dK and dV
@@ -749,7 +841,8 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
             constexpr bool EDGE = decltype(edge_tag)::value;
             constexpr int t = decltype(t_tag)::value;
             // the lane's 4 half moves to the bounds, so each test compares a constant
-            const int lo = mine.lo - q0 - 4 * half, hi = mine.hi - q0 - 4 * half;
+            const int lo = mine.lo - q0 - 4 * half;
+            const uint32_t width = (uint32_t)(mine.hi - mine.lo);
             const float dist = (float)(q0 + 4 * half - (int)my_key);
             float p[16], ds[16];
 #pragma unroll
@@ -774,7 +867,7 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
                     if constexpr (CAP) dj *= slope;
                     dj *= pj;
                     if constexpr (EDGE) {
-                        const bool hidden = off < lo || off >= hi;
+                        const bool hidden = (uint32_t)(off - lo) >= width;
                         pj = hidden ? 0.f : pj;
                         dj = hidden ? 0.f : dj;  // not 0 * dj: dP of a hidden pair may be anything
                     }
@@ -1254,13 +1347,12 @@ hipError_t launch_packed_bwd(const mc_packed_attn_desc& p, const void* q, const 
     a.ldst = (int64_t)a.nblk * 128;
     a.dq_blocks = (int64_t)a.nblk * a.B * a.H;
     a.sum_n8 = (int64_t)a.B * a.Hkv * a.S * a.D / 8;
-    const uint16_t* o16 = static_cast<const uint16_t*>(o);
-    const dim3 gprep((unsigned)(a.Sp / 64), (unsigned)(a.B * a.H));
+    const dim3 gprep((unsigned)((int64_t)a.nblk * a.B * a.H));
     const dim3 gkv((unsigned)((int64_t)a.nblk * a.B * a.Hkv * a.ngroups));
     by_variant(a.D, p.cap != 0.f, slopes != nullptr, [&](auto dim, auto cap, auto bias) {
         constexpr int D = decltype(dim)::value;
         constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
-        packed_prep<D><<<gprep, 256, 0, stream>>>(o16, a.dout, lse, a.H, a.S, a.Sp, lsd, qflags);
+        packed_prep<D, CAP, BIAS><<<gprep, 256, 0, stream>>>(a, static_cast<const uint16_t*>(o), lse, lsd, qflags);
         packed_dkdv<D, CAP, BIAS><<<gkv, 256, 0, stream>>>(a);
         if (from_ds) {
             // with partials, the dQ launch also sums them (see attn_bwd_dq_ds_bf16)

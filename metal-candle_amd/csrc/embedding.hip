@@ -164,53 +164,81 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
     }
 }
 
-// The columns of a wave: 4 per lane from d, one where VEC is 1 (then 64 apart).
+// The columns of a wave: 4 per lane from d (which may lie past the row), row by
+// row through buffer loads, whose range check drops the lanes past the row: no
+// branch stands between the loads of several rows. Rows of float32 start at any
+// 4 bytes, which a 16-byte buffer access takes; a row that is not whole 16-byte
+// vectors keeps its last columns in `rest`, one per lane.
 constexpr int kSlab = 256;
+struct Columns {
+    int d;        // this lane's first column
+    int rest;     // its column of the row's last dim % 4, or -1
+};
+__device__ __forceinline__ Columns columns_of(int64_t slab, int64_t dim) {
+    const int64_t d0 = slab * kSlab;
+    const int whole = (int)(dim & ~(int64_t)3), lane = lane_id();
+    const bool last = d0 + kSlab >= whole;  // of slabs_of(dim) (dim < 2^29)
+    return Columns{(int)d0 + 4 * lane, last && whole + lane < dim ? whole + lane : -1};
+}
+__host__ __device__ inline int64_t slabs_of(int64_t dim) { return dim < 4 ? 1 : ((dim & ~(int64_t)3) + kSlab - 1) / kSlab; }
+struct Sum {
+    float v[4], rest;
+};
+// 4 floats of a row at column c.d and the rest's; zeros past the row.
 template <typename T, int VEC>
-__device__ __forceinline__ void add_row(const T* row, int64_t d, int64_t dim, float (&acc)[4]) {
-    if constexpr (VEC == 4) {
-        if (d < dim) {
-            float v[4];
-            load_vec<T, 4>(row + d, v);
+__device__ __forceinline__ Sum load_row(const T* row, const Columns& c, int dim) {
+    Sum s;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(row, (int64_t)dim * (int)sizeof(T));
+    const uint32_t off = c.d + 4 <= dim ? (uint32_t)c.d * (uint32_t)sizeof(T) : kOOB;
+    if constexpr (sizeof(T) == 4) {
+        const i32x4 q = buf_load16(r, off);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] += v[e];
-        }
-    } else {
+        for (int e = 0; e < 4; ++e) s.v[e] = __int_as_float(q[e]);
+        s.rest = VEC == 4 ? 0.f
+                          : __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, c.rest >= 0 ? 4 * c.rest : (int)kOOB, 0, 0));
+    } else if constexpr (VEC == 4) {
+        const u32x2 q = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+        s.v[0] = bf16_lo(q[0]); s.v[1] = bf16_hi(q[0]); s.v[2] = bf16_lo(q[1]); s.v[3] = bf16_hi(q[1]);
+        s.rest = 0.f;
+    } else {  // rows of bf16 that start at any 2 bytes: one element at a time
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (d + e * kWave < dim) acc[e] += Elem<T>::load(row, d + e * kWave);
+            s.v[e] = bf16_to_f32((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                r, (int)(off == kOOB ? kOOB : off + 2u * (uint32_t)e), 0, 0));
+        s.rest = bf16_to_f32((uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, c.rest >= 0 ? 2 * c.rest : (int)kOOB, 0, 0));
     }
+    return s;
 }
 template <int VEC>
-__device__ __forceinline__ void put_row(float* row, int64_t d, int64_t dim, const float (&v)[4]) {
-    if constexpr (VEC == 4) {
-        if (d < dim) Vec16<float>::store(row + d, v);
-    } else {
+__device__ __forceinline__ void store_row(float* row, const Columns& c, int dim, const Sum& s) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(row, (int64_t)dim * 4);
+    const i32x4 q = {__float_as_int(s.v[0]), __float_as_int(s.v[1]), __float_as_int(s.v[2]), __float_as_int(s.v[3])};
+    __builtin_amdgcn_raw_buffer_store_b128(q, r, (int)(c.d + 4 <= dim ? (uint32_t)c.d * 4u : kOOB), 0, 0);
+    if constexpr (VEC != 4)
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(s.rest), r, c.rest >= 0 ? 4 * c.rest : (int)kOOB, 0, 0);
+}
+__device__ __forceinline__ void add(Sum& x, const Sum& y) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (d + e * kWave < dim) row[d + e * kWave] = v[e];
-    }
+    for (int e = 0; e < 4; ++e) x.v[e] += y.v[e];
+    x.rest += y.rest;
 }
 
 // acc += dout of sorted tokens [from, to), eight rows in flight.
 template <typename T, int VEC>
 __device__ __forceinline__ void add_run(const T* __restrict__ dout, const int32_t* __restrict__ order, int32_t from,
-                                        int32_t to, int64_t d, int64_t dim, float (&acc)[4]) {
+                                        int32_t to, const Columns& c, int dim, Sum& acc) {
     constexpr int U = 8;
     for (; from + U <= to; from += U) {
-        float part[U][4];
+        Sum part[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < U; ++u) part[u] = load_row<T, VEC>(dout + (int64_t)order[from + u] * dim, c, dim);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) part[u][e] = 0.f;
-            add_row<T, VEC>(dout + (int64_t)order[from + u] * dim, d, dim, part[u]);
-        }
+        for (int s = 1; s < U; s *= 2)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            acc[e] += ((part[0][e] + part[1][e]) + (part[2][e] + part[3][e])) +
-                      ((part[4][e] + part[5][e]) + (part[6][e] + part[7][e]));
+            for (int u = 0; u < U; u += 2 * s) add(part[u], part[u + s]);
+        add(acc, part[0]);
     }
-    for (; from < to; ++from) add_row<T, VEC>(dout + (int64_t)order[from] * dim, d, dim, acc);
+    for (; from < to; ++from) add(acc, load_row<T, VEC>(dout + (int64_t)order[from] * dim, c, dim));
 }
 
 // part[c][0]: the sum over unit c of the sorted tokens of the run that goes on
@@ -220,15 +248,15 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_long(const T* __restrict__ dout, const int32_t* __restrict__ ids,
                                                   const int32_t* __restrict__ order,
                                                   const int32_t* __restrict__ start, float* __restrict__ part,
-                                                  int64_t vocab, int64_t dim, int32_t unit) {
-    const int64_t slabs = (dim + kSlab - 1) / kSlab;
+                                                  int64_t vocab, int dim, int32_t unit) {
+    const int64_t slabs = slabs_of(dim);
     const int64_t job = (int64_t)blockIdx.x * 4 + wave_id();
-    const int64_t c = job / slabs, d0 = job % slabs * kSlab;
+    const int64_t c = job / slabs;
     const int32_t n = start[vocab];
     const int64_t from = c * unit;
     if (from >= n) return;
     const int32_t to = (int32_t)(from + unit < n ? from + unit : n);
-    const int64_t d = d0 + (VEC == 4 ? 4 * lane_id() : lane_id());
+    const Columns cols = columns_of(job % slabs, dim);
     int32_t id = ids[order[from]];
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
@@ -239,10 +267,10 @@ __global__ __launch_bounds__(256) void embed_long(const T* __restrict__ dout, co
         }
         const int32_t a = start[id], b = start[id + 1];
         if (b - a <= 2 * unit) continue;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        add_run<T, VEC>(dout, order, a > from ? a : (int32_t)from, b < to ? b : to, d, dim, acc);
+        Sum acc{};
+        add_run<T, VEC>(dout, order, a > from ? a : (int32_t)from, b < to ? b : to, cols, dim, acc);
         // a run that starts with the unit goes on through its start as well
-        put_row<VEC>(part + (2 * c + (a > from)) * dim, d, dim, acc);
+        store_row<VEC>(part + (2 * c + (a > from)) * dim, cols, dim, acc);
     }
 }
 
@@ -251,35 +279,31 @@ constexpr int kRows = 8;  // ids per workgroup of embed_grad
 template <typename T, int VEC, bool ADD>
 __global__ __launch_bounds__(256) void embed_grad(const T* __restrict__ dout, const int32_t* __restrict__ order,
                                                   const int32_t* __restrict__ start, const float* __restrict__ part,
-                                                  float* __restrict__ dtable, int64_t vocab, int64_t dim, float scale,
+                                                  float* __restrict__ dtable, int64_t vocab, int dim, float scale,
                                                   int32_t unit) {
     const int64_t v0 = (int64_t)blockIdx.x * kRows;
-    const int slabs = (int)((dim + kSlab - 1) / kSlab);
+    const int slabs = (int)slabs_of(dim);
     const int rows = (int)(vocab - v0 < kRows ? vocab - v0 : kRows);
     for (int job = wave_id(); job < rows * slabs; job += 4) {
         const int64_t v = v0 + job / slabs;
-        const int64_t d = (int64_t)(job % slabs) * kSlab + (VEC == 4 ? 4 * lane_id() : lane_id());
+        const Columns cols = columns_of(job % slabs, dim);
         const int32_t a = start[v], b = start[v + 1];
         if (ADD && a == b) continue;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        Sum acc{};
         if (b - a <= 2 * unit) {
-            add_run<T, VEC>(dout, order, a, b, d, dim, acc);
+            add_run<T, VEC>(dout, order, a, b, cols, dim, acc);
         } else {
             const int32_t c1 = (b - 1) / unit;
             for (int32_t c = a / unit; c <= c1; ++c)
-                add_row<float, VEC>(part + (2 * (int64_t)c + (a > (int64_t)c * unit)) * dim, d, dim, acc);
+                add(acc, load_row<float, VEC>(part + (2 * (int64_t)c + (a > (int64_t)c * unit)) * dim, cols, dim));
         }
         float* row = dtable + v * dim;
-        if constexpr (ADD) {
-            float old[4] = {0.f, 0.f, 0.f, 0.f};
-            add_row<float, VEC>(row, d, dim, old);
+        Sum old{};
+        if constexpr (ADD) old = load_row<float, VEC>(row, cols, dim);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(acc[e], scale, old[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] *= scale;
-        }
-        put_row<VEC>(row, d, dim, acc);
+        for (int e = 0; e < 4; ++e) acc.v[e] = __builtin_fmaf(acc.v[e], scale, old.v[e]);
+        acc.rest = __builtin_fmaf(acc.rest, scale, old.rest);
+        store_row<VEC>(row, cols, dim, acc);
     }
 }
 
@@ -336,7 +360,7 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
     const int32_t unit = unit_of(d.tokens);
     embed_sort<<<dim3((unsigned)((d.vocab + kIds - 1) / kIds)), kSortThreads, 0, stream>>>(
         ids, (int32_t)d.tokens, d.vocab, d.padding_id, order, start);
-    const int64_t slabs = (d.dim + kSlab - 1) / kSlab;
+    const int64_t slabs = slabs_of(d.dim);
     const dim3 glong((unsigned)(((d.tokens + unit - 1) / unit * slabs + 3) / 4));
     const dim3 ggrad((unsigned)((d.vocab + kRows - 1) / kRows));
     auto go = [&](auto elem, auto vec) {
@@ -344,12 +368,12 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
         constexpr int VEC = decltype(vec)::value;
         const T* g = static_cast<const T*>(dout);
         if (d.tokens > 2 * unit)
-            embed_long<T, VEC><<<glong, 256, 0, stream>>>(g, ids, order, start, part, d.vocab, d.dim, unit);
+            embed_long<T, VEC><<<glong, 256, 0, stream>>>(g, ids, order, start, part, d.vocab, (int)d.dim, unit);
         if (accumulate)
-            embed_grad<T, VEC, true><<<ggrad, 256, 0, stream>>>(g, order, start, part, dtable, d.vocab, d.dim,
+            embed_grad<T, VEC, true><<<ggrad, 256, 0, stream>>>(g, order, start, part, dtable, d.vocab, (int)d.dim,
                                                                 d.scale, unit);
         else
-            embed_grad<T, VEC, false><<<ggrad, 256, 0, stream>>>(g, order, start, part, dtable, d.vocab, d.dim,
+            embed_grad<T, VEC, false><<<ggrad, 256, 0, stream>>>(g, order, start, part, dtable, d.vocab, (int)d.dim,
                                                                  d.scale, unit);
     };
     if (d.dtype == MC_F32) {

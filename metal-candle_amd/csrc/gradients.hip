@@ -64,7 +64,7 @@ __device__ __forceinline__ int slot_of(const Batch& b, int blk) {
 
 template <typename T>
 __device__ __forceinline__ double sumsq_range(const T* __restrict__ p, int64_t n) {
-    constexpr int N = Vec<T>::N, U = 4;
+    constexpr int N = Vec<T>::N, U = 8;
     // elements before the first 16-byte boundary, then whole vectors, then the rest
     const int64_t mis = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
     const int64_t head = mis < n ? mis : n;
@@ -208,9 +208,11 @@ __global__ __launch_bounds__(kThreads) void grad_scale(GradScaleBatch b, const f
         f = *given;
     }
     if (b.count == 0) return;
-    const GradScaleSlot& t = b.slot[slot_of(b, (int)blockIdx.x)];
+    // backwards: the norm has left the last gradients that it read in the last-level cache
+    const int blk = (int)(gridDim.x - 1 - blockIdx.x);
+    const GradScaleSlot& t = b.slot[slot_of(b, blk)];
     if (f == 1.f && t.g == t.out) return;  // in place and nothing to clip
-    const int64_t base = (int64_t)((int)blockIdx.x - t.blk0) * b.chunk;
+    const int64_t base = (int64_t)(blk - t.blk0) * b.chunk;
     const int64_t n = t.n - base < b.chunk ? t.n - base : b.chunk;
     if (t.dtype == MC_F32) {
         const float* g = static_cast<const float*>(t.g) + base;

@@ -10,6 +10,7 @@ stream of the tensors' device and does not synchronise.
 import array
 import ctypes
 import itertools
+import operator
 
 import torch
 
@@ -18,6 +19,7 @@ from ._lib import (AdamWConfig, AdamWTensor, AttnDesc, DistillDesc, EmbeddingDes
                    McError, PackedAttnDesc, PolicyDesc, PreferenceDesc, XentDesc, check, lib)
 
 _DTYPES = {torch.float32: _lib.MC_F32, torch.bfloat16: _lib.MC_BF16}
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
 def _ptr(t):
@@ -914,21 +916,22 @@ def _tensors(group, name):
         raise McError(_lib.MC_ERR_NULL, f"{name} must hold tensors only")
     if not whole:
         raise McError(_lib.MC_ERR_LAYOUT, f"every tensor of {name} must be contiguous")
-    dtypes = [t.dtype for t in group]
-    devices = {t.device for t in group}
-    if len(devices) > 1:
-        raise McError(_lib.MC_ERR_LAYOUT, f"{name} are on {len(devices)} devices, expected one")
+    dtypes = list(map(_DTYPE_OF, group))
     for dtype in set(dtypes):
         if dtype not in _DTYPES:
             raise McError(_lib.MC_ERR_DTYPE, f"unsupported dtype {dtype} in {name} (float32 or bfloat16)")
-    return dtypes, list(map(torch.Tensor.numel, group)), list(map(torch.Tensor.data_ptr, group)), devices.pop()
+    indices = set(map(torch.Tensor.get_device, group))
+    if len(indices) > 1 or -1 in indices:  # the device objects take twice the time
+        devices = {t.device for t in group}
+        if len(devices) > 1:
+            raise McError(_lib.MC_ERR_LAYOUT, f"{name} are on {len(devices)} devices, expected one")
+    return dtypes, list(map(torch.Tensor.numel, group)), list(map(torch.Tensor.data_ptr, group)), group[0].device
 
 
 def _grad_table(grads, outs):
     """(address of the mc_grad_tensor table, its length, what keeps it alive) of gradients and where they go."""
     dtypes, sizes, at, device = _tensors(grads, "grads")
-    codes = [_DTYPES[t] for t in dtypes] if len(set(dtypes)) > 1 else [_DTYPES[dtypes[0]]] * len(dtypes)
-    to = at
+    to, out_dtypes = at, dtypes
     if outs is not None and outs is not grads:
         if len(outs) != len(grads):
             raise McError(_lib.MC_ERR_SHAPE, f"outs list has {len(outs)} entries, expected {len(grads)}")
@@ -938,9 +941,10 @@ def _grad_table(grads, outs):
             raise McError(_lib.MC_ERR_SHAPE, f"outs[{i}] has {out_sizes[i]} elements, expected {sizes[i]}")
         if out_device != device:
             raise McError(_lib.MC_ERR_LAYOUT, f"outs are on {out_device}, expected {device}")
-        codes = [c | _DTYPES[t] << 32 for c, t in zip(codes, out_dtypes)]
+    if len(set(dtypes)) == 1 and len(set(out_dtypes)) == 1:
+        codes = itertools.repeat(_DTYPES[dtypes[0]] | _DTYPES[out_dtypes[0]] << 32)
     else:
-        codes = [c | c << 32 for c in codes]
+        codes = [_DTYPES[a] | _DTYPES[b] << 32 for a, b in zip(dtypes, out_dtypes)]
     table = array.array("Q", itertools.chain.from_iterable(zip(at, to, sizes, codes)))
     return table.buffer_info()[0], len(sizes), table
 

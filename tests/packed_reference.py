@@ -12,7 +12,8 @@ their size; tanh to a few u, times the cap), so a probability by 2 d of its valu
   o    (r + p) sum_j P |v| + e |o|
   dv   (r + p) sum_i P |do| + e |dv|
   dS   (r + p) |dS| + P s (Eo |do| + r |do| |v| + 8 u (|dP| + |Delta|)), s the cap's
-       slope (<= 1, itself off by 8 u), Eo the bound of o, from which Delta is formed
+       slope (<= 1, itself off by 8 u), Eo the bound of o, from which Delta is formed;
+       where Delta is formed from P and dP (exact), r sum_j P |dP| in place of Eo |do|
   dq   scale (sum_j E_dS |k| + (S + D) u sum_j |dS| |k|) + e |dq|, dk alike over the
        queries, summed over the heads that share the key
 """
@@ -57,7 +58,7 @@ def spans_of(see):
     return out
 
 
-def attention(q, k, v, see, scale, cap=None, slopes=None, dout=None):
+def attention(q, k, v, see, scale, cap=None, slopes=None, dout=None, exact=False):
     """{name: (value, bound)} of o, lse and, with dout, dq, dk, dv; see [B, S, S] truth values."""
     B, H, S, D = q.shape
     Hkv = k.shape[1]
@@ -101,8 +102,8 @@ def attention(q, k, v, see, scale, cap=None, slopes=None, dout=None):
             G = torch.where(row[:, None], dout.view(B, S, H, D)[b, :, h].double(), 0.0)
             dP, delta = G @ V.t(), (G * O).sum(-1, keepdim=True)
             dS = p * (dP - delta) * s
-            EdS = (r + pr) * dS.abs() + p * s * ((Eo[b, :, h] * G.abs()).sum(-1, keepdim=True)
-                                                 + r * (G.abs() @ V.abs().t()))
+            off = r * (p * dP.abs()).sum(-1) if exact else (Eo[b, :, h] * G.abs()).sum(-1)
+            EdS = (r + pr) * dS.abs() + p * s * (off[:, None] + r * (G.abs() @ V.abs().t()))
             EdS = EdS + 8 * U * p * (dP.abs() + delta.abs())
             dq[b, h] = scale * (dS @ K)
             Eq[b, h] = scale * ((EdS + (S + D) * U * dS.abs()) @ K.abs()) + e * dq[b, h].abs()

@@ -49,94 +49,100 @@ using namespace attn;
 // 0 are padding. Two scans over the row, kItems tokens per thread and turn: from
 // the end, where each token's document ends, and the first token from it on that
 // is no prompt; from the start, where each document begins and where its prompt
-// ends. Latency is all there is: 16 KB of ids.
+// ends. Latency is all there is (8 KB of ids at 2048 tokens), so a row of one
+// turn stays in registers between the two.
 constexpr int kScanThreads = 1024, kScanWaves = kScanThreads / kWave, kItems = 4;
 constexpr int kScanTurn = kScanThreads * kItems;  // tokens per turn
 
-// The latest mark (>= 0; -1: none) of the threads before this one, or the carry
-// where they have none; the carry becomes the latest of all. `slots` must not be
-// the array of the call before.
-__device__ __forceinline__ int last_before(int mark, int& carry, int* slots) {
+// The latest mark (>= 0; -1: none) of the threads before this one (AFTER: the
+// first of those behind it), or the carry where they have none; the carry becomes
+// the last (first) of all. `slots` must not be the array of the call before.
+template <bool AFTER>
+__device__ __forceinline__ int nearest_mark(int mark, int& carry, int* slots) {
     const int lane = lane_id(), wave = wave_id();
+    auto from = [&](int v, int s) { return AFTER ? __shfl_down(v, s, kWave) : __shfl_up(v, s, kWave); };
     int m = mark;
 #pragma unroll
     for (int s = 1; s < kWave; s <<= 1) {
-        const int up = __shfl_up(m, s, kWave);
-        if (lane >= s && m < 0) m = up;
+        const int x = from(m, s);
+        m = m < 0 && (AFTER ? lane + s < kWave : lane >= s) ? x : m;
     }
-    if (lane == kWave - 1) slots[wave] = m;
+    if (lane == (AFTER ? 0 : kWave - 1)) slots[wave] = m;
     __syncthreads();
-    int before = __shfl_up(m, 1, kWave), earlier = carry;
+    int near = from(m, 1), other = carry;
 #pragma unroll
-    for (int w = 0; w < kScanWaves; ++w) {
-        const int x = slots[w];
-        if (x < 0) continue;
-        if (w < wave) earlier = x;
-        carry = x;
+    for (int i = 0; i < kScanWaves; ++i) {
+        const int w = AFTER ? kScanWaves - 1 - i : i, x = slots[w];
+        other = x >= 0 && (AFTER ? w > wave : w < wave) ? x : other;
+        carry = x >= 0 ? x : carry;
     }
-    return lane > 0 && before >= 0 ? before : earlier;
+    return lane != (AFTER ? kWave - 1 : 0) && near >= 0 ? near : other;
 }
 
 __global__ __launch_bounds__(kScanThreads) void packed_spans(const int32_t* __restrict__ documents,
                                                              const uint8_t* __restrict__ prefix, int S, int causal,
-                                                             int4* spans) {
+                                                             int4* __restrict__ spans) {
     __shared__ int slots[2][2][kScanWaves];
     const int64_t row = (int64_t)blockIdx.x * S;
     const int32_t* id = documents ? documents + row : nullptr;
     const uint8_t* pre = prefix ? prefix + row : nullptr;
     int4* out = spans + row;
     const int turns = (int)(((int64_t)S + kScanTurn - 1) / kScanTurn);
-    // a token's id (0 without documents) and whether it is marked as prompt; t is brought inside the row
+    // a token's id (0 without documents), t brought inside the row
     auto id_at = [&](int64_t t) { return id ? id[t < 0 ? 0 : t >= S ? S - 1 : t] : 0; };
-    auto prompt_at = [&](int64_t t) { return pre ? pre[t < 0 ? 0 : t >= S ? S - 1 : t] != 0 : false; };
-    // Backwards, item i at token S - 1 - i: a mark is seen by the items behind it.
-    int end_carry = S, stop_carry = S;
-    for (int turn = 0; turn < turns; ++turn) {
-        const int64_t i0 = (int64_t)turn * kScanTurn + (int64_t)threadIdx.x * kItems;
-        int ids[kItems + 1], end[kItems], stop[kItems], end_last = -1, stop_last = -1;
+    // this thread's tokens t0 .. t0 + kItems - 1 of a turn: ids[e + 1] is that of t0 + e
+    int ids[kItems + 2], end[kItems], stop[kItems];
+    int end_carry = S, stop_carry = S, k = 0;
+    for (int turn = turns - 1; turn >= 0; --turn, ++k) {
+        const int64_t t0 = (int64_t)turn * kScanTurn + (int64_t)threadIdx.x * kItems;
 #pragma unroll
-        for (int e = 0; e <= kItems; ++e) ids[e] = id_at(S - i0 - e);  // ids[e + 1]: of item e
+        for (int e = 0; e < kItems + 2; ++e) ids[e] = id_at(t0 + e - 1);
+        int first_end = -1, first_stop = -1;
 #pragma unroll
-        for (int e = 0; e < kItems; ++e) {
-            const int64_t i = i0 + e;
-            const int t = S - 1 - (int)(i < S ? i : S - 1);
-            const bool last = i == 0 || ids[e] != ids[e + 1];  // of its document
-            end[e] = i < S && last ? t + 1 : -1;
-            stop[e] = i < S && !prompt_at(t) ? t : end[e];
-            end_last = end[e] >= 0 ? end[e] : end_last;
-            stop_last = stop[e] >= 0 ? stop[e] : stop_last;
+        for (int e = kItems - 1; e >= 0; --e) {
+            const int64_t t = t0 + e;
+            const bool in = t < S, marked = pre ? pre[in ? t : S - 1] != 0 : false;
+            const bool last = t == S - 1 || ids[e + 1] != ids[e + 2];  // of its document
+            end[e] = in && last ? (int)t + 1 : -1;
+            stop[e] = in && !marked ? (int)t : end[e];
+            first_end = end[e] >= 0 ? end[e] : first_end;
+            first_stop = stop[e] >= 0 ? stop[e] : first_stop;
         }
-        int end_in = last_before(end_last, end_carry, slots[turn & 1][0]);
-        int stop_in = pre ? last_before(stop_last, stop_carry, slots[turn & 1][1]) : 0;
+        int end_in = nearest_mark<true>(first_end, end_carry, slots[k & 1][0]);
+        int stop_in = pre ? nearest_mark<true>(first_stop, stop_carry, slots[k & 1][1]) : 0;
 #pragma unroll
-        for (int e = 0; e < kItems; ++e) {
-            end_in = end[e] >= 0 ? end[e] : end_in;
-            stop_in = stop[e] >= 0 ? stop[e] : stop_in;
-            if (i0 + e < S) out[S - 1 - (i0 + e)] = make_int4(0, end_in, stop_in, 0);
+        for (int e = kItems - 1; e >= 0; --e) {
+            end[e] = end_in = end[e] >= 0 ? end[e] : end_in;
+            stop[e] = stop_in = stop[e] >= 0 ? stop[e] : stop_in;
+            // a row of several turns keeps them in its spans; the same thread reads them again
+            if (turns > 1 && t0 + e < S) out[t0 + e] = make_int4(0, end[e], stop[e], 0);
         }
     }
-    __syncthreads();  // out is read by other threads than wrote it
     int begin_carry = 0, prompt_carry = 0;
-    for (int turn = 0; turn < turns; ++turn) {
+    for (int turn = 0; turn < turns; ++turn, ++k) {
         const int64_t t0 = (int64_t)turn * kScanTurn + (int64_t)threadIdx.x * kItems;
-        int ids[kItems + 1], begin[kItems], prompt[kItems], end[kItems], begin_last = -1, prompt_last = -1;
+        if (turns > 1) {
 #pragma unroll
-        for (int e = 0; e <= kItems; ++e) ids[e] = id_at(t0 + e - 1);  // ids[e + 1]: of token t0 + e
+            for (int e = 0; e < kItems + 2; ++e) ids[e] = id_at(t0 + e - 1);
+#pragma unroll
+            for (int e = 0; e < kItems; ++e) {
+                const int4 x = t0 + e < S ? out[t0 + e] : make_int4(0, 0, 0, 0);
+                end[e] = x.y;
+                stop[e] = x.z;
+            }
+        }
+        int begin[kItems], prompt[kItems], last_begin = -1, last_prompt = -1;
 #pragma unroll
         for (int e = 0; e < kItems; ++e) {
             const int64_t t = t0 + e;
-            const int4 x = out[t < S ? t : S - 1];
             const bool first = t < S && (t == 0 || ids[e] != ids[e + 1]);
-            end[e] = x.y;
             begin[e] = first ? (int)t : -1;
-            prompt[e] = first ? x.z : -1;
-            begin_last = first ? begin[e] : begin_last;
-            prompt_last = first ? prompt[e] : prompt_last;
+            prompt[e] = first ? stop[e] : -1;
+            last_begin = first ? begin[e] : last_begin;
+            last_prompt = first ? prompt[e] : last_prompt;
         }
-        int begin_in = last_before(begin_last, begin_carry, slots[turn & 1][0]);
-        int prompt_in = pre ? last_before(prompt_last, prompt_carry, slots[turn & 1][1]) : 0;
-        // (each thread rewrites only what it has read itself, and another's clamped read of
-        // token S - 1 is not used)
+        int begin_in = nearest_mark<false>(last_begin, begin_carry, slots[k & 1][0]);
+        int prompt_in = pre ? nearest_mark<false>(last_prompt, prompt_carry, slots[k & 1][1]) : 0;
 #pragma unroll
         for (int e = 0; e < kItems; ++e) {
             const int t = (int)(t0 + e < S ? t0 + e : S - 1);
@@ -158,22 +164,27 @@ __global__ __launch_bounds__(kScanThreads) void packed_spans(const int32_t* __re
 struct WaveSpan {
     int lo, hi, all_lo, all_hi;
 };
+template <int CTRL>
+__device__ __forceinline__ int dpp_int(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false);
+}
+// The least (greatest) v of a wave half's 32 lanes, in every lane of it: within
+// 16 lanes by DPP as in wave_sum, then the two rows of 16 change places.
+template <bool GREATEST>
+__device__ __forceinline__ int half_extreme(int v) {
+    auto pick = [](int x, int y) { return GREATEST ? (x > y ? x : y) : (x < y ? x : y); };
+    v = pick(v, dpp_int<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = pick(v, dpp_int<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = pick(v, dpp_int<0x141>(v));  // row_half_mirror
+    v = pick(v, dpp_int<0x140>(v));  // row_mirror
+    const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    return pick((int)r[0], (int)r[1]);
+}
 __device__ __forceinline__ WaveSpan wave_span(Span s) {
-    WaveSpan w{s.lo < s.hi ? s.lo : 0x7fffffff, s.hi, s.lo, s.hi};
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        const int a = __shfl_xor(w.lo, m, kWave), b = __shfl_xor(w.hi, m, kWave);
-        const int c = __shfl_xor(w.all_lo, m, kWave), d = __shfl_xor(w.all_hi, m, kWave);
-        w.lo = a < w.lo ? a : w.lo;
-        w.hi = b > w.hi ? b : w.hi;
-        w.all_lo = c > w.all_lo ? c : w.all_lo;
-        w.all_hi = d < w.all_hi ? d : w.all_hi;
-    }
-    w.lo = __builtin_amdgcn_readfirstlane(w.lo);
-    w.hi = __builtin_amdgcn_readfirstlane(w.hi);
-    w.all_lo = __builtin_amdgcn_readfirstlane(w.all_lo);
-    w.all_hi = __builtin_amdgcn_readfirstlane(w.all_hi);
-    return w;
+    return WaveSpan{__builtin_amdgcn_readfirstlane(half_extreme<false>(s.lo < s.hi ? s.lo : 0x7fffffff)),
+                    __builtin_amdgcn_readfirstlane(half_extreme<true>(s.hi)),
+                    __builtin_amdgcn_readfirstlane(half_extreme<true>(s.lo)),
+                    __builtin_amdgcn_readfirstlane(half_extreme<false>(s.hi))};
 }
 // The union over the workgroup's four waves, as [lo, hi), empty as [0, 0).
 __device__ __forceinline__ Span workgroup_span(const WaveSpan& w, int (*slots)[2]) {
@@ -339,15 +350,6 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
     const i32x4 rk = rsrc_words(a.k + bhk * S * D, S * D * 2);
     const i32x4 rv = rsrc_words(a.vt + bhk * D * a.Sp, (int64_t)D * a.Sp * 2);
 
-    // what this lane's query sees, and with it the wave's and the workgroup's blocks of keys
-    const Span mine = query_span(a.spans, b, my_q, (int)S, a.causal);
-    const WaveSpan ws = wave_span(mine);
-    const Span wg = workgroup_span(ws, slots);
-    const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
-    const int wk0 = ws.lo < ws.hi ? ws.lo / KB : 0, wk1 = ws.lo < ws.hi ? (ws.hi + KB - 1) / KB : 0;
-    const bool bad_v = any_flag(a.vflags + bhk * (a.Sp / 64), wk0, wk1);
-    const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
-
     // K rows key0 .. key0+63 into the swizzled [64][D] layout, then V^T rows
     // d = 0 .. D-1 (64 positions each) into [D][64].
     auto issue = [&](int kb, int stage) {
@@ -371,6 +373,19 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
         }
     };
 
+    // Block kd holds this tile's own tokens, which see themselves: its rows are on
+    // the way while the spans are read. The others follow in order.
+    const int kd = 2 * qb;
+    issue(kd, 0);
+    // what this lane's query sees, and with it the wave's and the workgroup's blocks of keys
+    const Span mine = query_span(a.spans, b, my_q, (int)S, a.causal);
+    const WaveSpan ws = wave_span(mine);
+    const Span wg = workgroup_span(ws, slots);
+    const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
+    const int wk0 = ws.lo < ws.hi ? ws.lo / KB : 0, wk1 = ws.lo < ws.hi ? (ws.hi + KB - 1) / KB : 0;
+    const bool bad_v = any_flag(a.vflags + bhk * (a.Sp / 64), wk0, wk1);
+    const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+
     f32x16 oacc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -378,13 +393,16 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
         for (int j = 0; j < 16; ++j) oacc[t][j] = 0.f;
     float m_run = kNegInf, l_run = 0.f;
 
-    if (kb0 < kb1) issue(kb0, 0);
-    for (int kb = kb0; kb < kb1; ++kb) {
+    int kb = kd, next = 0, stage = 0;
+    for (bool more = kb0 < kb1; more; kb = next, stage ^= 1) {
+        next = kb == kd ? kb0 : kb + 1;
+        next += next == kd;
+        more = next < kb1;
         wait_vmcnt<0>();
         __syncthreads();
-        if (kb + 1 < kb1) issue(kb + 1, (kb + 1 - kb0) & 1);
+        if (more) issue(next, stage ^ 1);
         if (kb < wk0 || kb >= wk1) continue;  // wave-uniform: no query of this wave sees the block
-        const uint16_t* sk = smem + ((kb - kb0) & 1) * STAGE;
+        const uint16_t* sk = smem + stage * STAGE;
         const uint16_t* sv = sk + K_ELEMS;
 
         // S^T tiles t = 0, 1 (keys 32 t .. 32 t + 31) x the wave's 32 queries,
@@ -562,6 +580,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
 
     // O^T accumulator j of tile dt is dim 32 dt + 8 (j/4) + 4 half + j%4 of
     // query my_q: through a per-wave LDS patch to 16-byte row stores
+    wait_vmcnt<0>();  // the first DMA has landed also when the loop ran no block
     __syncthreads();
     static_assert(4 * 32 * (D + 8) <= 2 * STAGE, "the patches fit in the stages");
     store_rows<D, uint16_t>(oacc, inv, smem + wave * 32 * (D + 8), a.o + ((int64_t)b * S * a.H + h) * D,
@@ -616,6 +635,13 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
         gf[s] = __builtin_bit_cast(
             bf16x8, buf_load16(rdo, my_q < S ? (uint32_t)((my_q * ldo + 16 * s + 8 * half) * 2) : kOOB));
     const float x = my_q < S ? lse[(int64_t)bh * S + my_q] : kNegInf;
+    const i32x4 rk = rsrc_words(a.k + bhk * S * D, S * D * 2);
+    const i32x4 rv = rsrc_words(a.v + bhk * S * D, S * D * 2);
+    auto issue = [&](int kb, int stage) {
+        const uint32_t base = smem_byte + (uint32_t)(stage * STAGE * 2);
+        dma_rows<D>(rk, base, (uint32_t)kb * KB, D, wave, lane);
+        dma_rows<D>(rv, base + TILE * 2, (uint32_t)kb * KB, D, wave, lane);
+    };
     const Span mine = query_span(a.spans, b, my_q, (int)S, a.causal);
     const WaveSpan ws = wave_span(mine);
     const Span wg = workgroup_span(ws, slots);
@@ -649,13 +675,6 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
         uint32_t roff[KS];
 #pragma unroll
         for (int s = 0; s < KS; ++s) roff[s] = rows_off<D>(lane, 2 * s + half);
-        const i32x4 rk = rsrc_words(a.k + bhk * S * D, S * D * 2);
-        const i32x4 rv = rsrc_words(a.v + bhk * S * D, S * D * 2);
-        auto issue = [&](int kb, int stage) {
-            const uint32_t base = smem_byte + (uint32_t)(stage * STAGE * 2);
-            dma_rows<D>(rk, base, (uint32_t)kb * KB, D, wave, lane);
-            dma_rows<D>(rv, base + TILE * 2, (uint32_t)kb * KB, D, wave, lane);
-        };
         const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
         issue(kb0, 0);
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -761,18 +780,6 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
         dma_rows<D>(rv, kv_byte + 192 * D * 2, (uint32_t)key0 + 64, D, wave, lane);
     }
 
-    // The queries that the workgroup's keys meet, in whole blocks of 128: the dQ
-    // pass reads dS^T by those, and every one that it reads is written here.
-    const Span mine = key_span(a.spans, b, my_key, (int)S, a.causal);
-    const WaveSpan ws = wave_span(mine);
-    const Span wg = workgroup_span(ws, slots);
-    const int nqb = (int)((S + 63) / 64);
-    const int qstart = wg.lo / 128 * 2;
-    int qend = (int)(((int64_t)wg.hi + 127) / 128 * 2);
-    qend = qend < nqb ? qend : nqb;
-    const int nq = qend - qstart;       // query blocks per head
-    const int nit = hpg * nq;           // (head, query block) steps, head-major
-
     // step it of head h, query block qb
     auto issue = [&](int h, int qb, int stage) {
         const int64_t bh = (int64_t)b * a.H + h;
@@ -788,13 +795,33 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
                   lane < 32 ? (uint32_t)(qb * 512 + lane * 16) : kOOB);
     };
 
+    // Block kd holds the queries of the workgroup's own first keys: every head's
+    // steps start there and go round, and the first is on the way while the spans
+    // are read.
+    const int kd = 2 * kb;
+    issue(h0, kd, 0);
+
+    // The queries that the workgroup's keys meet, in whole blocks of 128: the dQ
+    // pass reads dS^T by those, and every one that it reads is written here.
+    const Span mine = key_span(a.spans, b, my_key, (int)S, a.causal);
+    const WaveSpan ws = wave_span(mine);
+    const Span wg = workgroup_span(ws, slots);
+    const int nqb = (int)((S + 63) / 64);
+    int qstart = wg.lo / 128 * 2, qend = (int)(((int64_t)wg.hi + 127) / 128 * 2);
+    if (wg.lo < wg.hi) {  // kd with them, whatever the spans hold
+        qstart = qstart < kd ? qstart : kd;
+        qend = qend > kd ? qend : kd + 1;
+    }
+    qend = qend < nqb ? qend : nqb;
+    const int nq = qend - qstart;       // query blocks per head
+    const int nit = hpg * nq;           // (head, query block) steps, head-major
+
     f32x16 dvacc[DT], dkacc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int j = 0; j < 16; ++j) dvacc[t][j] = dkacc[t][j] = 0.f;
 
-    if (nit > 0) issue(h0, qstart, 0);
     bool bad_q = false;
     for (int h = h0; h < h0 + hpg; ++h)
         bad_q |= any_flag(a.qflags + ((int64_t)b * a.H + h) * (a.Sp / 64), qstart, qend);
@@ -812,12 +839,13 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
     }
     bad_k = __syncthreads_or(bad_k);
     if (threadIdx.x == 0) a.kflags[bhk * a.nblk + kb] = bad_k;  // alike from every group
-    int h = h0, qb = qstart;
+    int h = h0, qb = kd, left = nq;  // of this head
     for (int it = 0; it < nit; ++it) {
         wait_vmcnt<0>();
         __syncthreads();
-        const bool wrap = qb + 1 == qend;
-        const int next_h = wrap ? h + 1 : h, next_qb = wrap ? qstart : qb + 1;
+        const bool wrap = --left == 0;
+        const int next_h = wrap ? h + 1 : h, next_qb = wrap ? kd : qb + 1 == qend ? qstart : qb + 1;
+        left = wrap ? nq : left;
         if (it + 1 < nit) issue(next_h, next_qb, (it + 1) & 1);
         uint16_t* sq = smem + (it & 1) * STAGE;
         uint16_t* sdo = sq + TILE;
@@ -1010,18 +1038,19 @@ __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
     const i32x4 rk = rsrc_words(a.k + bhk * S * D, S * D * 2);
     // dS^T rows of this head from column q0: rows past S fall outside
     const i32x4 rds = rsrc_words(a.dst + (int64_t)bh * S * a.ldst + q0, (S * a.ldst - q0) * 2);
-    const Span mine = query_span(a.spans, b, qw + (lane & 31), (int)S, a.causal);
-    const Span wg = workgroup_span(wave_span(mine), slots);
-    const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
-    const int32_t* kflags = a.kflags + bhk * a.nblk;
-    const bool bad_k = any_flag(kflags, kb0 / 2, (kb1 + 1) / 2);
-
     auto issue = [&](int kb, int stage) {
         const uint32_t base = smem_byte + (uint32_t)(stage * STAGE * 2);
         const uint32_t key0 = (uint32_t)kb * KB;
         dma_rows<D>(rk, base, key0, D, wave, lane);
         dma_rows<QB>(rds, base + KT * 2, key0, (uint32_t)a.ldst, wave, lane);
     };
+    const int kd = 2 * qb;  // the tile's own keys first, on the way while the spans are read
+    issue(kd, 0);
+    const Span mine = query_span(a.spans, b, qw + (lane & 31), (int)S, a.causal);
+    const Span wg = workgroup_span(wave_span(mine), slots);
+    const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
+    const int32_t* kflags = a.kflags + bhk * a.nblk;
+    const bool bad_k = any_flag(kflags, kb0 / 2, (kb1 + 1) / 2);
 
     f32x16 dqacc[DT];
 #pragma unroll
@@ -1029,12 +1058,15 @@ __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) dqacc[t][j] = 0.f;
 
-    if (kb0 < kb1) issue(kb0, 0);
-    for (int kb = kb0; kb < kb1; ++kb) {
+    int kb = kd, next = 0, stage = 0;
+    for (bool more = kb0 < kb1; more; kb = next, stage ^= 1) {
+        next = kb == kd ? kb0 : kb + 1;
+        next += next == kd;
+        more = next < kb1;
         wait_vmcnt<0>();
         __syncthreads();
-        if (kb + 1 < kb1) issue(kb + 1, (kb + 1 - kb0) & 1);
-        uint16_t* sk = smem + ((kb - kb0) & 1) * STAGE;
+        if (more) issue(next, stage ^ 1);
+        uint16_t* sk = smem + stage * STAGE;
         const uint16_t* sds = sk + KT;
         if (bad_k && kflags[kb / 2]) {  // workgroup-uniform
             clear_tile(sk, KT);

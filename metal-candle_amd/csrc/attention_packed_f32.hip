@@ -40,7 +40,7 @@ __device__ __forceinline__ float tanh_f32(float u) {
     p = __builtin_fmaf(p, x, 2.f / 15.f);
     p = __builtin_fmaf(p, x, -1.f / 3.f);
     const float small = __builtin_fmaf(p * x, u, u);
-    const float big = 1.f - 2.f / (exp2_hw(2.f * kLog2e * __builtin_fabsf(u)) + 1.f);
+    const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(exp2_hw(2.f * kLog2e * __builtin_fabsf(u)) + 1.f);
     return __builtin_fabsf(u) < 0.35f ? small : __builtin_copysignf(big, u);
 }
 // The score of a product s at distance far; slope: its derivative by scale s.

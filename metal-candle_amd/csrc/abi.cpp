@@ -808,8 +808,8 @@ static mc_status check_embedding(const char* op, const mc_embedding_desc* d) {
     MC_CHECK(d->tokens >= 1 && d->vocab >= 1 && d->dim >= 1, MC_ERR_SHAPE,
              "%s: tokens, vocab and dim must be >= 1, got %lld, %lld, %lld", op, (long long)d->tokens,
              (long long)d->vocab, (long long)d->dim);
-    MC_CHECK(d->tokens <= 2147483647 - 64 && d->vocab <= 2147483647, MC_ERR_SHAPE,
-             "%s: tokens must stay below 2^31 - 64 and vocab below 2^31, got %lld, %lld", op, (long long)d->tokens,
+    MC_CHECK(d->tokens < (1 << 28) && d->vocab <= 2147483647, MC_ERR_SHAPE,
+             "%s: tokens must stay below 2^28 and vocab below 2^31, got %lld, %lld", op, (long long)d->tokens,
              (long long)d->vocab);
     MC_CHECK((double)d->vocab * (double)d->dim < 1099511627776.0 && (double)d->tokens * (double)d->dim < 1099511627776.0,
              MC_ERR_SHAPE, "%s: vocab * dim and tokens * dim must stay below 2^40", op);
@@ -842,10 +842,10 @@ mc_status mc_embedding_bwd(const mc_embedding_desc* d, const int32_t* ids, const
     if (s != MC_OK) return s;
     MC_CHECK(ids && dout && dtable, MC_ERR_NULL, "embedding backward: ids, dout and dtable must not be NULL");
     MC_CHECK(accumulate == 0 || accumulate == 1, MC_ERR_VALUE, "embedding backward: accumulate must be 0 or 1");
-    // a launch holds at most 2^32 - 1 work-items: 256 per 8 ids, 64 per 256 columns of a unit of 64 tokens or more
-    MC_CHECK(d->vocab <= 134217720 && (double)((d->tokens + 63) / 64 < 1024 ? (d->tokens + 63) / 64 : 1024) *
-                                              (double)((d->dim + 255) / 256) < 6.0e7,
-             MC_ERR_SHAPE, "embedding backward: vocab must be <= 134217720 and dim <= 15000000");
+    // a launch holds at most 2^32 - 1 work-items: 256 per 4 ids, 64 per 256 columns of a unit (at most 1024 of them)
+    MC_CHECK(d->vocab <= 50000000 && d->dim <= 4000000, MC_ERR_SHAPE,
+             "embedding backward: vocab must be <= 50000000 and dim <= 4000000, got %lld, %lld", (long long)d->vocab,
+             (long long)d->dim);
     MC_CHECK(aligned16(dout) && aligned16(dtable), MC_ERR_LAYOUT,
              "embedding backward: dout and dtable must be 16-byte aligned");
     MC_CHECK(reinterpret_cast<uintptr_t>(ids) % 4 == 0, MC_ERR_LAYOUT, "embedding backward: ids must be 4-byte aligned");

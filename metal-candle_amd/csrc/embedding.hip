@@ -17,15 +17,16 @@
 //               tokens. One launch, no waiting between workgroups, no partial
 //               histograms in memory. 16 waves take a 16th of the tokens each, so
 //               that a batch of one repeated token is no slower than another.
-//  embed_long   runs of more than two units of the sorted tokens: the units'
-//               sums to the workspace, so that a frequent token's rows are read
-//               by many CUs.
-//  embed_grad   one wave per (id, slab of 256 columns): zeros, the run's sum, or
-//               the sum of its units', each row written once.
-#include <algorithm>
+//  embed_grad   one wave per (id, slab of 256 columns): zeros or the run's sum. Of
+//               runs longer than two units of the sorted tokens its first
+//               workgroups write the units' sums to the workspace, so that a
+//               frequent token's rows are read by many CUs.
+//  embed_join   the rows of those runs, from their units' sums.
+#include <type_traits>
 
 #include "common.hpp"
 #include "kernels.hpp"
+#include "rules.hpp"
 
 namespace mc {
 namespace {
@@ -74,40 +75,49 @@ constexpr int kIds = 512, kSortWaves = 16, kSortThreads = kSortWaves * kWave;
 
 // order[N]: the N tokens with an id of the table that is not padding, by id, in
 // their order within an id; start[v]: the first of id v there, start[vocab] = N.
+// AHEAD wave steps of ids are in flight, and stay in registers between the two
+// passes where they are all of a wave's. us, 2 / 4 / 8 / 16 ahead: 2036 tokens (2
+// steps a wave) 4.4 / 5.9 / 6.2 / 7.2, 16384 (16 steps) 12.3 / 12.0 / 12.0 / 11.1,
+// 65536 37.2 / 34.6 / 34.1 / 33.5: then the tests of every id bound it.
+template <int AHEAD>
 __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __restrict__ ids, int32_t tokens,
                                                            int64_t vocab, int64_t padding,
                                                            int32_t* __restrict__ order, int32_t* __restrict__ start) {
     __shared__ int32_t count[kSortWaves][kIds];
     __shared__ int32_t wsum[kSortWaves], before[kSortWaves];
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
-    const int64_t first = (int64_t)blockIdx.x * kIds;
-    const int32_t last = (int32_t)(first + kIds < vocab ? first + kIds : vocab);  // ids below 2^31
-    const int32_t lo = (int32_t)first;
-    const int32_t pad = padding < vocab ? (int32_t)padding : -1;
+    // this workgroup's ids [lo, lo + width); no token's key is -1 (unsigned)
+    const uint32_t lo = blockIdx.x * (uint32_t)kIds;
+    const uint32_t width = (uint32_t)(vocab - lo < kIds ? vocab - lo : kIds);
+    const uint32_t pad = padding >= 0 && padding < vocab ? (uint32_t)padding : 0xffffffffu;
     for (int i = tid; i < kSortWaves * kIds; i += kSortThreads) (&count[0][0])[i] = 0;
-    // this wave's tokens, whole wave steps
-    const int32_t steps = (int32_t)(((int64_t)tokens + kWave - 1) / kWave);
-    const int32_t per = (steps + kSortWaves - 1) / kSortWaves;
-    const int32_t s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
+    // this wave's tokens [t0, t1), whole wave steps
+    const int32_t per = (int32_t)((((int64_t)tokens + kWave - 1) / kWave + kSortWaves - 1) / kSortWaves);
+    const int64_t start0 = (int64_t)wave * per * kWave;
+    const int32_t t1 = (int32_t)(start0 + (int64_t)per * kWave < tokens ? start0 + (int64_t)per * kWave : tokens);
+    const int32_t t0 = (int32_t)(start0 < t1 ? start0 : t1);
+    const __amdgpu_buffer_rsrc_t rid = make_rsrc(ids, (int64_t)tokens * 4);
+    // AHEAD steps of tokens from t on: an id of the table, or -1
+    uint32_t key[AHEAD];
+    auto load_keys = [&](int32_t t) {
+        const int32_t mine = t + lane;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            key[u] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rid, (mine + u * kWave) * 4, 0, 0);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            key[u] = mine + u * kWave < t1 && key[u] != pad && (int32_t)key[u] >= 0 ? key[u] : 0xffffffffu;
+    };
     __syncthreads();
-    int32_t below = 0;
-    constexpr int U = 4;
-    for (int32_t s = s0; s < s1; s += U) {
-        int32_t id[U];
+    int32_t below = 0;  // tokens of smaller ids, wave-uniform
+    for (int32_t t = t0; t < t1; t += AHEAD * kWave) {
+        load_keys(t);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t t = (int64_t)(s + u) * kWave + lane;
-            id[u] = s + u < s1 && t < tokens ? ids[t] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool real = id[u] >= 0 && id[u] != pad;
-            below += real && id[u] < lo;
-            if (real && id[u] >= lo && id[u] < last) atomicAdd(&count[wave][id[u] - lo], 1);
+        for (int u = 0; u < AHEAD; ++u) {
+            below += __builtin_popcountll(__ballot(key[u] < lo));
+            if (key[u] - lo < width) atomicAdd(&count[wave][key[u] - lo], 1);
         }
     }
-#pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) below += __shfl_xor(below, m, kWave);
     if (lane == 0) before[wave] = below;
     __syncthreads();
     // exclusive scan over (id, wave): thread i < kIds owns id lo + i
@@ -129,7 +139,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
     }
     base += scan - mine;
     if (tid < kIds) {
-        if (lo + (int64_t)tid < last) start[lo + tid] = base;
+        if ((uint32_t)tid < width) start[lo + tid] = base;
         if (lo + (int64_t)tid + 1 == vocab) start[vocab] = base + mine;
         for (int w = 0; w < kSortWaves; ++w) {
             const int32_t c = count[w][tid];
@@ -138,25 +148,20 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
         }
     }
     __syncthreads();
-    for (int32_t s = s0; s < s1; s += U) {
-        int32_t id[U];
+    for (int32_t t = t0; t < t1; t += AHEAD * kWave) {
+        if (per > AHEAD) load_keys(t);  // otherwise they are still there
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t t = (int64_t)(s + u) * kWave + lane;
-            id[u] = s + u < s1 && t < tokens ? ids[t] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = id[u] >= 0 && id[u] != pad && id[u] >= lo && id[u] < last;
+        for (int u = 0; u < AHEAD; ++u) {
+            const bool in = key[u] - lo < width;
             uint64_t left = __ballot(in);
             while (left) {  // one id of this step at a time, its lanes in order
                 const int l = __builtin_ctzll(left);
-                const int32_t v = __builtin_amdgcn_readlane(id[u], l);
-                const uint64_t same = __ballot(in && id[u] == v);
+                const uint32_t v = (uint32_t)__builtin_amdgcn_readlane((int)key[u], l);
+                const uint64_t same = __ballot(in && key[u] == v);
                 volatile int32_t* place = &count[wave][v - lo];  // volatile: one lane moves it for the others
                 const int32_t at = *place;
-                if (in && id[u] == v)
-                    order[at + __builtin_popcountll(same & (((uint64_t)1 << lane) - 1))] = (s + u) * kWave + lane;
+                if (in && key[u] == v)
+                    order[at + __builtin_popcountll(same & (((uint64_t)1 << lane) - 1))] = t + u * kWave + lane;
                 if (lane == l) *place = at + __builtin_popcountll(same);
                 left &= ~same;
             }
@@ -209,11 +214,11 @@ __device__ __forceinline__ Sum load_row(const T* row, const Columns& c, int dim)
     }
     return s;
 }
-template <int VEC>
+template <int VEC, bool STREAM = false>
 __device__ __forceinline__ void store_row(float* row, const Columns& c, int dim, const Sum& s) {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(row, (int64_t)dim * 4);
     const i32x4 q = {__float_as_int(s.v[0]), __float_as_int(s.v[1]), __float_as_int(s.v[2]), __float_as_int(s.v[3])};
-    __builtin_amdgcn_raw_buffer_store_b128(q, r, (int)(c.d + 4 <= dim ? (uint32_t)c.d * 4u : kOOB), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(q, r, (int)(c.d + 4 <= dim ? (uint32_t)c.d * 4u : kOOB), 0, STREAM ? kStoreNT : 0);
     if constexpr (VEC != 4)
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(s.rest), r, c.rest >= 0 ? 4 * c.rest : (int)kOOB, 0, 0);
 }
@@ -241,70 +246,104 @@ __device__ __forceinline__ void add_run(const T* __restrict__ dout, const int32_
     for (; from < to; ++from) add(acc, load_row<T, VEC>(dout + (int64_t)order[from] * dim, c, dim));
 }
 
+// scale * acc, added to what the row holds or in its place.
+template <int VEC, bool ADD, bool STREAM>
+__device__ __forceinline__ void put_sum(float* row, const Columns& cols, int dim, float scale, Sum acc) {
+    Sum old{};
+    if constexpr (ADD) old = load_row<float, VEC>(row, cols, dim);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc.v[e] = __builtin_fmaf(acc.v[e], scale, old.v[e]);
+    acc.rest = __builtin_fmaf(acc.rest, scale, old.rest);
+    store_row<VEC, STREAM>(row, cols, dim, acc);
+}
+
+struct GradArgs {
+    const void* dout;
+    const int32_t *ids, *order, *start;
+    float *part, *dtable;
+    int64_t vocab;
+    int64_t long_blocks;  // the first workgroups: units of long runs
+    int dim, unit;
+    float scale;
+};
+
 // part[c][0]: the sum over unit c of the sorted tokens of the run that goes on
 // through its start, part[c][1]: of the run that starts inside it and goes on
 // through its end; only of runs longer than two units.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void embed_long(const T* __restrict__ dout, const int32_t* __restrict__ ids,
-                                                  const int32_t* __restrict__ order,
-                                                  const int32_t* __restrict__ start, float* __restrict__ part,
-                                                  int64_t vocab, int dim, int32_t unit) {
-    const int64_t slabs = slabs_of(dim);
+__device__ __forceinline__ void sum_unit(const GradArgs& a) {
+    const int64_t slabs = slabs_of(a.dim);
     const int64_t job = (int64_t)blockIdx.x * 4 + wave_id();
     const int64_t c = job / slabs;
-    const int32_t n = start[vocab];
-    const int64_t from = c * unit;
+    const int32_t n = a.start[a.vocab];
+    const int64_t from = c * a.unit;
     if (from >= n) return;
-    const int32_t to = (int32_t)(from + unit < n ? from + unit : n);
-    const Columns cols = columns_of(job % slabs, dim);
-    int32_t id = ids[order[from]];
+    const int32_t to = (int32_t)(from + a.unit < n ? from + a.unit : n);
+    const Columns cols = columns_of(job % slabs, a.dim);
+    int32_t id = a.ids[a.order[from]];
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         if (side == 1) {
-            const int32_t next = ids[order[to - 1]];
+            const int32_t next = a.ids[a.order[to - 1]];
             if (next == id) return;
             id = next;
         }
-        const int32_t a = start[id], b = start[id + 1];
-        if (b - a <= 2 * unit) continue;
+        const int32_t x = a.start[id], y = a.start[id + 1];
+        if (y - x <= 2 * a.unit) continue;
         Sum acc{};
-        add_run<T, VEC>(dout, order, a > from ? a : (int32_t)from, b < to ? b : to, cols, dim, acc);
+        add_run<T, VEC>(static_cast<const T*>(a.dout), a.order, x > from ? x : (int32_t)from, y < to ? y : to, cols,
+                        a.dim, acc);
         // a run that starts with the unit goes on through its start as well
-        store_row<VEC>(part + (2 * c + (a > from)) * dim, cols, dim, acc);
+        store_row<VEC>(a.part + (2 * c + (x > from)) * a.dim, cols, a.dim, acc);
     }
 }
 
-constexpr int kRows = 8;  // ids per workgroup of embed_grad
+// kRows ids per workgroup: 4 / 8 / 16 / 32 took 226 / 227 / 231 / 239 us for the
+// gradient of 16384 tokens into 151936 rows of 1536, with ordinary stores.
+constexpr int kRows = 4;
 
-template <typename T, int VEC, bool ADD>
-__global__ __launch_bounds__(256) void embed_grad(const T* __restrict__ dout, const int32_t* __restrict__ order,
-                                                  const int32_t* __restrict__ start, const float* __restrict__ part,
-                                                  float* __restrict__ dtable, int64_t vocab, int dim, float scale,
-                                                  int32_t unit) {
-    const int64_t v0 = (int64_t)blockIdx.x * kRows;
-    const int slabs = (int)slabs_of(dim);
-    const int rows = (int)(vocab - v0 < kRows ? vocab - v0 : kRows);
+// STREAM: stores past the caches, where rows are whole 128-byte lines and the
+// table is larger than they are; 226 -> 202 us at that size. Rows of 893 floats,
+// whose ends share lines, lost by it: 36 -> 52 us for 50257 of them.
+template <typename T, int VEC, bool ADD, bool STREAM>
+__global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
+    if ((int64_t)blockIdx.x < a.long_blocks) {
+        sum_unit<T, VEC>(a);
+        return;
+    }
+    const int64_t v0 = ((int64_t)blockIdx.x - a.long_blocks) * kRows;
+    const int slabs = (int)slabs_of(a.dim);
+    const int rows = (int)(a.vocab - v0 < kRows ? a.vocab - v0 : kRows);
     for (int job = wave_id(); job < rows * slabs; job += 4) {
         const int64_t v = v0 + job / slabs;
-        const Columns cols = columns_of(job % slabs, dim);
-        const int32_t a = start[v], b = start[v + 1];
-        if (ADD && a == b) continue;
+        const int32_t x = a.start[v], y = a.start[v + 1];
+        if ((ADD && x == y) || y - x > 2 * a.unit) continue;  // long runs: embed_join
+        const Columns cols = columns_of(job % slabs, a.dim);
         Sum acc{};
-        if (b - a <= 2 * unit) {
-            add_run<T, VEC>(dout, order, a, b, cols, dim, acc);
-        } else {
-            const int32_t c1 = (b - 1) / unit;
-            for (int32_t c = a / unit; c <= c1; ++c)
-                add(acc, load_row<float, VEC>(part + (2 * (int64_t)c + (a > (int64_t)c * unit)) * dim, cols, dim));
-        }
-        float* row = dtable + v * dim;
-        Sum old{};
-        if constexpr (ADD) old = load_row<float, VEC>(row, cols, dim);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc.v[e] = __builtin_fmaf(acc.v[e], scale, old.v[e]);
-        acc.rest = __builtin_fmaf(acc.rest, scale, old.rest);
-        store_row<VEC>(row, cols, dim, acc);
+        add_run<T, VEC>(static_cast<const T*>(a.dout), a.order, x, y, cols, a.dim, acc);
+        put_sum<VEC, ADD, STREAM>(a.dtable + v * a.dim, cols, a.dim, a.scale, acc);
     }
+}
+
+// The rows of long runs, one wave per (unit, slab) in which such a run ends.
+template <int VEC, bool ADD>
+__global__ __launch_bounds__(256) void embed_join(GradArgs a) {
+    const int64_t slabs = slabs_of(a.dim);
+    const int64_t job = (int64_t)blockIdx.x * 4 + wave_id();
+    const int64_t from = job / slabs * a.unit;
+    const int32_t n = a.start[a.vocab];
+    if (from >= n) return;
+    const int32_t to = (int32_t)(from + a.unit < n ? from + a.unit : n);
+    // the run at the unit's start is the only long one that can end in it
+    const int32_t id = a.ids[a.order[from]];
+    const int32_t x = a.start[id], y = a.start[id + 1];
+    if (y - x <= 2 * a.unit || y > to) return;
+    const Columns cols = columns_of(job % slabs, a.dim);
+    const int64_t c1 = (y - 1) / a.unit;
+    Sum acc{};
+    for (int64_t c = x / a.unit; c <= c1; ++c)
+        add(acc, load_row<float, VEC>(a.part + (2 * c + (x > c * a.unit)) * a.dim, cols, a.dim));
+    put_sum<VEC, ADD, false>(a.dtable + (int64_t)id * a.dim, cols, a.dim, a.scale, acc);
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -358,23 +397,40 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
     int32_t* start = reinterpret_cast<int32_t*>(ws + w.start);
     float* part = reinterpret_cast<float*>(ws + w.part);
     const int32_t unit = unit_of(d.tokens);
-    embed_sort<<<dim3((unsigned)((d.vocab + kIds - 1) / kIds)), kSortThreads, 0, stream>>>(
-        ids, (int32_t)d.tokens, d.vocab, d.padding_id, order, start);
-    const int64_t slabs = slabs_of(d.dim);
-    const dim3 glong((unsigned)(((d.tokens + unit - 1) / unit * slabs + 3) / 4));
-    const dim3 ggrad((unsigned)((d.vocab + kRows - 1) / kRows));
+    const dim3 gsort((unsigned)((d.vocab + kIds - 1) / kIds));
+    const int64_t steps = (d.tokens + kSortThreads - 1) / kSortThreads;  // of a wave
+    auto sort = [&](auto ahead) {
+        embed_sort<decltype(ahead)::value><<<gsort, kSortThreads, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab,
+                                                                              d.padding_id, order, start);
+    };
+    if (steps <= 2) sort(std::integral_constant<int, 2>{});
+    else if (steps <= 4) sort(std::integral_constant<int, 4>{});
+    else if (steps <= 8) sort(std::integral_constant<int, 8>{});
+    else sort(std::integral_constant<int, 16>{});
+    const int64_t slabs = slabs_of(d.dim), units = (d.tokens + unit - 1) / unit;
+    GradArgs a{};
+    a.dout = dout;
+    a.ids = ids;
+    a.order = order;
+    a.start = start;
+    a.part = part;
+    a.dtable = dtable;
+    a.vocab = d.vocab;
+    a.dim = (int)d.dim;
+    a.unit = unit;
+    a.scale = d.scale;
+    a.long_blocks = d.tokens > 2 * unit ? (units * slabs + 3) / 4 : 0;
+    const dim3 grid((unsigned)(a.long_blocks + (d.vocab + kRows - 1) / kRows));
+    const bool stream_out = embedding_stream_gradient(d.vocab, d.dim);
     auto go = [&](auto elem, auto vec) {
         typedef decltype(elem) T;
         constexpr int VEC = decltype(vec)::value;
-        const T* g = static_cast<const T*>(dout);
-        if (d.tokens > 2 * unit)
-            embed_long<T, VEC><<<glong, 256, 0, stream>>>(g, ids, order, start, part, d.vocab, (int)d.dim, unit);
-        if (accumulate)
-            embed_grad<T, VEC, true><<<ggrad, 256, 0, stream>>>(g, order, start, part, dtable, d.vocab, (int)d.dim,
-                                                                d.scale, unit);
-        else
-            embed_grad<T, VEC, false><<<ggrad, 256, 0, stream>>>(g, order, start, part, dtable, d.vocab, (int)d.dim,
-                                                                 d.scale, unit);
+        if (accumulate) embed_grad<T, VEC, true, false><<<grid, 256, 0, stream>>>(a);
+        else if (VEC == 4 && stream_out) embed_grad<T, VEC, false, VEC == 4><<<grid, 256, 0, stream>>>(a);
+        else embed_grad<T, VEC, false, false><<<grid, 256, 0, stream>>>(a);
+        if (a.long_blocks == 0) return;
+        if (accumulate) embed_join<VEC, true><<<dim3((unsigned)a.long_blocks), 256, 0, stream>>>(a);
+        else embed_join<VEC, false><<<dim3((unsigned)a.long_blocks), 256, 0, stream>>>(a);
     };
     if (d.dtype == MC_F32) {
         if (d.dim % 4 == 0) go(float{}, std::integral_constant<int, 4>{});

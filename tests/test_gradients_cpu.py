@@ -125,8 +125,8 @@ def test_embedding_abi(mc):
     for call in (fwd, bwd):
         assert call(None) == NULL
         assert call(desc(dtype=2)) == DTYPE
-        for bad in ({"tokens": 0}, {"vocab": 0}, {"dim": 0}, {"tokens": 2**31}, {"vocab": 2**31},
-                    {"vocab": 2**30, "dim": 1024}, {"tokens": 2**30, "dim": 1024}):
+        for bad in ({"tokens": 0}, {"vocab": 0}, {"dim": 0}, {"tokens": 2**28}, {"vocab": 2**31},
+                    {"vocab": 2**30, "dim": 1024}, {"tokens": 2**27, "dim": 8192}):
             assert call(desc(**bad)) == SHAPE, bad
         assert call(desc(scale=float("inf"))) == VALUE
         assert call(desc(), ids=None) == NULL
@@ -137,7 +137,7 @@ def test_embedding_abi(mc):
     assert bwd(desc(), dout=None) == NULL and bwd(desc(), dtable=None) == NULL
     assert bwd(desc(), dout=ctypes.c_void_p(264)) == LAYOUT and bwd(desc(), dtable=ctypes.c_void_p(264)) == LAYOUT
     assert bwd(desc(), add=2) == VALUE
-    assert bwd(desc(vocab=134217721, dim=1)) == SHAPE
+    assert bwd(desc(vocab=50000001, dim=1)) == SHAPE and bwd(desc(dim=4000001)) == SHAPE
     need = L.mc_embedding_bwd_workspace_size(desc())
     assert need == 256 + 512  # order and start; no run of 8 tokens is long
     assert bwd(desc(), have=need - 1) == WORKSPACE and bwd(desc(), ws=None) == WORKSPACE

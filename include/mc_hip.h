@@ -402,8 +402,8 @@ mc_status mc_clip_gradients(const mc_grad_tensor* tensors, int32_t count, float 
  * results are bitwise reproducible. */
 typedef struct mc_embedding_desc {
     int64_t tokens;      /* 1 .. 2^28 - 1 */
-    int64_t vocab;       /* 1 .. 2^31 - 1; backward 5e7 */
-    int64_t dim;         /* >= 1, backward 4e6; vocab * dim and tokens * dim < 2^40 */
+    int64_t vocab;       /* 1 .. 2^31 - 1 */
+    int64_t dim;         /* >= 1; vocab * dim < 2^40, tokens * dim < 2^40, backward < 1.7e10 */
     int64_t padding_id;  /* < 0: none */
     float scale;         /* finite */
     int32_t dtype;       /* mc_dtype of table, out and dout */

@@ -842,9 +842,9 @@ mc_status mc_embedding_bwd(const mc_embedding_desc* d, const int32_t* ids, const
     if (s != MC_OK) return s;
     MC_CHECK(ids && dout && dtable, MC_ERR_NULL, "embedding backward: ids, dout and dtable must not be NULL");
     MC_CHECK(accumulate == 0 || accumulate == 1, MC_ERR_VALUE, "embedding backward: accumulate must be 0 or 1");
-    // a launch holds at most 2^32 - 1 work-items: 256 per 4 ids, 64 per 256 columns of a unit (at most 1024 of them)
-    MC_CHECK(d->vocab <= 50000000 && d->dim <= 4000000, MC_ERR_SHAPE,
-             "embedding backward: vocab must be <= 50000000 and dim <= 4000000, got %lld, %lld", (long long)d->vocab,
+    // a launch holds at most 2^32 - 1 work-items: 64 per token and 256 columns, and per unit of tokens and 256 columns
+    MC_CHECK((double)(d->tokens + 1024) * std::ceil((double)d->dim / 256.0) < 67108860.0, MC_ERR_SHAPE,
+             "embedding backward: tokens (%lld) times dim / 256 (dim %lld) too large for a launch", (long long)d->tokens,
              (long long)d->dim);
     MC_CHECK(aligned16(dout) && aligned16(dtable), MC_ERR_LAYOUT,
              "embedding backward: dout and dtable must be 16-byte aligned");

@@ -17,11 +17,13 @@
 //               tokens. One launch, no waiting between workgroups, no partial
 //               histograms in memory. 16 waves take a 16th of the tokens each, so
 //               that a batch of one repeated token is no slower than another.
-//  embed_grad   one wave per (id, slab of 256 columns): zeros or the run's sum. Of
-//               runs longer than two units of the sorted tokens its first
-//               workgroups write the units' sums to the workspace, so that a
-//               frequent token's rows are read by many CUs.
+//               Its other workgroups clear the gradient meanwhile.
+//  embed_rows   one wave per (sorted token, slab of 256 columns): the first token
+//               of a run writes its row. Of runs longer than two units of the
+//               sorted tokens the first workgroups write the units' sums to the
+//               workspace, so that a frequent token's rows are read by many CUs.
 //  embed_join   the rows of those runs, from their units' sums.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.hpp"
@@ -71,7 +73,7 @@ __global__ __launch_bounds__(256) void embed_fwd(const T* __restrict__ table, co
 }
 
 // --------------------------------------------------------------- backward
-constexpr int kIds = 512, kSortWaves = 16, kSortThreads = kSortWaves * kWave;
+constexpr int kIds = 512, kSortWaves = 16, kSortThreads = kSortWaves * kWave, kClearBlocks = 2048;
 
 // order[N]: the N tokens with an id of the table that is not padding, by id, in
 // their order within an id; start[v]: the first of id v there, start[vocab] = N.
@@ -79,10 +81,29 @@ constexpr int kIds = 512, kSortWaves = 16, kSortThreads = kSortWaves * kWave;
 // passes where they are all of a wave's. us, 2 / 4 / 8 / 16 ahead: 2036 tokens (2
 // steps a wave) 4.4 / 5.9 / 6.2 / 7.2, 16384 (16 steps) 12.3 / 12.0 / 12.0 / 11.1,
 // 65536 37.2 / 34.6 / 34.1 / 33.5: then the tests of every id bound it.
-template <int AHEAD>
+//
+// The workgroups past sort_blocks clear the gradient meanwhile (`clear` floats of
+// it, 0 with accumulate): the sort leaves most of the device idle, and rows of ids
+// that do not occur are then written at the rate of a plain fill.
+template <int AHEAD, bool STREAM>
 __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __restrict__ ids, int32_t tokens,
                                                            int64_t vocab, int64_t padding,
-                                                           int32_t* __restrict__ order, int32_t* __restrict__ start) {
+                                                           int32_t* __restrict__ order, int32_t* __restrict__ start,
+                                                           int sort_blocks, float* __restrict__ dtable,
+                                                           int64_t clear) {
+    if ((int)blockIdx.x >= sort_blocks) {
+        const int64_t n = clear / 4, blocks = gridDim.x - sort_blocks;
+        const int64_t per = (n + blocks - 1) / blocks, first = ((int64_t)blockIdx.x - sort_blocks) * per;
+        const int64_t end = first + per < n ? first + per : n;
+        f32x4* out = reinterpret_cast<f32x4*>(dtable);
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        for (int64_t i = first + threadIdx.x; i < end; i += kSortThreads) {
+            if constexpr (STREAM) __builtin_nontemporal_store(zero, out + i);
+            else out[i] = zero;
+        }
+        if ((int)blockIdx.x == sort_blocks && threadIdx.x < (clear & 3)) dtable[n * 4 + threadIdx.x] = 0.f;
+        return;
+    }
     __shared__ int32_t count[kSortWaves][kIds];
     __shared__ int32_t wsum[kSortWaves], before[kSortWaves];
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
@@ -214,11 +235,11 @@ __device__ __forceinline__ Sum load_row(const T* row, const Columns& c, int dim)
     }
     return s;
 }
-template <int VEC, bool STREAM = false>
+template <int VEC>
 __device__ __forceinline__ void store_row(float* row, const Columns& c, int dim, const Sum& s) {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(row, (int64_t)dim * 4);
     const i32x4 q = {__float_as_int(s.v[0]), __float_as_int(s.v[1]), __float_as_int(s.v[2]), __float_as_int(s.v[3])};
-    __builtin_amdgcn_raw_buffer_store_b128(q, r, (int)(c.d + 4 <= dim ? (uint32_t)c.d * 4u : kOOB), 0, STREAM ? kStoreNT : 0);
+    __builtin_amdgcn_raw_buffer_store_b128(q, r, (int)(c.d + 4 <= dim ? (uint32_t)c.d * 4u : kOOB), 0, 0);
     if constexpr (VEC != 4)
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(s.rest), r, c.rest >= 0 ? 4 * c.rest : (int)kOOB, 0, 0);
 }
@@ -247,14 +268,14 @@ __device__ __forceinline__ void add_run(const T* __restrict__ dout, const int32_
 }
 
 // scale * acc, added to what the row holds or in its place.
-template <int VEC, bool ADD, bool STREAM>
+template <int VEC, bool ADD>
 __device__ __forceinline__ void put_sum(float* row, const Columns& cols, int dim, float scale, Sum acc) {
     Sum old{};
     if constexpr (ADD) old = load_row<float, VEC>(row, cols, dim);
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc.v[e] = __builtin_fmaf(acc.v[e], scale, old.v[e]);
     acc.rest = __builtin_fmaf(acc.rest, scale, old.rest);
-    store_row<VEC, STREAM>(row, cols, dim, acc);
+    store_row<VEC>(row, cols, dim, acc);
 }
 
 struct GradArgs {
@@ -298,31 +319,25 @@ __device__ __forceinline__ void sum_unit(const GradArgs& a) {
     }
 }
 
-// kRows ids per workgroup: 4 / 8 / 16 / 32 took 226 / 227 / 231 / 239 us for the
-// gradient of 16384 tokens into 151936 rows of 1536, with ordinary stores.
-constexpr int kRows = 4;
-
-// STREAM: stores past the caches, where rows are whole 128-byte lines and the
-// table is larger than they are; 226 -> 202 us at that size. Rows of 893 floats,
-// whose ends share lines, lost by it: 36 -> 52 us for 50257 of them.
-template <typename T, int VEC, bool ADD, bool STREAM>
-__global__ __launch_bounds__(256) void embed_grad(GradArgs a) {
+// One wave per (sorted token, slab): the first token of a run sums and writes its
+// row, the others have nothing to do.
+template <typename T, int VEC, bool ADD>
+__global__ __launch_bounds__(256) void embed_rows(GradArgs a) {
     if ((int64_t)blockIdx.x < a.long_blocks) {
         sum_unit<T, VEC>(a);
         return;
     }
-    const int64_t v0 = ((int64_t)blockIdx.x - a.long_blocks) * kRows;
-    const int slabs = (int)slabs_of(a.dim);
-    const int rows = (int)(a.vocab - v0 < kRows ? a.vocab - v0 : kRows);
-    for (int job = wave_id(); job < rows * slabs; job += 4) {
-        const int64_t v = v0 + job / slabs;
-        const int32_t x = a.start[v], y = a.start[v + 1];
-        if ((ADD && x == y) || y - x > 2 * a.unit) continue;  // long runs: embed_join
-        const Columns cols = columns_of(job % slabs, a.dim);
-        Sum acc{};
-        add_run<T, VEC>(static_cast<const T*>(a.dout), a.order, x, y, cols, a.dim, acc);
-        put_sum<VEC, ADD, STREAM>(a.dtable + v * a.dim, cols, a.dim, a.scale, acc);
-    }
+    const int64_t slabs = slabs_of(a.dim);
+    const int64_t job = ((int64_t)blockIdx.x - a.long_blocks) * 4 + wave_id();
+    const int64_t p = job / slabs;
+    if (p >= a.start[a.vocab]) return;
+    const int32_t id = a.ids[a.order[p]];
+    const int32_t x = a.start[id], y = a.start[id + 1];
+    if (p != x || y - x > 2 * a.unit) return;  // long runs: embed_join
+    const Columns cols = columns_of(job % slabs, a.dim);
+    Sum acc{};
+    add_run<T, VEC>(static_cast<const T*>(a.dout), a.order, x, y, cols, a.dim, acc);
+    put_sum<VEC, ADD>(a.dtable + (int64_t)id * a.dim, cols, a.dim, a.scale, acc);
 }
 
 // The rows of long runs, one wave per (unit, slab) in which such a run ends.
@@ -343,7 +358,7 @@ __global__ __launch_bounds__(256) void embed_join(GradArgs a) {
     Sum acc{};
     for (int64_t c = x / a.unit; c <= c1; ++c)
         add(acc, load_row<float, VEC>(a.part + (2 * c + (x > c * a.unit)) * a.dim, cols, a.dim));
-    put_sum<VEC, ADD, false>(a.dtable + (int64_t)id * a.dim, cols, a.dim, a.scale, acc);
+    put_sum<VEC, ADD>(a.dtable + (int64_t)id * a.dim, cols, a.dim, a.scale, acc);
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -397,11 +412,20 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
     int32_t* start = reinterpret_cast<int32_t*>(ws + w.start);
     float* part = reinterpret_cast<float*>(ws + w.part);
     const int32_t unit = unit_of(d.tokens);
-    const dim3 gsort((unsigned)((d.vocab + kIds - 1) / kIds));
+    // workgroups that clear the gradient: two per CU, or one per 64 KB of it
+    const int64_t clear = accumulate ? 0 : d.vocab * d.dim;
+    const int64_t clear_blocks = std::min<int64_t>((clear + (16 << 10) - 1) / (16 << 10), kClearBlocks);
+    const int sort_blocks = (int)((d.vocab + kIds - 1) / kIds);
+    const dim3 gsort((unsigned)(sort_blocks + clear_blocks));
     const int64_t steps = (d.tokens + kSortThreads - 1) / kSortThreads;  // of a wave
     auto sort = [&](auto ahead) {
-        embed_sort<decltype(ahead)::value><<<gsort, kSortThreads, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab,
-                                                                              d.padding_id, order, start);
+        constexpr int AHEAD = decltype(ahead)::value;
+        if (embedding_stream_gradient(d.vocab, d.dim))
+            embed_sort<AHEAD, true><<<gsort, kSortThreads, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id,
+                                                                       order, start, sort_blocks, dtable, clear);
+        else
+            embed_sort<AHEAD, false><<<gsort, kSortThreads, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id,
+                                                                        order, start, sort_blocks, dtable, clear);
     };
     if (steps <= 2) sort(std::integral_constant<int, 2>{});
     else if (steps <= 4) sort(std::integral_constant<int, 4>{});
@@ -420,14 +444,12 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
     a.unit = unit;
     a.scale = d.scale;
     a.long_blocks = d.tokens > 2 * unit ? (units * slabs + 3) / 4 : 0;
-    const dim3 grid((unsigned)(a.long_blocks + (d.vocab + kRows - 1) / kRows));
-    const bool stream_out = embedding_stream_gradient(d.vocab, d.dim);
+    const dim3 grid((unsigned)(a.long_blocks + (d.tokens * slabs + 3) / 4));
     auto go = [&](auto elem, auto vec) {
         typedef decltype(elem) T;
         constexpr int VEC = decltype(vec)::value;
-        if (accumulate) embed_grad<T, VEC, true, false><<<grid, 256, 0, stream>>>(a);
-        else if (VEC == 4 && stream_out) embed_grad<T, VEC, false, VEC == 4><<<grid, 256, 0, stream>>>(a);
-        else embed_grad<T, VEC, false, false><<<grid, 256, 0, stream>>>(a);
+        if (accumulate) embed_rows<T, VEC, true><<<grid, 256, 0, stream>>>(a);
+        else embed_rows<T, VEC, false><<<grid, 256, 0, stream>>>(a);
         if (a.long_blocks == 0) return;
         if (accumulate) embed_join<VEC, true><<<dim3((unsigned)a.long_blocks), 256, 0, stream>>>(a);
         else embed_join<VEC, false><<<dim3((unsigned)a.long_blocks), 256, 0, stream>>>(a);

@@ -401,9 +401,9 @@ mc_status mc_clip_gradients(const mc_grad_tensor* tensors, int32_t count, float 
  * holds there. Each row's sum runs in an order that the sizes and ids alone fix:
  * results are bitwise reproducible. */
 typedef struct mc_embedding_desc {
-    int64_t tokens;      /* 1 .. 2^28 - 1 */
+    int64_t tokens;      /* 1 .. 67108860; backward (tokens + 1024) * ceil(dim / 256) too */
     int64_t vocab;       /* 1 .. 2^31 - 1 */
-    int64_t dim;         /* >= 1; vocab * dim < 2^40, tokens * dim < 2^40, backward < 1.7e10 */
+    int64_t dim;         /* >= 1; vocab * dim and tokens * dim < 2^40, backward vocab * (dim + 2) < 1.7e10 */
     int64_t padding_id;  /* < 0: none */
     float scale;         /* finite */
     int32_t dtype;       /* mc_dtype of table, out and dout */

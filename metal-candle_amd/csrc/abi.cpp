@@ -842,9 +842,13 @@ mc_status mc_embedding_bwd(const mc_embedding_desc* d, const int32_t* ids, const
     if (s != MC_OK) return s;
     MC_CHECK(ids && dout && dtable, MC_ERR_NULL, "embedding backward: ids, dout and dtable must not be NULL");
     MC_CHECK(accumulate == 0 || accumulate == 1, MC_ERR_VALUE, "embedding backward: accumulate must be 0 or 1");
-    // a launch holds at most 2^32 - 1 work-items: 64 per token and 256 columns, and per unit of tokens and 256 columns
+    // a launch holds at most 2^32 - 1 work-items: 64 per token and 256 columns, and per unit of tokens (at most 1024)
+    // and 256 columns; of the sort 1024 per 512 ids, or 256 and as many per 1024 elements of the gradient
     MC_CHECK((double)(d->tokens + 1024) * std::ceil((double)d->dim / 256.0) < 67108860.0, MC_ERR_SHAPE,
              "embedding backward: tokens (%lld) times dim / 256 (dim %lld) too large for a launch", (long long)d->tokens,
+             (long long)d->dim);
+    MC_CHECK(d->vocab <= 2147482624 && (double)d->vocab * ((double)d->dim + 2.0) < 1.7e10, MC_ERR_SHAPE,
+             "embedding backward: vocab (%lld) times dim (%lld) too large for a launch", (long long)d->vocab,
              (long long)d->dim);
     MC_CHECK(aligned16(dout) && aligned16(dtable), MC_ERR_LAYOUT,
              "embedding backward: dout and dtable must be 16-byte aligned");

@@ -15,15 +15,20 @@
 //               its own run of tokens without another workgroup's help: counts
 //               per (id, wave) in LDS, a scan, and a second pass that places the
 //               tokens. One launch, no waiting between workgroups, no partial
-//               histograms in memory. 16 waves take a 16th of the tokens each, so
-//               that a batch of one repeated token is no slower than another.
+//               histograms in memory. The waves take a share of the tokens each,
+//               so that a batch of one repeated token is no slower than another.
 //               Its other workgroups clear the gradient meanwhile.
-//  embed_rows   one wave per (sorted token, slab of 256 columns): the first token
-//               of a run writes its row. Of runs longer than two units of the
-//               sorted tokens the first workgroups write the units' sums to the
-//               workspace, so that a frequent token's rows are read by many CUs.
+//  embed_rows   one wave per sorted token and 256 columns: the first token of a run
+//               sums the run. Of runs longer than two units of the sorted tokens the
+//               first workgroups write the units' sums to the workspace, so that a
+//               frequent token's rows are read by many CUs.
 //  embed_join   the rows of those runs, from their units' sums.
-#include <algorithm>
+//
+// 16384 tokens whose ids crowd at the table's start, 151936 x 1536 bf16: forward 21
+// us (100 MB, 4.7 TB/s); sort and clearing 136 us (933 MB, 6.8 TB/s: a fill's rate),
+// rows 38, join 5. A workgroup per sorted token, its waves taking the slabs of one
+// row in turn: 65 us for the rows. Sorted tokens as (token, id) pairs instead of two
+// arrays, whose consecutive tokens load at once: 54.
 #include <type_traits>
 
 #include "common.hpp"
@@ -39,11 +44,7 @@ namespace {
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
     if constexpr (VEC == 1) v[0] = Elem<T>::load(p, 0);
-    else if constexpr (VEC == Vec16<T>::N) Vec16<T>::load(p, v);
-    else {  // 4 bf16
-        const uint2 q = *reinterpret_cast<const uint2*>(p);
-        v[0] = bf16_lo(q.x); v[1] = bf16_hi(q.x); v[2] = bf16_lo(q.y); v[3] = bf16_hi(q.y);
-    }
+    else Vec16<T>::load(p, v);
 }
 
 template <typename T, int VEC>
@@ -73,35 +74,34 @@ __global__ __launch_bounds__(256) void embed_fwd(const T* __restrict__ table, co
 }
 
 // --------------------------------------------------------------- backward
-constexpr int kIds = 512, kSortWaves = 16, kSortThreads = kSortWaves * kWave, kClearBlocks = 2048;
+constexpr int kIds = 512;
 
-// order[N]: the N tokens with an id of the table that is not padding, by id, in
-// their order within an id; start[v]: the first of id v there, start[vocab] = N.
+// order[N]: the N tokens with an id of the table that is not padding, by id, in their
+// order within an id; sorted[N]: their ids; start[v]: the first of id v there,
+// start[vocab] = N.
 // AHEAD wave steps of ids are in flight, and stay in registers between the two
 // passes where they are all of a wave's. us, 2 / 4 / 8 / 16 ahead: 2036 tokens (2
 // steps a wave) 4.4 / 5.9 / 6.2 / 7.2, 16384 (16 steps) 12.3 / 12.0 / 12.0 / 11.1,
 // 65536 37.2 / 34.6 / 34.1 / 33.5: then the tests of every id bound it.
 //
 // The workgroups past sort_blocks clear the gradient meanwhile (`clear` floats of
-// it, 0 with accumulate): the sort leaves most of the device idle, and rows of ids
-// that do not occur are then written at the rate of a plain fill.
-template <int AHEAD, bool STREAM>
-__global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __restrict__ ids, int32_t tokens,
-                                                           int64_t vocab, int64_t padding,
-                                                           int32_t* __restrict__ order, int32_t* __restrict__ start,
-                                                           int sort_blocks, float* __restrict__ dtable,
-                                                           int64_t clear) {
+// it), one vector per thread, so that they sweep memory in order: 933 MB take 137
+// us, 155 with four vectors per thread, 172 with 16 or workgroups of 1024, and 165
+// in chunks of 64 KB and more. WAVES: workgroups that clear have 4, where the sort
+// of 16384 tokens takes 30 us instead of the 11 with 16 and hides behind them.
+template <int WAVES, int AHEAD>
+__global__ __launch_bounds__(WAVES * kWave) void embed_sort(const int32_t* __restrict__ ids, int32_t tokens,
+                                                            int64_t vocab, int64_t padding,
+                                                            int32_t* __restrict__ order, int32_t* __restrict__ sorted,
+                                                            int32_t* __restrict__ start,
+                                                            int sort_blocks, float* __restrict__ dtable,
+                                                            int64_t clear) {
+    constexpr int kSortWaves = WAVES, kSortThreads = WAVES * kWave;
     if ((int)blockIdx.x >= sort_blocks) {
-        const int64_t n = clear / 4, blocks = gridDim.x - sort_blocks;
-        const int64_t per = (n + blocks - 1) / blocks, first = ((int64_t)blockIdx.x - sort_blocks) * per;
-        const int64_t end = first + per < n ? first + per : n;
-        f32x4* out = reinterpret_cast<f32x4*>(dtable);
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        for (int64_t i = first + threadIdx.x; i < end; i += kSortThreads) {
-            if constexpr (STREAM) __builtin_nontemporal_store(zero, out + i);
-            else out[i] = zero;
-        }
-        if ((int)blockIdx.x == sort_blocks && threadIdx.x < (clear & 3)) dtable[n * 4 + threadIdx.x] = 0.f;
+        const int64_t i = (((int64_t)blockIdx.x - sort_blocks) * kSortThreads + threadIdx.x) * 4;
+        if (i + 4 <= clear) *reinterpret_cast<f32x4*>(dtable + i) = f32x4{0.f, 0.f, 0.f, 0.f};
+        else
+            for (int64_t e = i; e < clear; ++e) dtable[e] = 0.f;
         return;
     }
     __shared__ int32_t count[kSortWaves][kIds];
@@ -141,10 +141,13 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
     }
     if (lane == 0) before[wave] = below;
     __syncthreads();
-    // exclusive scan over (id, wave): thread i < kIds owns id lo + i
+    // exclusive scan over (id, wave): a thread owns kOwn ids
+    constexpr int kOwn = kIds / kSortThreads > 0 ? kIds / kSortThreads : 1;  // ids per thread
+    const bool owner = tid * kOwn < kIds;
     int32_t mine = 0;
-    if (tid < kIds)
-        for (int w = 0; w < kSortWaves; ++w) mine += count[w][tid];
+    if (owner)
+        for (int i = 0; i < kOwn; ++i)
+            for (int w = 0; w < kSortWaves; ++w) mine += count[w][tid * kOwn + i];
     int32_t scan = mine;
 #pragma unroll
     for (int m = 1; m < kWave; m <<= 1) {
@@ -159,15 +162,17 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
         if (w < wave) base += wsum[w];
     }
     base += scan - mine;
-    if (tid < kIds) {
-        if ((uint32_t)tid < width) start[lo + tid] = base;
-        if (lo + (int64_t)tid + 1 == vocab) start[vocab] = base + mine;
-        for (int w = 0; w < kSortWaves; ++w) {
-            const int32_t c = count[w][tid];
-            count[w][tid] = base;
-            base += c;
+    if (owner)
+        for (int i = 0; i < kOwn; ++i) {
+            const uint32_t k = (uint32_t)(tid * kOwn + i);
+            if (k < width) start[lo + k] = base;
+            for (int w = 0; w < kSortWaves; ++w) {
+                const int32_t c = count[w][k];
+                count[w][k] = base;
+                base += c;
+            }
+            if ((int64_t)lo + k + 1 == vocab) start[vocab] = base;
         }
-    }
     __syncthreads();
     for (int32_t t = t0; t < t1; t += AHEAD * kWave) {
         if (per > AHEAD) load_keys(t);  // otherwise they are still there
@@ -181,13 +186,23 @@ __global__ __launch_bounds__(kSortThreads) void embed_sort(const int32_t* __rest
                 const uint64_t same = __ballot(in && key[u] == v);
                 volatile int32_t* place = &count[wave][v - lo];  // volatile: one lane moves it for the others
                 const int32_t at = *place;
-                if (in && key[u] == v)
-                    order[at + __builtin_popcountll(same & (((uint64_t)1 << lane) - 1))] = t + u * kWave + lane;
+                if (in && key[u] == v) {
+                    const int32_t p = at + __builtin_popcountll(same & (((uint64_t)1 << lane) - 1));
+                    order[p] = t + u * kWave + lane;
+                    sorted[p] = (int32_t)v;
+                }
                 if (lane == l) *place = at + __builtin_popcountll(same);
                 left &= ~same;
             }
         }
     }
+}
+
+__global__ __launch_bounds__(256) void embed_clear(float* __restrict__ dtable, int64_t clear) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i + 4 <= clear) *reinterpret_cast<f32x4*>(dtable + i) = f32x4{0.f, 0.f, 0.f, 0.f};
+    else
+        for (int64_t e = i; e < clear; ++e) dtable[e] = 0.f;
 }
 
 // The columns of a wave: 4 per lane from d (which may lie past the row), row by
@@ -249,22 +264,35 @@ __device__ __forceinline__ void add(Sum& x, const Sum& y) {
     x.rest += y.rest;
 }
 
-// acc += dout of sorted tokens [from, to), eight rows in flight.
+// The sum of rows [from, to), row i at row(i): eight in flight, then four, two and
+// one.
+template <int U, typename T, int VEC, typename Row>
+__device__ __forceinline__ Sum sum_group(int64_t from, const Columns& c, int dim, Row&& row) {
+    Sum part[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) part[u] = load_row<T, VEC>(row(from + u), c, dim);
+#pragma unroll
+    for (int s = 1; s < U; s *= 2)
+#pragma unroll
+        for (int u = 0; u < U; u += 2 * s) add(part[u], part[u + s]);
+    return part[0];
+}
+template <typename T, int VEC, typename Row>
+__device__ __forceinline__ Sum sum_rows(int64_t from, int64_t to, const Columns& c, int dim, Row&& row) {
+    Sum acc{};
+    for (; from + 8 <= to; from += 8) add(acc, sum_group<8, T, VEC>(from, c, dim, row));
+    const int left = (int)(to - from);
+    if (left & 4) add(acc, sum_group<4, T, VEC>(from, c, dim, row)), from += 4;
+    if (left & 2) add(acc, sum_group<2, T, VEC>(from, c, dim, row)), from += 2;
+    if (left & 1) add(acc, sum_group<1, T, VEC>(from, c, dim, row));
+    return acc;
+}
+// Of dout over sorted tokens [from, to).
 template <typename T, int VEC>
-__device__ __forceinline__ void add_run(const T* __restrict__ dout, const int32_t* __restrict__ order, int32_t from,
-                                        int32_t to, const Columns& c, int dim, Sum& acc) {
-    constexpr int U = 8;
-    for (; from + U <= to; from += U) {
-        Sum part[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) part[u] = load_row<T, VEC>(dout + (int64_t)order[from + u] * dim, c, dim);
-#pragma unroll
-        for (int s = 1; s < U; s *= 2)
-#pragma unroll
-            for (int u = 0; u < U; u += 2 * s) add(part[u], part[u + s]);
-        add(acc, part[0]);
-    }
-    for (; from < to; ++from) add(acc, load_row<T, VEC>(dout + (int64_t)order[from] * dim, c, dim));
+__device__ __forceinline__ Sum sum_run(const void* dout, const int32_t* __restrict__ order, int64_t from, int64_t to,
+                                       const Columns& c, int dim) {
+    return sum_rows<T, VEC>(from, to, c, dim,
+                            [&](int64_t i) { return static_cast<const T*>(dout) + (int64_t)order[i] * dim; });
 }
 
 // scale * acc, added to what the row holds or in its place.
@@ -280,7 +308,7 @@ __device__ __forceinline__ void put_sum(float* row, const Columns& cols, int dim
 
 struct GradArgs {
     const void* dout;
-    const int32_t *ids, *order, *start;
+    const int32_t *order, *sorted, *start;
     float *part, *dtable;
     int64_t vocab;
     int64_t long_blocks;  // the first workgroups: units of long runs
@@ -301,19 +329,17 @@ __device__ __forceinline__ void sum_unit(const GradArgs& a) {
     if (from >= n) return;
     const int32_t to = (int32_t)(from + a.unit < n ? from + a.unit : n);
     const Columns cols = columns_of(job % slabs, a.dim);
-    int32_t id = a.ids[a.order[from]];
+    int32_t id = a.sorted[from];
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
         if (side == 1) {
-            const int32_t next = a.ids[a.order[to - 1]];
+            const int32_t next = a.sorted[to - 1];
             if (next == id) return;
             id = next;
         }
         const int32_t x = a.start[id], y = a.start[id + 1];
         if (y - x <= 2 * a.unit) continue;
-        Sum acc{};
-        add_run<T, VEC>(static_cast<const T*>(a.dout), a.order, x > from ? x : (int32_t)from, y < to ? y : to, cols,
-                        a.dim, acc);
+        const Sum acc = sum_run<T, VEC>(a.dout, a.order, x > from ? x : from, y < to ? y : to, cols, a.dim);
         // a run that starts with the unit goes on through its start as well
         store_row<VEC>(a.part + (2 * c + (x > from)) * a.dim, cols, a.dim, acc);
     }
@@ -329,15 +355,15 @@ __global__ __launch_bounds__(256) void embed_rows(GradArgs a) {
     }
     const int64_t slabs = slabs_of(a.dim);
     const int64_t job = ((int64_t)blockIdx.x - a.long_blocks) * 4 + wave_id();
-    const int64_t p = job / slabs;
+    const int32_t p = (int32_t)(job / slabs);
     if (p >= a.start[a.vocab]) return;
-    const int32_t id = a.ids[a.order[p]];
-    const int32_t x = a.start[id], y = a.start[id + 1];
-    if (p != x || y - x > 2 * a.unit) return;  // long runs: embed_join
+    const int32_t id = a.sorted[p];
+    if (p > 0 && a.sorted[p - 1] == id) return;
+    const int32_t end = a.start[id + 1];
+    if (end - p > 2 * a.unit) return;  // long runs: embed_join
     const Columns cols = columns_of(job % slabs, a.dim);
-    Sum acc{};
-    add_run<T, VEC>(static_cast<const T*>(a.dout), a.order, x, y, cols, a.dim, acc);
-    put_sum<VEC, ADD>(a.dtable + (int64_t)id * a.dim, cols, a.dim, a.scale, acc);
+    put_sum<VEC, ADD>(a.dtable + (int64_t)id * a.dim, cols, a.dim, a.scale,
+                      sum_run<T, VEC>(a.dout, a.order, p, end, cols, a.dim));
 }
 
 // The rows of long runs, one wave per (unit, slab) in which such a run ends.
@@ -350,14 +376,14 @@ __global__ __launch_bounds__(256) void embed_join(GradArgs a) {
     if (from >= n) return;
     const int32_t to = (int32_t)(from + a.unit < n ? from + a.unit : n);
     // the run at the unit's start is the only long one that can end in it
-    const int32_t id = a.ids[a.order[from]];
+    const int32_t id = a.sorted[from];
     const int32_t x = a.start[id], y = a.start[id + 1];
     if (y - x <= 2 * a.unit || y > to) return;
     const Columns cols = columns_of(job % slabs, a.dim);
     const int64_t c1 = (y - 1) / a.unit;
-    Sum acc{};
-    for (int64_t c = x / a.unit; c <= c1; ++c)
-        add(acc, load_row<float, VEC>(a.part + (2 * c + (x > c * a.unit)) * a.dim, cols, a.dim));
+    const Sum acc = sum_rows<float, VEC>(x / a.unit, c1 + 1, cols, a.dim, [&](int64_t c) {
+        return a.part + (2 * c + (x > c * a.unit)) * a.dim;
+    });
     put_sum<VEC, ADD>(a.dtable + (int64_t)id * a.dim, cols, a.dim, a.scale, acc);
 }
 
@@ -375,8 +401,9 @@ int32_t unit_of(int64_t tokens) {
 EmbeddingWs embedding_bwd_ws(const mc_embedding_desc& d) {
     EmbeddingWs w{};
     size_t off = 0;
-    w.order = off;  off += align256((size_t)d.tokens * 4);
-    w.start = off;  off += align256(((size_t)d.vocab + 1) * 4);
+    w.order = off;   off += align256((size_t)d.tokens * 4);
+    w.sorted = off;  off += align256((size_t)d.tokens * 4);
+    w.start = off;   off += align256(((size_t)d.vocab + 1) * 4);
     const int64_t unit = unit_of(d.tokens);
     if (d.tokens > 2 * unit) {
         w.part = off;
@@ -409,33 +436,38 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
                                 bool accumulate, char* ws, hipStream_t stream) {
     const EmbeddingWs w = embedding_bwd_ws(d);
     int32_t* order = reinterpret_cast<int32_t*>(ws + w.order);
+    int32_t* sorted = reinterpret_cast<int32_t*>(ws + w.sorted);
     int32_t* start = reinterpret_cast<int32_t*>(ws + w.start);
     float* part = reinterpret_cast<float*>(ws + w.part);
     const int32_t unit = unit_of(d.tokens);
-    // workgroups that clear the gradient: two per CU, or one per 64 KB of it
     const int64_t clear = accumulate ? 0 : d.vocab * d.dim;
-    const int64_t clear_blocks = std::min<int64_t>((clear + (16 << 10) - 1) / (16 << 10), kClearBlocks);
     const int sort_blocks = (int)((d.vocab + kIds - 1) / kIds);
-    const dim3 gsort((unsigned)(sort_blocks + clear_blocks));
-    const int64_t steps = (d.tokens + kSortThreads - 1) / kSortThreads;  // of a wave
+    // the sort in as many waves as it takes, or in those that clear
+    const bool together = embedding_sort_while_clearing(d.tokens, clear);
+    const int threads = together ? 256 : 1024;
+    const int64_t steps = (d.tokens + threads - 1) / threads;  // of a wave
     auto sort = [&](auto ahead) {
         constexpr int AHEAD = decltype(ahead)::value;
-        if (embedding_stream_gradient(d.vocab, d.dim))
-            embed_sort<AHEAD, true><<<gsort, kSortThreads, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id,
-                                                                       order, start, sort_blocks, dtable, clear);
+        const int64_t beside = together ? (clear + 1023) / 1024 : 0;
+        const dim3 grid((unsigned)(sort_blocks + beside));
+        if (together)
+            embed_sort<4, AHEAD><<<grid, 256, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id, order, sorted,
+                                                          start, sort_blocks, dtable, clear);
         else
-            embed_sort<AHEAD, false><<<gsort, kSortThreads, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id,
-                                                                        order, start, sort_blocks, dtable, clear);
+            embed_sort<16, AHEAD><<<grid, 1024, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id, order, sorted,
+                                                            start, sort_blocks, dtable, 0);
     };
     if (steps <= 2) sort(std::integral_constant<int, 2>{});
     else if (steps <= 4) sort(std::integral_constant<int, 4>{});
     else if (steps <= 8) sort(std::integral_constant<int, 8>{});
     else sort(std::integral_constant<int, 16>{});
+    if (clear && !together)
+        embed_clear<<<dim3((unsigned)((clear + 1023) / 1024)), 256, 0, stream>>>(dtable, clear);
     const int64_t slabs = slabs_of(d.dim), units = (d.tokens + unit - 1) / unit;
     GradArgs a{};
     a.dout = dout;
-    a.ids = ids;
     a.order = order;
+    a.sorted = sorted;
     a.start = start;
     a.part = part;
     a.dtable = dtable;

@@ -10,12 +10,19 @@
 // alone, so results are bitwise reproducible.
 //
 // Bound by memory: the norm reads each gradient, the clipping reads it again and
-// writes it. grad_sumsq gives each workgroup a chunk of one tensor (the table of
-// tensors travels by value as a kernel argument: no device allocation, nothing
-// to keep alive for a captured graph) and one 64-bit partial sum; the chunks are
-// so long that there are at most about kParts of them. The workgroups of
-// grad_scale then each add up the partials themselves while their gradients are
-// on the way, in place of a launch between the two that does it for all.
+// writes it. 281M bf16 gradients to float32: 97 us for the norm (562 MB, 5.8 TB/s),
+// 288 for the clipping (562 MB read, 1.12 GB written, 5.9 TB/s); 1 to 6 MB: 8 us,
+// the two launches. The table of tensors travels by value as a kernel argument: no
+// device allocation, nothing to keep alive for a captured graph.
+//
+//  grad_sumsq      a chunk of one tensor per workgroup, one 64-bit partial sum.
+//  grad_norm_join  the partials' sum, the norm and the scale. Where there are few
+//                  partials the workgroups of grad_scale add them up themselves
+//                  while their gradients are on the way, and the launch is saved.
+//  grad_scale      one vector per thread: the workgroups of such a launch sweep
+//                  memory in order, which writes reach 6.2 TB/s at (workgroups of
+//                  32 KB and more 5.0: the device's writes are then spread over as
+//                  many places as it runs workgroups).
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -50,21 +57,24 @@ __device__ __forceinline__ double wg_sum64(double v, double* red) {
     return t;
 }
 
-// The slot of a workgroup: the last whose first workgroup is not past it.
+// The slot of a workgroup: the last whose first workgroup is not past it, from a
+// coarse index on (few dependent scalar loads: a workgroup lives for 2 us).
 template <typename Batch>
-__device__ __forceinline__ int slot_of(const Batch& b, int blk) {
-    int lo = 0, hi = b.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (b.slot[mid].blk0 <= blk) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
+__device__ __forceinline__ int slot_of(const Batch& b, uint32_t blk) {
+    int s = b.first[blk >> b.shift];
+    while (s + 1 < b.count && b.slot[s + 1].blk0 <= blk) ++s;
+    return s;
+}
+// Addresses in the tables carry the tensor's type in their lowest bit (elements
+// are 2 bytes or 4): 1 for bf16.
+__device__ __forceinline__ bool is_bf16(uint64_t at) { return at & 1; }
+template <typename T> __device__ __forceinline__ T* pointer(uint64_t at) {
+    return reinterpret_cast<T*>(at & ~(uint64_t)1);
 }
 
 template <typename T>
 __device__ __forceinline__ double sumsq_range(const T* __restrict__ p, int64_t n) {
-    constexpr int N = Vec<T>::N, U = 8;
+    constexpr int N = Vec<T>::N, U = 4;
     // elements before the first 16-byte boundary, then whole vectors, then the rest
     const int64_t mis = ((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T);
     const int64_t head = mis < n ? mis : n;
@@ -104,11 +114,11 @@ __device__ __forceinline__ double sumsq_range(const T* __restrict__ p, int64_t n
 
 __global__ __launch_bounds__(kThreads) void grad_sumsq(GradNormBatch b, double* __restrict__ parts) {
     __shared__ double red[kThreads / kWave];
-    const GradNormSlot& t = b.slot[slot_of(b, (int)blockIdx.x)];
-    const int64_t base = (int64_t)((int)blockIdx.x - t.blk0) * b.chunk;
+    const GradNormSlot& t = b.slot[slot_of(b, blockIdx.x)];
+    const uint32_t base = (blockIdx.x - t.blk0) * b.chunk;
     const int64_t n = t.n - base < b.chunk ? t.n - base : b.chunk;
-    const double s = t.dtype == MC_F32 ? sumsq_range(static_cast<const float*>(t.g) + base, n)
-                                       : sumsq_range(static_cast<const uint16_t*>(t.g) + base, n);
+    const double s = is_bf16(t.g) ? sumsq_range(pointer<const uint16_t>(t.g) + base, n)
+                                  : sumsq_range(pointer<const float>(t.g) + base, n);
     const double total = wg_sum64(s, red);
     if (threadIdx.x == 0) parts[blockIdx.x] = total;
 }
@@ -134,64 +144,63 @@ __global__ __launch_bounds__(kThreads) void grad_norm_join(const double* __restr
     }
 }
 
-// out = f g over n elements. N elements at a time where both sides are 16-byte
-// aligned at the same element; otherwise one, which still writes whole lines.
-template <typename TI, typename TO>
-__device__ __forceinline__ void scale_range(const TI* g, TO* out, int64_t n, float f) {
-    constexpr int N = 16 / (sizeof(TI) < sizeof(TO) ? sizeof(TI) : sizeof(TO));
-    constexpr int VI = N * sizeof(TI) / 16, VO = N * sizeof(TO) / 16, U = 2;
-    const int64_t head0 = ((16 - (reinterpret_cast<uintptr_t>(g) & 15)) & 15) / sizeof(TI);
-    const int64_t head1 = ((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / sizeof(TO);
-    const bool vec = sizeof(TI) == sizeof(TO) ? head0 == head1
-                                              : ((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    if (!vec) {
-        for (int64_t i = threadIdx.x; i < n; i += kThreads) Elem<TO>::store(out, i, Elem<TI>::load(g, i) * f);
+// Four elements as loaded and stored by one thread.
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) { Vec16<float>::load(p, v); }
+__device__ __forceinline__ void load4(const uint16_t* p, float (&v)[4]) {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_lo(q.x); v[1] = bf16_hi(q.x); v[2] = bf16_lo(q.y); v[3] = bf16_hi(q.y);
+}
+template <bool STREAM, typename V, typename T>
+__device__ __forceinline__ void put(T* p, const V& v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+    else *reinterpret_cast<V*>(p) = v;
+}
+template <bool STREAM> __device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+    put<STREAM>(p, f32x4{v[0], v[1], v[2], v[3]});
+}
+template <bool STREAM> __device__ __forceinline__ void store4(uint16_t* p, const float (&v)[4]) {
+    put<STREAM>(p, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+}
+
+// out = f g over the n <= kScaleElems elements of a workgroup. Four at a time where
+// both sides are aligned to their four, all of a thread's loads before its stores;
+// otherwise one, which still writes whole lines.
+constexpr int kScaleVecs = 4, kScaleElems = kThreads * 4 * kScaleVecs;
+template <bool STREAM, typename TI, typename TO>
+__device__ __forceinline__ void scale_range(const TI* g, TO* out, int n, float f) {
+    const uintptr_t gm = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(TI)), om = reinterpret_cast<uintptr_t>(out) % (4 * sizeof(TO));
+    if (gm != 0 || om != 0) {
+        for (int i = threadIdx.x; i < n; i += kThreads) Elem<TO>::store(out, i, Elem<TI>::load(g, i) * f);
         return;
     }
-    const int64_t head = head0 < n ? head0 : n;
-    const int64_t nv = (n - head) / N;
-    const uint4* src = reinterpret_cast<const uint4*>(g + head);
-    TO* dst = out + head;
-    auto emit = [&](int64_t i, const uint4 (&q)[VI]) {
-        float x[N];
+    const int i0 = (int)threadIdx.x * 4;
+    float v[kScaleVecs][4];
+    if (n == kScaleElems) {
 #pragma unroll
-        for (int k = 0; k < VI; ++k) {
-            float y[Vec<TI>::N];
-            Vec<TI>::unpack(q[k], y);
+        for (int u = 0; u < kScaleVecs; ++u) load4(g + i0 + u * kThreads * 4, v[u]);
 #pragma unroll
-            for (int e = 0; e < Vec<TI>::N; ++e) x[k * Vec<TI>::N + e] = y[e] * f;
+        for (int u = 0; u < kScaleVecs; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[u][e] *= f;
+            store4<STREAM>(out + i0 + u * kThreads * 4, v[u]);
         }
+        return;
+    }
+    for (int i = i0; i < n; i += kThreads * 4) {
+        if (i + 4 <= n) {
+            load4(g + i, v[0]);
 #pragma unroll
-        for (int k = 0; k < VO; ++k) {
-            float y[Vec16<TO>::N];
-#pragma unroll
-            for (int e = 0; e < Vec16<TO>::N; ++e) y[e] = x[k * Vec16<TO>::N + e];
-            Vec16<TO>::store(dst + i * N + k * Vec16<TO>::N, y);
+            for (int e = 0; e < 4; ++e) v[0][e] *= f;
+            store4<STREAM>(out + i, v[0]);
+        } else {
+            for (int e = i; e < n; ++e) Elem<TO>::store(out, e, Elem<TI>::load(g, e) * f);
         }
-    };
-    int64_t i = threadIdx.x;
-    for (; i + (U - 1) * kThreads < nv; i += U * kThreads) {
-        uint4 q[U][VI];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < VI; ++k) q[u][k] = src[(i + u * kThreads) * VI + k];
-#pragma unroll
-        for (int u = 0; u < U; ++u) emit(i + u * kThreads, q[u]);
     }
-    for (; i < nv; i += kThreads) {
-        uint4 q[VI];
-#pragma unroll
-        for (int k = 0; k < VI; ++k) q[k] = src[i * VI + k];
-        emit(i, q);
-    }
-    const int64_t tail = head + nv * N;
-    if ((int64_t)threadIdx.x < head) Elem<TO>::store(out, threadIdx.x, Elem<TI>::load(g, threadIdx.x) * f);
-    if (tail + threadIdx.x < n) Elem<TO>::store(out, tail + threadIdx.x, Elem<TI>::load(g, tail + threadIdx.x) * f);
 }
 
 // The scale is given (parts null), or formed from the norm's partials; then the
 // first workgroup of the first launch also writes norm and scale.
+template <bool STREAM>
 __global__ __launch_bounds__(kThreads) void grad_scale(GradScaleBatch b, const float* __restrict__ given,
                                                        const double* __restrict__ parts, int nparts, float max_norm,
                                                        float* __restrict__ norm, float* __restrict__ scale) {
@@ -207,110 +216,140 @@ __global__ __launch_bounds__(kThreads) void grad_scale(GradScaleBatch b, const f
     } else {
         f = *given;
     }
-    if (b.count == 0) return;
-    // backwards: the norm has left the last gradients that it read in the last-level cache
-    const int blk = (int)(gridDim.x - 1 - blockIdx.x);
-    const GradScaleSlot& t = b.slot[slot_of(b, blk)];
+    const GradScaleSlot& t = b.slot[slot_of(b, blockIdx.x)];
     if (f == 1.f && t.g == t.out) return;  // in place and nothing to clip
-    const int64_t base = (int64_t)(blk - t.blk0) * b.chunk;
-    const int64_t n = t.n - base < b.chunk ? t.n - base : b.chunk;
-    if (t.dtype == MC_F32) {
-        const float* g = static_cast<const float*>(t.g) + base;
-        if (t.out_dtype == MC_F32) scale_range(g, static_cast<float*>(t.out) + base, n, f);
-        else scale_range(g, static_cast<uint16_t*>(t.out) + base, n, f);
+    const uint32_t base = (blockIdx.x - t.blk0) * b.chunk;
+    const int n = (int)(t.n - base < b.chunk ? t.n - base : b.chunk);
+    if (is_bf16(t.g)) {
+        const uint16_t* g = pointer<const uint16_t>(t.g) + base;
+        if (is_bf16(t.out)) scale_range<STREAM>(g, pointer<uint16_t>(t.out) + base, n, f);
+        else scale_range<STREAM>(g, pointer<float>(t.out) + base, n, f);
     } else {
-        const uint16_t* g = static_cast<const uint16_t*>(t.g) + base;
-        if (t.out_dtype == MC_F32) scale_range(g, static_cast<float*>(t.out) + base, n, f);
-        else scale_range(g, static_cast<uint16_t*>(t.out) + base, n, f);
+        const float* g = pointer<const float>(t.g) + base;
+        if (is_bf16(t.out)) scale_range<STREAM>(g, pointer<uint16_t>(t.out) + base, n, f);
+        else scale_range<STREAM>(g, pointer<float>(t.out) + base, n, f);
     }
 }
 
-// Elements per workgroup: 32 KB of float32 at least, and few enough chunks that
-// every workgroup of the clipping can add their sums.
-constexpr int64_t kMinChunk = 8192, kParts = 1024;
+// Elements per workgroup of the norm: 32 KB of float32 at least, and at most about
+// kParts of them. 562 MB of bf16 in chunks of 544 KB / 137 KB / 16 KB: 95 / 94 / 90 us.
+constexpr int64_t kMinChunk = 8192, kParts = 4096;
+// Partials that every workgroup of the clipping adds up itself (2 per thread).
+constexpr int64_t kFewParts = 512;
+// Elements of a slot: offsets in it stay below 2^32, chunk multiples.
+constexpr int64_t kSlotElems = (int64_t)1 << 31;
+// Outputs past this go past the caches: the optimizer finds smaller ones there.
+constexpr double kStreamBytes = 256.0 * 1048576.0;
 
 int64_t total_of(const mc_grad_tensor* t, int32_t count) {
     int64_t n = 0;
     for (int32_t i = 0; i < count; ++i) n += t[i].numel;
     return n;
 }
-int64_t chunk_of(int64_t total, int64_t parts) {
-    const int64_t per = (total + parts - 1) / parts;
-    return per <= kMinChunk ? kMinChunk : (per + kMinChunk - 1) / kMinChunk * kMinChunk;
+int64_t chunk_of(int64_t total) {
+    const int64_t per = (total + kParts - 1) / kParts;
+    int64_t chunk = kMinChunk;  // a power of two: it divides kSlotElems
+    while (chunk < per && chunk < kSlotElems) chunk *= 2;
+    return chunk;
 }
 int64_t blocks_of(int64_t n, int64_t chunk) { return (n + chunk - 1) / chunk; }
+
+// Fills batches with the pieces of every tensor and calls launch(batch, blocks)
+// for each full one and the last. make(tensor, first element): the slot without
+// its size and first workgroup.
+template <typename Batch, typename Make, typename Launch>
+hipError_t for_batches(const mc_grad_tensor* t, int32_t count, int64_t chunk, Make&& make, Launch&& launch) {
+    Batch b;
+    b.count = 0;
+    b.chunk = (uint32_t)chunk;
+    int64_t blocks = 0;
+    auto flush = [&]() {
+        if (b.count == 0) return hipSuccess;
+        b.shift = 0;
+        while (((blocks - 1) >> b.shift) >= kGradIndex) ++b.shift;
+        int s = 0;
+        for (int i = 0; i < kGradIndex; ++i) {
+            while (s + 1 < b.count && b.slot[s + 1].blk0 <= (uint64_t)i << b.shift) ++s;
+            b.first[i] = (uint8_t)s;
+        }
+        const hipError_t e = launch(b, (unsigned)blocks);
+        b.count = 0;
+        blocks = 0;
+        return e;
+    };
+    for (int32_t i = 0; i < count; ++i)
+        for (int64_t at = 0; at < t[i].numel; at += kSlotElems) {
+            const int64_t n = t[i].numel - at < kSlotElems ? t[i].numel - at : kSlotElems;
+            // a launch holds at most 2^32 - 1 work-items
+            if (blocks + blocks_of(n, chunk) > 16777215) {
+                const hipError_t e = flush();
+                if (e != hipSuccess) return e;
+            }
+            auto slot = make(t[i], at);
+            slot.n = (uint32_t)n;
+            slot.blk0 = (uint32_t)blocks;
+            b.slot[b.count++] = slot;
+            blocks += blocks_of(n, chunk);
+            if (b.count == Batch::kSlots) {
+                const hipError_t e = flush();
+                if (e != hipSuccess) return e;
+            }
+        }
+    return flush();
+}
+
+uint64_t tagged(const void* p, int64_t at, int32_t dtype) {
+    return (reinterpret_cast<uint64_t>(p) + (uint64_t)at * (dtype == MC_F32 ? 4 : 2)) | (dtype == MC_BF16 ? 1 : 0);
+}
+
+hipError_t launch_sumsq(const mc_grad_tensor* t, int32_t count, double* parts, hipStream_t stream) {
+    return for_batches<GradNormBatch>(
+        t, count, chunk_of(total_of(t, count)),
+        [](const mc_grad_tensor& x, int64_t at) { return GradNormSlot{tagged(x.grad, at, x.dtype), 0, 0}; },
+        [&](const GradNormBatch& b, unsigned blocks) {
+            grad_sumsq<<<dim3(blocks), kThreads, 0, stream>>>(b, parts);
+            parts += blocks;
+            return hipGetLastError();
+        });
+}
+
+hipError_t launch_join(const double* parts, int64_t n, float max_norm, float* norm, float* scale, hipStream_t stream) {
+    grad_norm_join<<<1, kThreads, 0, stream>>>(parts, (int)n, max_norm, norm, scale);
+    return hipGetLastError();
+}
+
+hipError_t launch_scale(const mc_grad_tensor* t, int32_t count, const float* given, const double* parts, int nparts,
+                        float max_norm, float* norm, float* scale, hipStream_t stream) {
+    double bytes = 0.0;
+    for (int32_t i = 0; i < count; ++i) bytes += (double)t[i].numel * (t[i].out_dtype == MC_F32 ? 4.0 : 2.0);
+    return for_batches<GradScaleBatch>(
+        t, count, kScaleElems,
+        [](const mc_grad_tensor& x, int64_t at) {
+            return GradScaleSlot{tagged(x.grad, at, x.dtype), tagged(x.out, at, x.out_dtype), 0, 0};
+        },
+        [&](const GradScaleBatch& b, unsigned blocks) {
+            if (bytes > kStreamBytes)
+                grad_scale<true><<<dim3(blocks), kThreads, 0, stream>>>(b, given, parts, nparts, max_norm, norm, scale);
+            else
+                grad_scale<false><<<dim3(blocks), kThreads, 0, stream>>>(b, given, parts, nparts, max_norm, norm, scale);
+            norm = nullptr;  // written by the first launch
+            return hipGetLastError();
+        });
+}
 
 }  // namespace
 
 int64_t gradient_parts(const mc_grad_tensor* t, int32_t count) {
-    const int64_t chunk = chunk_of(total_of(t, count), kParts);
+    const int64_t chunk = chunk_of(total_of(t, count));
     int64_t n = 0;
     for (int32_t i = 0; i < count; ++i) n += blocks_of(t[i].numel, chunk);
     return n;
 }
 
-static hipError_t launch_sumsq(const mc_grad_tensor* t, int32_t count, double* parts, hipStream_t stream) {
-    const int64_t chunk = chunk_of(total_of(t, count), kParts);
-    GradNormBatch b;
-    b.count = 0;
-    b.chunk = chunk;
-    int64_t blocks = 0;
-    auto flush = [&]() {
-        if (b.count == 0) return hipSuccess;
-        grad_sumsq<<<dim3((unsigned)blocks), kThreads, 0, stream>>>(b, parts);
-        parts += blocks;
-        b.count = 0;
-        blocks = 0;
-        return hipGetLastError();
-    };
-    for (int32_t i = 0; i < count; ++i) {
-        if (t[i].numel == 0) continue;
-        b.slot[b.count++] = GradNormSlot{t[i].grad, t[i].numel, (int)blocks, t[i].dtype};
-        blocks += blocks_of(t[i].numel, chunk);
-        if (b.count == kGradNormSlots) {
-            const hipError_t e = flush();
-            if (e != hipSuccess) return e;
-        }
-    }
-    return flush();
-}
-
 hipError_t launch_gradient_norm(const mc_grad_tensor* t, int32_t count, float max_norm, float* norm, float* scale,
                                 double* parts, hipStream_t stream) {
     const hipError_t e = launch_sumsq(t, count, parts, stream);
-    if (e != hipSuccess) return e;
-    grad_norm_join<<<1, kThreads, 0, stream>>>(parts, (int)gradient_parts(t, count), max_norm, norm, scale);
-    return hipGetLastError();
-}
-
-static hipError_t launch_scale(const mc_grad_tensor* t, int32_t count, const float* given, const double* parts,
-                               int nparts, float max_norm, float* norm, float* scale, hipStream_t stream) {
-    // a round or two of the CUs' workgroups
-    const int64_t chunk = chunk_of(total_of(t, count), 4096);
-    GradScaleBatch b;
-    b.count = 0;
-    b.chunk = chunk;
-    int64_t blocks = 0;
-    bool first = true;
-    auto flush = [&]() {
-        grad_scale<<<dim3((unsigned)(blocks ? blocks : 1)), kThreads, 0, stream>>>(b, given, parts, nparts, max_norm,
-                                                                                  first ? norm : nullptr, scale);
-        first = false;
-        b.count = 0;
-        blocks = 0;
-        return hipGetLastError();
-    };
-    for (int32_t i = 0; i < count; ++i) {
-        if (t[i].numel == 0) continue;
-        b.slot[b.count++] = GradScaleSlot{t[i].grad, t[i].out, t[i].numel, (int)blocks, (int16_t)t[i].dtype,
-                                          (int16_t)t[i].out_dtype};
-        blocks += blocks_of(t[i].numel, chunk);
-        if (b.count == kGradScaleSlots) {
-            const hipError_t e = flush();
-            if (e != hipSuccess) return e;
-        }
-    }
-    return b.count > 0 || (first && norm) ? flush() : hipSuccess;
+    return e != hipSuccess ? e : launch_join(parts, gradient_parts(t, count), max_norm, norm, scale, stream);
 }
 
 hipError_t launch_scale_gradients(const mc_grad_tensor* t, int32_t count, const float* scale, hipStream_t stream) {
@@ -319,9 +358,12 @@ hipError_t launch_scale_gradients(const mc_grad_tensor* t, int32_t count, const 
 
 hipError_t launch_clip_gradients(const mc_grad_tensor* t, int32_t count, float max_norm, float* norm, float* scale,
                                  double* parts, hipStream_t stream) {
-    const hipError_t e = launch_sumsq(t, count, parts, stream);
+    hipError_t e = launch_sumsq(t, count, parts, stream);
     if (e != hipSuccess) return e;
-    return launch_scale(t, count, nullptr, parts, (int)gradient_parts(t, count), max_norm, norm, scale, stream);
+    const int64_t n = gradient_parts(t, count);
+    if (n <= kFewParts) return launch_scale(t, count, nullptr, parts, (int)n, max_norm, norm, scale, stream);
+    e = launch_join(parts, n, max_norm, norm, scale, stream);
+    return e != hipSuccess ? e : launch_scale(t, count, scale, nullptr, 0, 0.f, nullptr, nullptr, stream);
 }
 
 }  // namespace mc

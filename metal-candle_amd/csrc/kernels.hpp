@@ -220,30 +220,31 @@ int adamw_blocks(int64_t n);  // workgroups one tensor of n elements takes
 hipError_t launch_adamw(const AdamWBatch& batch, int blocks, const float* grad_scale, hipStream_t stream);
 
 // ------------------------------------------------------ gradients' norm
-// The tables travel by value as kernel arguments (under 4 KB); blk0: first
-// workgroup of the slot, each of `chunk` elements.
-constexpr int kGradNormSlots = 160, kGradScaleSlots = 120;
+// The tables travel by value as kernel arguments (under 4 KB). g, out: addresses
+// with the type in the lowest bit; blk0: the slot's first workgroup, of `chunk`
+// elements each; first[i]: the slot of workgroup i << shift.
+constexpr int kGradIndex = 64;
 struct GradNormSlot {
-    const void* g;
-    int64_t n;
-    int blk0, dtype;
+    uint64_t g;
+    uint32_t n, blk0;
 };
 struct GradNormBatch {
-    GradNormSlot slot[kGradNormSlots];
-    int64_t chunk;
-    int count, pad;
+    static constexpr int kSlots = 240;
+    GradNormSlot slot[kSlots];
+    uint8_t first[kGradIndex];
+    uint32_t chunk;
+    int count, shift;
 };
 struct GradScaleSlot {
-    const void* g;
-    void* out;
-    int64_t n;
-    int blk0;
-    int16_t dtype, out_dtype;
+    uint64_t g, out;
+    uint32_t n, blk0;
 };
 struct GradScaleBatch {
-    GradScaleSlot slot[kGradScaleSlots];
-    int64_t chunk;
-    int count, pad;
+    static constexpr int kSlots = 160;
+    GradScaleSlot slot[kSlots];
+    uint8_t first[kGradIndex];
+    uint32_t chunk;
+    int count, shift;
 };
 int64_t gradient_parts(const mc_grad_tensor* t, int32_t count);  // f64 partial sums in the workspace
 hipError_t launch_gradient_norm(const mc_grad_tensor* t, int32_t count, float max_norm, float* norm, float* scale,
@@ -254,9 +255,10 @@ hipError_t launch_clip_gradients(const mc_grad_tensor* t, int32_t count, float m
 
 // -------------------------------------------------------------- embedding
 struct EmbeddingWs {
-    size_t order;  // int32 [tokens]
-    size_t start;  // int32 [vocab + 1]
-    size_t part;   // f32 [units][2][dim], where a run can be longer than two units
+    size_t order;   // int32 [tokens]
+    size_t sorted;  // int32 [tokens]
+    size_t start;   // int32 [vocab + 1]
+    size_t part;    // f32 [units][2][dim], where a run can be longer than two units
     size_t total;
 };
 EmbeddingWs embedding_bwd_ws(const mc_embedding_desc& d);

@@ -107,13 +107,10 @@ constexpr LossGrid loss_grad_grid(int64_t rows, int64_t row_bytes) {
     return LossGrid{row_bytes < 28 << 10 || rows <= 64 ? 512 : 1024, (unsigned)(wanted < most ? wanted : most)};
 }
 
-// The embedding's gradient stored past the caches: rows of whole 128-byte lines, a
-// table well over what the caches keep for the optimizer that reads it. Backward,
-// us, streamed / ordinary, 151936 rows of 1536 after 16384 tokens: 202 / 226; rows of
-// 893 floats, whose ends share lines, 50257 of them: 52 / 36.
-constexpr bool embedding_stream_gradient(int64_t vocab, int64_t dim) {
-    return dim % 32 == 0 && vocab * dim * 4 > (int64_t)256 << 20;
-}
+// The embedding's backward sorts its tokens in workgroups of 256 threads beside
+// those that clear the gradient, where the clearing (6.8 TB/s) takes as long as that
+// sort (1.9 us per 1024 tokens, 0.7 in workgroups of 1024); else one after the other.
+constexpr bool embedding_sort_while_clearing(int64_t tokens, int64_t clear) { return clear * 4 >= tokens * 12288; }
 
 // Softmax rows that are not whole 16-byte vectors: the covering vectors of the
 // one-wave kernels, or for short rows a lane per element (the scalar kernels),

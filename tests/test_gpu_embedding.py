@@ -64,7 +64,7 @@ def test_forward_and_backward(mc, dev, nan_outputs, T, V, D, dtype):
 
 
 @pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 136), (torch.float32, 37), (torch.bfloat16, 5)])
-@pytest.mark.parametrize("name", ["one_token", "two_runs", "unit_borders", "long_between", "unsorted_runs", "last_id"])
+@pytest.mark.parametrize("name", ["one_token", "two_runs", "unit_borders", "short_units", "long_between", "unsorted_runs", "last_id"])
 def test_long_runs(mc, dev, name, dtype, D):
     """Runs past two units of 64 sorted tokens: their units' sums, at every place of a run's ends in a unit."""
     V = 700
@@ -72,6 +72,7 @@ def test_long_runs(mc, dev, name, dtype, D):
         "one_token": [3] * 3001,
         "two_runs": [5] * 129 + [6] * 700,
         "unit_borders": [1] * 64 + [2] * 192 + [3] * 128 + [4] * 129 + [511] * 63 + [512] * 256,
+        "short_units": [1] * 16 + [2] * 32 + [3] * 33 + [4] * 31 + [5] * 48 + [6] * 47 + [7] * 49 + [8] * 34,
         "long_between": [0] * 20 + [9] * 500 + [10, 11, 12] + [13] * 300 + [14] * 5,
         "unsorted_runs": [i % 4 * 170 for i in range(2000)],
         "last_id": [V - 1] * 1000 + [V - 2] * 10,

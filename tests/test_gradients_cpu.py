@@ -80,13 +80,14 @@ def test_gradient_table_abi(mc):
 
 
 def test_gradient_partials(mc):
-    """Chunks of 8192 elements, longer ones where there would be more than about 1024 of them."""
+    """Chunks of 8192 elements, longer ones where there would be more than about 4096 of them."""
     L = mc._lib.lib()
     size = L.mc_gradient_norm_workspace_size
     assert size(table(mc, (256, 0, 8192, 0, 0)), 1) == 8
     assert size(table(mc, (256, 0, 8193, 1, 0)), 1) == 16
-    assert size(table(mc, (256, 0, 1024 * 8192, 0, 0)), 1) == 1024 * 8
-    assert size(table(mc, (256, 0, 1024 * 8192 + 1, 0, 0)), 1) == 513 * 8
+    assert size(table(mc, (256, 0, 4096 * 8192, 0, 0)), 1) == 4096 * 8
+    assert size(table(mc, (256, 0, 4096 * 8192 + 1, 0, 0)), 1) == 2049 * 8
+    assert size(table(mc, (256, 0, 2**34, 1, 0)), 1) == 4096 * 8
     assert size(table(mc, (None, 0, 0, 0, 0)), 1) == 0
 
 
@@ -137,10 +138,13 @@ def test_embedding_abi(mc):
     assert bwd(desc(), dout=None) == NULL and bwd(desc(), dtable=None) == NULL
     assert bwd(desc(), dout=ctypes.c_void_p(264)) == LAYOUT and bwd(desc(), dtable=ctypes.c_void_p(264)) == LAYOUT
     assert bwd(desc(), add=2) == VALUE
+    assert bwd(desc(vocab=2**24, dim=1024)) == SHAPE
+    assert bwd(desc(vocab=2**31 - 1, dim=1)) == SHAPE
     assert bwd(desc(tokens=2**26, dim=512)) == SHAPE and "too large for a launch" in mc._lib.last_error()
     need = L.mc_embedding_bwd_workspace_size(desc())
-    assert need == 256 + 512  # order and start; no run of 8 tokens is long
-    assert bwd(desc(), have=need - 1) == WORKSPACE and bwd(desc(), ws=None) == WORKSPACE
+    assert need == 256 + 256 + 512  # order, ids and start; no run of 8 tokens is long
+    assert L.mc_embedding_bwd_workspace_size(desc(tokens=128)) == 512 + 512 + 512
     # 129 tokens are three units of 64, with two sums of 16 columns each
-    assert L.mc_embedding_bwd_workspace_size(desc(tokens=129)) == 768 + 512 + 512
+    assert L.mc_embedding_bwd_workspace_size(desc(tokens=129)) == 768 + 768 + 512 + 512
+    assert bwd(desc(), have=need - 1) == WORKSPACE and bwd(desc(), ws=None) == WORKSPACE
     assert L.mc_embedding_bwd_workspace_size(desc(tokens=0)) == 0

@@ -60,23 +60,24 @@ constexpr int kScanTurn = kScanThreads * kItems;  // tokens per turn
 template <bool AFTER>
 __device__ __forceinline__ int nearest_mark(int mark, int& carry, int* slots) {
     const int lane = lane_id(), wave = wave_id();
-    auto from = [&](int v, int s) { return AFTER ? __shfl_down(v, s, kWave) : __shfl_up(v, s, kWave); };
-    int m = mark;
-#pragma unroll
-    for (int s = 1; s < kWave; s <<= 1) {
-        const int x = from(m, s);
-        m = m < 0 && (AFTER ? lane + s < kWave : lane >= s) ? x : m;
-    }
-    if (lane == (AFTER ? 0 : kWave - 1)) slots[wave] = m;
+    const uint64_t marked = __ballot(mark >= 0);
+    const uint64_t there = AFTER ? marked >> lane >> 1 : marked & (((uint64_t)1 << lane) - 1);
+    const int from = there == 0 ? lane : AFTER ? lane + 1 + __builtin_ctzll(there) : 63 - __builtin_clzll(there);
+    const int near = __shfl(mark, from, kWave);
+    // the mark of a wave that others see, and of each wave in lane w of 16
+    auto outer = [](int v, uint64_t lanes, int none) {
+        const int l = lanes == 0 ? 0 : AFTER ? __builtin_ctzll(lanes) : 63 - __builtin_clzll(lanes);
+        const int x = __builtin_amdgcn_readlane(v, l);
+        return lanes == 0 ? none : x;
+    };
+    if (lane == 0) slots[wave] = outer(mark, marked, -1);
     __syncthreads();
-    int near = from(m, 1), other = carry;
-#pragma unroll
-    for (int i = 0; i < kScanWaves; ++i) {
-        const int w = AFTER ? kScanWaves - 1 - i : i, x = slots[w];
-        other = x >= 0 && (AFTER ? w > wave : w < wave) ? x : other;
-        carry = x >= 0 ? x : carry;
-    }
-    return lane != (AFTER ? kWave - 1 : 0) && near >= 0 ? near : other;
+    const int of_wave = slots[lane % kScanWaves];
+    const uint64_t waves = __ballot(of_wave >= 0) & ((1 << kScanWaves) - 1);
+    const uint64_t beyond = AFTER ? waves >> wave >> 1 << wave << 1 : waves & (((uint64_t)1 << wave) - 1);
+    const int other = outer(of_wave, beyond, carry);
+    carry = outer(of_wave, waves, carry);
+    return there == 0 ? other : near;
 }
 
 __global__ __launch_bounds__(kScanThreads) void packed_spans(const int32_t* __restrict__ documents,
@@ -737,6 +738,7 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32;
     constexpr int TILE = 64 * D;                 // one [64][D] tile
     constexpr int STAGE = 2 * TILE + 512;        // Q, dO, lse/Delta (1 KB)
+    constexpr int kDsStores = 8;                 // of dS^T per step and wave
     constexpr int KV = 2 * 128 * D;              // the workgroup's K and V rows, [128][D] each, after the stages
     constexpr int PATCH = 4 * 32 * (D + 8) * 2;  // the epilogue's, over the stages
     constexpr int SMEM = 2 * STAGE + KV > PATCH ? 2 * STAGE + KV : PATCH;
@@ -840,8 +842,11 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
     bad_k = __syncthreads_or(bad_k);
     if (threadIdx.x == 0) a.kflags[bhk * a.nblk + kb] = bad_k;  // alike from every group
     int h = h0, qb = kd, left = nq;  // of this head
+    float slope2 = BIAS ? a.slopes[h0] * kLog2e : 0.f;  // its load waits for every store before it: once per head
     for (int it = 0; it < nit; ++it) {
-        wait_vmcnt<0>();
+        // step it has landed: behind it only the last step's stores of dS^T went out
+        // (the first's were waited for)
+        wait_vmcnt<kDsStores>();
         __syncthreads();
         const bool wrap = --left == 0;
         const int next_h = wrap ? h + 1 : h, next_qb = wrap ? kd : qb + 1 == qend ? qstart : qb + 1;
@@ -860,7 +865,6 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
         // Every wave runs every block, masked where its keys do not meet it.
         const int q0 = qb * 64;
         const bool edge = !(q0 >= ws.all_lo && q0 + 64 <= ws.all_hi);
-        const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
 
         // accumulator j of tile t: query q0 + 32 t + 8 (j/4) + 4 half + j%4, key my_key.
         // P and dS of query tile t; EDGE hides what this lane's key does not meet.
@@ -934,19 +938,18 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
             bf16x8 pb[2], db[2];
             if (edge) scores(std::true_type{}, t_tag, sacc, dpacc, pb, db);
             else scores(std::false_type{}, t_tag, sacc, dpacc, pb, db);
-            if (a.dst) {
-                // dS^T: elements 4 hh .. 4 hh + 3 of db[kk] are queries
-                // q0 + 32 t + 16 kk + 8 hh + 4 half + 0..3 of this lane's key;
-                // keys past S fall outside the buffer range and are dropped
+            // dS^T: elements 4 hh .. 4 hh + 3 of db[kk] are queries
+            // q0 + 32 t + 16 kk + 8 hh + 4 half + 0..3 of this lane's key; keys past S,
+            // and all where packed_dq_again forms dS, fall outside the buffer range and
+            // are dropped. kDsStores per step, which its first wait counts on.
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    const uint4 w4 = __builtin_bit_cast(uint4, db[kk]);
+            for (int kk = 0; kk < 2; ++kk) {
+                const uint4 w4 = __builtin_bit_cast(uint4, db[kk]);
 #pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        const int64_t qq = q0 + 32 * t + 16 * kk + 8 * hh + 4 * half;
-                        const u32x2 v2 = {hh ? w4.z : w4.x, hh ? w4.w : w4.y};
-                        __builtin_amdgcn_raw_buffer_store_b64(v2, rds, (int)(uint32_t)((my_key * a.ldst + qq) * 2), 0, 0);
-                    }
+                for (int hh = 0; hh < 2; ++hh) {
+                    const int64_t qq = q0 + 32 * t + 16 * kk + 8 * hh + 4 * half;
+                    const u32x2 v2 = {hh ? w4.z : w4.x, hh ? w4.w : w4.y};
+                    __builtin_amdgcn_raw_buffer_store_b64(v2, rds, (int)(uint32_t)((my_key * a.ldst + qq) * 2), 0, 0);
                 }
             }
             // dO^T and Q^T fragments one step ahead of their MFMAs; step u = 2 dt + kk
@@ -972,6 +975,8 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
         };
         tile(std::integral_constant<int, 0>{});
         tile(std::integral_constant<int, 1>{});
+        if constexpr (BIAS)
+            if (wrap && it + 1 < nit) slope2 = a.slopes[next_h] * kLog2e;
         h = next_h;
         qb = next_qb;
     }

@@ -928,7 +928,7 @@ def _tensors(group, name):
     return dtypes, list(map(torch.Tensor.numel, group)), list(map(torch.Tensor.data_ptr, group)), group[0].device
 
 
-def _grad_table(grads, outs):
+def _grad_table(grads, outs, written=True):
     """(address of the mc_grad_tensor table, its length, what keeps it alive) of gradients and where they go."""
     dtypes, sizes, at, device = _tensors(grads, "grads")
     to, out_dtypes = at, dtypes
@@ -941,6 +941,8 @@ def _grad_table(grads, outs):
             raise McError(_lib.MC_ERR_SHAPE, f"outs[{i}] has {out_sizes[i]} elements, expected {sizes[i]}")
         if out_device != device:
             raise McError(_lib.MC_ERR_LAYOUT, f"outs are on {out_device}, expected {device}")
+    if written and len(set(to)) < len(to) and len({p for p, n in zip(to, sizes) if n}) < sum(map(bool, sizes)):
+        raise McError(_lib.MC_ERR_LAYOUT, "a tensor is listed twice: it would be scaled twice")
     if len(set(dtypes)) == 1 and len(set(out_dtypes)) == 1:
         codes = itertools.repeat(_DTYPES[dtypes[0]] | _DTYPES[out_dtypes[0]] << 32)
     else:
@@ -955,7 +957,7 @@ def gradient_norm(grads, max_norm=None):
 
     norm = sqrt(sum of all squares), summed in 64 bits in a fixed order; scale = 1 where norm <= max_norm, else
     max_norm / norm. Pass scale to scale_gradients, or to adamw_step, which then clips as it reads."""
-    at, n, table = _grad_table(grads, None)
+    at, n, table = _grad_table(grads, None, written=False)
     dev = grads[0].device
     norm = torch.empty(1, dtype=torch.float32, device=dev)
     scale = None if max_norm is None else torch.empty(1, dtype=torch.float32, device=dev)

@@ -79,6 +79,22 @@ def test_gradient_table_abi(mc):
     assert L.mc_scale_gradients(None, 0, FAKE, None) == 0
 
 
+def test_same_tensor_twice(mc):
+    """It would be scaled twice or once, as the workgroups come; the norm may count it twice."""
+    a, b, empty = torch.ones(64), torch.ones(64), torch.ones(0)
+    scale = torch.ones(1)
+    raises(mc, LAYOUT, "listed twice", mc.clip_gradients, [a, b, a], 1.0)
+    raises(mc, LAYOUT, "listed twice", mc.scale_gradients, [a, b, a], scale)
+    raises(mc, LAYOUT, "listed twice", mc.clip_gradients, [b, b.clone(), b.clone()], 1.0, outs=[a, torch.ones(64), a])
+    # several empty tensors share the address 0: the call goes on to what refuses the CPU
+    with pytest.raises(Exception) as e:
+        mc.scale_gradients([a, empty, empty], scale)
+    assert "twice" not in str(e.value)
+    with pytest.raises(Exception) as e:
+        mc.gradient_norm([a, a])
+    assert "twice" not in str(e.value)
+
+
 def test_gradient_partials(mc):
     """Chunks of 8192 elements, longer ones where there would be more than about 4096 of them."""
     L = mc._lib.lib()

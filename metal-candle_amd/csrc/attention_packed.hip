@@ -31,6 +31,24 @@
 // The cap. With r = 1 / (1 + 2^(2 log2 e x / cap)), tanh(x / cap) = 1 - 2 r and
 // its slope is 4 (r - r^2): one exponential and one reciprocal more per score.
 // tanh grows with x, so the running maximum stays one of unscaled products.
+//
+// What bounds them, with us per call: (a) 4 x 28 x 4096 x 128, capped, one causal
+// document a row; (b) 8 x 12 x 2048 x 128 in documents of 345 tokens, a mean of 24 of
+// the 40 blocks of 64 x 128 pairs per CU visible; (c) 3 x 14 x 1021 x 64 in documents
+// of 156 tokens with prompts and a bias.
+//               (a)    (b)   (c)
+//  packed_spans        5.6   4.8   two scans of a row by one workgroup: latency
+//  packed_vt    10     7.1   3.6   memory
+//  packed_fwd   664    70    17    (a) 725 TFLOP/s: the scores' arithmetic, of whose
+//                                  time the cap's exponential and reciprocal are half
+//  packed_prep  52     37    12    (a) memory; (b, c) S and dP once more
+//  packed_dkdv  1582   165   28    one wave per SIMD: MFMA 31% of its cycles, scores
+//                                  37, waits 27, which follow each other (the scores
+//                                  of one query tile among the other's MFMAs: 1800
+//                                  and more, for what is moved between registers;
+//                                  tiles three steps ahead, fragments two or three:
+//                                  no change)
+//  packed_dq    458    64    12    (a) memory: dS^T, 1.9 GB, at 4.1 TB/s
 #include <algorithm>
 #include <type_traits>
 

@@ -8,6 +8,10 @@
 // by the float32 matrix rate, beside which the arithmetic of the cap is small: it
 // is chosen at run time, and its tanh is exact to about 2^-23.
 //
+// 4 x 12 (2) x 509 x 64 in documents of 75 tokens, capped: forward 25 us, dQ 35, dK/dV
+// 46, its groups' sum 5: 768 workgroups each, all resident, whose waves have one or two
+// blocks of 32 x 32 pairs: a chain of loads, products, scores and the waves' join.
+//
 // Row kernels (bf16 head dims other than 64 and 128, float32 ones that are no
 // multiple of 4 or past 128, and float32 rows of a few tokens): one wave per row,
 // lanes over the head dim, only what the row sees is read.

@@ -42,13 +42,13 @@
 //  packed_fwd   664    70    17    (a) 725 TFLOP/s: the scores' arithmetic, of whose
 //                                  time the cap's exponential and reciprocal are half
 //  packed_prep  52     37    12    (a) memory; (b, c) S and dP once more
-//  packed_dkdv  1582   165   28    one wave per SIMD: MFMA 31% of its cycles, scores
+//  packed_dkdv  1467   155   27    one wave per SIMD: MFMA 31% of its cycles, scores
 //                                  37, waits 27, which follow each other (the scores
 //                                  of one query tile among the other's MFMAs: 1800
 //                                  and more, for what is moved between registers;
 //                                  tiles three steps ahead, fragments two or three:
 //                                  no change)
-//  packed_dq    458    64    12    (a) memory: dS^T, 1.9 GB, at 4.1 TB/s
+//  packed_dq    452    65    12    (a) memory: dS^T, 1.9 GB, at 4.2 TB/s
 #include <algorithm>
 #include <type_traits>
 
@@ -273,8 +273,8 @@ struct PackedArgs {
     int32_t* kflags;       // backward: [B, Hkv, nblk], blocks of 128 rows of K
     uint16_t *dq, *dk, *dv;
     float *dk_part, *dv_part;  // [B, Hkv, ngroups, S, D]
-    uint16_t* dst;             // [B, H, S, ldst]: dS^T, key rows
-    int64_t ldst, dq_blocks, sum_n8;
+    uint16_t* dst;             // dS^T: [B, H] of head_ds bytes (kDsBlock), or null
+    int64_t head_ds, dq_blocks, sum_n8;
     int64_t S, Sp;
     int ngroups, B, H, Hkv, D, nblk, causal;
     float scale;       // of dq and dk (with a cap 4 times the scores')
@@ -282,6 +282,22 @@ struct PackedArgs {
     float cap_in;      // 2 log2 e scale / cap
     float cap_log2;    // cap log2 e
 };
+
+// dS^T in memory, in the order in which the dK/dV waves hold it, so that each of their
+// stores and each of the dQ pass's loads is 1 KB in a row (as key rows of queries a
+// store was 64 pieces of 8 bytes, and a seventh of the kernel's time): per head blocks
+// of 32 keys x 64 queries, in a block 16-query steps 2 t + kk, in a step lane (half,
+// key), in a lane the 8 queries from 8 half on. The blocks of 128 queries, which one
+// dQ workgroup reads, follow each other by keys (all queries of 32 keys together:
+// strides of a power of two between its reads, 472 us in place of 452).
+constexpr int kDsBlock = 32 * 64 * 2;  // bytes
+__device__ __forceinline__ uint32_t ds_block(int q64, int k32, int nblk) {
+    return ((uint32_t)((q64 >> 1) * 4 * nblk + k32) * 2u + (uint32_t)(q64 & 1)) * kDsBlock;
+}
+__host__ __device__ inline int64_t head_ds_bytes(int64_t S) {
+    const int64_t nblk = (S + 127) / 128;
+    return 4 * nblk * 2 * nblk * kDsBlock;
+}
 
 // Scores in log2 units from a product s.
 template <bool CAP>
@@ -756,7 +772,7 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
     constexpr int KS = D / 16, DT = D / 32;
     constexpr int TILE = 64 * D;                 // one [64][D] tile
     constexpr int STAGE = 2 * TILE + 512;        // Q, dO, lse/Delta (1 KB)
-    constexpr int kDsStores = 8;                 // of dS^T per step and wave
+    constexpr int kDsStores = 4;                 // of dS^T per step and wave
     constexpr int KV = 2 * 128 * D;              // the workgroup's K and V rows, [128][D] each, after the stages
     constexpr int PATCH = 4 * 32 * (D + 8) * 2;  // the epilogue's, over the stages
     constexpr int SMEM = 2 * STAGE + KV > PATCH ? 2 * STAGE + KV : PATCH;
@@ -879,7 +895,8 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
         }
         const int64_t bh = (int64_t)b * a.H + h;
         const __amdgpu_buffer_rsrc_t rds =
-            make_rsrc(a.dst ? a.dst + bh * S * a.ldst : nullptr, a.dst ? S * a.ldst * 2 : 0);
+            make_rsrc(a.dst ? a.dst + bh * (a.head_ds / 2) : nullptr, a.dst ? a.head_ds : 0);
+        const uint32_t ds_off = ds_block(qb, 4 * kb + wave, a.nblk) + (uint32_t)lane * 16u;
         // Every wave runs every block, masked where its keys do not meet it.
         const int q0 = qb * 64;
         const bool edge = !(q0 >= ws.all_lo && q0 + 64 <= ws.all_hi);
@@ -957,18 +974,18 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
             if (edge) scores(std::true_type{}, t_tag, sacc, dpacc, pb, db);
             else scores(std::false_type{}, t_tag, sacc, dpacc, pb, db);
             // dS^T: elements 4 hh .. 4 hh + 3 of db[kk] are queries
-            // q0 + 32 t + 16 kk + 8 hh + 4 half + 0..3 of this lane's key; keys past S,
-            // and all where packed_dq_again forms dS, fall outside the buffer range and
-            // are dropped. kDsStores per step, which its first wait counts on.
+            // q0 + 32 t + 16 kk + 8 hh + 4 half + 0..3 of this lane's key. The upper half's
+            // hh = 0 changes places with the lower's hh = 1, which gives each lane 8
+            // consecutive queries, 8 half from the first (zeros at keys past S). Where
+            // packed_dq_again forms dS they fall outside the buffer range and are
+            // dropped. kDsStores per step, which its first wait counts on.
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const uint4 w4 = __builtin_bit_cast(uint4, db[kk]);
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                    const int64_t qq = q0 + 32 * t + 16 * kk + 8 * hh + 4 * half;
-                    const u32x2 v2 = {hh ? w4.z : w4.x, hh ? w4.w : w4.y};
-                    __builtin_amdgcn_raw_buffer_store_b64(v2, rds, (int)(uint32_t)((my_key * a.ldst + qq) * 2), 0, 0);
-                }
+                const auto xz = __builtin_amdgcn_permlane32_swap(w4.x, w4.z, false, false);
+                const auto yw = __builtin_amdgcn_permlane32_swap(w4.y, w4.w, false, false);
+                const i32x4 v = {(int)xz[0], (int)yw[0], (int)xz[1], (int)yw[1]};
+                __builtin_amdgcn_raw_buffer_store_b128(v, rds, (int)(ds_off + 1024 * (2 * t + kk)), 0, 0);
             }
             // dO^T and Q^T fragments one step ahead of their MFMAs; step u = 2 dt + kk
             bf16x8 ot[2], qt[2];
@@ -1020,8 +1037,8 @@ __global__ __launch_bounds__(256) void packed_sum(PackedArgs a) {
 
 // ------------------------------------------------------------------- dQ
 // From the stored dS^T: per block of 64 keys that the workgroup's queries see, the
-// K tile [64][D] and the dS^T tile [64 keys][128 queries] go into LDS (two
-// stages); dQ^T (d x query) += K^T . dS^T takes both by transposed reads. A K tile
+// K tile [64][D] and dS^T of the 128 queries, four blocks as they are in memory, go
+// into LDS (two stages); dQ^T (d x query) += K^T . dS^T takes both by transposed reads. A K tile
 // with infinities or NaN is cleared of them first: dS is NaN where a query sees
 // such a key and 0 where it does not. Workgroups past dq_blocks sum the groups'
 // dK / dV partials.
@@ -1055,17 +1072,27 @@ __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) tk[dt][hh] = tr_off<D>(lane, 32 * dt, hh);
+    // the rows and columns that tr_off takes, in a block's order: of this wave's 32
+    // queries step g % 2, half i % 4 / 2, four queries i % 2
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) td[hh] = tr_off<QB>(lane, 32 * wave, hh);
+    for (int hh = 0; hh < 2; ++hh) {
+        const int i = lane & 15, g = lane >> 4, row = 4 * (g >> 1) + (i >> 2) + 8 * hh;
+        td[hh] = (uint32_t)((wave >> 1) * kDsBlock + (2 * (wave & 1) + (g & 1)) * 1024 + (32 * ((i >> 1) & 1) + row) * 16 +
+                            8 * (i & 1));
+    }
 
     const i32x4 rk = rsrc_words(a.k + bhk * S * D, S * D * 2);
-    // dS^T rows of this head from column q0: rows past S fall outside
-    const i32x4 rds = rsrc_words(a.dst + (int64_t)bh * S * a.ldst + q0, (S * a.ldst - q0) * 2);
+    const i32x4 rds = rsrc_words(a.dst + bh * (a.head_ds / 2), a.head_ds);
     auto issue = [&](int kb, int stage) {
         const uint32_t base = smem_byte + (uint32_t)(stage * STAGE * 2);
         const uint32_t key0 = (uint32_t)kb * KB;
         dma_rows<D>(rk, base, key0, D, wave, lane);
-        dma_rows<QB>(rds, base + KT * 2, key0, (uint32_t)a.ldst, wave, lane);
+        // two blocks of dS^T for each 32 keys, a wave one of the four
+        const uint32_t block = ds_block(2 * qb + (wave & 1), 2 * kb + (wave >> 1), a.nblk);
+#pragma unroll
+        for (int j = 0; j < kDsBlock / 1024; ++j)
+            dma16(rds, __builtin_amdgcn_readfirstlane(base + KT * 2 + (uint32_t)(wave * kDsBlock + j * 1024)),
+                  block + (uint32_t)(j * 1024 + lane * 16));
     };
     const int kd = 2 * qb;  // the tile's own keys first, on the way while the spans are read
     issue(kd, 0);
@@ -1097,7 +1124,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
         }
 #pragma unroll
         for (int kc = 0; kc < KB / 16; ++kc) {
-            const bf16x8 bfr = frag_tr_at(sds + 16 * kc * QB, td[0], td[1]);
+            const bf16x8 bfr = frag_tr_at(sds + ((kc >> 1) * 2 * kDsBlock + (kc & 1) * 256) / 2, td[0], td[1]);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
                 dqacc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_at(sk + 16 * kc * D, tk[dt][0], tk[dt][1]),
@@ -1256,6 +1283,11 @@ __global__ __launch_bounds__(256, 1) void packed_dq_again(PackedArgs a) {
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// dS^T is stored where a head's fits 32-bit buffer offsets (S <= 32640).
+bool dq_from_ds(const mc_attn_desc& d) {
+    return attention_uses_mfma(d) && head_ds_bytes(d.seq) < ((int64_t)1 << 31);
+}
+
 // The group rule of the causal kernels, which know the rows' shape; spans are
 // taken as causal.
 mc_attn_desc shape_of(const mc_packed_attn_desc& p, bool spans) {
@@ -1367,7 +1399,7 @@ PackedBwdWs packed_bwd_ws(const mc_packed_attn_desc& p, bool spans) {
         w.dv_part = off;  off += align256(B * Hkv * ng * S * D * 4);
     }
     w.dst = off;
-    if (attention_dq_from_ds(d)) off += align256(B * H * S * nblk * 128 * 2);
+    if (dq_from_ds(d)) off += B * H * (size_t)head_ds_bytes(d.seq);
     w.total = off;
     return w;
 }
@@ -1397,9 +1429,9 @@ hipError_t launch_packed_bwd(const mc_packed_attn_desc& p, const void* q, const 
     a.ngroups = attn_dkdv_groups(d);
     a.dk_part = a.ngroups > 1 ? dk_part : nullptr;
     a.dv_part = a.ngroups > 1 ? dv_part : nullptr;
-    const bool from_ds = attention_dq_from_ds(d);
+    const bool from_ds = dq_from_ds(d);
     a.dst = from_ds ? reinterpret_cast<uint16_t*>(ws + w.dst) : nullptr;
-    a.ldst = (int64_t)a.nblk * 128;
+    a.head_ds = head_ds_bytes(a.S);
     a.dq_blocks = (int64_t)a.nblk * a.B * a.H;
     a.sum_n8 = (int64_t)a.B * a.Hkv * a.S * a.D / 8;
     const dim3 gprep((unsigned)((int64_t)a.nblk * a.B * a.H));

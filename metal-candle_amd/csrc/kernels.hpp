@@ -168,7 +168,8 @@ struct PackedWs {
     size_t total;
 };
 struct PackedBwdWs {
-    size_t lsd, dk_part, dv_part, dst;  // as AttnBwdWs
+    size_t lsd, dk_part, dv_part;  // as AttnBwdWs
+    size_t dst;                    // bf16 dS^T in blocks, where a head's stays below 2^31 bytes
     size_t qflags, kflags;              // int32 [B, H, Sp / 64], [B, Hkv, S rounded up to 128 / 128]
     size_t total;
 };

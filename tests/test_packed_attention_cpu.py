@@ -100,9 +100,12 @@ def test_attention_abi(mc):
     assert need == 64 * 64 * 2 + 256  # V^T and a flag per 64 keys
     assert fwd(d, have=need - 1) == WORKSPACE
     need = L.mc_packed_attention_bwd_workspace_size(ctypes.byref(d), 0)
-    # lse and Delta, the flags of Q and of K, two heads' partials, dS^T
-    assert need == 2 * 512 + 256 + 256 + 2 * (2 * 64 * 64 * 4) + 2 * 64 * 128 * 2
+    # lse and Delta, the flags of Q and of K, two heads' partials, dS^T in blocks of 128 x 128
+    assert need == 2 * 512 + 256 + 256 + 2 * (2 * 64 * 64 * 4) + 2 * 128 * 128 * 2
     assert bwd(d, have=need - 1) == WORKSPACE
+    # a head's dS^T stays below 2^31 bytes, or none is stored
+    size = lambda S: L.mc_packed_attention_bwd_workspace_size(ctypes.byref(desc(mc, H=1, Hkv=1, S=S)), 0)  # noqa: E731
+    assert size(32640) > 255 * 255 * 32768 and size(32641) < 2**20
     assert L.mc_packed_attention_fwd_workspace_size(ctypes.byref(desc(mc, dtype=0))) == 0
     assert L.mc_packed_attention_fwd_workspace_size(ctypes.byref(desc(mc, cap=-1.0))) == 0
     assert L.mc_packed_attention_bwd_workspace_size(ctypes.byref(desc(mc, causal=1)), 1) == 0

@@ -15,7 +15,7 @@
 // The kernels are shaped as the causal ones of attention.hip (the same tiles, LDS
 // layouts and fragment orders, attention_tiles.hpp):
 //
-//  packed_vt    V^T for the forward, as there; infinities and NaN are left out of
+//  packed_vt    V^T for the forward of longer rows, as there; infinities and NaN are left out of
 //               it and their blocks of keys noted, since p = 0 times one of them
 //               would be NaN in every row of a tile that shares it. The forward
 //               adds them afterwards to the rows that see them.
@@ -56,6 +56,7 @@
 #include "attention_tiles.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
+#include "rules.hpp"
 
 namespace mc {
 namespace {
@@ -239,7 +240,8 @@ __device__ __forceinline__ uint32_t clear_nonfinite(uint32_t w) {
 }
 // Clears the infinities and NaN of a tile of `elems` bf16 in LDS; every thread of
 // the workgroup takes part.
-__device__ __forceinline__ void clear_tile(uint16_t* tile, int elems) {
+__device__ __forceinline__ bool clear_tile(uint16_t* tile, int elems) {
+    bool found = false;
     for (int i = threadIdx.x; i < elems / 8; i += 256) {
         uint4* p = reinterpret_cast<uint4*>(tile) + i;
         uint4 q = *p;
@@ -247,8 +249,10 @@ __device__ __forceinline__ void clear_tile(uint16_t* tile, int elems) {
             q.x = clear_nonfinite(q.x); q.y = clear_nonfinite(q.y);
             q.z = clear_nonfinite(q.z); q.w = clear_nonfinite(q.w);
             *p = q;
+            found = true;
         }
     }
+    return found;
 }
 // Any flag of [from, to) set: the same in every lane of a wave.
 __device__ __forceinline__ bool any_flag(const int32_t* flags, int from, int to) {
@@ -346,14 +350,16 @@ __global__ __launch_bounds__(256) void packed_vt(const uint16_t* __restrict__ V,
 }
 
 // ------------------------------------------------------- flash forward
-template <int D, bool CAP, bool BIAS>
+// ROWS: V as it is, through transposed reads, cleared of infinities and NaN block by
+// block in LDS; otherwise V^T from packed_vt.
+template <int D, bool CAP, bool BIAS, bool ROWS>
 __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
     constexpr int KB = 64;            // keys per block
     constexpr int QB = 128;           // queries per workgroup, 32 per wave
     constexpr int KS = D / 16;        // MFMA k-steps over the head dim
     constexpr int DT = D / 32;        // 32-row tiles of O^T
     constexpr int K_ELEMS = KB * D;   // K tile [64][D], rows of D bf16
-    constexpr int STAGE = 2 * KB * D; // K tile, then V^T tile [D][64]
+    constexpr int STAGE = 2 * KB * D; // K tile, then V^T tile [D][64] (ROWS: V [64][D])
     constexpr int CPR_K = D / 8, RPI_K = 64 / CPR_K;
     constexpr int LOADS_K = KB / RPI_K / 4, LOADS_V = D / 8 / 4;  // DMA per wave per block
     __shared__ __attribute__((aligned(1024))) uint16_t smem[2 * STAGE];
@@ -383,7 +389,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
 
     const int64_t bhk = (int64_t)b * a.Hkv + hk;
     const i32x4 rk = rsrc_words(a.k + bhk * S * D, S * D * 2);
-    const i32x4 rv = rsrc_words(a.vt + bhk * D * a.Sp, (int64_t)D * a.Sp * 2);
+    const i32x4 rv = ROWS ? rsrc_words(a.v + bhk * S * D, S * D * 2)
+                          : rsrc_words(a.vt + bhk * D * a.Sp, (int64_t)D * a.Sp * 2);
+    uint32_t troff[DT][2];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) troff[dt][hh] = ROWS ? tr_off<D>(lane, 32 * dt, hh) : 0;
 
     // K rows key0 .. key0+63 into the swizzled [64][D] layout, then V^T rows
     // d = 0 .. D-1 (64 positions each) into [D][64].
@@ -398,13 +410,17 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
             const uint32_t off = ((key0 + (uint32_t)row) * D + 8u * chunk) * 2u;
             dma16(rk, __builtin_amdgcn_readfirstlane(base + (uint32_t)blk * 1024u), off);
         }
+        if constexpr (ROWS) {
+            dma_rows<D>(rv, base + K_ELEMS * 2, key0, D, wave, lane);
+        } else {
 #pragma unroll
-        for (int j = 0; j < LOADS_V; ++j) {
-            const int blk = wave * LOADS_V + j;
-            const int row = blk * 8 + lane / 8;
-            const uint32_t chunk = (uint32_t)swz<64>(row, lane % 8);
-            const uint32_t off = ((uint32_t)row * (uint32_t)a.Sp + key0 + 8u * chunk) * 2u;
-            dma16(rv, __builtin_amdgcn_readfirstlane(base + (uint32_t)(K_ELEMS * 2) + (uint32_t)blk * 1024u), off);
+            for (int j = 0; j < LOADS_V; ++j) {
+                const int blk = wave * LOADS_V + j;
+                const int row = blk * 8 + lane / 8;
+                const uint32_t chunk = (uint32_t)swz<64>(row, lane % 8);
+                const uint32_t off = ((uint32_t)row * (uint32_t)a.Sp + key0 + 8u * chunk) * 2u;
+                dma16(rv, __builtin_amdgcn_readfirstlane(base + (uint32_t)(K_ELEMS * 2) + (uint32_t)blk * 1024u), off);
+            }
         }
     };
 
@@ -418,7 +434,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
     const Span wg = workgroup_span(ws, slots);
     const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
     const int wk0 = ws.lo < ws.hi ? ws.lo / KB : 0, wk1 = ws.lo < ws.hi ? (ws.hi + KB - 1) / KB : 0;
-    const bool bad_v = any_flag(a.vflags + bhk * (a.Sp / 64), wk0, wk1);
+    bool bad_v = ROWS ? false : any_flag(a.vflags + bhk * (a.Sp / 64), wk0, wk1);
     const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
 
     f32x16 oacc[DT];
@@ -436,6 +452,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
         wait_vmcnt<0>();
         __syncthreads();
         if (more) issue(next, stage ^ 1);
+        if constexpr (ROWS) bad_v |= __syncthreads_or(clear_tile(smem + stage * STAGE + K_ELEMS, K_ELEMS)) != 0;
         if (kb < wk0 || kb >= wk1) continue;  // wave-uniform: no query of this wave sees the block
         const uint16_t* sk = smem + stage * STAGE;
         const uint16_t* sv = sk + K_ELEMS;
@@ -557,15 +574,19 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
             const int row = 32 * (v >> 1) + col, t = v & 1;
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
-                vf[slot][kk] = *reinterpret_cast<const bf16x8*>(&sv[row * KB + 8 * swz<64>(row, 4 * t + 2 * kk + half)]);
+                if constexpr (ROWS)
+                    vf[slot][kk] = frag_tr_at(sv + (32 * t + 16 * kk) * D, troff[v >> 1][0], troff[v >> 1][1]);
+                else
+                    vf[slot][kk] = *reinterpret_cast<const bf16x8*>(&sv[row * KB + 8 * swz<64>(row, 4 * t + 2 * kk + half)]);
         };
+        constexpr int kReads = ROWS ? 4 : 2;
         vread(0, 0);
-        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReads, 0);
 #pragma unroll
         for (int v = 0; v < 2 * DT; ++v) {
             if (v + 1 < 2 * DT) {
                 vread(v + 1, (v + 1) & 1);
-                __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kReads, 0);
             }
             const int dt = v >> 1, t = v & 1;
 #pragma unroll
@@ -579,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
     if (bad_v) {
 #pragma unroll 1
         for (int kb = wk0; kb < wk1; ++kb) {
-            if (a.vflags[bhk * (a.Sp / 64) + kb] == 0) continue;
+            if (!ROWS && a.vflags[bhk * (a.Sp / 64) + kb] == 0) continue;
             const int last = (kb + 1) * KB < (int)S ? (kb + 1) * KB : (int)S;
 #pragma unroll 1
             for (int key = kb * KB; key < last; ++key) {
@@ -1346,7 +1367,7 @@ hipError_t launch_attention_spans(const int32_t* documents, const uint8_t* prefi
 PackedWs packed_fwd_ws(const mc_packed_attn_desc& p) {
     const mc_attn_desc& d = p.attn;
     PackedWs w{};
-    if (!attention_uses_mfma(d)) return w;
+    if (!attention_uses_mfma(d) || packed_fwd_from_rows(d.seq)) return w;
     const size_t Sp = (size_t)(d.seq + 63) / 64 * 64, bhk = (size_t)d.batch * d.kv_heads;
     w.vt = 0;
     w.flags = align256(bhk * d.head_dim * Sp * 2);
@@ -1373,8 +1394,13 @@ hipError_t launch_packed_fwd(const mc_packed_attn_desc& p, const void* q, const 
     const dim3 grid((unsigned)((int64_t)a.nblk * a.B * a.H));
     by_variant(a.D, p.cap != 0.f, slopes != nullptr, [&](auto dim, auto cap, auto bias) {
         constexpr int D = decltype(dim)::value;
-        packed_vt<D><<<gvt, 256, 0, stream>>>(a.v, a.S, a.Sp, vt, a.vflags);
-        packed_fwd<D, decltype(cap)::value, decltype(bias)::value><<<grid, 256, 0, stream>>>(a);
+        constexpr bool CAP = decltype(cap)::value, BIAS = decltype(bias)::value;
+        if (packed_fwd_from_rows(d.seq)) {
+            packed_fwd<D, CAP, BIAS, true><<<grid, 256, 0, stream>>>(a);
+        } else {
+            packed_vt<D><<<gvt, 256, 0, stream>>>(a.v, a.S, a.Sp, vt, a.vflags);
+            packed_fwd<D, CAP, BIAS, false><<<grid, 256, 0, stream>>>(a);
+        }
     });
     return hipGetLastError();
 }

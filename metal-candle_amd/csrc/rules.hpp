@@ -107,6 +107,14 @@ constexpr LossGrid loss_grad_grid(int64_t rows, int64_t row_bytes) {
     return LossGrid{row_bytes < 28 << 10 || rows <= 64 ? 512 : 1024, (unsigned)(wanted < most ? wanted : most)};
 }
 
+// The packed attention's bf16 forward takes V from its rows, without the launch that
+// writes V^T, where a row is one tile of queries: looking for infinities and NaN in
+// every block of V and twice the LDS reads cost more than the launch where there are
+// more blocks. us, rows / V^T, 8 x 12 x S x 128 causal: S = 65 8.5 / 10.3, 128 9.2 /
+// 10.8, 256 13.6 / 13.6, 512 23.1 / 20.7; 1 x 14 x S x 64 capped: 65 8.0 / 9.6, 128
+// 8.1 / 9.7, 256 11.8 / 11.9, 512 19.4 / 16.3.
+constexpr bool packed_fwd_from_rows(int64_t seq) { return seq <= 128; }
+
 // The embedding's backward sorts its tokens in workgroups of 256 threads beside
 // those that clear the gradient, where the clearing (6.8 TB/s) takes as long as that
 // sort (1.9 us per 1024 tokens, 0.7 in workgroups of 1024); else one after the other.

@@ -172,7 +172,8 @@ SPECIAL = [math.nan, math.inf, -math.inf]
 
 @pytest.mark.parametrize("cap", [None, 20.0])
 @pytest.mark.parametrize("dt,D,S", [(torch.bfloat16, 128, 300), (torch.bfloat16, 64, 200), (torch.float32, 64, 150),
-                                    (torch.float32, 128, 70), (torch.bfloat16, 40, 60), (torch.float32, 33, 40)])
+                                    (torch.float32, 128, 70), (torch.bfloat16, 40, 60), (torch.float32, 33, 40),
+                                    (torch.bfloat16, 128, 100), (torch.bfloat16, 64, 128)])
 def test_what_padding_holds(mc, dev, dt, D, S, cap):
     """Infinities and NaN in every tensor's padding change no bit of any result."""
     B, H, Hkv = 2, 4, 2
@@ -196,7 +197,7 @@ def test_what_padding_holds(mc, dev, dt, D, S, cap):
 @pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
 @pytest.mark.parametrize("value", SPECIAL)
 @pytest.mark.parametrize("dt,D,S", [(torch.bfloat16, 128, 300), (torch.bfloat16, 64, 140), (torch.float32, 64, 130),
-                                    (torch.bfloat16, 40, 50)])
+                                    (torch.bfloat16, 40, 50), (torch.bfloat16, 128, 128), (torch.bfloat16, 64, 90)])
 def test_one_document_that_is_not_finite(mc, dev, dt, D, S, which, value):
     """A NaN or an infinity in one document leaves the others' results as they are, and reaches its own."""
     B, H, Hkv = 1, 2, 1

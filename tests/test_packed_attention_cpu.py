@@ -94,11 +94,13 @@ def test_attention_abi(mc):
         assert call(desc(mc), q=None) == NULL and call(desc(mc), o=None) == NULL
         assert call(desc(mc), q=ctypes.c_void_p(264)) == LAYOUT
         assert call(desc(mc), spans=ctypes.c_void_p(264)) == LAYOUT
-        assert call(desc(mc), ws=None) == WORKSPACE
-    d = desc(mc)
+        assert call(desc(mc, S=129), ws=None) == WORKSPACE
+    d = desc(mc, S=129)
     need = L.mc_packed_attention_fwd_workspace_size(ctypes.byref(d))
-    assert need == 64 * 64 * 2 + 256  # V^T and a flag per 64 keys
+    assert need == 64 * 192 * 2 + 256  # V^T and a flag per 64 keys
     assert fwd(d, have=need - 1) == WORKSPACE
+    assert L.mc_packed_attention_fwd_workspace_size(ctypes.byref(desc(mc, S=128))) == 0  # V is read as it is
+    d = desc(mc)
     need = L.mc_packed_attention_bwd_workspace_size(ctypes.byref(d), 0)
     # lse and Delta, the flags of Q and of K, two heads' partials, dS^T in blocks of 128 x 128
     assert need == 2 * 512 + 256 + 256 + 2 * (2 * 64 * 64 * 4) + 2 * 128 * 128 * 2

@@ -918,7 +918,7 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
         const __amdgpu_buffer_rsrc_t rds =
             make_rsrc(a.dst ? a.dst + bh * (a.head_ds / 2) : nullptr, a.dst ? a.head_ds : 0);
         const uint32_t ds_off = ds_block(qb, 4 * kb + wave, a.nblk) + (uint32_t)lane * 16u;
-        // Every wave runs every block, masked where its keys do not meet it.
+        // Every wave stores every block's dS^T; a tile is masked where its keys do not meet it.
         const int q0 = qb * 64;
         const bool edge = !(q0 >= ws.all_lo && q0 + 64 <= ws.all_hi);
 
@@ -973,6 +973,15 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
         // then its share of dV^T (d x key) += dO^T . P and dK^T += Q^T . dS
         auto tile = [&](auto t_tag) {
             constexpr int t = decltype(t_tag)::value;
+            // none of the wave's keys meets the tile: 1 to 2% of documents' time, the
+            // workgroup's other waves set a step's
+            if (q0 + 32 * t >= ws.hi || q0 + 32 * t + 32 <= ws.lo) {
+                const i32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+                    __builtin_amdgcn_raw_buffer_store_b128(zero, rds, (int)(ds_off + 1024 * (2 * t + kk)), 0, 0);
+                return;
+            }
             f32x16 sacc, dpacc;
 #pragma unroll
             for (int j = 0; j < 16; ++j) sacc[j] = dpacc[j] = 0.f;

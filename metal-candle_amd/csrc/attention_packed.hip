@@ -41,7 +41,7 @@
 //  packed_vt    10     7.1   3.6   memory
 //  packed_fwd   664    70    17    (a) 725 TFLOP/s: the scores' arithmetic, of whose
 //                                  time the cap's exponential and reciprocal are half
-//  packed_prep  52     37    12    (a) memory; (b, c) S and dP once more
+//  packed_prep  52     39    12    (a) memory; (b, c) S and dP once more
 //  packed_dkdv  1467   155   27    one wave per SIMD: MFMA 31% of its cycles, scores
 //                                  37, waits 27, which follow each other (the scores
 //                                  of one query tile among the other's MFMAs: 1800
@@ -655,8 +655,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
 // dS = P (dP - Delta) does not average away where few keys share it: dq and dk of
 // 4 causal tokens were 6e-2 of their size off, of 30 9e-3, of 1021 4.9e-3, of 4096
 // 3.6e-3 (their own roundings and dS's to bf16 make 2.4e-3). Where a workgroup's
-// queries span at most kExactKeys keys it is formed as sum_j P_ij dP_ij instead,
-// S^T = K.Q^T and dP^T = V.dO^T once more, shaped as the forward. Both the error
+// queries span at most kExactKeys keys it is formed as sum_j P_ij dP_ij instead, over
+// sum_j P_ij, which is 1 but for lse's rounding (dS of the only key that a query sees
+// is 0): S^T = K.Q^T and dP^T = V.dO^T once more, shaped as the forward. Both the error
 // and what that costs end there: with 128 / 256 / 512 keys 8 rows of 2048 tokens
 // in documents of 340 are 4.1e-3 / 3.5e-3 / 2.9e-3 off.
 constexpr int kExactKeys = 256;
@@ -708,7 +709,7 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
     const float lse2 = empty ? __builtin_inff() : bad ? __builtin_nanf("") : x * kLog2e;
     const bool note = __any(my_q < S && (bad || !(__builtin_fabsf(x) < __builtin_inff())));
 
-    float delta = 0.f;
+    float delta = 0.f, sum_p = 0.f;
     if (wg.hi - wg.lo > kExactKeys) {  // alike in every wave
         const __amdgpu_buffer_rsrc_t ro = make_rsrc(o + ((int64_t)b * S * a.H + h) * D, (S * a.H - h) * D * 2);
 #pragma unroll
@@ -747,7 +748,7 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
             const uint32_t width = (uint32_t)(mine.hi - mine.lo);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                f32x16 sacc, dpacc;
+                f32x16 sacc, dpacc;  // products, then P and P dP
 #pragma unroll
                 for (int j = 0; j < 16; ++j) sacc[j] = dpacc[j] = 0.f;
 #pragma unroll
@@ -760,20 +761,26 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
                     const int ko = 32 * t + 8 * (j >> 2) + (j & 3);
                     float y = score_log2<CAP>(sacc[j], a);
                     if constexpr (BIAS) y = __builtin_fmaf(__builtin_fabsf(dist - (float)ko), -slope2, y);
-                    dpacc[j] *= exp2_hw(y - lse2);
+                    sacc[j] = exp2_hw(y - lse2);
+                    dpacc[j] *= sacc[j];
                 }
                 if (edge) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
-                        if ((uint32_t)(32 * t + 8 * (j >> 2) + (j & 3) - lo) >= width) dpacc[j] = 0.f;
+                        if ((uint32_t)(32 * t + 8 * (j >> 2) + (j & 3) - lo) >= width) sacc[j] = dpacc[j] = 0.f;
                 }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) delta += dpacc[j];
+                for (int j = 0; j < 16; ++j) {
+                    sum_p += sacc[j];
+                    delta += dpacc[j];
+                }
             }
         }
         wait_vmcnt<0>();
     }
     delta += __shfl_xor(delta, 32, kWave);
+    sum_p += __shfl_xor(sum_p, 32, kWave);
+    if (sum_p > 0.f) delta /= sum_p;  // only where P was formed
     // queries past S have lse = +inf too
     if (half == 0 && my_q < a.Sp) {
         float* blk = lsd + ((int64_t)bh * (a.Sp / 64) + my_q / 64) * 128 + my_q % 64;

@@ -170,6 +170,26 @@ def test_gradients_against_differences(mc, dev):
 SPECIAL = [math.nan, math.inf, -math.inf]
 
 
+@pytest.mark.parametrize("cap", [None, 50.0])
+@pytest.mark.parametrize("dt,D", [(torch.bfloat16, 64), (torch.bfloat16, 128)])
+def test_documents_of_one_token(mc, dev, dt, D, cap):
+    """P is 1 and dS nothing but what rounding leaves: with u = 2^-24, P dP / P is off by 2 u of dP, and dP, summed in
+    the same products in both kernels but for their order, by D u |dout| |v| each time; dq is scale dS k, rounded."""
+    B, H, Hkv, S = 2, 4, 2, 130
+    q, k, v, dout = inputs(dt, B, H, Hkv, S, D, dev, std=6.0)
+    spans = mc.attention_spans((torch.arange(S, dtype=torch.int32) % 2).repeat(B, 1).to(dev))
+    got = run(mc, q, k, v, dout, spans=spans, cap=cap)
+    rows = lambda x: x.double().cpu()  # noqa: E731
+    do = rows(dout).view(B, S, H, D).transpose(1, 2)
+    kk, vv = (rows(x).repeat_interleave(H // Hkv, 1) for x in (k, v))
+    most = 2.0**-24 * (2 * D + 8) * (do.abs() * vv.abs()).sum(-1) * D**-0.5  # scale |dS|
+    assert torch.equal(got["o"].view(B, S, H, D).transpose(1, 2), v.repeat_interleave(H // Hkv, 1))
+    assert (rows(got["dq"]).abs() <= most[..., None] * kk.abs() * 1.01).all()
+    sum_of = lambda x: x.view(B, Hkv, H // Hkv, S, -1).sum(2)  # noqa: E731
+    assert (rows(got["dk"]).abs() <= sum_of(most[..., None] * rows(q).abs()) * 1.01).all()
+    assert (rows(got["dv"]) - sum_of(do)).abs().le(2.0**-8 * sum_of(do.abs()) * 1.01).all()
+
+
 @pytest.mark.parametrize("cap", [None, 20.0])
 @pytest.mark.parametrize("dt,D,S", [(torch.bfloat16, 128, 300), (torch.bfloat16, 64, 200), (torch.float32, 64, 150),
                                     (torch.float32, 128, 70), (torch.bfloat16, 40, 60), (torch.float32, 33, 40),

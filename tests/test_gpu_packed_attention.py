@@ -170,6 +170,24 @@ def test_gradients_against_differences(mc, dev):
 SPECIAL = [math.nan, math.inf, -math.inf]
 
 
+@pytest.mark.parametrize("cap", [5.0, 50.0, 52.5, 1000.0])
+@pytest.mark.parametrize("dt,D,S", [(torch.bfloat16, 128, 300), (torch.bfloat16, 64, 70), (torch.float32, 64, 90)])
+def test_scores_at_the_cap(mc, dev, dt, D, S, cap):
+    """Rows whose scores are all minus the cap, all the cap, and both: no sum leaves float32."""
+    q, k, v, dout = inputs(dt, 1, 3, 1, S, D, dev)
+    k = torch.full_like(k, 4.0)
+    k[:, :, 1::2] *= -1.0
+    q = torch.full_like(q, 4.0)
+    ids = torch.zeros(1, S, dtype=torch.int32)
+    # the second head sees one sign only: tokens of one sign are documents of their own
+    ids[0] = torch.arange(S) % 2 if S < 100 else 0
+    q[:, 1] *= -1.0
+    how = {"spans": mc.attention_spans(ids.to(dev)), "cap": cap, "scale": 50.0}
+    got = run(mc, q, k, v, dout, **how)
+    want = ref.attention(q, k, v, ref.visible(S, ids[0].tolist())[None], 50.0, cap, None, dout)
+    ref.check(got, want)
+
+
 @pytest.mark.parametrize("cap", [None, 50.0])
 @pytest.mark.parametrize("dt,D", [(torch.bfloat16, 64), (torch.bfloat16, 128)])
 def test_documents_of_one_token(mc, dev, dt, D, cap):

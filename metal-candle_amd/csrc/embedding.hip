@@ -10,7 +10,7 @@
 // the tokens are sorted by id first (stable), then each row of the gradient adds
 // up the run of tokens that its id has.
 //
-//  embed_sort   one workgroup per kIds ids. Each reads every token's id (they are
+//  embed_sort   one workgroup per 16 to 512 ids. Each reads every token's id (they are
 //               few beside the rows, and stay in L2), which gives it the place of
 //               its own run of tokens without another workgroup's help: counts
 //               per (id, wave) in LDS, a scan, and a second pass that places the
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void embed_fwd(const T* __restrict__ table, co
 }
 
 // --------------------------------------------------------------- backward
-constexpr int kIds = 512;
+constexpr int kIds = 512;  // of a sorting workgroup, at most (embedding_sort_ids)
 
 // order[N]: the N tokens with an id of the table that is not padding, by id, in their
 // order within an id; sorted[N]: their ids; start[v]: the first of id v there,
@@ -93,7 +93,7 @@ template <int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES * kWave) void embed_sort(const int32_t* __restrict__ ids, int32_t tokens,
                                                             int64_t vocab, int64_t padding,
                                                             int32_t* __restrict__ order, int32_t* __restrict__ sorted,
-                                                            int32_t* __restrict__ start,
+                                                            int32_t* __restrict__ start, int id_block,
                                                             int sort_blocks, float* __restrict__ dtable,
                                                             int64_t clear) {
     constexpr int kSortWaves = WAVES, kSortThreads = WAVES * kWave;
@@ -108,8 +108,8 @@ __global__ __launch_bounds__(WAVES * kWave) void embed_sort(const int32_t* __res
     __shared__ int32_t wsum[kSortWaves], before[kSortWaves];
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_id();
     // this workgroup's ids [lo, lo + width); no token's key is -1 (unsigned)
-    const uint32_t lo = blockIdx.x * (uint32_t)kIds;
-    const uint32_t width = (uint32_t)(vocab - lo < kIds ? vocab - lo : kIds);
+    const uint32_t lo = blockIdx.x * (uint32_t)id_block;
+    const uint32_t width = (uint32_t)(vocab - lo < id_block ? vocab - lo : id_block);
     const uint32_t pad = padding >= 0 && padding < vocab ? (uint32_t)padding : 0xffffffffu;
     for (int i = tid; i < kSortWaves * kIds; i += kSortThreads) (&count[0][0])[i] = 0;
     // this wave's tokens [t0, t1), whole wave steps
@@ -162,16 +162,20 @@ __global__ __launch_bounds__(WAVES * kWave) void embed_sort(const int32_t* __res
         if (w < wave) base += wsum[w];
     }
     base += scan - mine;
+    uint32_t total_at = 0xffffffffu;  // the table's last id
     if (owner)
         for (int i = 0; i < kOwn; ++i) {
             const uint32_t k = (uint32_t)(tid * kOwn + i);
-            if (k < width) start[lo + k] = base;
+            if (k < width) {
+                start[lo + k] = base;
+                if ((int64_t)lo + k + 1 == vocab) total_at = k;
+            }
             for (int w = 0; w < kSortWaves; ++w) {
                 const int32_t c = count[w][k];
                 count[w][k] = base;
                 base += c;
             }
-            if ((int64_t)lo + k + 1 == vocab) start[vocab] = base;
+            if (k == total_at) start[vocab] = base;
         }
     __syncthreads();
     for (int32_t t = t0; t < t1; t += AHEAD * kWave) {
@@ -441,7 +445,9 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
     float* part = reinterpret_cast<float*>(ws + w.part);
     const int32_t unit = unit_of(d.tokens);
     const int64_t clear = accumulate ? 0 : d.vocab * d.dim;
-    const int sort_blocks = (int)((d.vocab + kIds - 1) / kIds);
+    const int id_block = embedding_sort_ids(d.vocab);
+    static_assert(embedding_sort_ids((int64_t)1 << 31) == kIds, "a workgroup's counts fit in LDS");
+    const int sort_blocks = (int)((d.vocab + id_block - 1) / id_block);
     // the sort in as many waves as it takes, or in those that clear
     const bool together = embedding_sort_while_clearing(d.tokens, clear);
     const int threads = together ? 256 : 1024;
@@ -452,10 +458,10 @@ hipError_t launch_embedding_bwd(const mc_embedding_desc& d, const int32_t* ids, 
         const dim3 grid((unsigned)(sort_blocks + beside));
         if (together)
             embed_sort<4, AHEAD><<<grid, 256, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id, order, sorted,
-                                                          start, sort_blocks, dtable, clear);
+                                                          start, id_block, sort_blocks, dtable, clear);
         else
             embed_sort<16, AHEAD><<<grid, 1024, 0, stream>>>(ids, (int32_t)d.tokens, d.vocab, d.padding_id, order, sorted,
-                                                            start, sort_blocks, dtable, 0);
+                                                            start, id_block, sort_blocks, dtable, 0);
     };
     if (steps <= 2) sort(std::integral_constant<int, 2>{});
     else if (steps <= 4) sort(std::integral_constant<int, 4>{});

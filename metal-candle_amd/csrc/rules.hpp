@@ -115,10 +115,24 @@ constexpr LossGrid loss_grad_grid(int64_t rows, int64_t row_bytes) {
 // 8.1 / 9.7, 256 11.8 / 11.9, 512 19.4 / 16.3.
 constexpr bool packed_fwd_from_rows(int64_t seq) { return seq <= 128; }
 
-// The embedding's backward sorts its tokens in workgroups of 256 threads beside
-// those that clear the gradient, where the clearing (6.8 TB/s) takes as long as that
-// sort (1.9 us per 1024 tokens, 0.7 in workgroups of 1024); else one after the other.
-constexpr bool embedding_sort_while_clearing(int64_t tokens, int64_t clear) { return clear * 4 >= tokens * 12288; }
+// Ids per workgroup of the embedding's sort: about one workgroup per CU, since each
+// places its own ids' tokens one id after the other. The backward with 512 ids in each
+// / by the rule, us, rows of 512: 16384 tokens of 2048 ids 88 / 22, of 16384 ids 38 /
+// 30, 65536 tokens of 2048 ids 317 / 55.
+constexpr int embedding_sort_ids(int64_t vocab) {
+    int ids = 16;
+    while (ids < 512 && vocab > 256 * (int64_t)ids) ids *= 2;
+    return ids;
+}
+
+// The embedding's backward sorts its tokens in workgroups of 256 threads beside those
+// that clear the gradient, where the clearing (6.8 TB/s) takes about as long as that
+// sort, or the launch saved is worth more than the difference; else in workgroups of
+// 1024 and one after the other. us, beside / after: 16384 tokens of 151936 x 896 118 /
+// 127, of 50257 x 512 40 / 39, of 16384 x 512 34 / 30; 1024 of 2048 x 512 10.3 / 11.9.
+constexpr bool embedding_sort_while_clearing(int64_t tokens, int64_t clear) {
+    return clear > 0 && (tokens <= 2048 || clear * 4 >= tokens * 8192);
+}
 
 // Softmax rows that are not whole 16-byte vectors: the covering vectors of the
 // one-wave kernels, or for short rows a lane per element (the scalar kernels),

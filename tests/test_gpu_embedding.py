@@ -37,6 +37,7 @@ def check_grad(got, ids, dout, vocab, scale, padding, before=None):
 CASES = [  # tokens, vocab, dim
     (1, 1, 1), (1, 7, 4), (5, 3, 7), (64, 512, 8), (65, 513, 256), (130, 511, 257), (63, 1025, 260), (1000, 100, 33),
     (777, 5000, 896), (2036, 50257, 893), (4096, 32000, 128), (300, 151936, 12),
+    (40, 16, 6), (90, 17, 6), (3000, 4096, 5), (3000, 4097, 5), (5000, 8193, 3), (2500, 131073, 2),  # ids per workgroup
 ]
 
 

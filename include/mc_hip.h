@@ -294,8 +294,9 @@ mc_status mc_attention_bwd(const mc_attn_desc* d, const void* q, const void* k, 
  *     causal only): a document's leading tokens of non-zero prefix, its prompt, also
  *     see each other. Non-zero tokens behind the first zero of a document are none.
  * The entry points below take the spans, or with spans NULL attn.causal (which is
- * 0 with spans). Spans of another origin are kept inside the row, but a query and a
- * key must agree on whether they meet, and both sides must be intervals.
+ * 0 with spans). Spans of another origin, a token that does not see itself included,
+ * are kept inside the row, but a query and a key must agree on whether they meet,
+ * and both sides must be intervals.
  *
  * The slopes are constants: they get no gradient. lse of a query whose q holds an
  * infinity or NaN is NaN under a cap. */

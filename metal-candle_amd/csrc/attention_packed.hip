@@ -274,7 +274,8 @@ struct PackedArgs {
     const float* lsd;      // backward: [B, H, Sp / 64, 2, 64]: lse * log2 e, Delta
     int32_t* vflags;       // forward: [B, Hkv, Sp / 64], blocks of V with infinities or NaN
     const int32_t* qflags; // backward: [B, H, Sp / 64], blocks of Q and dO
-    int32_t* kflags;       // backward: [B, Hkv, nblk], blocks of 128 rows of K
+    int4* kinfo;           // backward: [B, Hkv, nblk], blocks of 128 rows of K: whether they hold infinities
+                           // or NaN, and the blocks of 128 queries [y, z) whose dS^T is stored
     uint16_t *dq, *dk, *dv;
     float *dk_part, *dv_part;  // [B, Hkv, ngroups, S, D]
     uint16_t* dst;             // dS^T: [B, H] of head_ds bytes (kDsBlock), or null
@@ -865,17 +866,19 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
     const int kd = 2 * kb;
     issue(h0, kd, 0);
 
-    // The queries that the workgroup's keys meet, in whole blocks of 128: the dQ
-    // pass reads dS^T by those, and every one that it reads is written here.
+    // The queries that the workgroup's keys meet, in whole blocks of 128, by which
+    // the dQ pass reads dS^T. kd's are among them; a workgroup whose keys nobody
+    // sees stores none. kinfo says which, and dQ reads no others.
     const Span mine = key_span(a.spans, b, my_key, (int)S, a.causal);
     const WaveSpan ws = wave_span(mine);
     const Span wg = workgroup_span(ws, slots);
     const int nqb = (int)((S + 63) / 64);
     int qstart = wg.lo / 128 * 2, qend = (int)(((int64_t)wg.hi + 127) / 128 * 2);
-    if (wg.lo < wg.hi) {  // kd with them, whatever the spans hold
+    if (wg.lo < wg.hi) {
         qstart = qstart < kd ? qstart : kd;
-        qend = qend > kd ? qend : kd + 1;
+        qend = qend > kd ? qend : kd + 2;
     }
+    const int stored0 = qstart / 2, stored1 = qend / 2;
     qend = qend < nqb ? qend : nqb;
     const int nq = qend - qstart;       // query blocks per head
     const int nit = hpg * nq;           // (head, query block) steps, head-major
@@ -902,7 +905,7 @@ __global__ __launch_bounds__(256, 1) void packed_dkdv(PackedArgs a) {
         asm volatile("" : "+a"(kf[s]), "+a"(vf[s]));
     }
     bad_k = __syncthreads_or(bad_k);
-    if (threadIdx.x == 0) a.kflags[bhk * a.nblk + kb] = bad_k;  // alike from every group
+    if (threadIdx.x == 0) a.kinfo[bhk * a.nblk + kb] = make_int4(bad_k, stored0, stored1, 0);  // alike from every group
     int h = h0, qb = kd, left = nq;  // of this head
     float slope2 = BIAS ? a.slopes[h0] * kLog2e : 0.f;  // its load waits for every store before it: once per head
     for (int it = 0; it < nit; ++it) {
@@ -1075,10 +1078,11 @@ __global__ __launch_bounds__(256) void packed_sum(PackedArgs a) {
 // ------------------------------------------------------------------- dQ
 // From the stored dS^T: per block of 64 keys that the workgroup's queries see, the
 // K tile [64][D] and dS^T of the 128 queries, four blocks as they are in memory, go
-// into LDS (two stages); dQ^T (d x query) += K^T . dS^T takes both by transposed reads. A K tile
-// with infinities or NaN is cleared of them first: dS is NaN where a query sees
-// such a key and 0 where it does not. Workgroups past dq_blocks sum the groups'
-// dK / dV partials.
+// into LDS (two stages); dQ^T (d x query) += K^T . dS^T takes both by transposed reads.
+// A block between the first and the last of these keys that none of the queries
+// sees may have no dS^T in memory: it is left out, by kinfo. A K tile with infinities
+// or NaN is cleared of them first: dS is NaN where a query sees such a key and 0
+// where it does not. Workgroups past dq_blocks sum the groups' dK / dV partials.
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
     if ((int64_t)blockIdx.x >= a.dq_blocks) {
@@ -1136,8 +1140,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
     const Span mine = query_span(a.spans, b, qw + (lane & 31), (int)S, a.causal);
     const Span wg = workgroup_span(wave_span(mine), slots);
     const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
-    const int32_t* kflags = a.kflags + bhk * a.nblk;
-    const bool bad_k = any_flag(kflags, kb0 / 2, (kb1 + 1) / 2);
+    const int4* kinfo = a.kinfo + bhk * a.nblk;
+    bool bad = false, hole = false;
+    for (int i = kb0 / 2 + lane; i < (kb1 + 1) / 2; i += kWave) {
+        const int4 x = kinfo[i];
+        bad |= x.x != 0;
+        hole |= qb < x.y || qb >= x.z;
+    }
+    const bool bad_k = __any(bad), holes = __any(hole);
 
     f32x16 dqacc[DT];
 #pragma unroll
@@ -1153,9 +1163,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
         wait_vmcnt<0>();
         __syncthreads();
         if (more) issue(next, stage ^ 1);
+        if (kb < kb0 || kb >= kb1) continue;  // kd may be no key of these queries
+        if (holes && (qb < kinfo[kb / 2].y || qb >= kinfo[kb / 2].z)) continue;  // workgroup-uniform, as below
         uint16_t* sk = smem + stage * STAGE;
         const uint16_t* sds = sk + KT;
-        if (bad_k && kflags[kb / 2]) {  // workgroup-uniform
+        if (bad_k && kinfo[kb / 2].x) {
             clear_tile(sk, KT);
             __syncthreads();
         }
@@ -1232,8 +1244,10 @@ __global__ __launch_bounds__(256, 1) void packed_dq_again(PackedArgs a) {
     const WaveSpan ws = wave_span(mine);
     const Span wg = workgroup_span(ws, slots);
     const int kb0 = wg.lo / KB, kb1 = (wg.hi + KB - 1) / KB;
-    const int32_t* kflags = a.kflags + bhk * a.nblk;
-    const bool bad_k = any_flag(kflags, kb0 / 2, (kb1 + 1) / 2);
+    const int4* kinfo = a.kinfo + bhk * a.nblk;
+    bool bad = false;
+    for (int i = kb0 / 2 + lane; i < (kb1 + 1) / 2; i += kWave) bad |= kinfo[i].x != 0;
+    const bool bad_k = __any(bad);
     const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
 
     auto issue = [&](int kb, int stage) {
@@ -1256,7 +1270,7 @@ __global__ __launch_bounds__(256, 1) void packed_dq_again(PackedArgs a) {
         if (kb + 1 < kb1) issue(kb + 1, (kb + 1 - kb0) & 1);
         uint16_t* sk = smem + ((kb - kb0) & 1) * STAGE;
         const uint16_t* sv = sk + TILE;
-        const bool clear = bad_k && kflags[kb / 2];  // K for dQ, not for S
+        const bool clear = bad_k && kinfo[kb / 2].x;  // K for dQ, not for S
         const int key0 = kb * KB;
         // Every wave runs every block, masked where its queries do not see it.
         const bool edge = !(key0 >= ws.all_lo && key0 + KB <= ws.all_hi);
@@ -1432,7 +1446,7 @@ PackedBwdWs packed_bwd_ws(const mc_packed_attn_desc& p, bool spans) {
     off += align256(mfma ? B * H * (Sp / 64) * 128 * 4 : B * H * S * 4);
     if (mfma) {
         w.qflags = off;  off += align256(B * H * (Sp / 64) * 4);
-        w.kflags = off;  off += align256(B * Hkv * nblk * 4);
+        w.kinfo = off;   off += align256(B * Hkv * nblk * 16);
     }
     const size_t ng = mfma ? (size_t)attn_dkdv_groups(d)
                            : attention_f32_mfma_bwd(d) ? (size_t)attention_f32_groups(d) : 1;
@@ -1464,7 +1478,7 @@ hipError_t launch_packed_bwd(const mc_packed_attn_desc& p, const void* q, const 
     a.dout = static_cast<const uint16_t*>(dout);
     a.lsd = lsd;
     a.qflags = qflags;
-    a.kflags = reinterpret_cast<int32_t*>(ws + w.kflags);
+    a.kinfo = reinterpret_cast<int4*>(ws + w.kinfo);
     a.dq = static_cast<uint16_t*>(dq);
     a.dk = static_cast<uint16_t*>(dk);
     a.dv = static_cast<uint16_t*>(dv);

@@ -170,7 +170,7 @@ struct PackedWs {
 struct PackedBwdWs {
     size_t lsd, dk_part, dv_part;  // as AttnBwdWs
     size_t dst;                    // bf16 dS^T in blocks, where a head's stays below 2^31 bytes
-    size_t qflags, kflags;              // int32 [B, H, Sp / 64], [B, Hkv, S rounded up to 128 / 128]
+    size_t qflags, kinfo;          // int32 [B, H, Sp / 64], int32 [B, Hkv, S rounded up to 128 / 128, 4]
     size_t total;
 };
 PackedWs packed_fwd_ws(const mc_packed_attn_desc& d);

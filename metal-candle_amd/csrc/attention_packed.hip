@@ -655,12 +655,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
 // Delta_i = sum_d dO_id O_id carries o's rounding and that of P (bf16 both), which
 // dS = P (dP - Delta) does not average away where few keys share it: dq and dk of
 // 4 causal tokens were 6e-2 of their size off, of 30 9e-3, of 1021 4.9e-3, of 4096
-// 3.6e-3 (their own roundings and dS's to bf16 make 2.4e-3). Where a workgroup's
-// queries span at most kExactKeys keys it is formed as sum_j P_ij dP_ij instead, over
-// sum_j P_ij, which is 1 but for lse's rounding (dS of the only key that a query sees
-// is 0): S^T = K.Q^T and dP^T = V.dO^T once more, shaped as the forward. Both the error
-// and what that costs end there: with 128 / 256 / 512 keys 8 rows of 2048 tokens
-// in documents of 340 are 4.1e-3 / 3.5e-3 / 2.9e-3 off.
+// 3.6e-3 (their own roundings and dS's to bf16 make 2.4e-3). A query that sees at most
+// kExactKeys keys has it as sum_j P_ij dP_ij instead, over sum_j P_ij, which is 1 but
+// for lse's rounding (dS of the only key that a query sees is 0): S^T = K.Q^T and
+// dP^T = V.dO^T once more, shaped as the forward, over the keys of such queries. With
+// 64 / 128 / 256 / 512 / 1024 keys the backward of 8 x 12 x 2048 x 128 in documents of
+// 340 takes 222 / 223 / 228 / 241 / 241 us, and dq and dk of a row are 2.36 / 2.35 / 2.35 /
+// 2.34 / 2.34e-3 off.
 constexpr int kExactKeys = 256;
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16_t* __restrict__ o,
@@ -700,7 +701,10 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
         dma_rows<D>(rk, base, (uint32_t)kb * KB, D, wave, lane);
         dma_rows<D>(rv, base + TILE * 2, (uint32_t)kb * KB, D, wave, lane);
     };
-    const Span mine = query_span(a.spans, b, my_q, (int)S, a.causal);
+    // the keys of a query that sees few, and with them the wave's and the workgroup's
+    const Span all = query_span(a.spans, b, my_q, (int)S, a.causal);
+    const bool few = all.hi - all.lo <= kExactKeys;
+    const Span mine = few ? all : Span{0, 0};
     const WaveSpan ws = wave_span(mine);
     const Span wg = workgroup_span(ws, slots);
 #pragma unroll
@@ -710,8 +714,8 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
     const float lse2 = empty ? __builtin_inff() : bad ? __builtin_nanf("") : x * kLog2e;
     const bool note = __any(my_q < S && (bad || !(__builtin_fabsf(x) < __builtin_inff())));
 
-    float delta = 0.f, sum_p = 0.f;
-    if (wg.hi - wg.lo > kExactKeys) {  // alike in every wave
+    float from_o = 0.f, delta = 0.f, sum_p = 0.f;
+    if (__any(!few)) {
         const __amdgpu_buffer_rsrc_t ro = make_rsrc(o + ((int64_t)b * S * a.H + h) * D, (S * a.H - h) * D * 2);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -720,9 +724,11 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
                 buf_load16(ro, my_q < S ? (uint32_t)((my_q * ldo + 16 * s + 8 * half) * 2) : kOOB), u);
             BVec<uint16_t>::unpack(__builtin_bit_cast(i32x4, gf[s]), g);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) delta = __builtin_fmaf(u[e], g[e], delta);
+            for (int e = 0; e < 8; ++e) from_o = __builtin_fmaf(u[e], g[e], from_o);
         }
-    } else if (wg.lo < wg.hi) {
+        from_o += __shfl_xor(from_o, 32, kWave);
+    }
+    if (wg.lo < wg.hi) {  // alike in every wave
         const __amdgpu_buffer_rsrc_t rq = make_rsrc(a.q + (int64_t)bh * S * D, S * D * 2);
         bf16x8 qf[KS];
 #pragma unroll
@@ -781,7 +787,8 @@ __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16
     }
     delta += __shfl_xor(delta, 32, kWave);
     sum_p += __shfl_xor(sum_p, 32, kWave);
-    if (sum_p > 0.f) delta /= sum_p;  // only where P was formed
+    if (sum_p > 0.f) delta /= sum_p;
+    if (!few) delta = from_o;
     // queries past S have lse = +inf too
     if (half == 0 && my_q < a.Sp) {
         float* blk = lsd + ((int64_t)bh * (a.Sp / 64) + my_q / 64) * 128 + my_q % 64;

@@ -14,7 +14,9 @@
 //
 // Row kernels (bf16 head dims other than 64 and 128, float32 ones that are no
 // multiple of 4 or past 128, and float32 rows of a few tokens): one wave per row,
-// lanes over the head dim, only what the row sees is read.
+// lanes over the head dim, only what the row sees is read. Per key they wait for two
+// rows and one or two sums over the lanes: 2 x 8 (4) x 1024 x 256 bf16, causal and capped,
+// forward 3.5 ms, backward 8.4; of 96 1.3 and 3.8; 1 x 14 (2) x 300 x 40 0.16 and 1.4.
 #include <type_traits>
 
 #include "attention_f32_tiles.hpp"
@@ -541,7 +543,9 @@ __global__ __launch_bounds__(256) void packed_rows_fwd(Rows<T> a) {
     if (a.lse && lane_id() == 0) a.lse[row] = sees ? m + logf(l) : kNegInf;
 }
 
-// Also writes Delta, for packed_rows_dkdv.
+// Also writes Delta, for packed_rows_dkdv. bf16: as sum P dP / sum P, since o's
+// rounding to bf16 would stay in the gradients of queries that see few keys; it is
+// known behind the last key, so dq is scale (sum P dP slope k - Delta sum P slope k).
 template <typename T>
 __global__ __launch_bounds__(256) void packed_rows_dq(Rows<T> a) {
     const int64_t row = (int64_t)blockIdx.x * 4 + wave_id();
@@ -552,22 +556,44 @@ __global__ __launch_bounds__(256) void packed_rows_dq(Rows<T> a) {
     const int64_t orow = (((int64_t)b * a.S + qi) * a.H + h) * a.D;
     const Span see = query_span(a.spans, b, qi, (int)a.S, a.causal);
     const float bias = a.slopes ? a.slopes[h] : 0.f;
-    float qv[4], gv[4], ov[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr bool kFromP = sizeof(T) == 2;
+    float qv[4], gv[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, base[4] = {0.f, 0.f, 0.f, 0.f};
     row_load(a.q + row * a.D, a.D, qv);
     row_load(a.dout + orow, a.D, gv);
-    row_load(a.o + orow, a.D, ov);
-    const float di = row_dot(ov, gv), li = a.lse[row];
-    if (lane_id() == 0) a.delta[row] = di;
+    float di = 0.f, sum_p = 0.f;
+    if constexpr (!kFromP) {
+        float ov[4];
+        row_load(a.o + orow, a.D, ov);
+        di = row_dot(ov, gv);
+    }
+    const float li = a.lse[row];
     for (int key = see.lo; key < see.hi; ++key) {
         const int64_t kr = (bhk * a.S + key) * a.D;
         float kv[4], vv[4], slope;
         row_load(a.k + kr, a.D, kv);
         row_load(a.v + kr, a.D, vv);
         const float s = score_of(row_dot(qv, kv), __builtin_fabsf((float)((int)qi - key)), a.mods, bias, slope);
-        const float ds = exp2_hw((s - li) * kLog2e) * ((row_dot(gv, vv) - di) * slope);
+        const float p = exp2_hw((s - li) * kLog2e), dp = row_dot(gv, vv);
+        if constexpr (kFromP) {
+            sum_p += p;
+            di = __builtin_fmaf(p, dp, di);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] += ds * kv[i];
+            for (int i = 0; i < 4; ++i) {
+                acc[i] += p * dp * slope * kv[i];
+                base[i] += p * slope * kv[i];
+            }
+        } else {
+            const float ds = p * ((dp - di) * slope);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] += ds * kv[i];
+        }
     }
+    if constexpr (kFromP) {
+        if (sum_p > 0.f) di /= sum_p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(-di, base[i], acc[i]);
+    }
+    if (lane_id() == 0) a.delta[row] = di;
     row_store(a.dq + row * a.D, a.D, acc, a.mods.scale);
 }
 

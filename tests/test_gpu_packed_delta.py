@@ -1,5 +1,7 @@
-"""Delta = sum_j P_j dP_j of bf16 queries that see few keys (up to 256), whose gradients
-would carry o's rounding if it were formed from o: whatever lies beside them in the row.
+"""Delta = sum_j P_j dP_j of bf16 queries that see few keys, whose gradients would
+carry o's rounding if it were formed from o: whatever lies beside them in the row
+(the matrix kernels, up to 256 keys a query), and for every head dim (the row
+kernels, always).
 
 Against 64 bits with the bounds of packed_reference.py, `exact` for such queries."""
 import pytest
@@ -52,11 +54,24 @@ def test_few_keys_beside_many(mc, dev, name, causal, D, cap):
     ref.check(got, want_of(q, k, v, see, cap, dout, FEW))
 
 
+@pytest.mark.parametrize("D", [8, 40, 96, 192, 256])
+@pytest.mark.parametrize("cap", [None, 20.0])
+def test_other_head_dims(mc, dev, D, cap):
+    sizes = [40, 1, 4, 2, 1, 22]
+    S = sum(sizes)
+    ids = torch.repeat_interleave(torch.arange(len(sizes), dtype=torch.int32), torch.tensor(sizes))
+    for causal in (True, False):
+        q, k, v, dout = inputs(1, 4, 2, S, D, dev)
+        see = ref.visible(S, ids, causal=causal)[None]
+        got = run(mc, q, k, v, dout, spans=mc.attention_spans(ids[None].to(dev), causal=causal), cap=cap)
+        ref.check(got, want_of(q, k, v, see, cap, dout, S))
+
+
 @pytest.mark.parametrize("cap", [None, 50.0])
-@pytest.mark.parametrize("D,first", [(64, 300), (128, 300)])
+@pytest.mark.parametrize("D,first", [(64, 300), (128, 300), (40, 1), (96, 20), (256, 1)])
 def test_documents_of_one_token_behind_a_long_one(mc, dev, D, first, cap):
-    """P is 1 and dS nothing but what rounding leaves: dP twice, D u |dout| |v| each, u = 2^-24, P dP / P 2 u of it; dq is
-    scale dS k, rounded."""
+    """P is 1 and dS nothing but what rounding leaves: dP twice, D u |dout| |v| each, u = 2^-24, P dP / P 2 u of it, and
+    where dq is a difference of two sums 3 u more; dq is scale dS k, rounded."""
     B, H, Hkv, S = 1, 4, 2, first + 90
     q, k, v, dout = inputs(B, H, Hkv, S, D, dev, std=6.0)
     ids = torch.zeros(B, S, dtype=torch.int32)

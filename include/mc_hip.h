@@ -368,7 +368,8 @@ mc_status mc_adamw_scaled_step(const mc_adamw_config* cfg, const mc_adamw_tensor
  * norm, scale: fp32 [1] on the device. max_norm > 0, infinity for none. A norm past
  * fp32's range is stored as infinity, its scale is still max_norm / norm. Gradients
  * and outputs may start at any element; an output is its own gradient (of the same
- * dtype: in place) or apart from every gradient, and apart from every other output.
+ * dtype: in place) or apart from every gradient, and apart from every other output;
+ * others are refused.
  * The table is read on the host.
  * Sums run in a fixed order: results are bitwise reproducible. The workspace holds
  * nothing between calls. */

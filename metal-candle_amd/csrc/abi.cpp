@@ -9,10 +9,13 @@
 // exercised without a GPU.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <memory>
+#include <new>
 #include <string>
 
 #include "kernels.hpp"
@@ -707,6 +710,39 @@ mc_status mc_adamw_scaled_step(const mc_adamw_config* cfg, const mc_adamw_tensor
     return ok();
 }
 
+// Every output of the table apart from every other output and from every other
+// gradient: the workgroups of a call read and write them in any order. Sorted by
+// address (lists of tensors often are), then one pass over both.
+static mc_status check_apart(const char* op, const mc_grad_tensor* tensors, int32_t count) {
+    struct Range {
+        uintptr_t from, to;
+        int32_t tensor;
+    };
+    const std::unique_ptr<Range[]> ranges(new (std::nothrow) Range[2 * (size_t)count]);
+    MC_CHECK(ranges, MC_ERR_SHAPE, "%s: no host memory for a table of %d tensors", op, (int)count);
+    Range *outs = ranges.get(), *grads = outs + count, *out_end = outs, *grad_end = grads;
+    for (int32_t i = 0; i < count; ++i) {
+        const mc_grad_tensor& t = tensors[i];
+        if (t.numel == 0) continue;
+        const uintptr_t g = reinterpret_cast<uintptr_t>(t.grad), o = reinterpret_cast<uintptr_t>(t.out);
+        *out_end++ = Range{o, o + (size_t)t.numel * (t.out_dtype == MC_F32 ? 4 : 2), i};
+        if (g != o) *grad_end++ = Range{g, g + (size_t)t.numel * (t.dtype == MC_F32 ? 4 : 2), i};
+    }
+    const auto before = [](const Range& a, const Range& b) { return a.from < b.from; };
+    if (!std::is_sorted(outs, out_end, before)) std::sort(outs, out_end, before);
+    if (!std::is_sorted(grads, grad_end, before)) std::sort(grads, grad_end, before);
+    for (const Range* o = outs; o + 1 < out_end; ++o)
+        MC_CHECK(o->to <= o[1].from, MC_ERR_LAYOUT, "%s: the outs of tensors %d and %d overlap", op, (int)o->tensor,
+                 (int)o[1].tensor);
+    const Range* o = outs;
+    for (const Range* g = grads; g < grad_end; ++g) {
+        while (o < out_end && o->to <= g->from) ++o;
+        MC_CHECK(o == out_end || o->from >= g->to, MC_ERR_LAYOUT, "%s: out of tensor %d overlaps grad of tensor %d", op,
+                 (int)o->tensor, (int)g->tensor);
+    }
+    return MC_OK;
+}
+
 static mc_status check_grads(const char* op, const mc_grad_tensor* tensors, int32_t count, bool outs, double* elems) {
     MC_CHECK(count >= 0, MC_ERR_SHAPE, "%s: tensor count must be >= 0, got %d", op, (int)count);
     MC_CHECK(count == 0 || tensors, MC_ERR_NULL, "%s: tensor table is NULL", op);
@@ -736,7 +772,7 @@ static mc_status check_grads(const char* op, const mc_grad_tensor* tensors, int3
     }
     MC_CHECK(total < 1.0e15, MC_ERR_SHAPE, "%s: %g elements are too many", op, total);
     *elems = total;
-    return MC_OK;
+    return outs && count > 1 ? check_apart(op, tensors, count) : MC_OK;
 }
 
 static mc_status check_max_norm(const char* op, float max_norm) {

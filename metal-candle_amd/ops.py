@@ -970,7 +970,8 @@ def gradient_norm(grads, max_norm=None):
 
 def scale_gradients(grads, scale, outs=None):
     """Every gradient times scale (fp32 [1] on the device) into outs (fp32 or bf16 tensors of the same sizes; default:
-    in place), one rounding each. A tensor may be written once only: one that is listed twice is refused. Returns outs."""
+    in place), one rounding each. An output is its own gradient or apart from every gradient and output: one that is
+    listed twice, or overlaps another, is refused. Returns outs."""
     at, n, table = _grad_table(grads, outs)
     if scale is None:
         raise McError(_lib.MC_ERR_NULL, "scale must be a tensor")

@@ -863,17 +863,27 @@ def _ids(ids, device):
     return ids
 
 
+def _padding(padding_id):
+    """The id of padding, -1 for none. Ids past int32 arrive as 2**31 - 1, which is in no table and no padding."""
+    if padding_id is None or padding_id < 0:
+        return -1
+    if padding_id > 2**31 - 2:
+        raise McError(_lib.MC_ERR_VALUE, f"padding_id must be below 2**31 - 1, got {padding_id}")
+    return int(padding_id)
+
+
 def embedding_forward(table, ids, scale=1.0, padding_id=None):
     """scale * table[ids] for table [V, D] and ids int32 (or int64) [...]: [..., D] in the table's dtype, rounded once.
 
-    A token of padding_id gets zeros, one whose id is not in the table NaN."""
+    A token of padding_id gets zeros, one whose id is not in the table NaN. padding_id None or below 0: none (a token of
+    a negative id gets NaN then too)."""
     if not isinstance(table, torch.Tensor) or table.dim() != 2 or table.numel() == 0:
         raise McError(_lib.MC_ERR_SHAPE, "table must be [vocab, dim]")
     _contig(table, "table")
     code = _dtype_code(table)
     ids = _ids(ids, table.device)
     V, D = table.shape
-    d = EmbeddingDesc(ids.numel(), V, D, -1 if padding_id is None else int(padding_id), float(scale), code)
+    d = EmbeddingDesc(ids.numel(), V, D, _padding(padding_id), float(scale), code)
     out = torch.empty(*ids.shape, D, dtype=table.dtype, device=table.device)
     _launch(table, lib().mc_embedding_fwd, ctypes.byref(d), table.data_ptr(), ids.data_ptr(), out.data_ptr())
     return out
@@ -893,7 +903,7 @@ def embedding_backward(dout, ids, vocab, scale=1.0, padding_id=None, dtable=None
     if ids.shape != dout.shape[:-1]:
         raise McError(_lib.MC_ERR_SHAPE, f"ids has shape {tuple(ids.shape)}, expected {tuple(dout.shape[:-1])}")
     D, V = dout.shape[-1], int(vocab)
-    d = EmbeddingDesc(ids.numel(), V, D, -1 if padding_id is None else int(padding_id), float(scale), code)
+    d = EmbeddingDesc(ids.numel(), V, D, _padding(padding_id), float(scale), code)
     into = _address(dtable, "dtable", (V, D), torch.float32, dout.device)
     ws_n = lib().mc_embedding_bwd_workspace_size(ctypes.byref(d))
     if dtable is None and ws_n:

@@ -261,6 +261,27 @@ __device__ __forceinline__ bool any_flag(const int32_t* flags, int from, int to)
     return __any(bad);
 }
 
+// take(dt, j, value) for the infinities and NaN of rows [from, to) of x [S][D] that this
+// lane's query sees, at its accumulators j of tile dt (dim 32 dt + 8 (j/4) + 4 half + j%4).
+template <int D, typename F>
+__device__ __forceinline__ void each_nonfinite(const uint16_t* x, int from, int to, Span sees, int half, F&& take) {
+#pragma unroll 1
+    for (int key = from; key < to; ++key) {
+        if (key < sees.lo || key >= sees.hi) continue;
+        const uint16_t* row = x + (int64_t)key * D + 4 * half;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+            for (int jq = 0; jq < 4; ++jq) {
+                const uint2 w = *reinterpret_cast<const uint2*>(row + 32 * dt + 8 * jq);
+                const uint32_t e[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (nonfinite16(e[u])) take(dt, 4 * jq + u, __uint_as_float(e[u] << 16));
+            }
+    }
+}
+
 struct PackedArgs {
     const uint16_t* q;     // [B, H, S, D]
     const uint16_t* k;     // [B, Hkv, S, D]
@@ -602,22 +623,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
 #pragma unroll 1
         for (int kb = wk0; kb < wk1; ++kb) {
             if (!ROWS && a.vflags[bhk * (a.Sp / 64) + kb] == 0) continue;
-            const int last = (kb + 1) * KB < (int)S ? (kb + 1) * KB : (int)S;
-#pragma unroll 1
-            for (int key = kb * KB; key < last; ++key) {
-                if (key < mine.lo || key >= mine.hi) continue;
-                const uint16_t* row = a.v + (bhk * S + key) * D + 4 * half;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int jq = 0; jq < 4; ++jq) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(row + 32 * dt + 8 * jq);
-                        const uint32_t e[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            if (nonfinite16(e[u])) oacc[dt][4 * jq + u] += __uint_as_float(e[u] << 16);
-                    }
-            }
+            each_nonfinite<D>(a.v + bhk * S * D, kb * KB, (kb + 1) * KB < (int)S ? (kb + 1) * KB : (int)S, mine, half,
+                              [&](int dt, int j, float v) { oacc[dt][j] += v; });
         }
     }
 
@@ -1083,13 +1090,27 @@ __global__ __launch_bounds__(256) void packed_sum(PackedArgs a) {
 }
 
 // ------------------------------------------------------------------- dQ
+// dQ's share of the infinities and NaN that K's tiles were cleared of: dS of a query
+// that sees such a key is NaN, or 0 where its score is minus infinity or at the cap,
+// and 0 times an infinity is NaN as well.
+template <int D, typename Acc>
+__device__ __forceinline__ void nan_of_keys(const PackedArgs& a, int64_t bhk, int kb0, int kb1, Span sees, int half,
+                                            Acc& dqacc) {
+#pragma unroll 1
+    for (int i = kb0 / 2; i < (kb1 + 1) / 2; ++i) {
+        if (a.kinfo[bhk * a.nblk + i].x == 0) continue;
+        each_nonfinite<D>(a.k + bhk * a.S * D, i * 128, i * 128 + 128 < (int)a.S ? i * 128 + 128 : (int)a.S, sees, half,
+                          [&](int dt, int j, float) { dqacc[dt][j] = __builtin_nanf(""); });
+    }
+}
+
 // From the stored dS^T: per block of 64 keys that the workgroup's queries see, the
 // K tile [64][D] and dS^T of the 128 queries, four blocks as they are in memory, go
 // into LDS (two stages); dQ^T (d x query) += K^T . dS^T takes both by transposed reads.
 // A block between the first and the last of these keys that none of the queries
 // sees may have no dS^T in memory: it is left out, by kinfo. A K tile with infinities
-// or NaN is cleared of them first: dS is NaN where a query sees such a key and 0
-// where it does not. Workgroups past dq_blocks sum the groups' dK / dV partials.
+// or NaN is cleared of them first, and the rows that see such a key get NaN there
+// afterwards (nan_of_keys). Workgroups past dq_blocks sum the groups' dK / dV partials.
 template <int D>
 __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
     if ((int64_t)blockIdx.x >= a.dq_blocks) {
@@ -1188,6 +1209,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq(PackedArgs a) {
         }
     }
 
+    if (bad_k) nan_of_keys<D>(a, bhk, kb0, kb1, mine, lane >> 5, dqacc);
     wait_vmcnt<0>();  // every DMA has landed (also when the loop ran no block)
     __syncthreads();
     store_rows<D, uint16_t>(dqacc, a.scale, smem + wave * 32 * (D + 8), a.dq + (int64_t)bh * S * D, D, qw, S, lane);
@@ -1334,6 +1356,7 @@ __global__ __launch_bounds__(256, 1) void packed_dq_again(PackedArgs a) {
         tile(std::integral_constant<int, 1>{});
     }
 
+    if (bad_k) nan_of_keys<D>(a, bhk, kb0, kb1, mine, half, dqacc);
     wait_vmcnt<0>();  // every DMA has landed (also when the loop ran no block)
     __syncthreads();
     store_rows<D, uint16_t>(dqacc, a.scale, smem + wave * 32 * (D + 8), a.dq + (int64_t)bh * S * D, D, qw, S, lane);

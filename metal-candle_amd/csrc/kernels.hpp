@@ -162,14 +162,13 @@ hipError_t launch_attention_f32_bwd(const mc_attn_desc& d, const void* q, const 
 
 // Attention over packed rows (attention_packed.hip; float32 and row kernels in
 // attention_packed_f32.hip). spans: int32 [B, S, 4] or null (d.attn.causal).
-bool attention_dq_from_ds(const mc_attn_desc& d);  // the dQ pass reads a stored dS^T
 struct PackedWs {
     size_t vt, flags;  // bf16 [B, Hkv, D, Sp]; int32 [B, Hkv, Sp / 64]
     size_t total;
 };
 struct PackedBwdWs {
     size_t lsd, dk_part, dv_part;  // as AttnBwdWs
-    size_t dst;                    // bf16 dS^T in blocks, where a head's stays below 2^31 bytes
+    size_t dst;                    // bf16 dS^T in blocks, where a head's stays below 2^31 bytes (dq_from_ds there)
     size_t qflags, kinfo;          // int32 [B, H, Sp / 64], int32 [B, Hkv, S rounded up to 128 / 128, 4]
     size_t total;
 };

@@ -28,6 +28,12 @@
 //               past 2^31 bytes of one head's dS^T packed_dq_again forms S and dP
 //               once more.
 //
+// Roundings to bf16, each for the matrix rate of bf16, sixteen times float32's: P before
+// P.V and dV (its sum keeps it unrounded, so o is off by at most 2^-8 of sum P |v|), dS
+// before dK and dQ, which reads it from memory. Sums, maxima, lse and Delta are float32.
+// Of the size of a result that makes 2.4e-3 for dq and dk of random rows, where their
+// own rounding is 1.7e-3, and up to 3.4e-3 with Delta from o (packed_prep).
+//
 // The cap. With r = 1 / (1 + 2^(2 log2 e x / cap)), tanh(x / cap) = 1 - 2 r and
 // its slope is 4 (r - r^2): one exponential and one reciprocal more per score.
 // tanh grows with x, so the running maximum stays one of unscaled products.
@@ -41,7 +47,7 @@
 //  packed_vt    10     7.1   3.6   memory
 //  packed_fwd   664    70    17    (a) 725 TFLOP/s: the scores' arithmetic, of whose
 //                                  time the cap's exponential and reciprocal are half
-//  packed_prep  52     39    12    (a) memory; (b, c) S and dP once more
+//  packed_prep  52     44    14    (a) memory; (b, c) S and dP once more
 //  packed_dkdv  1467   155   27    one wave per SIMD: MFMA 31% of its cycles, scores
 //                                  37, waits 27, which follow each other (the scores
 //                                  of one query tile among the other's MFMAs: 1800
@@ -668,7 +674,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd(PackedArgs a) {
 // dP^T = V.dO^T once more, shaped as the forward, over the keys of such queries. With
 // 64 / 128 / 256 / 512 / 1024 keys the backward of 8 x 12 x 2048 x 128 in documents of
 // 340 takes 222 / 223 / 228 / 241 / 241 us, and dq and dk of a row are 2.36 / 2.35 / 2.35 /
-// 2.34 / 2.34e-3 off.
+// 2.34 / 2.34e-3 off; in documents of 64 to 1024, 3.0 / 2.6 / 2.4e-3 with 256 / 512 / 1024.
+// Formed so for every query of 4 x 28 x 4096 x 128, a call takes 24% longer.
 constexpr int kExactKeys = 256;
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void packed_prep(PackedArgs a, const uint16_t* __restrict__ o,
